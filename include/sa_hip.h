@@ -385,6 +385,59 @@ int sa_paged_kv_append(const void* k, const void* v, const float* log_gate,
                        int head_dim, int page_size, int max_pages, void* k_pages, void* v_pages,
                        float* gate_pages, void* stream);
 
+/*
+ * Paged KV cache in 8 bits (no counterpart in the reference, whose caches keep
+ * the model's dtype, inference/selective_attn_cache.py:3-42).  A block is one
+ * page of one kv head.  Full blocks: k_pages (num_pages, heads, page_size,
+ * head_dim) and v_pages (num_pages, heads, head_dim, page_size) e4m3 codes,
+ * k_scale and v_scale (num_pages, heads) f32, each the smallest power of two
+ * 2^e, e >= -126, with max|x| <= 448 * 2^e (1 for a block of zeros); a code
+ * stands for code * scale.  A row's open block, its seq_len % page_size tokens
+ * behind the last full page: k_tail (batch, heads, page_size, head_dim) and
+ * v_tail (batch, heads, head_dim, page_size) bf16.  gate_pages (num_pages,
+ * heads, page_size) f32, and log_gate, NULL for a cache without gates; tokens
+ * at -inf are left out of their block's maximum and stored as 0, the block's
+ * last one apart.  Infinities and NaN stay out of the maximum and are stored
+ * as NaN.  page_size in {64, 128}, head_dim in {64, 128}.
+ *
+ * append: one token per row, k and v (batch, heads, head_dim) bf16, log_gate
+ *   (batch, heads) f32: slot seq_lens[r] % page_size of the open block; a block
+ *   that it fills is rounded into page page_table[r][seq_lens[r] / page_size];
+ *   then seq_lens[r] += 1 on the device.  A page id outside the pool, or a slot
+ *   behind max_pages, leaves the pages as they are.
+ * build: tokens t < min(seq_lens[r], seqlen) of row r; k, v bf16 with element
+ *   strides sb (batch), st (token), sh (head), head_dim contiguous; log_gate
+ *   f32 with strides gb, gh, gt.  Slots behind a row's tokens in its open block
+ *   are 0 with -inf gates; nothing else is written.
+ */
+int sa_paged_kv_append_fp8(const void* k, const void* v, const float* log_gate,
+                           const int32_t* page_table, int32_t* seq_lens, int batch, int heads,
+                           int head_dim, int page_size, int max_pages, int num_pages,
+                           void* k_pages, void* v_pages, float* k_scale, float* v_scale,
+                           void* k_tail, void* v_tail, float* gate_pages, void* stream);
+int sa_paged_kv_build_fp8(const void* k, const void* v, long sb, long st, long sh,
+                          const float* log_gate, long gb, long gh, long gt,
+                          const int32_t* page_table, const int32_t* seq_lens, int batch,
+                          int seqlen, int heads, int head_dim, int page_size, int max_pages,
+                          int num_pages, void* k_pages, void* v_pages, float* k_scale,
+                          float* v_scale, void* k_tail, void* v_tail, float* gate_pages,
+                          void* stream);
+
+/*
+ * Paged GQA decode attention over that cache: sa_paged_decode_fwd's operation
+ * and workspace (sa_paged_decode_workspace_size), the keys and values as the
+ * codes stand for them.  q, o (batch, Hq, D) bf16; key_bias is gate_pages or
+ * NULL; a key whose bias is -inf (the newest apart) takes no part, whatever
+ * its codes.  Page ids outside the pool contribute no keys.
+ */
+int sa_paged_decode_fp8_fwd(const void* q, const void* k_pages, const void* v_pages,
+                            const float* k_scale, const float* v_scale, const void* k_tail,
+                            const void* v_tail, const int32_t* page_table,
+                            const int32_t* seq_lens, const float* key_bias, int batch,
+                            int num_q_heads, int num_kv_heads, int head_dim, int page_size,
+                            int max_pages, int num_pages, float softmax_scale, void* o,
+                            void* workspace, size_t workspace_bytes, void* stream);
+
 /* Workspace bytes of sa_paged_decode_fwd: segment partials for
  * batch * num_kv_heads + 8192 segments, plus a per-row tile prefix sum. */
 size_t sa_paged_decode_workspace_size(int batch, int num_q_heads, int num_kv_heads, int head_dim,

@@ -26,37 +26,6 @@
 
 namespace sa {
 
-// Online-softmax update for one block of keys.  s[kt][i]: log2-domain scores
-// of keys 16kt + 4g + i for query column (lane & 15); masked entries are
-// -inf.  Converts s to probabilities in place, rescales o, updates m and l.
-template <int KT, int DT>
-__device__ __forceinline__ void softmax_block(v4f (&s)[KT], v4f (&o)[DT], float& m, float& l) {
-  float mx = kNegInf;
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[kt][i]);
-  mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-  mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-  const float m_new = fmaxf(m, mx);
-  const float alpha = (m == kNegInf) ? 0.0f : fast_exp2(m - m_new);
-  float sum = 0.0f;
-#pragma unroll
-  for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float p = (s[kt][i] == kNegInf) ? 0.0f : fast_exp2(s[kt][i] - m_new);
-      s[kt][i] = p;
-      sum += p;
-    }
-  sum += __shfl_xor(sum, 16, 64);
-  sum += __shfl_xor(sum, 32, 64);
-  l = l * alpha + sum;
-  m = m_new;
-#pragma unroll
-  for (int t = 0; t < DT; ++t) o[t] *= alpha;
-}
-
 // ---------------------------------------------------------------------------
 // block-sparse varlen prefill.  One workgroup per (head, 64-query block),
 // four waves: wave w owns query rows 32 (w & 1) .. +31 and, of every selected
@@ -557,11 +526,6 @@ int launch_attn(int mode, int D, const void* q, const void* k, const void* v, co
 // outstanding.  Page ids are fetched 64 at a time, one per lane, and
 // broadcast with readlane.
 // ---------------------------------------------------------------------------
-template <bool B>
-struct BoolC {
-  static constexpr bool value = B;
-};
-
 struct DecodeSlot {
   long kidx;  // index of the tile's first key in the (page, kv head, key) pool
   int nk;     // valid keys of the tile (0: invalid page id)
@@ -596,11 +560,6 @@ __device__ __forceinline__ void decode_load_v(v8bf (&vf)[2][D / 16], const bf16*
       vf[ks][t] = buf_load_v8bf(r, voff, static_cast<unsigned>(32 * t * ps + 64 * ks));
 }
 
-// tiles of row r: ceil(clamp(seq_lens[r], 0, max_pages * ps) / 64)
-__device__ __forceinline__ int decode_row_len(const int32_t* seq_lens, int r, int max_pages, int ps) {
-  return min(max(seq_lens[r], 0), max_pages * ps);
-}
-
 // cum_row[r] = 64-key tiles of rows < r (per kv head), r = 0..b.  One block.
 __global__ __launch_bounds__(1024) void paged_decode_plan_kernel(
     const int32_t* __restrict__ seq_lens, int b, int ps, int max_pages,
@@ -629,14 +588,6 @@ __global__ __launch_bounds__(1024) void paged_decode_plan_kernel(
     carry += tot;
     __syncthreads();  // wtot is rewritten by the next chunk
   }
-}
-
-// first tile of wave w and the wave that holds tile g (W waves, T tiles)
-__device__ __forceinline__ long decode_wave_begin(int w, long T, int W) {
-  return static_cast<long>(w) * T / W;
-}
-__device__ __forceinline__ int decode_wave_of(long g, long T, int W) {
-  return static_cast<int>(((g + 1) * W + T - 1) / T - 1);
 }
 
 template <int D, bool BIAS>
@@ -922,23 +873,6 @@ __global__ __launch_bounds__(64) void paged_decode_merge_kernel(
   }
 }
 
-// waves of one resident round: CUs x resident 64-thread blocks per CU
-template <typename K>
-int decode_waves(K kern, int variant) {
-  static int cache[64][4] = {};
-  int dev = 0;
-  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 1024;
-  if (cache[dev][variant] == 0) {
-    int cus = 0, per_cu = 0;
-    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
-        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, 64, 0) != hipSuccess ||
-        cus <= 0 || per_cu <= 0)
-      return 1024;
-    cache[dev][variant] = min(cus * per_cu, kDecodeMaxWaves);
-  }
-  return cache[dev][variant];
-}
-
 }  // namespace sa
 
 extern "C" size_t sa_paged_decode_workspace_size(int batch, int num_q_heads, int num_kv_heads,
@@ -984,6 +918,28 @@ int decode_wave_count(int head_dim, bool bias) {
               : decode_waves(paged_decode_kernel<64, false>, 3);
 }
 
+// row plan of more than 64 rows (up to 64 the decode waves form it themselves)
+int decode_plan_launch(const int32_t* seq_lens, int batch, int page_size, int max_pages,
+                       const DecodeWs& ws, hipStream_t s) {
+  if (batch <= 64) return 0;
+  sa::ProfScope prof_("paged_decode_plan", s);
+  hipLaunchKernelGGL(sa::paged_decode_plan_kernel, dim3(1), dim3(1024), 0, s, seq_lens, batch,
+                     page_size, max_pages, ws.cum_row);
+  SA_CHECK_LAUNCH("paged_decode_plan");
+  return 0;
+}
+
+// merge of the segments that a W-wave stream-K decode left in ws
+int decode_merge_launch(int batch, int num_q_heads, int num_kv_heads, int head_dim, void* o,
+                        const DecodeWs& ws, int W, hipStream_t s) {
+  sa::ProfScope prof_("paged_decode_merge", s);
+  hipLaunchKernelGGL(sa::paged_decode_merge_kernel, dim3(batch * num_q_heads), dim3(64), 0, s,
+                     ws.part_o, ws.part_ml, ws.cum_row, static_cast<sa::bf16*>(o), batch,
+                     num_q_heads, num_kv_heads, head_dim, W);
+  SA_CHECK_LAUNCH("paged_decode_merge");
+  return 0;
+}
+
 // plan (more than 64 rows), stream-K decode and merge on workspace `ws` with W waves
 int decode_launch(const void* q, const void* k_pages, const void* v_pages,
                   const int32_t* page_table, const int32_t* seq_lens, const float* key_bias,
@@ -992,12 +948,7 @@ int decode_launch(const void* q, const void* k_pages, const void* v_pages,
                   int W, hipStream_t s) {
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(static_cast<float>(head_dim));
   const float sl2 = scale * sa::kLog2e;
-  if (batch > 64) {   // up to 64 rows the decode waves form the plan themselves
-    sa::ProfScope prof_("paged_decode_plan", s);
-    hipLaunchKernelGGL(sa::paged_decode_plan_kernel, dim3(1), dim3(1024), 0, s, seq_lens, batch,
-                       page_size, max_pages, ws.cum_row);
-    SA_CHECK_LAUNCH("paged_decode_plan");
-  }
+  if (const int rc = decode_plan_launch(seq_lens, batch, page_size, max_pages, ws, s)) return rc;
   {
     sa::ProfScope prof_("paged_decode", s);
     auto launch = [&](auto kern) {
@@ -1013,14 +964,7 @@ int decode_launch(const void* q, const void* k_pages, const void* v_pages,
       key_bias ? launch(sa::paged_decode_kernel<64, true>) : launch(sa::paged_decode_kernel<64, false>);
     SA_CHECK_LAUNCH("paged_decode");
   }
-  {
-    sa::ProfScope prof_("paged_decode_merge", s);
-    hipLaunchKernelGGL(sa::paged_decode_merge_kernel, dim3(batch * num_q_heads), dim3(64), 0, s,
-                       ws.part_o, ws.part_ml, ws.cum_row, static_cast<sa::bf16*>(o), batch,
-                       num_q_heads, num_kv_heads, head_dim, W);
-    SA_CHECK_LAUNCH("paged_decode_merge");
-  }
-  return 0;
+  return decode_merge_launch(batch, num_q_heads, num_kv_heads, head_dim, o, ws, W, s);
 }
 
 }  // namespace sa

@@ -1,0 +1,351 @@
+// Paged GQA decode attention over a cache held in 8 bits (gfx950).
+//
+// A block is one page of tokens of one kv head.  A full block's keys are e4m3
+// codes k_pages (num_pages, Hkv, ps, D) with one scale k_scale (num_pages,
+// Hkv), its values codes v_pages (num_pages, Hkv, D, ps), transposed, with
+// v_scale; a code stands for code * scale, and the scales are powers of two.
+// A row's open block, the seq_len % ps tokens behind its last full page, is in
+// bfloat16: k_tail (batch, Hkv, ps, D), v_tail (batch, Hkv, D, ps).
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(log2(e) (scale q.k_j +
+//   [j not the newest] bias_j) - m),  m the running maximum
+//
+// The split is stream-K over 64-key tiles, as in the bf16 decode (attention.hip):
+// one resident round of W one-wave workgroups, each the same number of tiles
+// of the (row, kv head, tile) list, partial sums joined by the merge kernel.
+// What differs is the tile: 64 D codes are a quarter to a half of the
+// registers of the bf16 tile, widened to bf16 MFMA operands right before
+// their product (v_cvt_scalef32_pk_bf16_fp8, two codes an instruction, which
+// multiplies by the block's power of two on the way: exact, every e4m3 number
+// times 2^e is a bf16 number).
+//
+// Operand order.  Lane (c, g) = (lane & 15, lane >> 4) loads 16 codes at once.
+// K: dims 64 s + 16 g .. + 15 of key 16 (c >> 2) + 4 kt + (c & 3), the k-steps
+// 2 s and 2 s + 1 of the contraction over dims (q is loaded in the same
+// order).  The score tile kt then leaves lane (c, g) the keys 16 g + 4 kt + i,
+// i = 0..3, of query column c, so the four tiles give it keys 16 g .. + 15:
+// what its V^T load of 16 codes (dim 16 t + c, keys 16 g .. + 15) contracts.
+#include "common.h"
+#include "decode.h"
+#include "prof.h"
+
+namespace sa {
+namespace {
+
+// 8 e4m3 codes (two words) times the power of two `scale` as a bf16 fragment
+__device__ __forceinline__ v8bf widen8(uint32_t lo, uint32_t hi, float scale) {
+  const uint4 r = {
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(lo, scale, true)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, false)),
+      __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(hi, scale, true))};
+  return __builtin_bit_cast(v8bf, r);
+}
+
+struct Slot8 {
+  long blk;          // (page, kv head) of the tile in the pool
+  int k0;            // the tile's first key inside its page
+  bool ok;           // a valid page id: else the tile has no keys
+  float ks, vs;      // the block's scales
+};
+
+template <int D, bool BIAS>
+__global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
+    const bf16* __restrict__ q, const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp,
+    const float* __restrict__ ksc, const float* __restrict__ vsc, const bf16* __restrict__ kt_p,
+    const bf16* __restrict__ vt_p, const int32_t* __restrict__ page_table,
+    const int32_t* __restrict__ seq_lens, const float* __restrict__ key_bias,
+    int32_t* __restrict__ cum_row, float* __restrict__ part_o, float* __restrict__ part_ml, int b,
+    int Hq, int Hkv, int ps, int max_pages, int num_pages, int W, float scale_log2) {
+  constexpr int DT = D / 16, KS = D / 32, K2 = D / 64;
+  const int w = blockIdx.x;
+  const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
+  // row plan: up to 64 rows each wave forms it in its lanes (lane r holds row
+  // r's 64-key tiles and the tiles before it), wave 0 stores it for the merge
+  const bool lane_plan = b <= 64;
+  int ex_l = 0, tot = 0;
+  if (lane_plan) {
+    const int nb = lane < b ? (decode_row_len(seq_lens, lane, max_pages, ps) + 63) >> 6 : 0;
+    int incl = nb;
+#pragma unroll
+    for (int o2 = 1; o2 < 64; o2 <<= 1) {
+      const int t = __shfl_up(incl, o2, 64);
+      if (lane >= o2) incl += t;
+    }
+    ex_l = incl - nb;
+    tot = __builtin_amdgcn_readlane(incl, 63);
+    if (w == 0 && lane < b) {
+      cum_row[lane + 1] = incl;
+      if (lane == 0) cum_row[0] = 0;
+    }
+  }
+  auto crow = [&](int r) -> int {   // tiles of the rows before r, r in [0, b]
+    return lane_plan ? (r < 64 ? __builtin_amdgcn_readlane(ex_l, r) : tot) : cum_row[r];
+  };
+  const long T = static_cast<long>(Hkv) * crow(b);
+  W = static_cast<int>(min(static_cast<long>(W), T));   // every wave gets a tile
+  if (w >= W) return;
+  long gt = decode_wave_begin(w, T, W);
+  const long gt_end = decode_wave_begin(w + 1, T, W);
+  const int grp = Hq / Hkv;
+  const int tshift = ps == 128 ? 1 : 0;   // log2(64-key tiles per page)
+
+  // row of the first tile: the largest r with Hkv * cum_row[r] <= gt
+  int bi = 0;
+  if (lane_plan) {
+    bi = __popcll(__ballot(lane < b && static_cast<long>(Hkv) * ex_l <= gt)) - 1;
+  } else {
+    int lo = 0, span = b;   // 64-ary search, answer in [lo, lo + span)
+    while (span > 1) {
+      const int step = (span + 63) >> 6;
+      const int r = lo + lane * step;
+      const bool le = r < lo + span && static_cast<long>(Hkv) * cum_row[r] <= gt;
+      const int k = __popcll(__ballot(le));   // >= 1: lane 0 reads cum_row[lo]
+      const int nlo = lo + (k - 1) * step;
+      span = min(step, lo + span - nlo);
+      lo = nlo;
+    }
+    bi = lo;
+  }
+
+  while (gt < gt_end) {
+    long rb = static_cast<long>(Hkv) * crow(bi);
+    int tb = crow(bi + 1) - crow(bi);
+    while (gt >= rb + static_cast<long>(Hkv) * tb) {   // rows with no tiles
+      ++bi;
+      rb = static_cast<long>(Hkv) * crow(bi);
+      tb = crow(bi + 1) - crow(bi);
+    }
+    const int off = static_cast<int>(gt - rb);
+    const int kvh = off / tb;
+    const int t_begin = off - kvh * tb;
+    const int t_end = t_begin + static_cast<int>(min(gt_end - gt, static_cast<long>(tb - t_begin)));
+    const int n = decode_row_len(seq_lens, bi, max_pages, ps);
+    const int t_open = (n / ps) << tshift;   // first tile of the open block
+    const int t_close = min(t_end, t_open);
+    const int32_t* prow = page_table + static_cast<long>(bi) * max_pages;
+
+    const bf16* qrow = q + (static_cast<long>(bi) * Hq + kvh * grp + min(c, grp - 1)) * D;
+    v8bf qf[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+      qf[ks] = c < grp ? load_v8bf(qrow + 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)) : zero_v8bf();
+    float m = kNegInf, l = 0.0f;
+    v4f acc[DT];
+#pragma unroll
+    for (int t = 0; t < DT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    // scale, bias (not on the newest key) and mask of the score tiles; entry
+    // (kt, i) is key 16 g + 4 kt + i of the tile at sequence position pos0.
+    // keep[kt] gets the byte mask of the keys that take part.
+    auto finish = [&](v4f (&sc)[4], const float* brow, int nk, int pos0, uint32_t (&keep)[4])
+                      __attribute__((always_inline)) {
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
+        if constexpr (BIAS) bv = *reinterpret_cast<const float4*>(brow + 16 * g + 4 * kt);
+        const float bs[4] = {bv.x, bv.y, bv.z, bv.w};
+        keep[kt] = 0u;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = 16 * g + 4 * kt + i;
+          bool on = key < nk;
+          float val = sc[kt][i] * scale_log2;
+          if constexpr (BIAS) {
+            const bool newest = key == n - 1 - pos0;
+            val = newest ? val : val + bs[i] * kLog2e;
+            on = on && (newest || bs[i] != kNegInf);   // a dropped key counts for nothing, whatever it holds
+          }
+          sc[kt][i] = on && c < grp ? val : kNegInf;
+          keep[kt] |= on ? 0xffu << (8 * i) : 0u;
+        }
+      }
+    };
+
+    // full blocks, in runs of at most 64 pages: lane j holds the id and the
+    // scales of the run's page p0 + j
+    for (int r0 = t_begin; r0 < t_close;) {
+      const int p0 = r0 >> tshift;
+      const int r1 = min(t_close, (p0 + 64) << tshift);
+      const int my_page = lane <= ((r1 - 1) >> tshift) - p0 ? prow[p0 + lane] : -1;
+      const bool my_ok = my_page >= 0 && my_page < num_pages;
+      // invalid ids read page 0, which exists, and contribute no keys
+      const long my_blk = static_cast<long>(my_ok ? my_page : 0) * Hkv + kvh;
+      const float my_ks = ksc[my_blk], my_vs = vsc[my_blk];
+      auto slot_of = [&](int t) {
+        const int j = (t >> tshift) - p0;
+        const int page = __builtin_amdgcn_readlane(my_page, j);
+        Slot8 sl;
+        sl.ok = page >= 0 && page < num_pages;
+        sl.blk = static_cast<long>(sl.ok ? page : 0) * Hkv + kvh;
+        sl.k0 = (t & tshift) * 64;
+        sl.ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_ks), j));
+        sl.vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_vs), j));
+        return sl;
+      };
+      uint4 kf[4][K2], vf[DT];
+      auto load_k = [&](const Slot8& sl) __attribute__((always_inline)) {
+        const uint8_t* base = kp + (sl.blk * ps + sl.k0) * D;
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int s = 0; s < K2; ++s)
+            kf[kt][s] = *reinterpret_cast<const uint4*>(
+                base + static_cast<unsigned>((16 * (c >> 2) + 4 * kt + (c & 3)) * D + 64 * s + 16 * g));
+      };
+      auto load_v = [&](const Slot8& sl) __attribute__((always_inline)) {
+        const uint8_t* base = vp + sl.blk * ps * D + sl.k0;
+#pragma unroll
+        for (int t = 0; t < DT; ++t)
+          vf[t] = *reinterpret_cast<const uint4*>(base + static_cast<unsigned>((16 * t + c) * ps + 16 * g));
+      };
+      Slot8 cur = slot_of(r0);
+      load_k(cur);
+      load_v(cur);
+      auto tile = [&](auto more_c, int t, const Slot8& nxt) __attribute__((always_inline)) {
+        constexpr bool kMore = decltype(more_c)::value;
+        v4f sc[4];
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+          sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int s = 0; s < K2; ++s) {
+            const uint4 x = kf[kt][s];
+            sc[kt] = mfma_bf16(widen8(x.x, x.y, cur.ks), qf[2 * s], sc[kt]);
+            sc[kt] = mfma_bf16(widen8(x.z, x.w, cur.ks), qf[2 * s + 1], sc[kt]);
+          }
+        }
+        if constexpr (kMore) load_k(nxt);
+        uint32_t keep[4];
+        finish(sc, key_bias + cur.blk * ps + cur.k0, cur.ok ? 64 : 0, 64 * t, keep);
+        softmax_block<4, DT>(sc, acc, m, l);
+        const v8bf p0b = pack_p(sc[0], sc[1]), p1b = pack_p(sc[2], sc[3]);
+        if (cur.ok) {
+#pragma unroll
+          for (int tt = 0; tt < DT; ++tt) {
+            uint4 x = vf[tt];
+            if constexpr (BIAS) x = uint4{x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]};
+            acc[tt] = mfma_bf16(widen8(x.x, x.y, cur.vs), p0b, acc[tt]);
+            acc[tt] = mfma_bf16(widen8(x.z, x.w, cur.vs), p1b, acc[tt]);
+          }
+        }
+        if constexpr (kMore) load_v(nxt);
+      };
+      for (int t = r0; t + 1 < r1; ++t) {
+        const Slot8 nxt = slot_of(t + 1);
+        tile(BoolC<true>{}, t, nxt);
+        cur = nxt;
+      }
+      tile(BoolC<false>{}, r1 - 1, cur);
+      r0 = r1;
+    }
+
+    // the open block, in bf16
+    for (int t = max(t_begin, t_open); t < t_end; ++t) {
+      const int page = prow[t >> tshift];
+      if (page < 0 || page >= num_pages) continue;   // wave-uniform
+      const int k0 = (t & tshift) * 64, nk = min(64, n - 64 * t);
+      const long tail = (static_cast<long>(bi) * Hkv + kvh) * ps * D;
+      const bf16* kb = kt_p + tail + k0 * D;
+      const bf16* vb = vt_p + tail + k0;
+      v4f sc[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+          sc[kt] = mfma_bf16(load_v8bf(kb + (16 * (c >> 2) + 4 * kt + (c & 3)) * D + 64 * (ks >> 1) +
+                                       16 * g + 8 * (ks & 1)),
+                             qf[ks], sc[kt]);
+      }
+      uint32_t keep[4];
+      finish(sc, key_bias + (static_cast<long>(page) * Hkv + kvh) * ps + k0, nk, 64 * t, keep);
+      softmax_block<4, DT>(sc, acc, m, l);
+      // two keys a word: byte masks to 16-bit masks (slots past nk hold what
+      // the buffer held, NaN perhaps)
+      uint32_t km[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        km[i] = __builtin_amdgcn_perm(0u, keep[i >> 1], (i & 1) ? 0x03030202u : 0x01010000u);
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const v8bf pb = pack_p(sc[2 * h], sc[2 * h + 1]);
+#pragma unroll
+        for (int tt = 0; tt < DT; ++tt) {
+          uint4 x = *reinterpret_cast<const uint4*>(vb + (16 * tt + c) * ps + 16 * g + 8 * h);
+          x = uint4{x.x & km[4 * h], x.y & km[4 * h + 1], x.z & km[4 * h + 2], x.w & km[4 * h + 3]};
+          acc[tt] = mfma_bf16(__builtin_bit_cast(v8bf, x), pb, acc[tt]);
+        }
+      }
+    }
+
+    // partial of this segment: O^T[d][q] unnormalised, with m (log2 domain) and l
+    const long seg = static_cast<long>(bi) * Hkv + kvh + w;
+    if (c < grp) {
+      float* po = part_o + (seg * grp + c) * D;
+#pragma unroll
+      for (int t = 0; t < DT; ++t)
+        *reinterpret_cast<float4*>(po + 16 * t + 4 * g) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+      if (g == 0) {
+        part_ml[(seg * grp + c) * 2] = m;
+        part_ml[(seg * grp + c) * 2 + 1] = l;
+      }
+    }
+    gt += t_end - t_begin;
+  }
+}
+
+int fp8_wave_count(int head_dim, bool bias) {
+  if (head_dim == 128)
+    return bias ? decode_waves(paged_decode_fp8_kernel<128, true>, 4)
+                : decode_waves(paged_decode_fp8_kernel<128, false>, 5);
+  return bias ? decode_waves(paged_decode_fp8_kernel<64, true>, 6)
+              : decode_waves(paged_decode_fp8_kernel<64, false>, 7);
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" int sa_paged_decode_fp8_fwd(
+    const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
+    const float* v_scale, const void* k_tail, const void* v_tail, const int32_t* page_table,
+    const int32_t* seq_lens, const float* key_bias, int batch, int num_q_heads, int num_kv_heads,
+    int head_dim, int page_size, int max_pages, int num_pages, float softmax_scale, void* o,
+    void* workspace, size_t workspace_bytes, void* stream) {
+  const char* who = "sa_paged_decode_fp8_fwd";
+  if (const int rc = sa::decode_check(sa::kBF16, q, k_pages, v_pages, page_table, seq_lens,
+                                      key_bias, batch, num_q_heads, num_kv_heads, head_dim,
+                                      page_size, max_pages, num_pages, o, who))
+    return rc;
+  SA_CHECK_ARG(k_scale && v_scale && k_tail && v_tail && workspace, "%s: null pointer", who);
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) |
+                 reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(k_tail) |
+                 reinterpret_cast<uintptr_t>(v_tail)) & 15) == 0,
+               "%s: q, the pages and the tails must be 16-byte aligned", who);
+  sa::DecodeWs ws;
+  const size_t need = sa::decode_ws_layout(batch, num_q_heads, num_kv_heads, head_dim,
+                                           sa::kDecodeMaxWaves, workspace, &ws);
+  SA_CHECK_ARG(workspace_bytes >= need, "%s: workspace %zu B < %zu B", who, workspace_bytes, need);
+  if (batch == 0) return 0;
+  const int W = sa::fp8_wave_count(head_dim, key_bias != nullptr);
+  const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(static_cast<float>(head_dim));
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  if (const int rc = sa::decode_plan_launch(seq_lens, batch, page_size, max_pages, ws, s)) return rc;
+  {
+    sa::ProfScope prof_("paged_decode_fp8", s);
+    auto launch = [&](auto kern) {
+      hipLaunchKernelGGL(kern, dim3(W), dim3(64), 0, s, static_cast<const sa::bf16*>(q),
+                         static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages),
+                         k_scale, v_scale, static_cast<const sa::bf16*>(k_tail),
+                         static_cast<const sa::bf16*>(v_tail), page_table, seq_lens, key_bias,
+                         ws.cum_row, ws.part_o, ws.part_ml, batch, num_q_heads, num_kv_heads,
+                         page_size, max_pages, num_pages, W, scale * sa::kLog2e);
+    };
+    if (head_dim == 128)
+      key_bias ? launch(sa::paged_decode_fp8_kernel<128, true>) : launch(sa::paged_decode_fp8_kernel<128, false>);
+    else
+      key_bias ? launch(sa::paged_decode_fp8_kernel<64, true>) : launch(sa::paged_decode_fp8_kernel<64, false>);
+    SA_CHECK_LAUNCH("paged_decode_fp8");
+  }
+  return sa::decode_merge_launch(batch, num_q_heads, num_kv_heads, head_dim, o, ws, W, s);
+}

@@ -37,6 +37,14 @@ def require_device(*tensors: torch.Tensor | None) -> torch.device:
     return dev
 
 
+def call_on(t: torch.Tensor, name: str, *args) -> None:
+    """_lib.call with t's device current (its stream belongs to that device)."""
+    if torch._C._cuda_getDevice() == t.device.index:
+        return _lib.call(name, *args)
+    with torch.cuda.device(t.device):
+        return _lib.call(name, *args)
+
+
 def limits(delta_limit) -> tuple[float, float]:
     lo, hi = float(delta_limit[0]), float(delta_limit[1])
     return lo, hi

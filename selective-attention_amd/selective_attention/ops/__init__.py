@@ -1,4 +1,5 @@
 from .attention import attn_varlen, paged_decode_attn, sparse_attn_varlen
+from .kv_fp8 import paged_decode_attn_fp8, paged_kv_append_fp8, paged_kv_build_fp8
 from .selective_mha import (PagedSelectiveAttnCache, ScoreStdFn, cross_attention_train,
                            gated_attention_train, selective_mha_prefill)
 from .ssd_scan import SSDScanFn
@@ -8,4 +9,5 @@ from .ssu import SSUFn
 __all__ = ["SSDScanFn", "SSUFn", "sparse_attn_varlen", "paged_decode_attn", "SSMConvFn",
            "SSMGateFn", "SSDScanGatedFn", "build_conv_ctx", "ssm_conv_step",
            "selective_mha_prefill", "PagedSelectiveAttnCache", "attn_varlen", "ScoreStdFn",
-           "gated_attention_train", "cross_attention_train"]
+           "gated_attention_train", "cross_attention_train", "paged_decode_attn_fp8",
+           "paged_kv_append_fp8", "paged_kv_build_fp8"]
