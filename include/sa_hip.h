@@ -337,6 +337,54 @@ int sa_gemv_bf16_multi(const void* x, const void* xscale, int M, int K, int nseg
                        void* stream);
 
 /*
+ * Linear layers with 4-bit weights for 1 to 64 rows (inference; the reference
+ * has none): y_i = x W_i^T + bias_i, i < nseg <= 4, all of the same x,
+ *   W[n, k] = scale[n, k / group] (code[n, k] - zero[n, k / group]),
+ * zero = 8 where zeros is NULL, group in {32, 64, 128}.  x (M, K) bf16 with row
+ * stride ldx (a multiple of 8 elements; columns K..ldx-1 hold zeros), 16-byte
+ * aligned; with xscale (laid out as x, or NULL) the input is bf16(x * xscale).
+ * packed: (ceil(N / 16), ceil(K / 128), 64, 16) bytes, lane 16 g + c of a tile
+ * being its row c, byte 4 j + i of it columns 32 j + 8 g + 2 i (low half) and
+ * + 1 (high half).  scales, zeros: (ceil(N / 16), ceil(K / 128) 128 / group,
+ * 16) bf16, finite in the padding.  bias (N) bf16 or NULL, y (M, N) bf16.
+ * zeros, bias: NULL, or arrays of nseg pointers (zero points for all or none).
+ */
+int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int K, int ldx, int group,
+                        int nseg, const void* const* packed, const void* const* scales,
+                        const void* const* zeros, const void* const* bias, const int* N,
+                        void* const* y, void* stream);
+
+/* The weights that such a packed matrix stands for, rounded to bf16: out (N, K). */
+int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zeros, int N, int K,
+                         int group, void* out, void* stream);
+
+/*
+ * Log probabilities of given tokens (no kernel in the reference, which takes
+ * softmax and argmax of its logits, models/causal_lm.py:143-221).  logits
+ * (rows, vocab) in `dtype` (f32 or bf16) with row stride ld (elements), targets
+ * (rows) int64; all outputs f32 unless said:
+ *   logprob (rows): log p of targets[r]; 0 at ignore_index, NaN for any other id
+ *   outside the vocabulary.  entropy (rows): -sum p log p.  stats (rows, 2): the
+ *   row's maximum and log sum e^(x - maximum), for the backward.  top_ids (rows,
+ *   top) int64 and top_logprobs (rows, top): the largest, ties to the lowest id;
+ *   top 0..64 and <= vocab, both may be NULL for 0.
+ * Backward: dlogits (rows, vocab) in `dtype`, row stride ldd, for the upstream
+ * gradients g_logprob (rows), g_entropy (rows), g_top (rows, top), each NULL for
+ * zero; entropy, stats, top_ids as the forward wrote them.
+ */
+int sa_token_logprobs_fwd(int dtype, const void* logits, long ld, const int64_t* targets,
+                          long rows, int vocab, int top, long ignore_index, float* logprob,
+                          float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
+                          void* stream);
+int sa_token_logprobs_bwd(int dtype, const void* logits, long ld, const int64_t* targets,
+                          long rows, int vocab, int top, long ignore_index, const float* entropy,
+                          const float* stats, const int64_t* top_ids, const float* g_logprob,
+                          const float* g_entropy, const float* g_top, void* dlogits, long ldd,
+                          void* stream);
+
+
+
+/*
  * SwiGLU's gated product (modules/feed_forward.py:10-11): out = bf16(a *
  * bf16(silu(c))), n bf16 elements (n % 8 == 0, 16-byte aligned).
  */

@@ -1,0 +1,285 @@
+// Linear layers with 4-bit weights and group scales, for few rows (gfx950).
+//
+//   y[m, n] = sum_k x[m, k] W[n, k] + bias[n],  W[n, k] = s[n, k / G] (c[n, k] - z[n, k / G])
+//
+// c in 0..15, G in {32, 64, 128}, z = 8 where no zero points are given.  At
+// decode sizes the layer is bound by the bytes of the weights, a quarter of
+// bf16's, so the widening must cost less than their loads: a code becomes the
+// bf16 number 1 + c / 16 by placing its four bits under the exponent of 1 (one
+// shift and one and-or for two codes), exactly, and the group's factors are
+// applied to sums in fp32:
+//
+//   sum_k x (c - z) = 16 (sum_k x (1 + c / 16) - (1 + z / 16) sum_k x)
+//
+// both sums on the matrix cores (16x16x32, the weights as the A operand, x as
+// B; sum_k x as the product with ones, once for all tiles of a wave).  The
+// difference costs at most three to four bits of fp32's 24, so a result is
+// off by about 2^-20 of sum |x w| before its one rounding to bf16.
+//
+// Packed weights: tiles of 16 rows and 128 columns, (N / 16, K / 128, 64, 16)
+// bytes, so that one 16-byte load a lane is a tile.  Lane 16 g + c holds row c;
+// its byte 4 j + i has, in its low and high half, columns 32 j + 8 g + 2 i and
+// + 1.  Scales and zero points: (N / 16, groups, 16) bf16, groups = (K / 128)
+// 128 / G.  N and K are padded to whole tiles; columns at or behind K meet
+// x = 0 and rows behind N are not stored.
+#include "common.h"
+#include "prof.h"
+
+#include <type_traits>
+
+namespace sa {
+namespace {
+
+constexpr int kInt4Segs = 4;
+struct Int4Segs {
+  const uint4* W[kInt4Segs];
+  const bf16* scale[kInt4Segs];
+  const bf16* zero[kInt4Segs];
+  const bf16* bias[kInt4Segs];
+  bf16* y[kInt4Segs];
+  int N[kInt4Segs];
+  int blk0[kInt4Segs + 1];
+  int nseg;
+};
+
+// codes of one k-step (8 of a lane, one word) as 1 + c / 16; the operand's
+// pairs are codes (q, q + 4), four bits apart by 16 in the word
+__device__ __forceinline__ v8bf widen_codes(uint32_t w) {
+  constexpr uint32_t kMask = 0x00780078u, kOne = 0x3f803f80u;
+  const uint4 r = {((w << 3) & kMask) | kOne, ((w >> 1) & kMask) | kOne, ((w >> 5) & kMask) | kOne,
+                   ((w >> 9) & kMask) | kOne};
+  return __builtin_bit_cast(v8bf, r);
+}
+// eight consecutive x in that order: (0, 4), (1, 5), (2, 6), (3, 7)
+__device__ __forceinline__ v8bf pair_x(const uint4& x) {
+  const uint4 r = {__builtin_amdgcn_perm(x.z, x.x, 0x05040100u), __builtin_amdgcn_perm(x.z, x.x, 0x07060302u),
+                   __builtin_amdgcn_perm(x.w, x.y, 0x05040100u), __builtin_amdgcn_perm(x.w, x.y, 0x07060302u)};
+  return __builtin_bit_cast(v8bf, r);
+}
+__device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
+  return pack_bf16x2(bf16lo_to_f32(a) * bf16lo_to_f32(b), bf16hi_to_f32(a) * bf16hi_to_f32(b));
+}
+
+// A workgroup of NW waves computes R tiles of 16 columns of y for up to 16 CT
+// rows of x; the waves take the 128-column blocks of K in turn and their sums
+// meet in LDS.
+template <int CT, int G, bool Z, int R, int NW>
+__global__ __launch_bounds__(64 * NW) void int4_linear_kernel(const bf16* __restrict__ x,
+                                                              const bf16* __restrict__ xscale,
+                                                              const Int4Segs sg, int M, int K,
+                                                              int ldx) {
+  constexpr int GN = 128 / G, GS = G / 32;   // groups of a block, k-steps of a group
+  __shared__ float part[NW][R][CT][256];
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = lane & 15, g = lane >> 4;
+  const int bid = blockIdx.x;
+  int seg = 0;
+#pragma unroll
+  for (int i = 1; i < kInt4Segs; ++i) seg += (i < sg.nseg && bid >= sg.blk0[i]) ? 1 : 0;
+  const int N = sg.N[seg], tiles = (N + 15) >> 4, kb_n = (K + 127) >> 7;
+  const int t0 = (bid - sg.blk0[seg]) * R;
+  const uint4* W = sg.W[seg];
+  const uint2* S = reinterpret_cast<const uint2*>(sg.scale[seg]);
+  const uint2* ZP = reinterpret_cast<const uint2*>(sg.zero[seg]);
+
+  v4f acc[R][CT];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < CT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
+  v8bf ones;
+  {
+    const uint4 o = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    ones = __builtin_bit_cast(v8bf, o);
+  }
+  auto tile_of = [&](int r) { return static_cast<long>(min(t0 + r, tiles - 1)); };   // (behind the last: not stored)
+
+  for (int kb = wid; kb < kb_n; kb += NW) {
+    uint4 w[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) w[r] = W[(tile_of(r) * kb_n + kb) * 64 + lane];
+    uint2 s[R][GN], z[R][GN];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+      for (int i = 0; i < GN; ++i) {
+        const long at = ((tile_of(r) * kb_n + kb) * GN + i) * 4 + g;
+        s[r][i] = S[at];
+        if constexpr (Z) z[r][i] = ZP[at];
+      }
+    v8bf xf[CT][4];
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int row = 16 * t + c, k = 128 * kb + 32 * j + 8 * g;
+        const bool ok = row < M && k < K;
+        uint4 v = ld16(x + static_cast<long>(row) * ldx + k, ok);
+        if (xscale) {
+          const uint4 f = ld16(xscale + static_cast<long>(row) * ldx + k, ok);
+          v = uint4{mul_pair(v.x, f.x), mul_pair(v.y, f.y), mul_pair(v.z, f.z), mul_pair(v.w, f.w)};
+        }
+        xf[t][j] = pair_x(v);
+      }
+#pragma unroll
+    for (int i = 0; i < GN; ++i) {
+#pragma unroll
+      for (int t = 0; t < CT; ++t) {
+        v4f xs = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < GS; ++j) xs = mfma_bf16(ones, xf[t][GS * i + j], xs);
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+          const uint32_t wj[4] = {w[r].x, w[r].y, w[r].z, w[r].w};
+          v4f d = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < GS; ++j) d = mfma_bf16(widen_codes(wj[GS * i + j]), xf[t][GS * i + j], d);
+          const float sv[4] = {bf16lo_to_f32(s[r][i].x), bf16hi_to_f32(s[r][i].x), bf16lo_to_f32(s[r][i].y),
+                               bf16hi_to_f32(s[r][i].y)};
+          float zv[4] = {8.f, 8.f, 8.f, 8.f};
+          if constexpr (Z) {
+            zv[0] = bf16lo_to_f32(z[r][i].x);
+            zv[1] = bf16hi_to_f32(z[r][i].x);
+            zv[2] = bf16lo_to_f32(z[r][i].y);
+            zv[3] = bf16hi_to_f32(z[r][i].y);
+          }
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[r][t][e] = fmaf(16.0f * sv[e], fmaf(-(1.0f + 0.0625f * zv[e]), xs[e], d[e]), acc[r][t][e]);
+        }
+      }
+    }
+  }
+  // lane (c, g) holds columns 4 g + e of the tile for row 16 t + c of x
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+      *reinterpret_cast<float4*>(&part[wid][r][t][c * 16 + 4 * g]) =
+          make_float4(acc[r][t][0], acc[r][t][1], acc[r][t][2], acc[r][t][3]);
+  __syncthreads();
+  const bf16* bias = sg.bias[seg];
+  bf16* y = sg.y[seg];
+  for (int e = tid; e < R * CT * 256; e += 64 * NW) {
+    const int row = (e >> 4) % (16 * CT), n = 16 * (t0 + e / (CT * 256)) + (e & 15);
+    const float* p = &part[0][0][0][0] + e;
+    float v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) v += p[i * R * CT * 256];
+    if (row < M && n < N) y[static_cast<long>(row) * N + n] = from_f32<bf16>(v + (bias ? to_f32(bias[n]) : 0.0f));
+  }
+}
+
+// the weights in bf16, (N, K) row-major: for many rows, where a plain matrix
+// product follows.  One workgroup a tile and 128 columns.
+__global__ __launch_bounds__(256) void int4_dequant_kernel(const uint32_t* __restrict__ W,
+                                                           const bf16* __restrict__ scale,
+                                                           const bf16* __restrict__ zero,
+                                                           bf16* __restrict__ out, int N, int K,
+                                                           int G) {
+  const int kb_n = (K + 127) >> 7, kb = blockIdx.x % kb_n, tile = blockIdx.x / kb_n;
+  const int gn = 128 / G;
+  const uint32_t* w = W + static_cast<long>(blockIdx.x) * 256;
+  // thread: row c, columns 8 u .. + 7 of the block
+  const int c = threadIdx.x >> 4, u = threadIdx.x & 15, j = u >> 2, g = u & 3;
+  const int n = 16 * tile + c, k = 128 * kb + 8 * u;
+  if (n >= N || k >= K) return;
+  const uint32_t v = w[(16 * g + c) * 4 + j];
+  const long at = ((static_cast<long>(tile) * kb_n + kb) * gn + 8 * u / G) * 16 + c;
+  const float s = to_f32(scale[at]), z = zero ? to_f32(zero[at]) : 8.0f;
+  bf16* o = out + static_cast<long>(n) * K + k;
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (k + i < K) o[i] = from_f32<bf16>(s * (static_cast<float>((v >> (4 * i)) & 15u) - z));
+}
+
+template <int CT, int G, bool Z, int R, int NW>
+void int4_go(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int ldx, hipStream_t s) {
+  sg.blk0[0] = 0;
+  for (int i = 0; i < kInt4Segs; ++i)
+    sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? ((sg.N[i] + 15) / 16 + R - 1) / R : 0);
+  hipLaunchKernelGGL((int4_linear_kernel<CT, G, Z, R, NW>), dim3(sg.blk0[sg.nseg]), dim3(64 * NW), 0,
+                     s, static_cast<const bf16*>(x), static_cast<const bf16*>(xscale), sg, M, K, ldx);
+}
+
+template <int G, bool Z>
+void int4_rows(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int ldx, hipStream_t s) {
+  if (M <= 16)
+    int4_go<1, G, Z, 1, 4>(x, xscale, sg, M, K, ldx, s);
+  else if (M <= 32)
+    int4_go<2, G, Z, 2, 4>(x, xscale, sg, M, K, ldx, s);
+  else
+    int4_go<4, G, Z, 2, 4>(x, xscale, sg, M, K, ldx, s);
+}
+
+bool int4_group_ok(int G) { return G == 32 || G == 64 || G == 128; }
+
+}  // namespace
+}  // namespace sa
+
+extern "C" int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int K, int ldx,
+                                   int group, int nseg, const void* const* packed,
+                                   const void* const* scales, const void* const* zeros,
+                                   const void* const* bias, const int* N, void* const* y,
+                                   void* stream) {
+  const char* who = "sa_int4_linear_bf16";
+  SA_CHECK_ARG(M >= 1 && M <= 64 && K > 0 && K <= (1 << 24), "%s: M %d must be 1..64 and K %d positive",
+               who, M, K);
+  SA_CHECK_ARG(ldx % 8 == 0 && ldx >= K, "%s: row stride %d must be a multiple of 8, at least K %d", who,
+               ldx, K);
+  SA_CHECK_ARG(sa::int4_group_ok(group), "%s: group %d not in {32, 64, 128}", who, group);
+  SA_CHECK_ARG(nseg >= 1 && nseg <= sa::kInt4Segs, "%s: %d weight matrices, 1..%d allowed", who, nseg,
+               sa::kInt4Segs);
+  SA_CHECK_ARG(x && packed && scales && N && y, "%s: null pointer", who);
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xscale)) & 15) == 0,
+               "%s: x and xscale must be 16-byte aligned", who);
+  sa::Int4Segs sg{};
+  sg.nseg = nseg;
+  const bool z = zeros && zeros[0];
+  long tiles = 0;
+  for (int i = 0; i < nseg; ++i) {
+    SA_CHECK_ARG(packed[i] && scales[i] && y[i] && N[i] > 0, "%s: weight matrix %d: null pointer or N %d",
+                 who, i, N[i]);
+    SA_CHECK_ARG((zeros && zeros[i]) == z, "%s: zero points for all weight matrices or for none", who);
+    SA_CHECK_ARG((reinterpret_cast<uintptr_t>(packed[i]) & 15) == 0 &&
+                     (reinterpret_cast<uintptr_t>(scales[i]) & 7) == 0 &&
+                     (!z || (reinterpret_cast<uintptr_t>(zeros[i]) & 7) == 0),
+                 "%s: weight matrix %d is not aligned", who, i);
+    tiles += (N[i] + 15L) / 16;
+    SA_CHECK_ARG(tiles < (1 << 27), "%s: too many columns", who);
+    sg.W[i] = static_cast<const uint4*>(packed[i]);
+    sg.scale[i] = static_cast<const sa::bf16*>(scales[i]);
+    sg.zero[i] = z ? static_cast<const sa::bf16*>(zeros[i]) : nullptr;
+    sg.bias[i] = bias ? static_cast<const sa::bf16*>(bias[i]) : nullptr;
+    sg.y[i] = static_cast<sa::bf16*>(y[i]);
+    sg.N[i] = N[i];
+  }
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  sa::ProfScope prof_("int4_linear", s);
+  auto go = [&](auto zc) {
+    constexpr bool Z = decltype(zc)::value;
+    if (group == 32) sa::int4_rows<32, Z>(x, xscale, sg, M, K, ldx, s);
+    else if (group == 64) sa::int4_rows<64, Z>(x, xscale, sg, M, K, ldx, s);
+    else sa::int4_rows<128, Z>(x, xscale, sg, M, K, ldx, s);
+  };
+  z ? go(std::integral_constant<bool, true>{}) : go(std::integral_constant<bool, false>{});
+  SA_CHECK_LAUNCH(who);
+  return 0;
+}
+
+extern "C" int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zeros, int N,
+                                    int K, int group, void* out, void* stream) {
+  const char* who = "sa_int4_dequant_bf16";
+  SA_CHECK_ARG(N > 0 && K > 0 && sa::int4_group_ok(group), "%s: bad sizes N=%d K=%d group=%d", who, N, K,
+               group);
+  SA_CHECK_ARG(packed && scales && out, "%s: null pointer", who);
+  SA_CHECK_ARG((reinterpret_cast<uintptr_t>(packed) & 3) == 0, "%s: packed weights are not aligned", who);
+  const long blocks = ((N + 15L) / 16) * ((K + 127L) / 128);
+  SA_CHECK_ARG(blocks < (1L << 31), "%s: weights too large", who);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  sa::ProfScope prof_("int4_dequant", s);
+  hipLaunchKernelGGL(sa::int4_dequant_kernel, dim3(blocks), dim3(256), 0, s,
+                     static_cast<const uint32_t*>(packed), static_cast<const sa::bf16*>(scales),
+                     static_cast<const sa::bf16*>(zeros), static_cast<sa::bf16*>(out), N, K, group);
+  SA_CHECK_LAUNCH("int4_dequant");
+  return 0;
+}

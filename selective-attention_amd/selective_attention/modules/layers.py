@@ -9,8 +9,10 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..kernels.int4 import MAX_MATRICES
 from ..kernels.lm_ops import (add_rms_norm, add_rms_norm_supported, gemv, gemv_multi,
                               gemv_supported, rms_norm, rope_qk, silu_mul)
+from ..ops.int4 import int4_linear, int4_linear_multi, quantize_int4
 
 
 def _gemv_ok(x: torch.Tensor, lin: nn.Linear) -> bool:
@@ -42,11 +44,88 @@ class Linear(nn.Linear):
         return list(torch.split(self(x), sizes, dim=-1))
 
 
+class Int4Linear(nn.Module):
+    """A linear layer whose weight is kept as 4-bit codes with a scale for each
+    group of input features (ops/int4.py), for inference: bfloat16 rows, no
+    weight gradient.  Buffers: packed, scales, zeros (None: symmetric), bias, in
+    bfloat16 whatever the module is cast to."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True,
+                 group_size: int = 128, symmetric: bool = True, device=None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        self.group_size, self.symmetric = group_size, symmetric
+        nt, kb = (out_features + 15) // 16, (in_features + 127) // 128
+        f = (nt, kb * 128 // group_size, 16)
+
+        def make(shape):
+            return torch.zeros(shape, dtype=torch.bfloat16, device=device)
+        self.register_buffer("packed", torch.zeros(nt, kb, 64, 16, dtype=torch.uint8, device=device))
+        self.register_buffer("scales", make(f))
+        self.register_buffer("zeros", None if symmetric else make(f))
+        self.register_buffer("bias", make(out_features) if bias else None)
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear, group_size: int = 128, symmetric: bool = True) -> "Int4Linear":
+        """lin's weight rounded to its nearest codes (quantize_int4)."""
+        q = cls(lin.in_features, lin.out_features, lin.bias is not None, group_size, symmetric,
+                lin.weight.device)
+        q.packed, q.scales, q.zeros = quantize_int4(lin.weight, group_size, symmetric)
+        if lin.bias is not None:
+            q.bias = lin.bias.detach().to(torch.bfloat16)
+        return q
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = {n: getattr(self, n) for n in ("scales", "zeros", "bias")}
+        super()._apply(fn, *args, **kwargs)
+        for n, t in kept.items():   # moved, not cast
+            new = getattr(self, n)
+            if t is not None and new.dtype != torch.bfloat16:
+                setattr(self, n, t.to(new.device))
+        return self
+
+    def weights(self):
+        return self.packed, self.scales, self.zeros
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return int4_linear(x, self.packed, self.scales, self.zeros, self.bias, self.out_features)
+
+    def split_forward(self, x: torch.Tensor, sizes) -> list:
+        """torch.split(self(x), sizes, dim=-1), each piece a contiguous tensor; one
+        launch of several matrices where the pieces are whole tiles."""
+        if len(sizes) <= MAX_MATRICES and min(sizes) > 0 and all(n % 16 == 0 for n in sizes[:-1]):
+            tiles = [(n + 15) // 16 for n in sizes]
+            cut = [[None] * len(sizes) if t is None else torch.split(t, tiles) for t in self.weights()]
+            bs = [None] * len(sizes) if self.bias is None else torch.split(self.bias, sizes)
+            return int4_linear_multi(x, list(zip(*cut)), bs, sizes)
+        return [p.contiguous() for p in torch.split(self(x), sizes, dim=-1)]
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, "
+                f"bias={self.bias is not None}, group_size={self.group_size}, symmetric={self.symmetric}")
+
+
+def quantize_linears(module: nn.Module, group_size: int = 128, symmetric: bool = True) -> nn.Module:
+    """Replace every linear layer inside `module` by its Int4Linear, in place."""
+    for name, child in module.named_children():
+        if isinstance(child, nn.Linear):
+            setattr(module, name, Int4Linear.from_linear(child, group_size, symmetric))
+        else:
+            quantize_linears(child, group_size, symmetric)
+    return module
+
+
 def project(x: torch.Tensor, linears, xscale: torch.Tensor | None = None) -> list:
     """[lin(x * xscale if xscale is given else x) for lin in linears]: one
     multi-GEMV launch on the decode shape (at most 4 layers), where the
-    product x * xscale is taken in bf16 as torch does."""
-    if len(linears) <= 4 and all(_gemv_ok(x, lin) for lin in linears):
+    product x * xscale is taken in bf16 as torch does; 4-bit layers of one kind
+    likewise."""
+    if all(isinstance(lin, Int4Linear) for lin in linears):
+        if len(linears) <= MAX_MATRICES and len({(lin.group_size, lin.symmetric) for lin in linears}) == 1:
+            return int4_linear_multi(x, [lin.weights() for lin in linears],
+                                     [lin.bias for lin in linears],
+                                     [lin.out_features for lin in linears], xscale)
+    elif len(linears) <= 4 and all(isinstance(lin, nn.Linear) and _gemv_ok(x, lin) for lin in linears):
         return gemv_multi(x, [lin.weight for lin in linears], [lin.bias for lin in linears], xscale)
     xs = x if xscale is None else x * xscale
     return [lin(xs) for lin in linears]

@@ -1,0 +1,71 @@
+"""Log probabilities of given tokens, the entropy of their distribution and its
+largest alternatives, with the logits' gradient: what a decode step answers
+with, what scoring a text needs, and (with a minus) a language model's loss.
+
+New op (the reference takes softmax and argmax of its logits,
+models/causal_lm.py:143-221, and leaves the loss to its caller).
+"""
+from __future__ import annotations
+
+from typing import NamedTuple
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..kernels import logprobs as _k
+from ..utils import check_shape
+
+
+class TokenLogprobs(NamedTuple):
+    logprob: torch.Tensor       # (...) float32: log p of the given tokens
+    entropy: torch.Tensor       # (...) float32: -sum p log p
+    top_ids: torch.Tensor       # (..., top) int64, most probable first
+    top_logprobs: torch.Tensor  # (..., top) float32
+
+
+class TokenLogprobsFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, targets, top, ignore_index):
+        lp, H, stats, ids, tl = _k.token_logprobs_forward(logits, targets, top, ignore_index)
+        ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(logits, targets, H, stats, ids)
+        ctx.top, ctx.ignore_index = top, ignore_index
+        return lp, H, ids, tl
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g_lp, g_h, _, g_top):
+        logits, targets, H, stats, ids = ctx.saved_tensors
+        if g_lp is None and g_h is None and g_top is None:
+            return None, None, None, None
+        dx = _k.token_logprobs_backward(logits, targets, ctx.top, ctx.ignore_index, H, stats, ids,
+                                        g_lp, g_h, g_top)
+        return dx, None, None, None
+
+
+def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
+                   ignore_index: int = -100) -> TokenLogprobs:
+    """
+    Args:
+        logits: (..., vocab) float32 or bfloat16; -inf rules a token out
+        targets: (...) int32 or int64 token ids.  ignore_index: logprob 0 and no
+            gradient from it; any other id outside the vocabulary: NaN
+        top: alternatives a row, 0..64 and at most vocab; equal logits in the
+            order of their ids
+    Returns:
+        TokenLogprobs, in float32; a row of -inf alone, or with NaN or +inf, gives
+        NaN.  Differentiable once in logits (logprob, entropy and top_logprobs);
+        the gradient has the logits' dtype.
+    """
+    if logits.dim() < 1 or logits.shape[-1] == 0:
+        raise ValueError(f"token_logprobs: logits need a vocabulary, got {tuple(logits.shape)}")
+    if logits.dtype not in (torch.float32, torch.bfloat16):
+        raise TypeError(f"token_logprobs: logits must be float32 or bfloat16, got {logits.dtype}")
+    if targets.dtype not in (torch.int32, torch.int64):
+        raise TypeError(f"token_logprobs: targets must be int32 or int64, got {targets.dtype}")
+    check_shape(targets, tuple(logits.shape[:-1]), name="targets")
+    if not 0 <= top <= min(_k.MAX_TOP, logits.shape[-1]):
+        raise ValueError(f"token_logprobs: top {top} must be 0..{_k.MAX_TOP} and at most the "
+                         f"vocabulary {logits.shape[-1]}")
+    return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets, int(top), int(ignore_index)))
