@@ -1,8 +1,8 @@
 """Inference state of the causal LM: the same containers as the reference's
 `selective_attention.inference` (ssm_cache.py:3-43, selective_attn_cache.py:3-42,
 causal_block_cache.py, infer_state.py:4-14, generation_config.py:5-14), with
-SelectiveMHA's KV cache kept in pages (PagedSelectiveAttnCache) instead of
-dense per-head compacted tensors.
+SelectiveMHA's KV cache kept in pages (PagedSelectiveAttnCache, in 8 bits
+PagedSelectiveAttnCacheFP8) instead of dense per-head compacted tensors.
 """
 from __future__ import annotations
 
@@ -11,7 +11,7 @@ from typing import List
 
 import torch
 
-from ..ops.selective_mha import PagedSelectiveAttnCache
+from ..ops.selective_mha import PagedSelectiveAttnCache, PagedSelectiveAttnCacheFP8
 from ..ops.ssm_io import build_conv_ctx as _build_conv_ctx
 
 
@@ -36,6 +36,9 @@ class SSMCache:
         self.conv_ctx[:, :, -1] = x
 
 
+KV_DTYPES = {"bf16": PagedSelectiveAttnCache, "fp8": PagedSelectiveAttnCacheFP8}
+
+
 class SelectiveAttnCache:
     """inference/selective_attn_cache.py:3-42 on pages.
 
@@ -44,17 +47,21 @@ class SelectiveAttnCache:
     and compact() (the reference's _reset_cache, modules/selective_attention.py:
     11-25) frees pages whose keys every head has dropped.  `reserve` is the
     number of decode tokens the pages are sized for beyond the prefill; the
-    pool doubles when it runs out.
+    pool doubles when it runs out.  `kv_dtype`: "bf16", or "fp8" for pages in 8
+    bits with a scale for each page and head (half the bytes a step reads).
     """
 
-    def __init__(self, reserve: int = 256, page_size: int = 64):
+    def __init__(self, reserve: int = 256, page_size: int = 64, kv_dtype: str = "bf16"):
+        if kv_dtype not in KV_DTYPES:
+            raise ValueError(f"kv_dtype {kv_dtype!r} must be one of {sorted(KV_DTYPES)}")
         self.reserve = reserve
         self.page_size = page_size
+        self.kv_dtype = kv_dtype
         self.pages: PagedSelectiveAttnCache | None = None
 
     def _make(self, b, H, D, tokens, device):
-        self.pages = PagedSelectiveAttnCache(b, H, D, tokens + self.reserve + 1, device,
-                                             page_size=self.page_size, grow=True)
+        self.pages = KV_DTYPES[self.kv_dtype](b, H, D, tokens + self.reserve + 1, device,
+                                              page_size=self.page_size, grow=True)
 
     def build_kv(self, k_rot, v, log_gate, lengths=None):
         """k_rot, v (batch, heads, seq_len, head_dim); log_gate (batch, heads, seq_len)."""
@@ -113,18 +120,18 @@ class CrossSelectiveAttnCache:
 class CrossBlockCache:
     """inference/cross_block_cache.py: SSM, self-attention and cross-attention caches."""
 
-    def __init__(self, reserve: int = 256):
+    def __init__(self, reserve: int = 256, kv_dtype: str = "bf16"):
         self.ssm_cache = SSMCache()
-        self.attn_cache = SelectiveAttnCache(reserve)
+        self.attn_cache = SelectiveAttnCache(reserve, kv_dtype=kv_dtype)
         self.cross_attn_cache = CrossSelectiveAttnCache()
 
 
 class CausalBlockCache:
     """inference/causal_block_cache.py: one SSM cache and one attention cache per block."""
 
-    def __init__(self, reserve: int = 256):
+    def __init__(self, reserve: int = 256, kv_dtype: str = "bf16"):
         self.ssm_cache = SSMCache()
-        self.attn_cache = SelectiveAttnCache(reserve)
+        self.attn_cache = SelectiveAttnCache(reserve, kv_dtype=kv_dtype)
 
 
 class InferenceState:
@@ -150,6 +157,7 @@ class GenerationConfig:
     cross_attn_gate_thresholds: torch.Tensor | List | None = None
     enc_attn_gate_thresholds: torch.Tensor | List | None = None
     cache_update_interval: int = 100
+    kv_cache_dtype: str = "bf16"    # or "fp8": self-attention caches in 8 bits
 
 
 __all__ = ["SSMCache", "SelectiveAttnCache", "CrossSelectiveAttnCache", "CausalBlockCache",

@@ -19,8 +19,9 @@ import torch
 import torch.nn as nn
 
 from ..inference import CausalBlockCache, GenerationConfig, InferenceState
-from ..modules.layers import Linear
+from ..modules.layers import Int4Linear, Linear, quantize_linears
 from ..modules import CausalBlock, RMSNorm
+from ..ops.logprobs import TokenLogprobs, token_logprobs
 from ._graph import graph_decode
 
 
@@ -77,6 +78,13 @@ class CausalLM(nn.Module):
         self.norm.weight.data = self.norm.weight.data.float()
         return self
 
+    def quantize_int4(self, group_size: int = 128, symmetric: bool = True) -> "CausalLM":
+        """Every linear layer and the head to 4-bit weights (Int4Linear), in place,
+        for inference in bfloat16; the embedding keeps its own table."""
+        quantize_linears(self.layers, group_size, symmetric)
+        self.lm_head = Int4Linear.from_linear(self.lm_head, group_size, symmetric)
+        return self
+
     def _hidden(self, input_ids, lengths=None, attn_gate_thresholds=None, cache=None):
         h = self.embedding(input_ids)
         for i, layer in enumerate(self.layers):
@@ -91,6 +99,24 @@ class CausalLM(nn.Module):
         """input_ids (batch_size, seq_len) -> logits (batch_size, seq_len, vocab_size)."""
         return self.lm_head(self.norm(self._hidden(input_ids, lengths, attn_gate_thresholds, cache)))
 
+    def score(self, input_ids: torch.Tensor, lengths: torch.Tensor | None = None,
+              attn_gate_thresholds: torch.Tensor | List | None = None, top: int = 0) -> TokenLogprobs:
+        """Log probability of each token after the first given those before it, with
+        the entropy and `top` alternatives at its place: TokenLogprobs of
+        (batch_size, seq_len - 1[, top]).  Tokens at or past a length have logprob
+        0 and pass no gradient; in training, minus the sum over the others'
+        number is the language model's loss."""
+        b, L = input_ids.shape
+        logits = self.forward(input_ids, lengths, attn_gate_thresholds)
+        # targets one place to the left, the last place without one: the logits'
+        # rows are read where they are
+        targets = torch.full_like(input_ids, -100, dtype=torch.int64)
+        targets[:, :-1] = input_ids[:, 1:]
+        if lengths is not None:
+            past = torch.arange(1, L + 1, device=targets.device)[None, :] >= lengths.to(targets.device)[:, None]
+            targets.masked_fill_(past, -100)
+        return TokenLogprobs(*(t[:, :-1] for t in token_logprobs(logits, targets, top)))
+
     def step(self, input_ids: torch.Tensor, cache: list, state: InferenceState,
              gen_cfg: GenerationConfig, analysis_cfg=None, stats=None):
         """input_ids (batch_size,) -> logits (batch_size, vocab_size).  Each
@@ -104,10 +130,12 @@ class CausalLM(nn.Module):
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, gen_cfg: GenerationConfig, analysis_cfg=None,
-                 use_graph: bool = True, check_every: int = 16):
+                 use_graph: bool = True, check_every: int = 16, logprobs: int | None = None):
         """Greedy decoding (models/causal_lm.py:143-221): prefill, then up to
         max_new_tokens steps; tokens after the first eos become eos.
-        Returns seq_ids (batch_size, seq_len + max_new_tokens).
+        Returns seq_ids (batch_size, seq_len + max_new_tokens); with `logprobs`, a
+        number of alternatives, also the new tokens' TokenLogprobs
+        (batch_size, max_new_tokens[, logprobs]), zeros behind a row's first eos.
 
         With use_graph, one decode step (the six blocks, the head, the argmax
         and the length update) is captured once in a HIP graph and replayed
@@ -120,7 +148,7 @@ class CausalLM(nn.Module):
         b, L = input_ids.shape
         dev = input_ids.device
         new = gen_cfg.max_new_tokens
-        cache = [CausalBlockCache(reserve=new) for _ in self.layers]
+        cache = [CausalBlockCache(reserve=new, kv_dtype=gen_cfg.kv_cache_dtype) for _ in self.layers]
         lengths = (input_ids != gen_cfg.pad_token_id).sum(dim=1)
         state = InferenceState(lengths.clone())
         h = self._hidden(input_ids, lengths, gen_cfg.attn_gate_thresholds, cache)
@@ -128,24 +156,31 @@ class CausalLM(nn.Module):
         logits = self.lm_head(self.norm(h[torch.arange(b, device=dev), lengths - 1]))
         seq_ids = torch.full((b, L + new), gen_cfg.pad_token_id, dtype=input_ids.dtype, device=dev)
         seq_ids[:, :L] = input_ids
-        if new <= 0:
-            return seq_ids
-        if use_graph and dev.type == "cuda":
-            self._generate_graph(logits, cache, state, gen_cfg, seq_ids, L, check_every)
-        else:
-            finished = torch.zeros(b, dtype=torch.bool, device=dev)
-            for _ in range(new):
-                nxt = torch.argmax(torch.softmax(logits, dim=-1), dim=-1)
-                seq_ids[:, L + state.step] = nxt
-                finished |= nxt == gen_cfg.eos_token_id
-                if bool(finished.all()):
-                    break
-                logits = self.step(nxt, cache, state, gen_cfg)
-                state.update()
+        lps = None if logprobs is None else _LogprobLog(b, max(new, 0), logprobs, dev)
+        if new > 0:
+            if use_graph and dev.type == "cuda":
+                self._generate_graph(logits, cache, state, gen_cfg, seq_ids, L, check_every, lps)
+            else:
+                finished = torch.zeros(b, dtype=torch.bool, device=dev)
+                for _ in range(new):
+                    nxt = torch.argmax(torch.softmax(logits, dim=-1), dim=-1)
+                    seq_ids[:, L + state.step] = nxt
+                    if lps is not None:
+                        lps.take(logits, nxt)
+                        lps.keep(state.step)
+                    finished |= nxt == gen_cfg.eos_token_id
+                    if bool(finished.all()):
+                        break
+                    logits = self.step(nxt, cache, state, gen_cfg)
+                    state.update()
         first_eos = (seq_ids == gen_cfg.eos_token_id).float().cumsum(dim=1) >= 1
-        return torch.where(first_eos, gen_cfg.eos_token_id, seq_ids)
+        if lps is not None:   # places whose token before is an eos already
+            lps = lps.result(first_eos[:, L - 1:-1] if new > 0 else None)
+        if new > 0:
+            seq_ids = torch.where(first_eos, gen_cfg.eos_token_id, seq_ids)
+        return seq_ids if lps is None else (seq_ids, lps)
 
-    def _generate_graph(self, logits, cache, state, gen_cfg, seq_ids, L, check_every):
+    def _generate_graph(self, logits, cache, state, gen_cfg, seq_ids, L, check_every, lps=None):
         new = gen_cfg.max_new_tokens
         H, D = self.cfg.model_dim // self.cfg.head_dim, self.cfg.head_dim
         like = torch.empty(logits.shape[0], H, D, device=logits.device)
@@ -154,15 +189,22 @@ class CausalLM(nn.Module):
         try:
             tok = torch.argmax(torch.softmax(logits, dim=-1), dim=-1)
             seq_ids[:, L] = tok
+            if lps is not None:
+                lps.take(logits, tok)
+                lps.keep(0)
             state.step = 0
 
             def body():
                 lg = self.step(tok, cache, state, gen_cfg)
                 tok.copy_(torch.argmax(torch.softmax(lg, dim=-1), dim=-1))
+                if lps is not None:
+                    lps.take(lg, tok)
                 state.lengths.add_(1)
 
             def on_token(i):
                 seq_ids[:, L + i] = tok
+                if lps is not None:
+                    lps.keep(i)
                 state.step = i
 
             eos = gen_cfg.eos_token_id
@@ -171,3 +213,31 @@ class CausalLM(nn.Module):
         finally:
             for c in cache:
                 c.attn_cache.pages.exit_device_mode()
+
+
+class _LogprobLog:
+    """The new tokens' log probabilities during generate: take() fills one step's
+    buffers (inside the captured step), keep(i) files them under token i."""
+
+    def __init__(self, b: int, new: int, top: int, device):
+        self.top = top
+        f = dict(dtype=torch.float32, device=device)
+        self.now = TokenLogprobs(torch.zeros(b, **f), torch.zeros(b, **f),
+                                 torch.zeros(b, top, dtype=torch.int64, device=device),
+                                 torch.zeros(b, top, **f))
+        self.all = TokenLogprobs(*(t.new_zeros(b, new, *t.shape[1:]) for t in self.now))
+
+    def take(self, logits, tokens):
+        for dst, src in zip(self.now, token_logprobs(logits, tokens, self.top)):
+            dst.copy_(src)
+
+    def keep(self, i: int):
+        for dst, src in zip(self.all, self.now):
+            dst[:, i] = src
+
+    def result(self, behind) -> TokenLogprobs:
+        """behind (b, new): places behind a row's first eos, or None for no token."""
+        if behind is None:
+            return self.all
+        return TokenLogprobs(*(t.masked_fill(behind if t.dim() == 2 else behind[..., None], 0)
+                               for t in self.all))

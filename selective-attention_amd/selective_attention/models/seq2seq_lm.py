@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from ..inference import CrossBlockCache, GenerationConfig, InferenceState
-from ..modules.layers import Linear
+from ..modules.layers import Linear, quantize_linears
 from ..modules import SSM, BiBlock, CrossBlock, RMSNorm
 from ._graph import graph_decode
 
@@ -78,6 +78,12 @@ class Seq2SeqLM(nn.Module):
                 m.score_std_ema.data = m.score_std_ema.data.float()
         return self
 
+    def quantize_int4(self, group_size: int = 128, symmetric: bool = True) -> "Seq2SeqLM":
+        """Every linear layer and the head to 4-bit weights (Int4Linear), in place,
+        for inference in bfloat16; the embedding keeps its own table."""
+        quantize_linears(self, group_size, symmetric)
+        return self
+
     def encode(self, input_ids, lengths, enc_attn_gate_thresholds=None):
         """Encoder output (batch, enc_len, model_dim) and the decoders' initial
         SSM state (batch, heads, head_dim, state_dim) float32 (:151-169)."""
@@ -129,7 +135,7 @@ class Seq2SeqLM(nn.Module):
         b = input_ids.shape[0]
         dev = input_ids.device
         new = gen_cfg.max_new_tokens
-        cache = [CrossBlockCache(reserve=new) for _ in self.decoder_layers]
+        cache = [CrossBlockCache(reserve=new, kv_dtype=gen_cfg.kv_cache_dtype) for _ in self.decoder_layers]
         state = InferenceState(torch.ones(b, dtype=torch.long, device=dev))
         lengths = (input_ids != gen_cfg.pad_token_id).sum(dim=1)
         seq_ids = torch.full((b, new), gen_cfg.pad_token_id, dtype=input_ids.dtype, device=dev)

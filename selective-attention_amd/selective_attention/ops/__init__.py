@@ -2,7 +2,7 @@ from .attention import attn_varlen, paged_decode_attn, sparse_attn_varlen
 from .int4 import dequantize_int4, int4_linear, int4_linear_multi, pack_int4, quantize_int4
 from .kv_fp8 import paged_decode_attn_fp8, paged_kv_append_fp8, paged_kv_build_fp8
 from .logprobs import TokenLogprobs, TokenLogprobsFn, token_logprobs
-from .selective_mha import (PagedSelectiveAttnCache, ScoreStdFn, cross_attention_train,
+from .selective_mha import (PagedSelectiveAttnCache, PagedSelectiveAttnCacheFP8, ScoreStdFn, cross_attention_train,
                            gated_attention_train, selective_mha_prefill)
 from .ssd_scan import SSDScanFn
 from .ssm_io import SSDScanGatedFn, SSMConvFn, SSMGateFn, build_conv_ctx, ssm_conv_step
@@ -14,4 +14,4 @@ __all__ = ["SSDScanFn", "SSUFn", "sparse_attn_varlen", "paged_decode_attn", "SSM
            "gated_attention_train", "cross_attention_train", "paged_decode_attn_fp8",
            "paged_kv_append_fp8", "paged_kv_build_fp8", "int4_linear", "int4_linear_multi",
            "pack_int4", "quantize_int4", "dequantize_int4", "token_logprobs", "TokenLogprobs",
-           "TokenLogprobsFn"]
+           "TokenLogprobsFn", "PagedSelectiveAttnCacheFP8"]

@@ -18,6 +18,7 @@ ops:
   key_bias pages (-inf for dropped keys; the newest key is exempt, as in
   mode "pos").  Compaction becomes a page-table rewrite: drop_evicted_pages
   removes pages whose keys every head has dropped, without moving data.
+* PagedSelectiveAttnCacheFP8: the same cache held in 8 bits.
 
 * ScoreStdFn: the per-head std of the valid scores that SelectiveMHA's
   training forward scales the log-gate by (:234-247), from the count, sum and
@@ -35,8 +36,11 @@ import torch
 from ..kernels.attention import (TRAIN_HEAD_DIMS, gated_attn_train_backward,
                                  gated_attn_train_forward, mha_prefill, score_moments,
                                  score_std_backward)
+from ..kernels import kv_fp8 as _kv8
+from ..kernels.common import require_device
 from ..kernels.lm_ops import paged_kv_append, paged_kv_build
-from ..utils import check_shape
+from ..utils import check_ndim, check_shape
+from . import kv_fp8 as _kv8_ops
 from .attention import paged_decode_attn
 
 
@@ -245,10 +249,7 @@ class PagedSelectiveAttnCache:
         self.grow = grow
         self.max_pages = max(1, (max_tokens + page_size - 1) // page_size)
         n = batch_size * self.max_pages
-        self.k_pages = torch.zeros(n, num_heads, page_size, head_dim, dtype=torch.bfloat16, device=device)
-        self.v_pages = torch.zeros(n, num_heads, head_dim, page_size, dtype=torch.bfloat16, device=device)
-        self.gate_pages = torch.full((n, num_heads, page_size), float("-inf"), dtype=torch.float32,
-                                     device=device)
+        self._make_pools(n, device)
         self.free = list(range(n - 1, -1, -1))
         self.rows = [[] for _ in range(batch_size)]   # page ids per batch row
         self.lens = [0] * batch_size
@@ -261,20 +262,38 @@ class PagedSelectiveAttnCache:
         # device mode (see enter_device_mode): lengths live on the device
         self.lens_dev = None
 
-    # --- bookkeeping -------------------------------------------------------
-    def _grow(self):
-        """Double the page pool (rows keep their page ids; the page table gets
-        twice the columns)."""
-        n = self.k_pages.shape[0]
-        dev = self.device
+    # --- storage -------------------------------------------------------------
+    def _make_pools(self, n: int, device):
+        H, D, ps = self.H, self.D, self.ps
+        self.k_pages = torch.zeros(n, H, ps, D, dtype=torch.bfloat16, device=device)
+        self.v_pages = torch.zeros(n, H, D, ps, dtype=torch.bfloat16, device=device)
+        self.gate_pages = torch.full((n, H, ps), float("-inf"), dtype=torch.float32, device=device)
 
+    def _grow_pools(self, n: int):
+        """n pages more, behind those that are there."""
         def bigger(t, fill):
-            out = torch.full((2 * n,) + tuple(t.shape[1:]), fill, dtype=t.dtype, device=dev)
-            out[:n] = t
+            out = torch.full((t.shape[0] + n,) + tuple(t.shape[1:]), fill, dtype=t.dtype,
+                             device=self.device)
+            out[:t.shape[0]] = t
             return out
         self.k_pages = bigger(self.k_pages, 0)
         self.v_pages = bigger(self.v_pages, 0)
         self.gate_pages = bigger(self.gate_pages, float("-inf"))
+
+    def _build_pages(self, k_rot, v, log_gate):
+        paged_kv_build(k_rot, v, log_gate, self.page_table(), self.seq_lens(), self.k_pages,
+                       self.v_pages, self.gate_pages)
+
+    def _append_pages(self, k_rot, v, log_gate, table, lens):
+        paged_kv_append(k_rot, v, log_gate, table, lens, self.k_pages, self.v_pages,
+                        self.gate_pages)
+
+    # --- bookkeeping -------------------------------------------------------
+    def _grow(self):
+        """Double the page pool (rows keep their page ids; the page table gets
+        twice the columns)."""
+        n = self.gate_pages.shape[0]
+        self._grow_pools(n)
         self.free = list(range(2 * n - 1, n - 1, -1)) + self.free
         self.max_pages *= 2
         self._pt_dirty = True
@@ -339,8 +358,7 @@ class PagedSelectiveAttnCache:
                 self.rows[i] = [self._alloc(fill=False) for _ in range((lens[i] + ps - 1) // ps)]
                 self.lens[i] = lens[i]
             self._pt_dirty = self._sl_dirty = True
-            paged_kv_build(k_rot, v, log_gate, self.page_table(), self.seq_lens(), self.k_pages,
-                           self.v_pages, self.gate_pages)
+            self._build_pages(k_rot, v, log_gate)
             return
         for i in range(self.b):
             for pid in self.rows[i]:
@@ -395,8 +413,7 @@ class PagedSelectiveAttnCache:
         self._sl_dirty = True
 
     def _append_device(self, k_rot, v, log_gate):
-        paged_kv_append(k_rot, v, log_gate, self._pt, self.lens_dev, self.k_pages, self.v_pages,
-                        self.gate_pages)
+        self._append_pages(k_rot, v, log_gate, self._pt, self.lens_dev)
 
     def append(self, k_rot, v, log_gate):
         """SelectiveAttnCache.update_kv (:30-47): one token per batch row;
@@ -410,8 +427,7 @@ class PagedSelectiveAttnCache:
             # of the slots, three indexed stores and a copy of the lengths are
             # 70 us of host time
             lens = torch.tensor(self.lens, dtype=torch.int32).to(self.device)
-            paged_kv_append(k_rot, v, log_gate, self.page_table(), lens, self.k_pages,
-                            self.v_pages, self.gate_pages)
+            self._append_pages(k_rot, v, log_gate, self.page_table(), lens)
             self.lens[:] = [n + 1 for n in self.lens]   # (in place, as everywhere)
             self._sl, self._sl_dirty = lens, False
             return
@@ -473,6 +489,129 @@ class PagedSelectiveAttnCache:
             self.rows[i] = keep
         if freed:
             self._pt_dirty = self._sl_dirty = True
+        return freed
+
+
+class PagedSelectiveAttnCacheFP8(PagedSelectiveAttnCache):
+    """The paged decode cache held in 8 bits (ops/kv_fp8.py), on the GPU.
+
+    k / v pages: float8_e4m3fn codes of the full blocks in the parent's layouts
+    with k_scale / v_scale (num_pages, num_heads), powers of two; k_tail / v_tail
+    (batch, num_heads, ...) bfloat16 hold each row's open block until it is
+    full.  Page table, lengths, gates and device mode are the parent's; head_dim
+    and page_size 64 or 128.
+
+    unappend takes back the newest token of a block that still stands in the
+    tail: a token before it, whose block has been rounded and overwritten by the
+    next one's tokens, is refused.  In device mode that is one unappend for each
+    append.
+    """
+
+    def __init__(self, batch_size: int, num_heads: int, head_dim: int, max_tokens: int, device,
+                 page_size: int = 64, grow: bool = False):
+        if head_dim not in _kv8.HEAD_DIMS or page_size not in _kv8.PAGE_SIZES:
+            raise ValueError(f"PagedSelectiveAttnCacheFP8: head_dim {head_dim} must be one of "
+                             f"{_kv8.HEAD_DIMS} and page_size {page_size} one of {_kv8.PAGE_SIZES}")
+        super().__init__(batch_size, num_heads, head_dim, max_tokens, device, page_size, grow)
+        # block whose tokens the row's tail holds (-1: none that can be told)
+        self._tail_block = [-1] * batch_size
+        self._dev_newest = False     # device mode: an append that unappend may take back
+
+    # --- storage -------------------------------------------------------------
+    def _make_pools(self, n: int, device):
+        H, D, ps, b = self.H, self.D, self.ps, self.b
+        self.k_pages = torch.zeros(n, H, ps, D, dtype=torch.uint8, device=device).view(_kv8.FP8)
+        self.v_pages = torch.zeros(n, H, D, ps, dtype=torch.uint8, device=device).view(_kv8.FP8)
+        self.k_scale = torch.ones(n, H, dtype=torch.float32, device=device)
+        self.v_scale = torch.ones(n, H, dtype=torch.float32, device=device)
+        self.gate_pages = torch.full((n, H, ps), float("-inf"), dtype=torch.float32, device=device)
+        self.k_tail = torch.zeros(b, H, ps, D, dtype=torch.bfloat16, device=device)
+        self.v_tail = torch.zeros(b, H, D, ps, dtype=torch.bfloat16, device=device)
+
+    def _grow_pools(self, n: int):
+        def bigger(t, fill):
+            raw = t.view(torch.uint8) if t.dtype == _kv8.FP8 else t
+            out = torch.full((raw.shape[0] + n,) + tuple(raw.shape[1:]), fill, dtype=raw.dtype,
+                             device=self.device)
+            out[:raw.shape[0]] = raw
+            return out.view(t.dtype)
+        self.k_pages, self.v_pages = bigger(self.k_pages, 0), bigger(self.v_pages, 0)
+        self.k_scale, self.v_scale = bigger(self.k_scale, 1.0), bigger(self.v_scale, 1.0)
+        self.gate_pages = bigger(self.gate_pages, float("-inf"))
+
+    def _cache(self):
+        return (self.k_pages, self.v_pages, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
+
+    def _build_pages(self, k_rot, v, log_gate):
+        _kv8_ops.paged_kv_build_fp8(k_rot, v, log_gate, self.page_table(), self.seq_lens(),
+                                    *self._cache(), self.gate_pages)
+
+    def _append_pages(self, k_rot, v, log_gate, table, lens):
+        _kv8_ops.paged_kv_append_fp8(k_rot, v, log_gate, table, lens, *self._cache(),
+                                     self.gate_pages)
+
+    # --- the reference's cache operations --------------------------------------
+    def build(self, k_rot, v, log_gate, lengths=None):
+        b, H, D = self.b, self.H, self.D
+        check_ndim(k_rot, 4, name="k_rot")
+        L = k_rot.shape[2]
+        check_shape(k_rot, (b, H, L, D), name="k_rot")
+        check_shape(v, (b, H, L, D), name="v")
+        check_shape(log_gate, (b, H, L), name="log_gate")
+        require_device(k_rot, v, log_gate)
+        super().build(k_rot, v, log_gate, lengths)
+        self._note_tails()
+
+    def _note_tails(self):
+        """The tails hold the open blocks; behind a full one nothing can be told."""
+        self._tail_block = [n // self.ps if n % self.ps else -1 for n in self.lens]
+
+    def append(self, k_rot, v, log_gate):
+        shape = (self.b, self.H, self.D)
+        check_shape(k_rot, shape, name="k_rot")
+        check_shape(v, shape, name="v")
+        check_shape(log_gate, shape[:2], name="log_gate")
+        require_device(k_rot, v, log_gate)
+        super().append(k_rot, v, log_gate)
+        if self.lens_dev is None:
+            self._tail_block = [(n - 1) // self.ps for n in self.lens]
+        else:
+            self._dev_newest = True
+
+    def unappend(self, rows=None):
+        if self.lens_dev is not None:
+            if not self._dev_newest:
+                raise RuntimeError("PagedSelectiveAttnCacheFP8: one unappend for each append in "
+                                   "device mode")
+            self._dev_newest = False
+            return super().unappend(rows)
+        rows = list(range(self.b) if rows is None else rows)
+        for i in rows:
+            n = self.lens[i] - rows.count(i)
+            if n < 0 or (n % self.ps and n // self.ps != self._tail_block[i]):
+                raise RuntimeError(f"PagedSelectiveAttnCacheFP8: row {i} has no token to take back "
+                                   "that is still in its open block")
+        super().unappend(rows)
+
+    def enter_device_mode(self, extra_tokens: int):
+        super().enter_device_mode(extra_tokens)
+        self._dev_newest = False
+
+    def exit_device_mode(self):
+        super().exit_device_mode()
+        self._note_tails()
+
+    def attend(self, q_rot) -> torch.Tensor:
+        return _kv8_ops.paged_decode_attn_fp8(q_rot.to(torch.bfloat16), *self._cache(),
+                                              self.page_table(), self.seq_lens(),
+                                              key_bias=self.gate_pages)
+
+    def drop_evicted_pages(self) -> int:
+        before = list(self.lens)
+        freed = super().drop_evicted_pages()
+        for i, n in enumerate(self.lens):   # the blocks before the open one move up
+            if self._tail_block[i] >= 0:
+                self._tail_block[i] -= (before[i] - n) // self.ps
         return freed
 
 
