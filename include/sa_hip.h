@@ -364,18 +364,20 @@ int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zer
  * (rows, vocab) in `dtype` (f32 or bf16) with row stride ld (elements), targets
  * (rows) int64; all outputs f32 unless said:
  *   logprob (rows): log p of targets[r]; 0 at ignore_index, NaN for any other id
- *   outside the vocabulary.  entropy (rows): -sum p log p.  stats (rows, 2): the
- *   row's maximum and log sum e^(x - maximum), for the backward.  top_ids (rows,
+ *   outside the vocabulary.  entropy (rows): -sum p log p.  stats (rows, 2): n
+ *   and log2 sum 2^(x log2(e) + n), for the backward.  top_ids (rows,
  *   top) int64 and top_logprobs (rows, top): the largest, ties to the lowest id;
- *   top 0..64 and <= vocab, both may be NULL for 0.
+ *   top 0..64 and <= vocab, both may be NULL for 0.  workspace: of the size that
+ *   sa_token_logprobs_workspace_size says, 16-byte aligned (0 bytes: NULL).
  * Backward: dlogits (rows, vocab) in `dtype`, row stride ldd, for the upstream
  * gradients g_logprob (rows), g_entropy (rows), g_top (rows, top), each NULL for
  * zero; entropy, stats, top_ids as the forward wrote them.
  */
+size_t sa_token_logprobs_workspace_size(long rows, int vocab, int top);
 int sa_token_logprobs_fwd(int dtype, const void* logits, long ld, const int64_t* targets,
                           long rows, int vocab, int top, long ignore_index, float* logprob,
                           float* entropy, float* stats, int64_t* top_ids, float* top_logprobs,
-                          void* stream);
+                          void* workspace, size_t workspace_bytes, void* stream);
 int sa_token_logprobs_bwd(int dtype, const void* logits, long ld, const int64_t* targets,
                           long rows, int vocab, int top, long ignore_index, const float* entropy,
                           const float* stats, const int64_t* top_ids, const float* g_logprob,

@@ -76,7 +76,9 @@ SIGNATURES: dict[str, list] = {
                             ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i),
                             ctypes.POINTER(_vp), _vp],
     "sa_int4_dequant_bf16": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
-    "sa_token_logprobs_fwd": [_i, _vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp],
+    "sa_token_logprobs_workspace_size": [_i64, _i, _i],
+    "sa_token_logprobs_fwd": [_i, _vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                              _sz, _vp],
     "sa_token_logprobs_bwd": [_i, _vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                               _vp, _i64, _vp],
     "sa_ssd_bwd": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
@@ -105,6 +107,7 @@ RESTYPES = {"sa_last_error": ctypes.c_char_p, "sa_profile_enable": None, "sa_ssd
             "sa_ssd_bwd_gated_workspace_size": ctypes.c_size_t,
             "sa_paged_decode_workspace_size": ctypes.c_size_t,
             "sa_paged_decode_noalloc_limit": ctypes.c_size_t,
+            "sa_token_logprobs_workspace_size": ctypes.c_size_t,
             "sa_ssm_conv_bwd_workspace_size": ctypes.c_size_t,
             "sa_ssm_gate_bwd_workspace_size": ctypes.c_size_t,
             "sa_score_stats_workspace_size": ctypes.c_size_t,

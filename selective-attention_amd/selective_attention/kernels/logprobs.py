@@ -37,9 +37,12 @@ def token_logprobs_forward(logits, targets, top, ignore_index):
     stats = torch.empty((rows, 2), **f32)
     ids = torch.empty((*shape, top), dtype=torch.int64, device=dev)
     tl = torch.empty((*shape, top), **f32)
+    nbytes = _lib.load().sa_token_logprobs_workspace_size(rows, V, top)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
     call_on(x, "sa_token_logprobs_fwd", act_dtype_code(x.dtype), _lib.ptr(x), _stride(x),
             _lib.ptr(tg), rows, V, top, int(ignore_index), _lib.ptr(lp), _lib.ptr(H),
-            _lib.ptr(stats), _lib.ptr(ids), _lib.ptr(tl), _lib.stream_of(x))
+            _lib.ptr(stats), _lib.ptr(ids), _lib.ptr(tl), _lib.ptr(ws), nbytes,
+            _lib.stream_of(x))
     return lp, H, stats, ids, tl
 
 

@@ -2,7 +2,7 @@
 float64.
 
 Tolerances (half a step of fp32 is u = 2^-24).  With d = x - m the relative error
-of e^d is at most (3 |d| + 4) u: d's rounding, d log2(e)'s two, exp2's.  Summed
+of e^d is at most (3 |d| + 4) u: log2(e)'s rounding, the exponent's, exp2's.  Summed
 over the terms, s is off by (3 |t / s| + 4) u, |t / s| <= log V < 12, and by the
 sum's order, 64 terms a thread, then 20 levels: 84 u.  So log s is off by
 (40 + 84) u < 8e-6, a logprob by that and two roundings of its own (4 u of it).
@@ -128,14 +128,31 @@ def test_alternatives_in_hard_orders(V, order):
         lanes = (torch.arange(V) // 8) % 64
         x[0, lanes < 20] += 10.0
     for dtype in (torch.float32, torch.bfloat16):
-        check(x.to(dtype), torch.tensor([V - 1]), top)
+        one = check(x.to(dtype), torch.tensor([V - 1]), top)
+        # many rows: another split of the row, the same answer
+        many = token_logprobs(x.to(dtype).cuda().expand(512, V).contiguous(),
+                              torch.full((512,), V - 1, device="cuda"), top=top)
+        assert torch.equal(many.top_ids, one.top_ids.expand(512, top))
+        # (rows stand at different places to a 16-byte boundary: other threads add
+        # other logits, each row within the bound of the exact value)
+        assert (many.logprob - many.logprob[:1]).abs().max() <= 2 * E_LP
+        for a, b, tol in zip(many, one, (E_LP, E_H, 0, E_LP)):
+            near(a[:1], b.cpu(), "many rows", 2 * tol)
 
 
 @pytest.mark.gpu
-def test_rows_of_no_numbers():
+@pytest.mark.parametrize("V,top", [(20001, 7), (40001, 0), (40001, 20)])
+def test_many_rows_of_several_pieces(V, top):
+    x, t = make(515, V, torch.bfloat16, seed=V, banned=0.1)
+    check(x, t, top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [6, 600])
+def test_rows_of_no_numbers(rows):
     """Rows of -inf alone, with NaN, with +inf: NaN; the rows beside them stand."""
     for V in (100, 5000, 40000):
-        x, t = make(6, V, torch.float32, seed=1)
+        x, t = make(rows, V, torch.float32, seed=1)
         x[1] = -INF
         x[2, V // 3] = math.nan
         x[3, V // 2] = INF
@@ -150,6 +167,20 @@ def test_rows_of_no_numbers():
             assert torch.isnan(out.logprob[r]) and torch.isnan(out.entropy[r])
         assert out.top_ids[1].tolist() == [0, 1, 2, 3]
         assert out.top_ids[2, 0] == V // 3 and out.top_ids[3, 0] == V // 2
+
+
+@pytest.mark.gpu
+def test_one_large_logit():
+    """All the probability at one token, at any size of its logit: log p is 0 to
+    fp32's step at 1, never above, and the entropy 0, never below."""
+    for size in (30.0, 127.5, 1000.0, -1000.0, 3.0e4):
+        x = torch.full((3, 500), size - 50.0)
+        x[:, 7] = size
+        out = token_logprobs(x.cuda(), torch.tensor([7, 8, 7]).cuda(), top=2)
+        assert (out.logprob[[0, 2]] <= 0).all() and (out.logprob[[0, 2]] >= -2.0 ** -23).all()
+        assert abs(float(out.logprob[1]) + 50.0) <= 2.0 ** -22 * 50
+        assert (out.entropy >= 0).all() and (out.entropy <= 2.0 ** -22).all()
+        assert (out.top_logprobs <= 0).all() and out.top_ids[0].tolist() == [7, 0]
 
 
 @pytest.mark.gpu
