@@ -340,19 +340,18 @@ int sa_gemv_bf16_multi(const void* x, const void* xscale, int M, int K, int nseg
  * Linear layers with 4-bit weights for 1 to 64 rows (inference; the reference
  * has none): y_i = x W_i^T + bias_i, i < nseg <= 4, all of the same x,
  *   W[n, k] = scale[n, k / group] (code[n, k] - zero[n, k / group]),
- * zero = 8 where zeros is NULL, group in {32, 64, 128}.  x (M, K) bf16 with row
+ * zero = 8 where there are no zeros, group in {32, 64, 128}.  x (M, K) bf16 with row
  * stride ldx (a multiple of 8 elements; columns K..ldx-1 hold zeros), 16-byte
  * aligned; with xscale (laid out as x, or NULL) the input is bf16(x * xscale).
  * packed: (ceil(N / 16), ceil(K / 128), 64, 16) bytes, lane 16 g + c of a tile
  * being its row c, byte 4 j + i of it columns 32 j + 8 g + 2 i (low half) and
  * + 1 (high half).  scales, zeros: (ceil(N / 16), ceil(K / 128) 128 / group,
  * 16) bf16, finite in the padding.  bias (N) bf16 or NULL, y (M, N) bf16.
- * zeros, bias: NULL, or arrays of nseg pointers (zero points for all or none).
+ * matrices: six words each, the addresses of packed, scales, zeros (0: none; for
+ * all or for none), bias (0: none) and y, and N.
  */
 int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int K, int ldx, int group,
-                        int nseg, const void* const* packed, const void* const* scales,
-                        const void* const* zeros, const void* const* bias, const int* N,
-                        void* const* y, void* stream);
+                        int nseg, const int64_t* matrices, void* stream);
 
 /* The weights that such a packed matrix stands for, rounded to bf16: out (N, K). */
 int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zeros, int N, int K,

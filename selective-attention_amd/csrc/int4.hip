@@ -25,6 +25,7 @@
 #include "common.h"
 #include "prof.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace sa {
@@ -60,6 +61,54 @@ __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
   return pack_bf16x2(bf16lo_to_f32(a) * bf16lo_to_f32(b), bf16hi_to_f32(a) * bf16hi_to_f32(b));
 }
 
+// J blocks of 128 columns and 16 rows of x, those outside x as 0 (buffer loads,
+// whose range check answers for them without a branch), times xscale, rounded to
+// bf16, where that is given.  They are read along the rows (16 lanes a row, 4 rows
+// a load) and turned into operand order in the wave's own LDS (16 rows of 272
+// bytes): loads in operand order take 64 bytes from each of 16 rows, which at K =
+// 4096 lie in one channel of the L2 (64 rows, 4096 -> 4096: 13.3 us, turned 10.4;
+// 32 rows, 4096 -> 32000: 24.6 and 22).
+constexpr int kTurnRow = 17;   // uint4
+template <int J>
+__device__ __forceinline__ void load_x_rows(uint4 (&v)[J][4], const bf16* x, const bf16* xscale, int row0,
+                                            int k0, int M, int K, int ldx) {
+  const int lane = threadIdx.x & 63, bytes = M * ldx * 2;
+  const __amdgpu_buffer_rsrc_t rx =
+      __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(x), static_cast<short>(0), bytes, 0x00020000);
+  auto at = [&](int j, int i) {
+    const int row = row0 + 4 * i + (lane >> 4), k = k0 + 128 * j + 8 * (lane & 15);
+    return row < M && k < K ? (row * ldx + k) * 2 : bytes;
+  };
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      v[j][i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, at(j, i), 0, 0));
+  if (xscale) {
+    const __amdgpu_buffer_rsrc_t rf =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(xscale), static_cast<short>(0), bytes, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint4 f = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rf, at(j, i), 0, 0));
+        uint4& u = v[j][i];
+        u = uint4{mul_pair(u.x, f.x), mul_pair(u.y, f.y), mul_pair(u.z, f.z), mul_pair(u.w, f.w)};
+      }
+  }
+}
+__device__ __forceinline__ void turn_x(v8bf (&xf)[4], const uint4 (&v)[4], uint4* lds) {
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) lds[(4 * i + g) * kTurnRow + c] = v[i];
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#pragma unroll
+  for (int j = 0; j < 4; ++j) xf[j] = pair_x(lds[c * kTurnRow + 4 * j + g]);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
+
 // A workgroup of NW waves computes R tiles of 16 columns of y for up to 16 CT
 // rows of x; the waves take the 128-column blocks of K in turn and their sums
 // meet in LDS.
@@ -69,7 +118,8 @@ __global__ __launch_bounds__(64 * NW) void int4_linear_kernel(const bf16* __rest
                                                               const Int4Segs sg, int M, int K,
                                                               int ldx) {
   constexpr int GN = 128 / G, GS = G / 32;   // groups of a block, k-steps of a group
-  __shared__ float part[NW][R][CT][256];
+  constexpr int kPart = NW * R * CT * 64, kTurn = 16 * kTurnRow;   // uint4, a wave's uint4
+  __shared__ uint4 smem[NW * kTurn > kPart ? NW * kTurn : kPart];     // x turned, then the sums
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = lane & 15, g = lane >> 4;
   const int bid = blockIdx.x;
   int seg = 0;
@@ -107,19 +157,11 @@ __global__ __launch_bounds__(64 * NW) void int4_linear_kernel(const bf16* __rest
         if constexpr (Z) z[r][i] = ZP[at];
       }
     v8bf xf[CT][4];
+    uint4 xr[CT][1][4];
 #pragma unroll
-    for (int t = 0; t < CT; ++t)
+    for (int t = 0; t < CT; ++t) load_x_rows(xr[t], x, xscale, 16 * t, 128 * kb, M, K, ldx);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int row = 16 * t + c, k = 128 * kb + 32 * j + 8 * g;
-        const bool ok = row < M && k < K;
-        uint4 v = ld16(x + static_cast<long>(row) * ldx + k, ok);
-        if (xscale) {
-          const uint4 f = ld16(xscale + static_cast<long>(row) * ldx + k, ok);
-          v = uint4{mul_pair(v.x, f.x), mul_pair(v.y, f.y), mul_pair(v.z, f.z), mul_pair(v.w, f.w)};
-        }
-        xf[t][j] = pair_x(v);
-      }
+    for (int t = 0; t < CT; ++t) turn_x(xf[t], xr[t][0], smem + wid * kTurn);
 #pragma unroll
     for (int i = 0; i < GN; ++i) {
 #pragma unroll
@@ -150,22 +192,163 @@ __global__ __launch_bounds__(64 * NW) void int4_linear_kernel(const bf16* __rest
     }
   }
   // lane (c, g) holds columns 4 g + e of the tile for row 16 t + c of x
+  float* part = reinterpret_cast<float*>(smem);
+  __syncthreads();   // the turned rows are read
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int t = 0; t < CT; ++t)
-      *reinterpret_cast<float4*>(&part[wid][r][t][c * 16 + 4 * g]) =
+      *reinterpret_cast<float4*>(part + ((wid * R + r) * CT + t) * 256 + c * 16 + 4 * g) =
           make_float4(acc[r][t][0], acc[r][t][1], acc[r][t][2], acc[r][t][3]);
   __syncthreads();
   const bf16* bias = sg.bias[seg];
   bf16* y = sg.y[seg];
   for (int e = tid; e < R * CT * 256; e += 64 * NW) {
     const int row = (e >> 4) % (16 * CT), n = 16 * (t0 + e / (CT * 256)) + (e & 15);
-    const float* p = &part[0][0][0][0] + e;
+    const float* p = part + e;
     float v = 0.0f;
 #pragma unroll
     for (int i = 0; i < NW; ++i) v += p[i * R * CT * 256];
     if (row < M && n < N) y[static_cast<long>(row) * N + n] = from_f32<bf16>(v + (bias ? to_f32(bias[n]) : 0.0f));
+  }
+}
+
+// The same for K up to 8 KW blocks of 128 columns: wave w of a workgroup keeps x
+// of its KW blocks in registers, in operand order and with the groups' sums, and
+// the workgroup goes through the tiles t, t + gridDim.x, ..., so that only the
+// weights are streamed: x is read and put in order once a workgroup, not once a
+// tile (4096 -> 32000, 8 rows: 25.7 us by tiles, 16.2 here; 32 rows: 36.4 and 22;
+// the weights' bytes at 6 TB/s are 11.4 us).  The next tile's codes and factors are
+// in flight while this one's are multiplied (two in flight: no faster); the eight
+// waves' sums meet in one of two LDS buffers, one barrier a tile.
+template <int CT, int G, bool Z, int KW>
+__global__ __launch_bounds__(512, CT == 1 && KW < 4 ? 3 : 2) void int4_stream_kernel(
+    const bf16* __restrict__ x, const bf16* __restrict__ xscale, const Int4Segs sg, int M, int K,
+    int ldx) {
+  constexpr int GN = 128 / G, GS = G / 32, NW = 8;
+  constexpr int kPart = NW * CT * 256, kTurn = 16 * kTurnRow;   // floats, uint4 a wave
+  __shared__ uint4 smem[(NW * kTurn > 2 * kPart / 4) ? NW * kTurn : 2 * kPart / 4];   // x turned, then the sums
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = lane & 15, g = lane >> 4;
+  const int kb_n = (K + 127) >> 7, kb0 = wid * KW, m0 = blockIdx.y * 16 * CT;
+  const int total = sg.blk0[kInt4Segs];   // tiles of all matrices
+
+  struct Tile {
+    uint4 w[KW];
+    uint2 s[KW * GN], z[Z ? KW * GN : 1];
+  };
+  auto seg_of = [&](int t) {
+    int seg = 0;
+#pragma unroll
+    for (int i = 1; i < kInt4Segs; ++i) seg += (i < sg.nseg && t >= sg.blk0[i]) ? 1 : 0;
+    return seg;
+  };
+  auto load = [&](int t, Tile& q) __attribute__((always_inline)) {
+    const int seg = seg_of(t);
+    const long first = static_cast<long>(t - sg.blk0[seg]) * kb_n;
+    const uint4* W = sg.W[seg];
+    const uint2* S = reinterpret_cast<const uint2*>(sg.scale[seg]);
+    const uint2* ZP = reinterpret_cast<const uint2*>(sg.zero[seg]);
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const long kb = first + min(kb0 + k, kb_n - 1);   // (blocks behind the last meet x = 0)
+      q.w[k] = W[kb * 64 + lane];
+#pragma unroll
+      for (int i = 0; i < GN; ++i) {
+        q.s[k * GN + i] = S[(kb * GN + i) * 4 + g];
+        if constexpr (Z) q.z[k * GN + i] = ZP[(kb * GN + i) * 4 + g];
+      }
+    }
+  };
+  int t = blockIdx.x;   // (gridDim.x <= total)
+  const int step = gridDim.x;
+  Tile q0, q1;      // one is multiplied, the next in flight
+  load(t, q0);
+
+  v8bf xf[CT][KW][4];
+  float xs[CT][KW * GN];
+  {
+    const uint4 o = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
+    const v8bf ones = __builtin_bit_cast(v8bf, o);
+    uint4 xr[CT][KW][4];
+#pragma unroll
+    for (int t = 0; t < CT; ++t) load_x_rows(xr[t], x, xscale, m0 + 16 * t, 128 * kb0, M, K, ldx);
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int k = 0; k < KW; ++k) turn_x(xf[t][k], xr[t][k], smem + wid * kTurn);
+#pragma unroll
+    for (int t = 0; t < CT; ++t)
+#pragma unroll
+      for (int i = 0; i < KW * GN; ++i) {
+        v4f s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < GS; ++j) s = mfma_bf16(ones, xf[t][i / GN][GS * (i % GN) + j], s);
+        xs[t][i] = s[0];   // every row of the product is the same
+      }
+  }
+
+  __syncthreads();   // the turned rows are read
+  int flip = 0;
+  auto tile = [&](const Tile& cur, Tile& free) __attribute__((always_inline)) {
+    load(min(t + step, total - 1), free);
+    v4f acc[CT];
+#pragma unroll
+    for (int u = 0; u < CT; ++u) acc[u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int k = 0; k < KW; ++k) {
+      const uint32_t wj[4] = {cur.w[k].x, cur.w[k].y, cur.w[k].z, cur.w[k].w};
+#pragma unroll
+      for (int i = 0; i < GN; ++i) {
+        const int gi = k * GN + i;
+        v4f d[CT];
+#pragma unroll
+        for (int u = 0; u < CT; ++u) d[u] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < GS; ++j) {
+          const v8bf a = widen_codes(wj[GS * i + j]);
+#pragma unroll
+          for (int u = 0; u < CT; ++u) d[u] = mfma_bf16(a, xf[u][k][GS * i + j], d[u]);
+        }
+        const float sv[4] = {bf16lo_to_f32(cur.s[gi].x), bf16hi_to_f32(cur.s[gi].x),
+                             bf16lo_to_f32(cur.s[gi].y), bf16hi_to_f32(cur.s[gi].y)};
+        float zv[4] = {8.f, 8.f, 8.f, 8.f};
+        if constexpr (Z) {
+          zv[0] = bf16lo_to_f32(cur.z[gi].x);
+          zv[1] = bf16hi_to_f32(cur.z[gi].x);
+          zv[2] = bf16lo_to_f32(cur.z[gi].y);
+          zv[3] = bf16hi_to_f32(cur.z[gi].y);
+        }
+#pragma unroll
+        for (int u = 0; u < CT; ++u)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            acc[u][e] = fmaf(16.0f * sv[e], fmaf(-(1.0f + 0.0625f * zv[e]), xs[u][gi], d[u][e]), acc[u][e]);
+      }
+    }
+    float* buf = reinterpret_cast<float*>(smem) + flip * kPart;
+#pragma unroll
+    for (int u = 0; u < CT; ++u)
+      *reinterpret_cast<float4*>(buf + (wid * CT + u) * 256 + c * 16 + 4 * g) = make_float4(acc[u][0], acc[u][1], acc[u][2], acc[u][3]);
+    __syncthreads();
+    const int seg = seg_of(t), N = sg.N[seg];
+    const bf16* bias = sg.bias[seg];
+    bf16* y = sg.y[seg];
+    for (int e = tid; e < CT * 256; e += 64 * NW) {
+      const int row = m0 + (e >> 4), n = 16 * (t - sg.blk0[seg]) + (e & 15);
+      float v = 0.0f;
+#pragma unroll
+      for (int i = 0; i < NW; ++i) v += buf[i * CT * 256 + e];
+      if (row < M && n < N) y[static_cast<long>(row) * N + n] = from_f32<bf16>(v + (bias ? to_f32(bias[n]) : 0.0f));
+    }
+    flip ^= 1;
+    t += step;
+  };
+  // (two copies of the body, so that no register of a load in flight is moved)
+  while (true) {
+    tile(q0, q1);
+    if (t >= total) break;
+    tile(q1, q0);
+    if (t >= total) break;
   }
 }
 
@@ -201,14 +384,33 @@ void int4_go(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int 
                      s, static_cast<const bf16*>(x), static_cast<const bf16*>(xscale), sg, M, K, ldx);
 }
 
+template <int CT, int G, bool Z, int KW>
+void int4_stream(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int ldx, hipStream_t s) {
+  sg.blk0[0] = 0;
+  for (int i = 0; i < kInt4Segs; ++i)
+    sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? (sg.N[i] + 15) / 16 : 0);
+  const int parts = (M + 16 * CT - 1) / (16 * CT);
+  // one workgroup a CU where its registers leave room for no second one (KW = 4),
+  // else two (1024 -> 32000, 4 rows: 8.3 and 6.8 us; 4096 -> 32000: 16.3 and 19)
+  const int grid = std::min(sg.blk0[kInt4Segs], (KW == 4 ? 256 : 512) / parts);
+  hipLaunchKernelGGL((int4_stream_kernel<CT, G, Z, KW>), dim3(grid, parts), dim3(512), 0, s,
+                     static_cast<const bf16*>(x), static_cast<const bf16*>(xscale), sg, M, K, ldx);
+}
+
 template <int G, bool Z>
 void int4_rows(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int ldx, hipStream_t s) {
-  if (M <= 16)
-    int4_go<1, G, Z, 1, 4>(x, xscale, sg, M, K, ldx, s);
-  else if (M <= 32)
-    int4_go<2, G, Z, 2, 4>(x, xscale, sg, M, K, ldx, s);
-  else
-    int4_go<4, G, Z, 2, 4>(x, xscale, sg, M, K, ldx, s);
+  const int kb = (K + 127) / 128;
+  auto stream = [&](auto kw) {
+    constexpr int KW = decltype(kw)::value;
+    M <= 16 ? int4_stream<1, G, Z, KW>(x, xscale, sg, M, K, ldx, s)
+            : int4_stream<2, G, Z, KW>(x, xscale, sg, M, K, ldx, s);
+  };
+  if (kb <= 8) stream(std::integral_constant<int, 1>{});
+  else if (kb <= 16) stream(std::integral_constant<int, 2>{});
+  else if (kb <= 32 && G > 32) stream(std::integral_constant<int, (G > 32 ? 4 : 2)>{});
+  else if (M <= 16) int4_go<1, G, Z, 2, 8>(x, xscale, sg, M, K, ldx, s);
+  else if (M <= 32) int4_go<2, G, Z, 2, 8>(x, xscale, sg, M, K, ldx, s);
+  else int4_go<4, G, Z, 2, 8>(x, xscale, sg, M, K, ldx, s);
 }
 
 bool int4_group_ok(int G) { return G == 32 || G == 64 || G == 128; }
@@ -217,41 +419,36 @@ bool int4_group_ok(int G) { return G == 32 || G == 64 || G == 128; }
 }  // namespace sa
 
 extern "C" int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int K, int ldx,
-                                   int group, int nseg, const void* const* packed,
-                                   const void* const* scales, const void* const* zeros,
-                                   const void* const* bias, const int* N, void* const* y,
-                                   void* stream) {
+                                   int group, int nseg, const int64_t* matrices, void* stream) {
   const char* who = "sa_int4_linear_bf16";
-  SA_CHECK_ARG(M >= 1 && M <= 64 && K > 0 && K <= (1 << 24), "%s: M %d must be 1..64 and K %d positive",
+  SA_CHECK_ARG(M >= 1 && M <= 64 && K > 0 && K <= (1 << 22), "%s: M %d must be 1..64 and K %d 1..2^22",
                who, M, K);
-  SA_CHECK_ARG(ldx % 8 == 0 && ldx >= K, "%s: row stride %d must be a multiple of 8, at least K %d", who,
+  SA_CHECK_ARG(ldx % 8 == 0 && ldx >= K && ldx <= (1 << 23), "%s: row stride %d must be a multiple of 8, at least K %d", who,
                ldx, K);
   SA_CHECK_ARG(sa::int4_group_ok(group), "%s: group %d not in {32, 64, 128}", who, group);
   SA_CHECK_ARG(nseg >= 1 && nseg <= sa::kInt4Segs, "%s: %d weight matrices, 1..%d allowed", who, nseg,
                sa::kInt4Segs);
-  SA_CHECK_ARG(x && packed && scales && N && y, "%s: null pointer", who);
+  SA_CHECK_ARG(x && matrices, "%s: null pointer", who);
   SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xscale)) & 15) == 0,
                "%s: x and xscale must be 16-byte aligned", who);
   sa::Int4Segs sg{};
   sg.nseg = nseg;
-  const bool z = zeros && zeros[0];
+  const bool z = matrices[2] != 0;
   long tiles = 0;
   for (int i = 0; i < nseg; ++i) {
-    SA_CHECK_ARG(packed[i] && scales[i] && y[i] && N[i] > 0, "%s: weight matrix %d: null pointer or N %d",
-                 who, i, N[i]);
-    SA_CHECK_ARG((zeros && zeros[i]) == z, "%s: zero points for all weight matrices or for none", who);
-    SA_CHECK_ARG((reinterpret_cast<uintptr_t>(packed[i]) & 15) == 0 &&
-                     (reinterpret_cast<uintptr_t>(scales[i]) & 7) == 0 &&
-                     (!z || (reinterpret_cast<uintptr_t>(zeros[i]) & 7) == 0),
-                 "%s: weight matrix %d is not aligned", who, i);
-    tiles += (N[i] + 15L) / 16;
+    const int64_t* m = matrices + 6 * i;   // packed, scales, zeros, bias, y, N
+    SA_CHECK_ARG(m[0] && m[1] && m[4] && m[5] > 0 && m[5] <= (1L << 30),
+                 "%s: weight matrix %d: null pointer or N %ld", who, i, static_cast<long>(m[5]));
+    SA_CHECK_ARG((m[2] != 0) == z, "%s: zero points for all weight matrices or for none", who);
+    SA_CHECK_ARG((m[0] & 15) == 0 && ((m[1] | m[2]) & 7) == 0, "%s: weight matrix %d is not aligned", who, i);
+    tiles += (m[5] + 15) / 16;
     SA_CHECK_ARG(tiles < (1 << 27), "%s: too many columns", who);
-    sg.W[i] = static_cast<const uint4*>(packed[i]);
-    sg.scale[i] = static_cast<const sa::bf16*>(scales[i]);
-    sg.zero[i] = z ? static_cast<const sa::bf16*>(zeros[i]) : nullptr;
-    sg.bias[i] = bias ? static_cast<const sa::bf16*>(bias[i]) : nullptr;
-    sg.y[i] = static_cast<sa::bf16*>(y[i]);
-    sg.N[i] = N[i];
+    sg.W[i] = reinterpret_cast<const uint4*>(m[0]);
+    sg.scale[i] = reinterpret_cast<const sa::bf16*>(m[1]);
+    sg.zero[i] = reinterpret_cast<const sa::bf16*>(m[2]);
+    sg.bias[i] = reinterpret_cast<const sa::bf16*>(m[3]);
+    sg.y[i] = reinterpret_cast<sa::bf16*>(m[4]);
+    sg.N[i] = static_cast<int>(m[5]);
   }
   hipStream_t s = static_cast<hipStream_t>(stream);
   sa::ProfScope prof_("int4_linear", s);

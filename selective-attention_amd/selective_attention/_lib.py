@@ -72,9 +72,7 @@ SIGNATURES: dict[str, list] = {
     "sa_gemv_bf16": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
     "sa_gemv_bf16_multi": [_vp, _vp, _i, _i, _i, ctypes.POINTER(_vp), ctypes.POINTER(_vp),
                            ctypes.POINTER(_i), ctypes.POINTER(_vp), _vp],
-    "sa_int4_linear_bf16": [_vp, _vp, _i, _i, _i, _i, _i, ctypes.POINTER(_vp), ctypes.POINTER(_vp),
-                            ctypes.POINTER(_vp), ctypes.POINTER(_vp), ctypes.POINTER(_i),
-                            ctypes.POINTER(_vp), _vp],
+    "sa_int4_linear_bf16": [_vp, _vp, _i, _i, _i, _i, _i, ctypes.POINTER(_i64), _vp],
     "sa_int4_dequant_bf16": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
     "sa_token_logprobs_workspace_size": [_i64, _i, _i],
     "sa_token_logprobs_fwd": [_i, _vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp,

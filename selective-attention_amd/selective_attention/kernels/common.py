@@ -37,6 +37,19 @@ def require_device(*tensors: torch.Tensor | None) -> torch.device:
     return dev
 
 
+def require_one_device(*tensors: torch.Tensor | None) -> None:
+    """require_device for the decode steps' calls: without the device objects,
+    which for a dozen tensors take longer than a launch."""
+    dev = -2
+    for t in tensors:
+        if t is not None:
+            d = t.get_device()
+            if d != dev:
+                if d < 0 or dev != -2:
+                    require_device(*tensors)    # says what is wrong
+                dev = d
+
+
 def call_on(t: torch.Tensor, name: str, *args) -> None:
     """_lib.call with t's device current (its stream belongs to that device)."""
     if torch._C._cuda_getDevice() == t.device.index:

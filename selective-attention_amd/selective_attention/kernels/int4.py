@@ -7,7 +7,7 @@ import ctypes
 import torch
 
 from .. import _lib
-from .common import call_on, require_device
+from .common import call_on, require_device, require_one_device
 
 GROUPS = (32, 64, 128)
 MAX_ROWS = 64      # rows of one launch; more go through the widened weights
@@ -16,36 +16,38 @@ MAX_MATRICES = 4
 
 def group_size(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None) -> int:
     """The group size that the tensors' shapes say, checked."""
-    if packed.dim() != 4 or tuple(packed.shape[2:]) != (64, 16) or packed.dtype != torch.uint8:
+    shape, f = packed.shape, scales.shape
+    if len(shape) != 4 or shape[2] != 64 or shape[3] != 16 or packed.dtype != torch.uint8:
         raise ValueError(f"int4: packed must be (tiles, blocks, 64, 16) uint8, got "
-                         f"{tuple(packed.shape)} {packed.dtype}")
-    nt, kb = packed.shape[:2]
+                         f"{tuple(shape)} {packed.dtype}")
+    nt, kb = shape[0], shape[1]
     if nt == 0 or kb == 0:
         raise ValueError("int4: empty weight")
-    if scales.dim() != 3 or scales.shape[0] != nt or scales.shape[2] != 16:
-        raise ValueError(f"int4: scales must be ({nt}, groups, 16), got {tuple(scales.shape)}")
-    G = 128 * kb // max(scales.shape[1], 1)
-    if G not in GROUPS or G * scales.shape[1] != 128 * kb:
-        raise ValueError(f"int4: {scales.shape[1]} groups over {128 * kb} columns are groups of "
-                         f"none of {GROUPS}")
-    if zeros is not None and zeros.shape != scales.shape:
-        raise ValueError(f"int4: zeros must be {tuple(scales.shape)}, got {tuple(zeros.shape)}")
-    for t, name in ((scales, "scales"), (zeros, "zeros")):
-        if t is not None and t.dtype != torch.bfloat16:
-            raise TypeError(f"int4: {name} must be bfloat16, got {t.dtype}")
+    if len(f) != 3 or f[0] != nt or f[2] != 16:
+        raise ValueError(f"int4: scales must be ({nt}, groups, 16), got {tuple(f)}")
+    G = 128 * kb // max(f[1], 1)
+    if G not in GROUPS or G * f[1] != 128 * kb:
+        raise ValueError(f"int4: {f[1]} groups over {128 * kb} columns are groups of none of {GROUPS}")
+    if zeros is not None and zeros.shape != f:
+        raise ValueError(f"int4: zeros must be {tuple(f)}, got {tuple(zeros.shape)}")
     for t, name in ((packed, "packed"), (scales, "scales"), (zeros, "zeros")):
-        if t is not None and (not t.is_contiguous() or t.data_ptr() % 16):
-            raise ValueError(f"int4: {name} must be contiguous on a 16-byte boundary")
+        if t is not None:
+            if t is not packed and t.dtype != torch.bfloat16:
+                raise TypeError(f"int4: {name} must be bfloat16, got {t.dtype}")
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"int4: {name} must be contiguous on a 16-byte boundary")
     return G
 
 
 def _rows(x: torch.Tensor, K: int) -> torch.Tensor:
     """x (..., K) as (M, K) rows that the kernel reads: 16-byte aligned, the row
     length padded with zeros to a multiple of 8."""
-    x = x.reshape(-1, K)
+    if x.dim() != 2:
+        x = x.reshape(-1, K)
     if K % 8:
         return torch.nn.functional.pad(x, (0, 8 - K % 8))
-    x = x.contiguous()
+    if not x.is_contiguous():
+        return x.contiguous()
     return x if x.data_ptr() % 16 == 0 else x.clone()
 
 
@@ -53,19 +55,24 @@ def int4_linear_multi(x, weights, biases, sizes, G, xscale=None):
     """x (..., K) bf16 of 1..64 rows; weights: [(packed, scales, zeros or None)],
     1..4 of them with one group size; biases: [(N_i,) bf16 or None]; sizes: [N_i]
     -> [(..., N_i)], one launch."""
-    require_device(x, xscale, *[t for w in weights for t in w], *biases)
+    for w in weights:
+        require_one_device(x, *w)
+    require_one_device(x, xscale, *biases)
     K, n = x.shape[-1], len(weights)
     xr = _rows(x, K)
     xs = None if xscale is None else _rows(xscale, K)
     M = xr.shape[0]
-    ys = [torch.empty(*x.shape[:-1], N, dtype=torch.bfloat16, device=x.device) for N in sizes]
-    bs = [None if b is None else b.contiguous() for b in biases]
-    arr = ctypes.c_void_p * n
-    call_on(x, "sa_int4_linear_bf16", _lib.ptr(xr), _lib.ptr(xs), M, K, xr.shape[1], G, n,
-            arr(*[w[0].data_ptr() for w in weights]), arr(*[w[1].data_ptr() for w in weights]),
-            None if weights[0][2] is None else arr(*[w[2].data_ptr() for w in weights]),
-            arr(*[_lib.ptr(b) for b in bs]), (ctypes.c_int * n)(*sizes),
-            arr(*[y.data_ptr() for y in ys]), _lib.stream_of(x))
+    ys, words, kept = [], [], []
+    for (packed, scales, zeros), b, N in zip(weights, biases, sizes):
+        y = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
+        if b is not None and not b.is_contiguous():
+            b = b.contiguous()
+            kept.append(b)
+        words += (packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
+                  0 if b is None else b.data_ptr(), y.data_ptr(), N)
+        ys.append(y)
+    call_on(x, "sa_int4_linear_bf16", xr.data_ptr(), _lib.ptr(xs), M, K, xr.shape[1], G, n,
+            (ctypes.c_int64 * (6 * n))(*words), _lib.stream_of(x))
     return ys
 
 

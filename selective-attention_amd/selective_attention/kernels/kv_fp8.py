@@ -12,7 +12,7 @@ import torch
 
 from .. import _lib
 from .attention import _i32, _rows16
-from .common import call_on, require_device
+from .common import call_on, require_one_device
 
 FP8 = torch.float8_e4m3fn
 PAGE_SIZES = (64, 128)
@@ -38,7 +38,7 @@ def _check_cache(who, batch, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
     if gate_pages is not None:
         want.append(("gate_pages" if written else "key_bias", gate_pages, (n, H, ps), torch.float32))
     for name, t, shape, dtype in want:
-        if tuple(t.shape) != shape:
+        if t.shape != shape:
             raise ValueError(f"{who}: {name} must be {shape}, got {tuple(t.shape)}")
         if t.dtype != dtype:
             raise TypeError(f"{who}: {name} must be {dtype}, got {t.dtype}")
@@ -76,7 +76,7 @@ def paged_decode_attn_fp8(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
     b, Hq, D = q.shape
     n, Hkv, ps, _ = _check_cache(who, b, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
                                  page_table, key_bias, False)
-    require_device(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail, page_table, seq_lens,
+    require_one_device(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail, page_table, seq_lens,
                    key_bias)
     q = _rows16(q)
     pt, sl = _i32(page_table), _i32(seq_lens)
@@ -92,11 +92,15 @@ def paged_decode_attn_fp8(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
     return o
 
 
+def _dense(t, dtype):
+    return t if t.dtype == dtype and t.is_contiguous() else t.to(dtype).contiguous()
+
+
 def _lens_and_table(who, page_table, seq_lens, batch):
     for t, name in ((page_table, "page_table"), (seq_lens, "seq_lens")):
         if t.dtype != torch.int32 or not t.is_contiguous():
             raise ValueError(f"{who}: {name} must be a contiguous int32 tensor")
-    if tuple(seq_lens.shape) != (batch,):
+    if seq_lens.shape != (batch,):
         raise ValueError(f"{who}: seq_lens must be ({batch},), got {tuple(seq_lens.shape)}")
     if page_table.shape[1] == 0:
         raise ValueError(f"{who}: page_table has no columns")
@@ -113,11 +117,10 @@ def paged_kv_append_fp8(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, 
     n, _, ps, _ = _check_cache(who, b, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
                                page_table, gate_pages, True)
     _lens_and_table(who, page_table, seq_lens, b)
-    require_device(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale, v_scale,
+    require_one_device(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale, v_scale,
                    k_tail, v_tail, gate_pages)
-    k = k.to(torch.bfloat16).contiguous()
-    v = v.to(torch.bfloat16).contiguous()
-    lg = None if log_gate is None else log_gate.to(torch.float32).contiguous()
+    k, v = _dense(k, torch.bfloat16), _dense(v, torch.bfloat16)
+    lg = None if log_gate is None else _dense(log_gate, torch.float32)
     call_on(k, "sa_paged_kv_append_fp8", _lib.ptr(k), _lib.ptr(v), _lib.ptr(lg),
               _lib.ptr(page_table), _lib.ptr(seq_lens), b, H, D, ps, page_table.shape[1], n,
               _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(k_scale), _lib.ptr(v_scale),
@@ -136,7 +139,7 @@ def paged_kv_build_fp8(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k
     n, _, ps, _ = _check_cache(who, b, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
                                page_table, gate_pages, True)
     _lens_and_table(who, page_table, seq_lens, b)
-    require_device(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale, v_scale,
+    require_one_device(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale, v_scale,
                    k_tail, v_tail, gate_pages)
     if b == 0 or L == 0:
         return   # no tokens: no row has a page to write

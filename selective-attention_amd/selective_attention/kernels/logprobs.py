@@ -5,7 +5,7 @@ from __future__ import annotations
 import torch
 
 from .. import _lib
-from .common import act_dtype_code, call_on, require_device
+from .common import act_dtype_code, call_on, require_one_device
 
 MAX_TOP = 64
 
@@ -13,7 +13,7 @@ MAX_TOP = 64
 def _rows(logits):
     """(rows, vocab) rows of logits whose last dimension is dense, in place where
     one stride leads from row to row."""
-    x = logits.reshape(-1, logits.shape[-1])
+    x = logits if logits.dim() == 2 else logits.reshape(-1, logits.shape[-1])
     return x if x.stride(1) == 1 or x.shape[1] == 1 else x.contiguous()
 
 
@@ -21,16 +21,23 @@ def _stride(x):
     return x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
+def _targets(t):
+    if t.dim() == 1 and t.dtype == torch.int64 and t.is_contiguous():
+        return t
+    return t.reshape(-1).to(torch.int64).contiguous()
+
+
 def token_logprobs_forward(logits, targets, top, ignore_index):
     """logits (..., vocab) float32 or bfloat16, targets (...) integers -> (logprob
     (...), entropy (...), stats (rows, 2), top_ids (..., top) int64, top_logprobs
     (..., top) float32)."""
-    dev = require_device(logits, targets)
+    require_one_device(logits, targets)
+    dev = logits.device
     x = _rows(logits)
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         x = x.contiguous()     # overlapping (expanded) rows
     rows, V = x.shape
-    tg = targets.reshape(-1).to(torch.int64).contiguous()
+    tg = _targets(targets)
     shape = logits.shape[:-1]
     f32 = dict(dtype=torch.float32, device=dev)
     lp, H = torch.empty(shape, **f32), torch.empty(shape, **f32)
@@ -53,7 +60,7 @@ def token_logprobs_backward(logits, targets, top, ignore_index, entropy, stats, 
     if x.shape[0] > 1 and x.stride(0) < x.shape[1]:
         x = x.contiguous()
     rows, V = x.shape
-    tg = targets.reshape(-1).to(torch.int64).contiguous()
+    tg = _targets(targets)
     dx = torch.empty((rows, V), dtype=x.dtype, device=x.device)
     g = [None if t is None else t.to(torch.float32).contiguous() for t in (g_lp, g_h, g_top)]
     call_on(x, "sa_token_logprobs_bwd", act_dtype_code(x.dtype), _lib.ptr(x), _stride(x),

@@ -124,16 +124,22 @@ def int4_linear_multi(x: torch.Tensor, weights, biases, sizes,
     if xscale is not None and (xscale.shape != x.shape or xscale.dtype != torch.bfloat16):
         raise ValueError("int4_linear: xscale must be bfloat16 of x's shape")
     K = x.shape[-1]
-    G = _k.group_size(*weights[0])
+    if K == 0:
+        raise ValueError("int4_linear: x has no features")
+    G, zeros = 0, weights[0][2] is None
     for w, b, N in zip(weights, biases, sizes):
-        if _k.group_size(*w) != G or (w[2] is None) != (weights[0][2] is None):
+        g = _k.group_size(*w)
+        if (G and g != G) or (w[2] is None) != zeros:
             raise ValueError("int4_linear_multi: the weights differ in group size or zero points")
+        G = g
         _sizes(w[0], N, K)
-        check_shape(b, (N,), name="bias", optional=True)
-        if b is not None and b.dtype != torch.bfloat16:
-            raise TypeError(f"int4_linear: bias must be bfloat16, got {b.dtype}")
-    grad = torch.is_grad_enabled() and any(
-        t is not None and t.requires_grad for t in (x, xscale, *biases))
+        if b is not None:
+            check_shape(b, (N,), name="bias")
+            if b.dtype != torch.bfloat16:
+                raise TypeError(f"int4_linear: bias must be bfloat16, got {b.dtype}")
+    grad = torch.is_grad_enabled() and (
+        x.requires_grad or (xscale is not None and xscale.requires_grad)
+        or any(b is not None and b.requires_grad for b in biases))
     rows = x.numel() // K
     if rows == 0:
         return [x.new_empty(*x.shape[:-1], N) for N in sizes]

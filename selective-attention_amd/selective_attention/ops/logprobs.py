@@ -68,4 +68,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     if not 0 <= top <= min(_k.MAX_TOP, logits.shape[-1]):
         raise ValueError(f"token_logprobs: top {top} must be 0..{_k.MAX_TOP} and at most the "
                          f"vocabulary {logits.shape[-1]}")
-    return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets, int(top), int(ignore_index)))
+    top, ignore_index = int(top), int(ignore_index)
+    if torch.is_grad_enabled() and logits.requires_grad:
+        return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets, top, ignore_index))
+    lp, H, _, ids, tl = _k.token_logprobs_forward(logits, targets, top, ignore_index)
+    return TokenLogprobs(lp, H, ids, tl)

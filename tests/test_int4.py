@@ -146,10 +146,25 @@ def test_linear(M, N, K, G, zeros):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20, 64])
+@pytest.mark.parametrize("N,K,G,zeros", [(40, 4096, 64, True), (5000, 1100, 128, False),
+                                         (40, 4100, 128, False), (50, 2100, 32, True)])
+def test_linear_long(M, N, K, G, zeros):
+    """The widest x that stays in registers, more tiles than workgroups, and the
+    columns behind that."""
+    codes, scales, z, b = make(N, K, G, zeros, seed=M, bias=True)
+    packed = pack_int4(codes, scales, z, G)
+    x = torch.randn(M, K, generator=torch.Generator().manual_seed(M)).to(torch.bfloat16)
+    y = int4_linear(x.cuda(), *dev(packed), bias=b.cuda(), out_features=N)
+    check(y, x, packed, N, K, b)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [3, 40])
-def test_multi_with_xscale(M):
+@pytest.mark.parametrize("K", [384, 4300])
+def test_multi_with_xscale(M, K):
     """Four weights of one x * xscale in one launch, outputs of their own."""
-    K, G, sizes = 384, 64, [16, 100, 33, 1]
+    G, sizes = 64, [16, 100, 33, 1]
     g = torch.Generator().manual_seed(5)
     x, f = (torch.randn(M, K, generator=g).to(torch.bfloat16) for _ in range(2))
     ws, bs = [], []
