@@ -42,6 +42,16 @@ __device__ __forceinline__ v8bf widen8(uint32_t lo, uint32_t hi, float scale) {
   return __builtin_bit_cast(v8bf, r);
 }
 
+// 16 bytes of a buffer at a lane's and a constant offset.  NT: non-temporal, the
+// line is not kept.  The codes are read once a step, and without it the caches'
+// own traffic costs a tenth: 64 rows of 1 to 32 thousand keys, 8 heads of 128,
+// 456 us; 410 with it, 5.9 TB/s.  Only where a tile takes whole lines: at 128 keys a
+// page the two tiles of a V^T row share its line (5.1 TB/s without, 4.2 with).
+template <bool NT>
+__device__ __forceinline__ uint4 buf_load16(__amdgpu_buffer_rsrc_t r, unsigned off) {
+  return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0));
+}
+
 struct Slot8 {
   long blk;          // (page, kv head) of the tile in the pool
   int k0;            // the tile's first key inside its page
@@ -49,15 +59,16 @@ struct Slot8 {
   float ks, vs;      // the block's scales
 };
 
-template <int D, bool BIAS>
+template <int D, bool BIAS, int PS>
 __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
     const bf16* __restrict__ q, const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp,
     const float* __restrict__ ksc, const float* __restrict__ vsc, const bf16* __restrict__ kt_p,
     const bf16* __restrict__ vt_p, const int32_t* __restrict__ page_table,
     const int32_t* __restrict__ seq_lens, const float* __restrict__ key_bias,
     int32_t* __restrict__ cum_row, float* __restrict__ part_o, float* __restrict__ part_ml, int b,
-    int Hq, int Hkv, int ps, int max_pages, int num_pages, int W, float scale_log2) {
+    int Hq, int Hkv, int max_pages, int num_pages, int W, float scale_log2) {
   constexpr int DT = D / 16, KS = D / 32, K2 = D / 64;
+  constexpr int ps = PS, tshift = PS == 128 ? 1 : 0;   // log2(64-key tiles per page)
   const int w = blockIdx.x;
   const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
   // row plan: up to 64 rows each wave forms it in its lanes (lane r holds row
@@ -88,7 +99,9 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
   long gt = decode_wave_begin(w, T, W);
   const long gt_end = decode_wave_begin(w + 1, T, W);
   const int grp = Hq / Hkv;
-  const int tshift = ps == 128 ? 1 : 0;   // log2(64-key tiles per page)
+  // the lane's place in a tile of codes, K (key, dim) and V^T (dim, key)
+  const unsigned koff = static_cast<unsigned>((16 * (c >> 2) + (c & 3)) * D + 16 * g);
+  const unsigned voff = static_cast<unsigned>(c * ps + 16 * g);
 
   // row of the first tile: the largest r with Hkv * cum_row[r] <= gt
   int bi = 0;
@@ -185,19 +198,16 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
       };
       uint4 kf[4][K2], vf[DT];
       auto load_k = [&](const Slot8& sl) __attribute__((always_inline)) {
-        const uint8_t* base = kp + (sl.blk * ps + sl.k0) * D;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(kp + (sl.blk * ps + sl.k0) * D);
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-          for (int s = 0; s < K2; ++s)
-            kf[kt][s] = *reinterpret_cast<const uint4*>(
-                base + static_cast<unsigned>((16 * (c >> 2) + 4 * kt + (c & 3)) * D + 64 * s + 16 * g));
+          for (int s = 0; s < K2; ++s) kf[kt][s] = buf_load16<true>(r, koff + (4 * kt * D + 64 * s));
       };
       auto load_v = [&](const Slot8& sl) __attribute__((always_inline)) {
-        const uint8_t* base = vp + sl.blk * ps * D + sl.k0;
+        const __amdgpu_buffer_rsrc_t r = make_rsrc(vp + sl.blk * ps * D + sl.k0);
 #pragma unroll
-        for (int t = 0; t < DT; ++t)
-          vf[t] = *reinterpret_cast<const uint4*>(base + static_cast<unsigned>((16 * t + c) * ps + 16 * g));
+        for (int t = 0; t < DT; ++t) vf[t] = buf_load16<PS == 64>(r, voff + 16 * t * ps);
       };
       Slot8 cur = slot_of(r0);
       load_k(cur);
@@ -246,16 +256,14 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
       if (page < 0 || page >= num_pages) continue;   // wave-uniform
       const int k0 = (t & tshift) * 64, nk = min(64, n - 64 * t);
       const long tail = (static_cast<long>(bi) * Hkv + kvh) * ps * D;
-      const bf16* kb = kt_p + tail + k0 * D;
-      const bf16* vb = vt_p + tail + k0;
+      const __amdgpu_buffer_rsrc_t kb = make_rsrc(kt_p + tail + k0 * D), vb = make_rsrc(vt_p + tail + k0);
       v4f sc[4];
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
         sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks)
-          sc[kt] = mfma_bf16(load_v8bf(kb + (16 * (c >> 2) + 4 * kt + (c & 3)) * D + 64 * (ks >> 1) +
-                                       16 * g + 8 * (ks & 1)),
+          sc[kt] = mfma_bf16(buf_load_v8bf(kb, 2 * koff + 2 * (4 * kt * D + 64 * (ks >> 1) + 8 * (ks & 1)), 0),
                              qf[ks], sc[kt]);
       }
       uint32_t keep[4];
@@ -272,7 +280,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
         const v8bf pb = pack_p(sc[2 * h], sc[2 * h + 1]);
 #pragma unroll
         for (int tt = 0; tt < DT; ++tt) {
-          uint4 x = *reinterpret_cast<const uint4*>(vb + (16 * tt + c) * ps + 16 * g + 8 * h);
+          uint4 x = buf_load16<false>(vb, 2 * voff + 16 * h + 32 * tt * ps);
           x = uint4{x.x & km[4 * h], x.y & km[4 * h + 1], x.z & km[4 * h + 2], x.w & km[4 * h + 3]};
           acc[tt] = mfma_bf16(__builtin_bit_cast(v8bf, x), pb, acc[tt]);
         }
@@ -295,12 +303,88 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
   }
 }
 
-int fp8_wave_count(int head_dim, bool bias) {
-  if (head_dim == 128)
-    return bias ? decode_waves(paged_decode_fp8_kernel<128, true>, 4)
-                : decode_waves(paged_decode_fp8_kernel<128, false>, 5);
-  return bias ? decode_waves(paged_decode_fp8_kernel<64, true>, 6)
-              : decode_waves(paged_decode_fp8_kernel<64, false>, 7);
+// Joins the segments of one (batch row, query head): sum_s w_s o_s / sum_s w_s l_s,
+// w_s = 2^(m_s - max m), in the order of the segments whatever the launch.  A step
+// behind the stream-K launch with little data, so latency is what counts: four
+// waves, each a quarter of the segments with eight loads in flight (attention of 1
+// row of 32000 keys, 8 heads of 128, 256 segments a head: 42 us with one wave a
+// head, as the bf16 cache's merge has it, 24 so; 4 rows of 6600, 16 heads of 64:
+// 22.9 and 20).
+template <int D>
+__global__ __launch_bounds__(256) void paged_decode_fp8_merge_kernel(
+    const float* __restrict__ part_o, const float* __restrict__ part_ml,
+    const int32_t* __restrict__ cum_row, bf16* __restrict__ o, int b, int Hq, int Hkv, int W) {
+  constexpr int SPW = 128 / D;   // segments a wave takes at once, two dims a lane
+  constexpr int kMergeSegs = 512;   // segments whose weights stand in LDS at once
+  __shared__ float wsh[kMergeSegs];
+  __shared__ float red[4][128];
+  __shared__ float lred[4];
+  const int qh = blockIdx.x % Hq, bi = blockIdx.x / Hq;
+  const int grp = Hq / Hkv, kvh = qh / grp, qi = qh % grp;
+  const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6;
+  bf16* orow = o + (static_cast<long>(bi) * Hq + qh) * D;
+  const int c0 = cum_row[bi], tb = cum_row[bi + 1] - c0;
+  if (tb <= 0) {   // no keys
+    if (2 * tid < D) *reinterpret_cast<uint32_t*>(orow + 2 * tid) = 0u;
+    return;
+  }
+  const long T = static_cast<long>(Hkv) * cum_row[b];
+  W = static_cast<int>(min(static_cast<long>(W), T));   // as in the decode kernel
+  const long g0 = static_cast<long>(Hkv) * c0 + static_cast<long>(kvh) * tb;
+  const int w0 = decode_wave_of(g0, T, W), nseg = decode_wave_of(g0 + tb - 1, T, W) - w0 + 1;
+  const long slot0 = static_cast<long>(bi) * Hkv + kvh + w0;
+  auto ml_of = [&](int s) { return *reinterpret_cast<const float2*>(part_ml + ((slot0 + s) * grp + qi) * 2); };
+  float M = kNegInf;
+  for (int s = lane; s < nseg; s += 64) M = fmaxf(M, ml_of(s).x);
+  M = wave_max(M);   // every wave for itself
+  float L = 0.0f, a0 = 0.0f, a1 = 0.0f;
+  const int half = lane / (D / 2), d = 2 * (lane % (D / 2));
+  for (int s0 = 0; s0 < nseg; s0 += kMergeSegs) {
+    const int ns = min(kMergeSegs, nseg - s0);
+    if (s0 > 0) __syncthreads();
+    for (int s = tid; s < ns; s += 256) {
+      const float2 ml = ml_of(s0 + s);
+      const float w = ml.x == kNegInf ? 0.0f : fast_exp2(ml.x - M);
+      wsh[s] = w;
+      L += w * ml.y;
+    }
+    __syncthreads();
+#pragma unroll 8
+    for (int s = SPW * wid + half; s < ns; s += 4 * SPW) {
+      const float2 v = *reinterpret_cast<const float2*>(part_o + ((slot0 + s0 + s) * grp + qi) * D + d);
+      a0 = fmaf(wsh[s], v.x, a0);
+      a1 = fmaf(wsh[s], v.y, a1);
+    }
+  }
+  L = wave_sum(L);
+  if (lane == 0) lred[wid] = L;
+  if constexpr (SPW == 2) {
+    a0 += __shfl_xor(a0, 32, 64);
+    a1 += __shfl_xor(a1, 32, 64);
+  }
+  if (half == 0) *reinterpret_cast<float2*>(&red[wid][d]) = make_float2(a0, a1);
+  __syncthreads();
+  if (2 * tid < D) {
+    const float l = (lred[0] + lred[1]) + (lred[2] + lred[3]);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    const float2 r0 = *reinterpret_cast<const float2*>(&red[0][2 * tid]), r1 = *reinterpret_cast<const float2*>(&red[1][2 * tid]);
+    const float2 r2 = *reinterpret_cast<const float2*>(&red[2][2 * tid]), r3 = *reinterpret_cast<const float2*>(&red[3][2 * tid]);
+    *reinterpret_cast<uint32_t*>(orow + 2 * tid) =
+        pack_bf16x2(((r0.x + r1.x) + (r2.x + r3.x)) * inv, ((r0.y + r1.y) + (r2.y + r3.y)) * inv);
+  }
+}
+
+// the kernel for these sizes, and its number among the eight
+template <typename F>
+auto with_fp8_kernel(int head_dim, int page_size, bool bias, F f) {
+  if (head_dim == 128) {
+    if (page_size == 64)
+      return bias ? f(paged_decode_fp8_kernel<128, true, 64>, 0) : f(paged_decode_fp8_kernel<128, false, 64>, 1);
+    return bias ? f(paged_decode_fp8_kernel<128, true, 128>, 2) : f(paged_decode_fp8_kernel<128, false, 128>, 3);
+  }
+  if (page_size == 64)
+    return bias ? f(paged_decode_fp8_kernel<64, true, 64>, 4) : f(paged_decode_fp8_kernel<64, false, 64>, 5);
+  return bias ? f(paged_decode_fp8_kernel<64, true, 128>, 6) : f(paged_decode_fp8_kernel<64, false, 128>, 7);
 }
 
 }  // namespace
@@ -327,25 +411,30 @@ extern "C" int sa_paged_decode_fp8_fwd(
                                            sa::kDecodeMaxWaves, workspace, &ws);
   SA_CHECK_ARG(workspace_bytes >= need, "%s: workspace %zu B < %zu B", who, workspace_bytes, need);
   if (batch == 0) return 0;
-  const int W = sa::fp8_wave_count(head_dim, key_bias != nullptr);
+  const int W = sa::with_fp8_kernel(head_dim, page_size, key_bias != nullptr,
+                                    [](auto kern, int i) { return sa::decode_waves(kern, i); });
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(static_cast<float>(head_dim));
   hipStream_t s = static_cast<hipStream_t>(stream);
   if (const int rc = sa::decode_plan_launch(seq_lens, batch, page_size, max_pages, ws, s)) return rc;
   {
     sa::ProfScope prof_("paged_decode_fp8", s);
-    auto launch = [&](auto kern) {
+    sa::with_fp8_kernel(head_dim, page_size, key_bias != nullptr, [&](auto kern, int) {
       hipLaunchKernelGGL(kern, dim3(W), dim3(64), 0, s, static_cast<const sa::bf16*>(q),
                          static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages),
                          k_scale, v_scale, static_cast<const sa::bf16*>(k_tail),
                          static_cast<const sa::bf16*>(v_tail), page_table, seq_lens, key_bias,
                          ws.cum_row, ws.part_o, ws.part_ml, batch, num_q_heads, num_kv_heads,
-                         page_size, max_pages, num_pages, W, scale * sa::kLog2e);
-    };
-    if (head_dim == 128)
-      key_bias ? launch(sa::paged_decode_fp8_kernel<128, true>) : launch(sa::paged_decode_fp8_kernel<128, false>);
-    else
-      key_bias ? launch(sa::paged_decode_fp8_kernel<64, true>) : launch(sa::paged_decode_fp8_kernel<64, false>);
+                         max_pages, num_pages, W, scale * sa::kLog2e);
+      return 0;
+    });
     SA_CHECK_LAUNCH("paged_decode_fp8");
   }
-  return sa::decode_merge_launch(batch, num_q_heads, num_kv_heads, head_dim, o, ws, W, s);
+  sa::ProfScope prof_("paged_decode_fp8_merge", s);
+  auto merge = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(batch * num_q_heads), dim3(256), 0, s, ws.part_o, ws.part_ml,
+                       ws.cum_row, static_cast<sa::bf16*>(o), batch, num_q_heads, num_kv_heads, W);
+  };
+  head_dim == 128 ? merge(sa::paged_decode_fp8_merge_kernel<128>) : merge(sa::paged_decode_fp8_merge_kernel<64>);
+  SA_CHECK_LAUNCH("paged_decode_fp8_merge");
+  return 0;
 }

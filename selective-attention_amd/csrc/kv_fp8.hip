@@ -65,68 +65,79 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
 
 // One token per row.  One workgroup per row: the token into the open block
 // (and its gate into the page), and where that was the block's last slot, the
-// block's codes and scales, a wave per (head, keys or values).
+// block's codes and scales, a wave per (head, keys or values) with its block in
+// registers between the maximum and the codes (128 x 128 blocks are read twice).
+// Bound by latency, one chain of length, page, tail and block: 64 rows, 8 heads of
+// 128, 7 us where no row closes a block, 14 where one or all of them do (between
+// events; 12 and 16 with the block read twice).
+template <int D, int PS>
 __global__ __launch_bounds__(1024) void kv_fp8_append_kernel(
     const bf16* __restrict__ k, const bf16* __restrict__ v, const float* __restrict__ log_gate,
-    const int32_t* __restrict__ page_table, int32_t* __restrict__ seq_lens, int heads, int D, int ps,
+    const int32_t* __restrict__ page_table, int32_t* __restrict__ seq_lens, int heads,
     int max_pages, int num_pages, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages,
     float* __restrict__ k_scale, float* __restrict__ v_scale, bf16* k_tail, bf16* v_tail,
     float* gate_pages) {
+  constexpr int NV = PS * D / 8 / 64, NR = NV < 16 ? NV : 16;   // 16-byte pieces a lane; kept
   const int row = blockIdx.x;
   const int t = max(seq_lens[row], 0);
-  const int col = min(t / ps, max_pages - 1), s = t % ps;
+  const int col = min(t / PS, max_pages - 1), s = t % PS;
   const int page = page_table[static_cast<long>(row) * max_pages + col];
   // an invalid id, or a row past its table: the tail alone is written
-  const bool ok = page >= 0 && page < num_pages && t / ps < max_pages;
-  const long tail0 = static_cast<long>(row) * heads * ps * D;
+  const bool ok = page >= 0 && page < num_pages && t / PS < max_pages;
+  const long tail0 = static_cast<long>(row) * heads * PS * D;
   const long page0 = static_cast<long>(ok ? page : 0) * heads;
   for (int e = threadIdx.x; e < heads * D; e += blockDim.x) {
-    const int h = e / D, d = e - h * D;
+    const int h = e / D, d = e % D;
     const long src = static_cast<long>(row) * heads * D + e;
-    const long dst = tail0 + static_cast<long>(h) * ps * D;
-    k_tail[dst + static_cast<long>(s) * D + d] = k[src];
-    v_tail[dst + static_cast<long>(d) * ps + s] = v[src];
+    const long dst = tail0 + static_cast<long>(h) * PS * D;
+    k_tail[dst + s * D + d] = k[src];
+    v_tail[dst + d * PS + s] = v[src];
     if (d == 0 && gate_pages && ok)
-      gate_pages[(page0 + h) * ps + s] = log_gate[static_cast<long>(row) * heads + h];
+      gate_pages[(page0 + h) * PS + s] = log_gate[static_cast<long>(row) * heads + h];
   }
   __syncthreads();   // the row's stores are visible to the whole workgroup
   if (threadIdx.x == 0) seq_lens[row] = t + 1;
-  if (s != ps - 1 || !ok) return;
+  if (s != PS - 1 || !ok) return;
   const int lane = threadIdx.x & 63;
-  const int nv = ps * D / 8;   // 16-byte pieces of a block
   for (int it = threadIdx.x >> 6; it < 2 * heads; it += blockDim.x >> 6) {
     const int h = it >> 1;
     const bool val = it & 1;
-    const uint4* src = reinterpret_cast<const uint4*>((val ? v_tail : k_tail) + tail0 + static_cast<long>(h) * ps * D);
-    uint2* dst = reinterpret_cast<uint2*>((val ? v_pages : k_pages) + (page0 + h) * ps * D);
-    const float* gr = gate_pages ? gate_pages + (page0 + h) * ps : nullptr;
-    // the piece with its dropped tokens at 0: a row of D keys is one token, a
-    // row of ps values one dim
-    auto piece = [&](int i) {
-      uint4 x = src[i];
-      if (gr) {
-        if (!val) {
-          const int tok = 8 * i / D;
-          if (tok != ps - 1 && gr[tok] == -__builtin_inff()) x = uint4{0u, 0u, 0u, 0u};
-        } else {
-          const int tok = 8 * i % ps;
-          uint32_t u[4] = {x.x, x.y, x.z, x.w};
+    const uint4* src = reinterpret_cast<const uint4*>((val ? v_tail : k_tail) + tail0 + static_cast<long>(h) * PS * D);
+    uint2* dst = reinterpret_cast<uint2*>((val ? v_pages : k_pages) + (page0 + h) * PS * D);
+    const float* gr = gate_pages ? gate_pages + (page0 + h) * PS : nullptr;
+    // dropped tokens are 0.  Values: a lane's pieces are all of the same eight
+    // tokens (512 % PS = 0), one mask; keys: a piece is of one token.
+    uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
+    if (gr && val) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (tok + j != ps - 1 && gr[tok + j] == -__builtin_inff())
-              u[j >> 1] &= (j & 1) ? 0x0000ffffu : 0xffff0000u;
-          x = uint4{u[0], u[1], u[2], u[3]};
-        }
+      for (int j = 0; j < 8; ++j) {
+        const int tok = (8 * lane) % PS + j;
+        if (tok != PS - 1 && gr[tok] == -__builtin_inff()) keep[j >> 1] &= (j & 1) ? 0x0000ffffu : 0xffff0000u;
       }
-      return x;
+    }
+    auto mask = [&](const uint4& x, int i) {
+      const int tok = 8 * i / D;
+      const bool dead = gr && !val && tok != PS - 1 && gr[tok] == -__builtin_inff();
+      return dead ? uint4{0u, 0u, 0u, 0u}
+                  : uint4{x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]};
     };
+    uint4 x[NR];
+#pragma unroll
+    for (int i = 0; i < NR; ++i) x[i] = src[lane + 64 * i];
     uint32_t top = 0u;
+#pragma unroll
+    for (int i = 0; i < NR; ++i) {
+      x[i] = mask(x[i], lane + 64 * i);
+      top = max(top, mag_max(x[i]));
+    }
 #pragma unroll 4
-    for (int i = lane; i < nv; i += 64) top = max(top, mag_max(piece(i)));
+    for (int i = NR; i < NV; ++i) top = max(top, mag_max(mask(src[lane + 64 * i], lane + 64 * i)));
     const int e = block_exp(wave_umax(top) << 16);
     const float inv = pow2f(-e);
+#pragma unroll
+    for (int i = 0; i < NR; ++i) dst[lane + 64 * i] = encode8(x[i], inv);
 #pragma unroll 4
-    for (int i = lane; i < nv; i += 64) dst[i] = encode8(piece(i), inv);
+    for (int i = NR; i < NV; ++i) dst[lane + 64 * i] = encode8(mask(src[lane + 64 * i], lane + 64 * i), inv);
     if (lane == 0) (val ? v_scale : k_scale)[page0 + h] = pow2f(e);
   }
 }
@@ -262,12 +273,17 @@ extern "C" int sa_paged_kv_append_fp8(const void* k, const void* v, const float*
   if (batch == 0) return 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   sa::ProfScope prof_("kv_fp8_append", s);
-  hipLaunchKernelGGL(sa::kv_fp8_append_kernel, dim3(batch), dim3(1024), 0, s,
-                     static_cast<const sa::bf16*>(k), static_cast<const sa::bf16*>(v), log_gate,
-                     page_table, seq_lens, heads, head_dim, page_size, max_pages, num_pages,
-                     static_cast<uint8_t*>(k_pages), static_cast<uint8_t*>(v_pages), k_scale,
-                     v_scale, static_cast<sa::bf16*>(k_tail), static_cast<sa::bf16*>(v_tail),
-                     gate_pages);
+  auto launch = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3(batch), dim3(1024), 0, s, static_cast<const sa::bf16*>(k),
+                       static_cast<const sa::bf16*>(v), log_gate, page_table, seq_lens, heads,
+                       max_pages, num_pages, static_cast<uint8_t*>(k_pages),
+                       static_cast<uint8_t*>(v_pages), k_scale, v_scale,
+                       static_cast<sa::bf16*>(k_tail), static_cast<sa::bf16*>(v_tail), gate_pages);
+  };
+  if (head_dim == 64)
+    page_size == 64 ? launch(sa::kv_fp8_append_kernel<64, 64>) : launch(sa::kv_fp8_append_kernel<64, 128>);
+  else
+    page_size == 64 ? launch(sa::kv_fp8_append_kernel<128, 64>) : launch(sa::kv_fp8_append_kernel<128, 128>);
   SA_CHECK_LAUNCH("kv_fp8_append");
   return 0;
 }
