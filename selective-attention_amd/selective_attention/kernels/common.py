@@ -61,3 +61,23 @@ def call_on(t: torch.Tensor, name: str, *args) -> None:
 def limits(delta_limit) -> tuple[float, float]:
     lo, hi = float(delta_limit[0]), float(delta_limit[1])
     return lo, hi
+
+
+def needs_torch_ops(*ts: torch.Tensor) -> bool:
+    """Whether something has to see torch's own ops on ts, which a kernel launch
+    hides or cannot serve: forward-mode AD, a dispatch mode, tracing, a functorch
+    transform, or a legacy batched tensor (is_grads_batched)."""
+    return (torch._C._are_functorch_transforms_active()
+            or torch.autograd.forward_ad._current_level >= 0
+            or torch._C._len_torch_dispatch_stack() > 0
+            or torch.compiler.is_compiling() or torch.jit.is_tracing()
+            # (on the tensors too: a GPU backward runs on a thread of its own)
+            or any(torch._C._functorch.is_functorch_wrapped_tensor(t)
+                   or torch._C._functorch.is_legacy_batchedtensor(t) for t in ts))
+
+
+def in_forward_mode() -> bool:
+    """Whether a dual level of forward-mode AD is open: a kernel launch would drop
+    the tangents without a word.  (Wrapped and batched tensors refuse the launch
+    by themselves, having no address.)"""
+    return torch.autograd.forward_ad._current_level >= 0

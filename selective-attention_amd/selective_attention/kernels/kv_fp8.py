@@ -8,6 +8,8 @@ behind its last full page) stays in bfloat16 until it is full.
 """
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -17,6 +19,11 @@ from .common import call_on, require_one_device
 FP8 = torch.float8_e4m3fn
 PAGE_SIZES = (64, 128)
 HEAD_DIMS = (64, 128)
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(b, Hq, Hkv, D, max_pages):
+    return _lib.load().sa_paged_decode_workspace_size(b, Hq, Hkv, D, max_pages)
 
 
 def _check_cache(who, batch, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail, page_table,
@@ -31,19 +38,31 @@ def _check_cache(who, batch, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
                          f"of {HEAD_DIMS}")
     if n == 0 or H == 0:
         raise ValueError(f"{who}: empty page pool")
-    want = [("k_pages", k_pages, (n, H, ps, D), FP8), ("v_pages", v_pages, (n, H, D, ps), FP8),
-            ("k_scale", k_scale, (n, H), torch.float32), ("v_scale", v_scale, (n, H), torch.float32),
-            ("k_tail", k_tail, (batch, H, ps, D), torch.bfloat16),
-            ("v_tail", v_tail, (batch, H, D, ps), torch.bfloat16)]
-    if gate_pages is not None:
-        want.append(("gate_pages" if written else "key_bias", gate_pages, (n, H, ps), torch.float32))
-    for name, t, shape, dtype in want:
-        if t.shape != shape:
-            raise ValueError(f"{who}: {name} must be {shape}, got {tuple(t.shape)}")
-        if t.dtype != dtype:
-            raise TypeError(f"{who}: {name} must be {dtype}, got {t.dtype}")
-        if not t.is_contiguous() or t.data_ptr() % 16:
-            raise ValueError(f"{who}: {name} must be contiguous on a 16-byte boundary")
+    # (one plain chain where all is well: a loop over names costs more than a launch)
+    sh, f32 = (n, H), torch.float32
+    gates_ok = gate_pages is None or (gate_pages.shape == (n, H, ps) and gate_pages.dtype == f32
+                                      and gate_pages.is_contiguous() and not gate_pages.data_ptr() % 16)
+    if not (gates_ok and v_pages.shape == (n, H, D, ps) and k_scale.shape == sh == v_scale.shape
+            and k_tail.shape == (batch, H, ps, D) and v_tail.shape == (batch, H, D, ps)
+            and k_pages.dtype == FP8 == v_pages.dtype and k_scale.dtype == f32 == v_scale.dtype
+            and k_tail.dtype == torch.bfloat16 == v_tail.dtype
+            and k_pages.is_contiguous() and v_pages.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous() and k_tail.is_contiguous() and v_tail.is_contiguous()
+            and not (k_pages.data_ptr() | v_pages.data_ptr() | k_scale.data_ptr()
+                     | v_scale.data_ptr() | k_tail.data_ptr() | v_tail.data_ptr()) % 16):
+        want = [("k_pages", k_pages, (n, H, ps, D), FP8), ("v_pages", v_pages, (n, H, D, ps), FP8),
+                ("k_scale", k_scale, sh, f32), ("v_scale", v_scale, sh, f32),
+                ("k_tail", k_tail, (batch, H, ps, D), torch.bfloat16),
+                ("v_tail", v_tail, (batch, H, D, ps), torch.bfloat16)]
+        if gate_pages is not None:
+            want.append(("gate_pages" if written else "key_bias", gate_pages, (n, H, ps), f32))
+        for name, t, shape, dtype in want:
+            if t.shape != shape:
+                raise ValueError(f"{who}: {name} must be {shape}, got {tuple(t.shape)}")
+            if t.dtype != dtype:
+                raise TypeError(f"{who}: {name} must be {dtype}, got {t.dtype}")
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                raise ValueError(f"{who}: {name} must be contiguous on a 16-byte boundary")
     if page_table.dim() != 2 or page_table.shape[0] != batch:
         raise ValueError(f"{who}: page_table must be ({batch}, max_pages), got {tuple(page_table.shape)}")
     return n, H, ps, D
@@ -81,14 +100,16 @@ def paged_decode_attn_fp8(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
     q = _rows16(q)
     pt, sl = _i32(page_table), _i32(seq_lens)
     max_pages = pt.shape[1]
-    nbytes = _lib.load().sa_paged_decode_workspace_size(b, Hq, Hkv, D, max_pages)
+    if b == 0 or max_pages == 0:
+        return torch.zeros_like(q)   # no row has a key
+    nbytes = _workspace_bytes(b, Hq, Hkv, D, max_pages)
     ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=q.device)
     o = torch.empty_like(q)
     scale = -1.0 if softmax_scale is None else float(softmax_scale)
-    call_on(q, "sa_paged_decode_fp8_fwd", _lib.ptr(q), _lib.ptr(k_pages), _lib.ptr(v_pages),
-              _lib.ptr(k_scale), _lib.ptr(v_scale), _lib.ptr(k_tail), _lib.ptr(v_tail),
-              _lib.ptr(pt), _lib.ptr(sl), _lib.ptr(key_bias), b, Hq, Hkv, D, ps, max_pages, n,
-              scale, _lib.ptr(o), _lib.ptr(ws), nbytes, _lib.stream_of(q))
+    call_on(q, "sa_paged_decode_fp8_fwd", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
+            k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
+            pt.data_ptr(), sl.data_ptr(), _lib.ptr(key_bias), b, Hq, Hkv, D, ps, max_pages, n,
+            scale, o.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(q))
     return o
 
 
@@ -119,12 +140,14 @@ def paged_kv_append_fp8(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, 
     _lens_and_table(who, page_table, seq_lens, b)
     require_one_device(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale, v_scale,
                    k_tail, v_tail, gate_pages)
+    if b == 0:
+        return
     k, v = _dense(k, torch.bfloat16), _dense(v, torch.bfloat16)
     lg = None if log_gate is None else _dense(log_gate, torch.float32)
-    call_on(k, "sa_paged_kv_append_fp8", _lib.ptr(k), _lib.ptr(v), _lib.ptr(lg),
-              _lib.ptr(page_table), _lib.ptr(seq_lens), b, H, D, ps, page_table.shape[1], n,
-              _lib.ptr(k_pages), _lib.ptr(v_pages), _lib.ptr(k_scale), _lib.ptr(v_scale),
-              _lib.ptr(k_tail), _lib.ptr(v_tail), _lib.ptr(gate_pages), _lib.stream_of(k))
+    call_on(k, "sa_paged_kv_append_fp8", k.data_ptr(), v.data_ptr(), _lib.ptr(lg),
+            page_table.data_ptr(), seq_lens.data_ptr(), b, H, D, ps, page_table.shape[1], n,
+            k_pages.data_ptr(), v_pages.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+            k_tail.data_ptr(), v_tail.data_ptr(), _lib.ptr(gate_pages), _lib.stream_of(k))
 
 
 def paged_kv_build_fp8(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale, v_scale,

@@ -82,7 +82,8 @@ class CausalLM(nn.Module):
         """Every linear layer and the head to 4-bit weights (Int4Linear), in place,
         for inference in bfloat16; the embedding keeps its own table."""
         quantize_linears(self.layers, group_size, symmetric)
-        self.lm_head = Int4Linear.from_linear(self.lm_head, group_size, symmetric)
+        if isinstance(self.lm_head, nn.Linear):
+            self.lm_head = Int4Linear.from_linear(self.lm_head, group_size, symmetric)
         return self
 
     def _hidden(self, input_ids, lengths=None, attn_gate_thresholds=None, cache=None):

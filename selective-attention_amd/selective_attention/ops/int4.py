@@ -17,6 +17,7 @@ import torch
 import torch.nn.functional as F
 
 from ..kernels import int4 as _k
+from ..kernels.common import in_forward_mode
 from ..kernels.int4 import MAX_MATRICES, MAX_ROWS
 from ..utils import check_ndim, check_shape
 
@@ -139,7 +140,7 @@ def int4_linear_multi(x: torch.Tensor, weights, biases, sizes,
                 raise TypeError(f"int4_linear: bias must be bfloat16, got {b.dtype}")
     grad = torch.is_grad_enabled() and (
         x.requires_grad or (xscale is not None and xscale.requires_grad)
-        or any(b is not None and b.requires_grad for b in biases))
+        or any(b is not None and b.requires_grad for b in biases)) or in_forward_mode()
     rows = x.numel() // K
     if rows == 0:
         return [x.new_empty(*x.shape[:-1], N) for N in sizes]

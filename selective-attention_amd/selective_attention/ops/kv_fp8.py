@@ -7,6 +7,8 @@ any launch.
 """
 from __future__ import annotations
 
+import math
+
 import torch
 
 from ..kernels import kv_fp8 as _k
@@ -18,15 +20,18 @@ def paged_decode_attn_fp8(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch
                           v_tail: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
                           softmax_scale: float | None = None,
                           key_bias: torch.Tensor | None = None) -> torch.Tensor:
-    check_ndim(q, 3, name="q")
+    if q.dim() != 3 or k_pages.dim() != 4:
+        check_ndim(q, 3, name="q")
+        check_ndim(k_pages, 4, name="k_pages")
     b, Hq, D = q.shape
-    check_ndim(k_pages, 4, name="k_pages")
     Hkv = k_pages.shape[1]
     if k_pages.shape[3] != D:
         raise ValueError(f"[k_pages] Shape mismatch: expected head_dim {D}, got {k_pages.shape[3]}")
     if Hkv == 0 or Hq % Hkv or Hq // Hkv > 16:
         raise ValueError(f"num_q_heads {Hq} must be a multiple of num_kv_heads {Hkv}, at most 16 times it")
     check_shape(seq_lens, (b,), name="seq_lens")
+    if softmax_scale is not None and not 0.0 < softmax_scale < math.inf:
+        raise ValueError(f"softmax_scale must be positive and finite, got {softmax_scale}")
     return _k.paged_decode_attn_fp8(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
                                     page_table, seq_lens, softmax_scale, key_bias)
 

@@ -13,6 +13,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from ..kernels import logprobs as _k
+from ..kernels.common import in_forward_mode, needs_torch_ops
 from ..utils import check_shape
 
 
@@ -39,6 +40,9 @@ class TokenLogprobsFn(torch.autograd.Function):
         logits, targets, H, stats, ids = ctx.saved_tensors
         if g_lp is None and g_h is None and g_top is None:
             return None, None, None, None
+        if needs_torch_ops(*(g for g in (g_lp, g_h, g_top) if g is not None)):
+            raise RuntimeError("token_logprobs: the backward takes plain upstream gradients (no "
+                               "batched ones, transforms or forward mode)")
         dx = _k.token_logprobs_backward(logits, targets, ctx.top, ctx.ignore_index, H, stats, ids,
                                         g_lp, g_h, g_top)
         return dx, None, None, None
@@ -69,7 +73,7 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
         raise ValueError(f"token_logprobs: top {top} must be 0..{_k.MAX_TOP} and at most the "
                          f"vocabulary {logits.shape[-1]}")
     top, ignore_index = int(top), int(ignore_index)
-    if torch.is_grad_enabled() and logits.requires_grad:
+    if (torch.is_grad_enabled() and logits.requires_grad) or in_forward_mode():
         return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets, top, ignore_index))
     lp, H, _, ids, tl = _k.token_logprobs_forward(logits, targets, top, ignore_index)
     return TokenLogprobs(lp, H, ids, tl)

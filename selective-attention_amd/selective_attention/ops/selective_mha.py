@@ -37,7 +37,7 @@ from ..kernels.attention import (TRAIN_HEAD_DIMS, gated_attn_train_backward,
                                  gated_attn_train_forward, mha_prefill, score_moments,
                                  score_std_backward)
 from ..kernels import kv_fp8 as _kv8
-from ..kernels.common import require_device
+from ..kernels.common import needs_torch_ops, require_device
 from ..kernels.lm_ops import paged_kv_append, paged_kv_build
 from ..utils import check_ndim, check_shape
 from . import kv_fp8 as _kv8_ops
@@ -81,7 +81,7 @@ class ScoreStdFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         q, k, stats = ctx.saved_tensors
-        if torch.is_grad_enabled() or _needs_torch_ops(g):   # torch ops by query chunks
+        if torch.is_grad_enabled() or needs_torch_ops(g):   # torch ops by query chunks
             dq, dk = _score_std_backward_dense(q, k, stats, g, ctx)
         else:
             dq, dk = score_std_backward(q, k, ctx.q_lengths, ctx.k_lengths, ctx.causal, stats, g)
@@ -124,19 +124,6 @@ def _gated_attention_dense(q, k, v, log_gate, causal):
     return torch.matmul(torch.softmax(s, dim=-1), v)
 
 
-def _needs_torch_ops(*ts: torch.Tensor) -> bool:
-    """Whether something has to see torch's own ops on ts, which a kernel launch
-    hides or cannot serve: forward-mode AD, a dispatch mode, tracing, a functorch
-    transform, or a legacy batched tensor (is_grads_batched)."""
-    return (torch._C._are_functorch_transforms_active()
-            or torch.autograd.forward_ad._current_level >= 0
-            or torch._C._len_torch_dispatch_stack() > 0
-            or torch.compiler.is_compiling() or torch.jit.is_tracing()
-            # (on the tensors too: a GPU backward runs on a thread of its own)
-            or any(torch._C._functorch.is_functorch_wrapped_tensor(t)
-                   or torch._C._functorch.is_legacy_batchedtensor(t) for t in ts))
-
-
 class GatedAttnTrainFn(torch.autograd.Function):
     """gated_attention_train on the fp32 MFMA kernels.  A backward that is itself
     recorded (create_graph), batched over upstream gradients or in forward mode
@@ -153,7 +140,7 @@ class GatedAttnTrainFn(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, log_gate, out, stats = ctx.saved_tensors
         recorded = torch.is_grad_enabled()
-        if recorded or _needs_torch_ops(dout):
+        if recorded or needs_torch_ops(dout):
             need = ctx.needs_input_grad[:4]
             # aliases of their own: where one input was made from another, the
             # derivative with respect to the inputs themselves would hold that
@@ -180,7 +167,7 @@ def _train_kernel_ok(q, k, v, log_gate) -> bool:
             and q.shape[-1] in TRAIN_HEAD_DIMS and 0 < q.numel()
             and q.shape[0] * q.shape[1] * ((q.shape[2] + 63) // 64) < 2 ** 31
             and not torch.is_autocast_enabled("cuda")
-            and not _needs_torch_ops(*ts))
+            and not needs_torch_ops(*ts))
 
 
 def gated_attention_train(q_rot, k_rot, v, log_gate, causal=True):

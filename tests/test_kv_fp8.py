@@ -210,7 +210,8 @@ def test_append_and_build_refuse(what):
         build(k4, k4, None if lg is None else lg[..., None].expand(-1, -1, 5), table, lens, c)
 
 
-@pytest.mark.parametrize("what", ["heads", "group", "dtype", "D", "bias", "lens", "scale", "cpu"])
+@pytest.mark.parametrize("what", ["heads", "group", "dtype", "D", "bias", "lens", "scale",
+                                  "softmax", "cpu"])
 def test_attention_refuses(what):
     table, lens, c = _args()
     q = torch.zeros(2, 4, 64, dtype=torch.bfloat16)
@@ -228,8 +229,9 @@ def test_attention_refuses(what):
         lens = torch.zeros(3, dtype=torch.int32)
     elif what == "scale":
         c["v_scale"] = c["v_scale"][:, :1]
+    kw = dict(softmax_scale=0.0) if what == "softmax" else {}
     with pytest.raises((ValueError, TypeError)):
-        attend(q, c, table, lens)
+        attend(q, c, table, lens, **kw)
 
 
 # --- the writes ------------------------------------------------------------------
@@ -448,6 +450,31 @@ def test_masked_places_hold_anything(D, ps):
     # the refs round page 0 of row 0 anew without its gates, which takes no part
     check_attention(o0, q[:1], rows[:1], lens[:1])
     assert torch.equal(got[2], clean[2])
+
+
+@pytest.mark.gpu
+def test_no_rows_and_no_pages():
+    table, c = make_cache(2, 2, 64, 64, 2, True, "cuda")
+    z = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device="cuda")
+    i32 = dict(dtype=torch.int32, device="cuda")
+    empty = dict(c, k_tail=c["k_tail"][:0], v_tail=c["v_tail"][:0])
+    assert attend(z, empty, table[:0], torch.zeros(0, **i32)).shape == (0, 2, 64)
+    append(z, z, torch.zeros(0, 2, device="cuda"), table[:0], torch.zeros(0, **i32), empty)
+    q = torch.ones(2, 2, 64, dtype=torch.bfloat16, device="cuda")
+    assert not attend(q, c, table[:, :0], torch.zeros(2, **i32)).any()
+
+
+@pytest.mark.gpu
+def test_other_index_types_and_strides_of_q():
+    """int64 lengths and tables, q as a transposed view: the same answer."""
+    b, H, D, ps = 2, 4, 64, 64
+    k, v, lg = tokens(b, H, 100, D, True, seed=13, spread=False)
+    table, c = make_cache(b, H, D, ps, 2, True, "cuda")
+    sl = torch.tensor([100, 70], dtype=torch.int32, device="cuda")
+    build(k.cuda(), v.cuda(), lg.cuda(), table, sl, c)
+    q = torch.randn(b, H, D, device="cuda").to(torch.bfloat16)
+    want = attend(q, c, table, sl)
+    assert torch.equal(attend(q.transpose(0, 1).contiguous().transpose(0, 1), c, table.long(), sl.long()), want)
 
 
 @pytest.mark.gpu

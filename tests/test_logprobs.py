@@ -289,6 +289,12 @@ def test_targets_outside_give_no_number_and_double_backward_is_refused():
     with pytest.raises(RuntimeError):
         torch.autograd.grad(d.sum(), leaf)
     assert not token_logprobs(x.cuda(), t.cuda()).logprob.requires_grad
+    out = token_logprobs(leaf, t.cuda())
+    with pytest.raises(RuntimeError):     # batched upstream gradients
+        torch.autograd.grad(out.logprob, leaf, torch.eye(3, device="cuda"), is_grads_batched=True)
+    import torch.autograd.forward_ad as fwd
+    with pytest.raises(RuntimeError), fwd.dual_level():
+        token_logprobs(fwd.make_dual(x.cuda(), torch.ones_like(x).cuda()), t.cuda())
 
 
 @pytest.mark.gpu
