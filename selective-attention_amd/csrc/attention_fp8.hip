@@ -13,7 +13,8 @@
 // The split is stream-K over 64-key tiles, as in the bf16 decode (attention.hip):
 // one resident round of W one-wave workgroups, each the same number of tiles
 // of the (row, kv head, tile) list, partial sums joined by the merge kernel.
-// What differs is the tile: 64 D codes are a quarter to a half of the
+// Short tables take one workgroup a (row, kv head) instead and need no merge.
+// What differs from the bf16 cache is the tile: 64 D codes are a quarter to a half of the
 // registers of the bf16 tile, widened to bf16 MFMA operands right before
 // their product (v_cvt_scalef32_pk_bf16_fp8, two codes an instruction, which
 // multiplies by the block's power of two on the way: exact, every e4m3 number
@@ -28,6 +29,8 @@
 #include "common.h"
 #include "decode.h"
 #include "prof.h"
+
+#include <type_traits>
 
 namespace sa {
 namespace {
@@ -59,16 +62,195 @@ struct Slot8 {
   float ks, vs;      // the block's scales
 };
 
-template <int D, bool BIAS, int PS>
-__global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
-    const bf16* __restrict__ q, const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp,
-    const float* __restrict__ ksc, const float* __restrict__ vsc, const bf16* __restrict__ kt_p,
-    const bf16* __restrict__ vt_p, const int32_t* __restrict__ page_table,
-    const int32_t* __restrict__ seq_lens, const float* __restrict__ key_bias,
-    int32_t* __restrict__ cum_row, float* __restrict__ part_o, float* __restrict__ part_ml, int b,
-    int Hq, int Hkv, int max_pages, int num_pages, int W, float scale_log2) {
+struct Fp8Cache {
+  const uint8_t *k, *v;
+  const float *k_scale, *v_scale;
+  const bf16 *k_tail, *v_tail;
+  const int32_t* page_table;
+  const float* bias;
+  int Hkv, max_pages, num_pages;
+};
+
+// One wave over the tiles t_begin, t_begin + S, ... < t_end of the n keys of (row
+// bi, kv head kvh): its sums O^T (acc), their reference m and weight l, for the
+// query heads in qf, those of columns c < grp.
+template <int D, bool BIAS, int PS, int S>
+__device__ __forceinline__ void row_tiles(const Fp8Cache& kv, int bi, int kvh, int n, int t_begin, int t_end,
+                                          int grp, float scale_log2, const v8bf (&qf)[D / 32],
+                                          v4f (&acc)[D / 16], float& m, float& l) {
   constexpr int DT = D / 16, KS = D / 32, K2 = D / 64;
   constexpr int ps = PS, tshift = PS == 128 ? 1 : 0;   // log2(64-key tiles per page)
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const int Hkv = kv.Hkv, num_pages = kv.num_pages;
+  const float* key_bias = kv.bias;
+  // the lane's place in a tile of codes, K (key, dim) and V^T (dim, key)
+  const unsigned koff = static_cast<unsigned>((16 * (c >> 2) + (c & 3)) * D + 16 * g);
+  const unsigned voff = static_cast<unsigned>(c * ps + 16 * g);
+  const int t_open = (n / ps) << tshift;   // first tile of the open block
+  const int t_close = min(t_end, t_open);
+  const int32_t* prow = kv.page_table + static_cast<long>(bi) * kv.max_pages;
+
+  // scale, bias (not on the newest key) and mask of the score tiles; entry
+  // (kt, i) is key 16 g + 4 kt + i of the tile at sequence position pos0.
+  // keep[kt] gets the byte mask of the keys that take part.
+  auto finish = [&](v4f (&sc)[4], const float* brow, int nk, int pos0, uint32_t (&keep)[4])
+                    __attribute__((always_inline)) {
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
+      if constexpr (BIAS) bv = *reinterpret_cast<const float4*>(brow + 16 * g + 4 * kt);
+      const float bs[4] = {bv.x, bv.y, bv.z, bv.w};
+      keep[kt] = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = 16 * g + 4 * kt + i;
+        bool on = key < nk;
+        float val = sc[kt][i] * scale_log2;
+        if constexpr (BIAS) {
+          const bool newest = key == n - 1 - pos0;
+          val = newest ? val : val + bs[i] * kLog2e;
+          on = on && (newest || bs[i] != kNegInf);   // a dropped key counts for nothing, whatever it holds
+        }
+        sc[kt][i] = on && c < grp ? val : kNegInf;
+        keep[kt] |= on ? 0xffu << (8 * i) : 0u;
+      }
+    }
+  };
+
+  // full blocks, in runs of at most 64 pages: lane j holds the id and the
+  // scales of the run's page p0 + j
+  int r0 = t_begin;
+  while (r0 < t_close) {
+    const int p0 = r0 >> tshift;
+    const int r1 = min(t_close, (p0 + 64) << tshift);
+    const int my_page = lane <= ((r1 - 1) >> tshift) - p0 ? prow[p0 + lane] : -1;
+    const bool my_ok = my_page >= 0 && my_page < num_pages;
+    // invalid ids read page 0, which exists, and contribute no keys
+    const long my_blk = static_cast<long>(my_ok ? my_page : 0) * Hkv + kvh;
+    const float my_ks = kv.k_scale[my_blk], my_vs = kv.v_scale[my_blk];
+    auto slot_of = [&](int t) {
+      const int j = (t >> tshift) - p0;
+      const int page = __builtin_amdgcn_readlane(my_page, j);
+      Slot8 sl;
+      sl.ok = page >= 0 && page < num_pages;
+      sl.blk = static_cast<long>(sl.ok ? page : 0) * Hkv + kvh;
+      sl.k0 = (t & tshift) * 64;
+      sl.ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_ks), j));
+      sl.vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_vs), j));
+      return sl;
+    };
+    uint4 kf[4][K2], vf[DT];
+    auto load_k = [&](const Slot8& sl) __attribute__((always_inline)) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(kv.k + (sl.blk * ps + sl.k0) * D);
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int s = 0; s < K2; ++s) kf[kt][s] = buf_load16<true>(r, koff + (4 * kt * D + 64 * s));
+    };
+    auto load_v = [&](const Slot8& sl) __attribute__((always_inline)) {
+      const __amdgpu_buffer_rsrc_t r = make_rsrc(kv.v + sl.blk * ps * D + sl.k0);
+#pragma unroll
+      for (int t = 0; t < DT; ++t) vf[t] = buf_load16<PS == 64>(r, voff + 16 * t * ps);
+    };
+    Slot8 cur = slot_of(r0);
+    load_k(cur);
+    load_v(cur);
+    auto tile = [&](auto more_c, int t, const Slot8& nxt) __attribute__((always_inline)) {
+      constexpr bool kMore = decltype(more_c)::value;
+      v4f sc[4];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) {
+        sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s < K2; ++s) {
+          const uint4 x = kf[kt][s];
+          sc[kt] = mfma_bf16(widen8(x.x, x.y, cur.ks), qf[2 * s], sc[kt]);
+          sc[kt] = mfma_bf16(widen8(x.z, x.w, cur.ks), qf[2 * s + 1], sc[kt]);
+        }
+      }
+      if constexpr (kMore) load_k(nxt);
+      uint32_t keep[4];
+      finish(sc, key_bias + cur.blk * ps + cur.k0, cur.ok ? 64 : 0, 64 * t, keep);
+      softmax_block<4, DT>(sc, acc, m, l);
+      const v8bf p0b = pack_p(sc[0], sc[1]), p1b = pack_p(sc[2], sc[3]);
+      if (cur.ok) {
+#pragma unroll
+        for (int tt = 0; tt < DT; ++tt) {
+          uint4 x = vf[tt];
+          if constexpr (BIAS) x = uint4{x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]};
+          acc[tt] = mfma_bf16(widen8(x.x, x.y, cur.vs), p0b, acc[tt]);
+          acc[tt] = mfma_bf16(widen8(x.z, x.w, cur.vs), p1b, acc[tt]);
+        }
+      }
+      if constexpr (kMore) load_v(nxt);
+    };
+    int t = r0;
+    for (; t + S < r1; t += S) {
+      const Slot8 nxt = slot_of(t + S);
+      tile(BoolC<true>{}, t, nxt);
+      cur = nxt;
+    }
+    tile(BoolC<false>{}, t, cur);
+    r0 = t + S;
+  }
+
+  // the open block, in bf16
+  int t_first = t_begin;
+  if (t_open > t_begin) t_first += (t_open - t_begin + S - 1) / S * S;
+  for (int t = t_first; t < t_end; t += S) {
+    const int page = prow[t >> tshift];
+    if (page < 0 || page >= num_pages) continue;   // wave-uniform
+    const int k0 = (t & tshift) * 64, nk = min(64, n - 64 * t);
+    const long tail = (static_cast<long>(bi) * Hkv + kvh) * ps * D;
+    const __amdgpu_buffer_rsrc_t kb = make_rsrc(kv.k_tail + tail + k0 * D), vb = make_rsrc(kv.v_tail + tail + k0);
+    v4f sc[4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+      sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+        sc[kt] = mfma_bf16(buf_load_v8bf(kb, 2 * koff + 2 * (4 * kt * D + 64 * (ks >> 1) + 8 * (ks & 1)), 0),
+                           qf[ks], sc[kt]);
+    }
+    uint32_t keep[4];
+    finish(sc, key_bias + (static_cast<long>(page) * Hkv + kvh) * ps + k0, nk, 64 * t, keep);
+    softmax_block<4, DT>(sc, acc, m, l);
+    // two keys a word: byte masks to 16-bit masks (slots past nk hold what
+    // the buffer held, NaN perhaps)
+    uint32_t km[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      km[i] = __builtin_amdgcn_perm(0u, keep[i >> 1], (i & 1) ? 0x03030202u : 0x01010000u);
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const v8bf pb = pack_p(sc[2 * h], sc[2 * h + 1]);
+#pragma unroll
+      for (int tt = 0; tt < DT; ++tt) {
+        uint4 x = buf_load16<false>(vb, 2 * voff + 16 * h + 32 * tt * ps);
+        x = uint4{x.x & km[4 * h], x.y & km[4 * h + 1], x.z & km[4 * h + 2], x.w & km[4 * h + 3]};
+        acc[tt] = mfma_bf16(__builtin_bit_cast(v8bf, x), pb, acc[tt]);
+      }
+    }
+  }
+}
+
+// the group's query heads, column c = lane & 15, dims in the order of the K operand
+template <int D>
+__device__ __forceinline__ void load_q(v8bf (&qf)[D / 32], const bf16* q, int grp) {
+  const int lane = threadIdx.x & 63, c = lane & 15, g = lane >> 4;
+  const bf16* row = q + min(c, grp - 1) * D;
+#pragma unroll
+  for (int ks = 0; ks < D / 32; ++ks)
+    qf[ks] = c < grp ? load_v8bf(row + 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)) : zero_v8bf();
+}
+
+template <int D, bool BIAS, int PS>
+__global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
+    const bf16* __restrict__ q, const Fp8Cache kv, const int32_t* __restrict__ seq_lens,
+    int32_t* __restrict__ cum_row, float* __restrict__ part_o, float* __restrict__ part_ml, int b,
+    int Hq, int W, float scale_log2) {
+  constexpr int DT = D / 16, ps = PS;
+  const int Hkv = kv.Hkv, max_pages = kv.max_pages;
   const int w = blockIdx.x;
   const int lane = threadIdx.x, c = lane & 15, g = lane >> 4;
   // row plan: up to 64 rows each wave forms it in its lanes (lane r holds row
@@ -99,9 +281,6 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
   long gt = decode_wave_begin(w, T, W);
   const long gt_end = decode_wave_begin(w + 1, T, W);
   const int grp = Hq / Hkv;
-  // the lane's place in a tile of codes, K (key, dim) and V^T (dim, key)
-  const unsigned koff = static_cast<unsigned>((16 * (c >> 2) + (c & 3)) * D + 16 * g);
-  const unsigned voff = static_cast<unsigned>(c * ps + 16 * g);
 
   // row of the first tile: the largest r with Hkv * cum_row[r] <= gt
   int bi = 0;
@@ -134,158 +313,13 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
     const int t_begin = off - kvh * tb;
     const int t_end = t_begin + static_cast<int>(min(gt_end - gt, static_cast<long>(tb - t_begin)));
     const int n = decode_row_len(seq_lens, bi, max_pages, ps);
-    const int t_open = (n / ps) << tshift;   // first tile of the open block
-    const int t_close = min(t_end, t_open);
-    const int32_t* prow = page_table + static_cast<long>(bi) * max_pages;
-
-    const bf16* qrow = q + (static_cast<long>(bi) * Hq + kvh * grp + min(c, grp - 1)) * D;
-    v8bf qf[KS];
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-      qf[ks] = c < grp ? load_v8bf(qrow + 64 * (ks >> 1) + 16 * g + 8 * (ks & 1)) : zero_v8bf();
+    v8bf qf[D / 32];
+    load_q<D>(qf, q + (static_cast<long>(bi) * Hq + kvh * grp) * D, grp);
     float m = kNegInf, l = 0.0f;
     v4f acc[DT];
 #pragma unroll
     for (int t = 0; t < DT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
-
-    // scale, bias (not on the newest key) and mask of the score tiles; entry
-    // (kt, i) is key 16 g + 4 kt + i of the tile at sequence position pos0.
-    // keep[kt] gets the byte mask of the keys that take part.
-    auto finish = [&](v4f (&sc)[4], const float* brow, int nk, int pos0, uint32_t (&keep)[4])
-                      __attribute__((always_inline)) {
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        float4 bv = make_float4(0.f, 0.f, 0.f, 0.f);
-        if constexpr (BIAS) bv = *reinterpret_cast<const float4*>(brow + 16 * g + 4 * kt);
-        const float bs[4] = {bv.x, bv.y, bv.z, bv.w};
-        keep[kt] = 0u;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int key = 16 * g + 4 * kt + i;
-          bool on = key < nk;
-          float val = sc[kt][i] * scale_log2;
-          if constexpr (BIAS) {
-            const bool newest = key == n - 1 - pos0;
-            val = newest ? val : val + bs[i] * kLog2e;
-            on = on && (newest || bs[i] != kNegInf);   // a dropped key counts for nothing, whatever it holds
-          }
-          sc[kt][i] = on && c < grp ? val : kNegInf;
-          keep[kt] |= on ? 0xffu << (8 * i) : 0u;
-        }
-      }
-    };
-
-    // full blocks, in runs of at most 64 pages: lane j holds the id and the
-    // scales of the run's page p0 + j
-    for (int r0 = t_begin; r0 < t_close;) {
-      const int p0 = r0 >> tshift;
-      const int r1 = min(t_close, (p0 + 64) << tshift);
-      const int my_page = lane <= ((r1 - 1) >> tshift) - p0 ? prow[p0 + lane] : -1;
-      const bool my_ok = my_page >= 0 && my_page < num_pages;
-      // invalid ids read page 0, which exists, and contribute no keys
-      const long my_blk = static_cast<long>(my_ok ? my_page : 0) * Hkv + kvh;
-      const float my_ks = ksc[my_blk], my_vs = vsc[my_blk];
-      auto slot_of = [&](int t) {
-        const int j = (t >> tshift) - p0;
-        const int page = __builtin_amdgcn_readlane(my_page, j);
-        Slot8 sl;
-        sl.ok = page >= 0 && page < num_pages;
-        sl.blk = static_cast<long>(sl.ok ? page : 0) * Hkv + kvh;
-        sl.k0 = (t & tshift) * 64;
-        sl.ks = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_ks), j));
-        sl.vs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(my_vs), j));
-        return sl;
-      };
-      uint4 kf[4][K2], vf[DT];
-      auto load_k = [&](const Slot8& sl) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(kp + (sl.blk * ps + sl.k0) * D);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int s = 0; s < K2; ++s) kf[kt][s] = buf_load16<true>(r, koff + (4 * kt * D + 64 * s));
-      };
-      auto load_v = [&](const Slot8& sl) __attribute__((always_inline)) {
-        const __amdgpu_buffer_rsrc_t r = make_rsrc(vp + sl.blk * ps * D + sl.k0);
-#pragma unroll
-        for (int t = 0; t < DT; ++t) vf[t] = buf_load16<PS == 64>(r, voff + 16 * t * ps);
-      };
-      Slot8 cur = slot_of(r0);
-      load_k(cur);
-      load_v(cur);
-      auto tile = [&](auto more_c, int t, const Slot8& nxt) __attribute__((always_inline)) {
-        constexpr bool kMore = decltype(more_c)::value;
-        v4f sc[4];
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) {
-          sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-          for (int s = 0; s < K2; ++s) {
-            const uint4 x = kf[kt][s];
-            sc[kt] = mfma_bf16(widen8(x.x, x.y, cur.ks), qf[2 * s], sc[kt]);
-            sc[kt] = mfma_bf16(widen8(x.z, x.w, cur.ks), qf[2 * s + 1], sc[kt]);
-          }
-        }
-        if constexpr (kMore) load_k(nxt);
-        uint32_t keep[4];
-        finish(sc, key_bias + cur.blk * ps + cur.k0, cur.ok ? 64 : 0, 64 * t, keep);
-        softmax_block<4, DT>(sc, acc, m, l);
-        const v8bf p0b = pack_p(sc[0], sc[1]), p1b = pack_p(sc[2], sc[3]);
-        if (cur.ok) {
-#pragma unroll
-          for (int tt = 0; tt < DT; ++tt) {
-            uint4 x = vf[tt];
-            if constexpr (BIAS) x = uint4{x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]};
-            acc[tt] = mfma_bf16(widen8(x.x, x.y, cur.vs), p0b, acc[tt]);
-            acc[tt] = mfma_bf16(widen8(x.z, x.w, cur.vs), p1b, acc[tt]);
-          }
-        }
-        if constexpr (kMore) load_v(nxt);
-      };
-      for (int t = r0; t + 1 < r1; ++t) {
-        const Slot8 nxt = slot_of(t + 1);
-        tile(BoolC<true>{}, t, nxt);
-        cur = nxt;
-      }
-      tile(BoolC<false>{}, r1 - 1, cur);
-      r0 = r1;
-    }
-
-    // the open block, in bf16
-    for (int t = max(t_begin, t_open); t < t_end; ++t) {
-      const int page = prow[t >> tshift];
-      if (page < 0 || page >= num_pages) continue;   // wave-uniform
-      const int k0 = (t & tshift) * 64, nk = min(64, n - 64 * t);
-      const long tail = (static_cast<long>(bi) * Hkv + kvh) * ps * D;
-      const __amdgpu_buffer_rsrc_t kb = make_rsrc(kt_p + tail + k0 * D), vb = make_rsrc(vt_p + tail + k0);
-      v4f sc[4];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-        sc[kt] = v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-          sc[kt] = mfma_bf16(buf_load_v8bf(kb, 2 * koff + 2 * (4 * kt * D + 64 * (ks >> 1) + 8 * (ks & 1)), 0),
-                             qf[ks], sc[kt]);
-      }
-      uint32_t keep[4];
-      finish(sc, key_bias + (static_cast<long>(page) * Hkv + kvh) * ps + k0, nk, 64 * t, keep);
-      softmax_block<4, DT>(sc, acc, m, l);
-      // two keys a word: byte masks to 16-bit masks (slots past nk hold what
-      // the buffer held, NaN perhaps)
-      uint32_t km[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        km[i] = __builtin_amdgcn_perm(0u, keep[i >> 1], (i & 1) ? 0x03030202u : 0x01010000u);
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const v8bf pb = pack_p(sc[2 * h], sc[2 * h + 1]);
-#pragma unroll
-        for (int tt = 0; tt < DT; ++tt) {
-          uint4 x = buf_load16<false>(vb, 2 * voff + 16 * h + 32 * tt * ps);
-          x = uint4{x.x & km[4 * h], x.y & km[4 * h + 1], x.z & km[4 * h + 2], x.w & km[4 * h + 3]};
-          acc[tt] = mfma_bf16(__builtin_bit_cast(v8bf, x), pb, acc[tt]);
-        }
-      }
-    }
+    row_tiles<D, BIAS, PS, 1>(kv, bi, kvh, n, t_begin, t_end, grp, scale_log2, qf, acc, m, l);
 
     // partial of this segment: O^T[d][q] unnormalised, with m (log2 domain) and l
     const long seg = static_cast<long>(bi) * Hkv + kvh + w;
@@ -300,6 +334,61 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
       }
     }
     gt += t_end - t_begin;
+  }
+}
+
+// Short tables: one workgroup a (row, kv head), its waves taking the row's tiles in
+// turn and joining in LDS, so that no second launch and no workspace follow.  The
+// rows' own lengths stand on the device; the table's width, which bounds them, is
+// what the host can go by.
+template <int D>
+constexpr int kShortWaves = 512 / D;   // their sums O^T fill 32 KB: 16 columns of D fp32 each
+template <int D, bool BIAS, int PS>
+__global__ __launch_bounds__(64 * kShortWaves<D>) void paged_decode_fp8_short_kernel(
+    const bf16* __restrict__ q, const Fp8Cache kv, const int32_t* __restrict__ seq_lens,
+    bf16* __restrict__ o, int Hq, float scale_log2) {
+  constexpr int DT = D / 16, NW = kShortWaves<D>;
+  __shared__ float so[NW][16][D];
+  __shared__ float sm[NW][16], sl[NW][16];
+  const int kvh = blockIdx.x % kv.Hkv, bi = blockIdx.x / kv.Hkv, grp = Hq / kv.Hkv;
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, g = lane >> 4;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int n = decode_row_len(seq_lens, bi, kv.max_pages, PS);
+  const bf16* qg = q + (static_cast<long>(bi) * Hq + kvh * grp) * D;
+  v8bf qf[D / 32];
+  load_q<D>(qf, qg, grp);
+  float m = kNegInf, l = 0.0f;
+  v4f acc[DT];
+#pragma unroll
+  for (int t = 0; t < DT; ++t) acc[t] = v4f{0.f, 0.f, 0.f, 0.f};
+  row_tiles<D, BIAS, PS, NW>(kv, bi, kvh, n, wid, (n + 63) >> 6, grp, scale_log2, qf, acc, m, l);
+  if (c < grp) {
+#pragma unroll
+    for (int t = 0; t < DT; ++t)
+      *reinterpret_cast<float4*>(&so[wid][c][16 * t + 4 * g]) = make_float4(acc[t][0], acc[t][1], acc[t][2], acc[t][3]);
+    if (g == 0) {
+      sm[wid][c] = m;
+      sl[wid][c] = l;
+    }
+  }
+  __syncthreads();
+  bf16* og = o + (static_cast<long>(bi) * Hq + kvh * grp) * D;
+  for (int e = tid; e < grp * D / 2; e += 64 * NW) {
+    const int col = 2 * e / D, d = 2 * e % D;
+    float M = kNegInf;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) M = fmaxf(M, sm[i][col]);
+    float L = 0.0f, a0 = 0.0f, a1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const float w = sm[i][col] == kNegInf ? 0.0f : fast_exp2(sm[i][col] - M);
+      const float2 v = *reinterpret_cast<const float2*>(&so[i][col][d]);
+      L = fmaf(w, sl[i][col], L);
+      a0 = fmaf(w, v.x, a0);
+      a1 = fmaf(w, v.y, a1);
+    }
+    const float inv = L > 0.0f ? 1.0f / L : 0.0f;
+    *reinterpret_cast<uint32_t*>(og + 2 * e) = pack_bf16x2(a0 * inv, a1 * inv);
   }
 }
 
@@ -374,18 +463,27 @@ __global__ __launch_bounds__(256) void paged_decode_fp8_merge_kernel(
   }
 }
 
-// the kernel for these sizes, and its number among the eight
+// f(D, bias, page size, their number among the eight), the first three as constants
 template <typename F>
-auto with_fp8_kernel(int head_dim, int page_size, bool bias, F f) {
-  if (head_dim == 128) {
-    if (page_size == 64)
-      return bias ? f(paged_decode_fp8_kernel<128, true, 64>, 0) : f(paged_decode_fp8_kernel<128, false, 64>, 1);
-    return bias ? f(paged_decode_fp8_kernel<128, true, 128>, 2) : f(paged_decode_fp8_kernel<128, false, 128>, 3);
-  }
-  if (page_size == 64)
-    return bias ? f(paged_decode_fp8_kernel<64, true, 64>, 4) : f(paged_decode_fp8_kernel<64, false, 64>, 5);
-  return bias ? f(paged_decode_fp8_kernel<64, true, 128>, 6) : f(paged_decode_fp8_kernel<64, false, 128>, 7);
+auto with_sizes(int head_dim, int page_size, bool bias, F f) {
+  using std::integral_constant;
+  auto page = [&](auto d, auto bi, int i) {
+    return page_size == 64 ? f(d, bi, integral_constant<int, 64>{}, i)
+                           : f(d, bi, integral_constant<int, 128>{}, i + 1);
+  };
+  auto gate = [&](auto d, int i) {
+    return bias ? page(d, integral_constant<bool, true>{}, i) : page(d, integral_constant<bool, false>{}, i + 2);
+  };
+  return head_dim == 128 ? gate(integral_constant<int, 128>{}, 0) : gate(integral_constant<int, 64>{}, 4);
 }
+
+// Whether the one-launch kernel takes a call, by the table's width in keys and the
+// number of (row, kv head) pairs.  Measured, GPU time of one and of two launches in
+// us (rows of half to all of the width, gated heads of 64 / ungated of 128): one
+// row, 16 / 8 heads, 256 keys 4.1, 8.3 / 4.7, 8.1; 1024 keys 6.9, 8.8 / 9.9, 9.2
+// (a launch costs the host some 4 us besides); 2048 keys 12.6, 10.0 / 16.7, 8.8.
+// 16 rows, 2048 keys 15.3, 20.8 / 19.6, 22.6; 4096 keys 25.3, 29.4 / 35.5, 31.7.
+inline bool short_table(long keys, long pairs) { return keys <= 1024 || (keys <= 2048 && pairs >= 128); }
 
 }  // namespace
 }  // namespace sa
@@ -411,20 +509,39 @@ extern "C" int sa_paged_decode_fp8_fwd(
                                            sa::kDecodeMaxWaves, workspace, &ws);
   SA_CHECK_ARG(workspace_bytes >= need, "%s: workspace %zu B < %zu B", who, workspace_bytes, need);
   if (batch == 0) return 0;
-  const int W = sa::with_fp8_kernel(head_dim, page_size, key_bias != nullptr,
-                                    [](auto kern, int i) { return sa::decode_waves(kern, i); });
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(static_cast<float>(head_dim));
+  const float sl2 = scale * sa::kLog2e;
   hipStream_t s = static_cast<hipStream_t>(stream);
+  const sa::Fp8Cache kv{static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages),
+                        k_scale, v_scale, static_cast<const sa::bf16*>(k_tail),
+                        static_cast<const sa::bf16*>(v_tail), page_table, key_bias,
+                        num_kv_heads, max_pages, num_pages};
+  const auto* qp = static_cast<const sa::bf16*>(q);
+  const bool bias = key_bias != nullptr;
+  if (sa::short_table(static_cast<long>(max_pages) * page_size, static_cast<long>(batch) * num_kv_heads)) {
+    sa::ProfScope prof_("paged_decode_fp8_short", s);
+    sa::with_sizes(head_dim, page_size, bias, [&](auto d, auto bi, auto ps, int) {
+      constexpr int D = decltype(d)::value;
+      hipLaunchKernelGGL((sa::paged_decode_fp8_short_kernel<D, decltype(bi)::value, decltype(ps)::value>),
+                         dim3(batch * num_kv_heads), dim3(64 * sa::kShortWaves<D>), 0, s, qp, kv, seq_lens,
+                         static_cast<sa::bf16*>(o), num_q_heads, sl2);
+      return 0;
+    });
+    SA_CHECK_LAUNCH("paged_decode_fp8_short");
+    return 0;
+  }
+  const int W = sa::with_sizes(head_dim, page_size, bias, [](auto d, auto bi, auto ps, int i) {
+    return sa::decode_waves(
+        sa::paged_decode_fp8_kernel<decltype(d)::value, decltype(bi)::value, decltype(ps)::value>, i);
+  });
   if (const int rc = sa::decode_plan_launch(seq_lens, batch, page_size, max_pages, ws, s)) return rc;
   {
     sa::ProfScope prof_("paged_decode_fp8", s);
-    sa::with_fp8_kernel(head_dim, page_size, key_bias != nullptr, [&](auto kern, int) {
-      hipLaunchKernelGGL(kern, dim3(W), dim3(64), 0, s, static_cast<const sa::bf16*>(q),
-                         static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages),
-                         k_scale, v_scale, static_cast<const sa::bf16*>(k_tail),
-                         static_cast<const sa::bf16*>(v_tail), page_table, seq_lens, key_bias,
-                         ws.cum_row, ws.part_o, ws.part_ml, batch, num_q_heads, num_kv_heads,
-                         max_pages, num_pages, W, scale * sa::kLog2e);
+    sa::with_sizes(head_dim, page_size, bias, [&](auto d, auto bi, auto ps, int) {
+      hipLaunchKernelGGL(
+          (sa::paged_decode_fp8_kernel<decltype(d)::value, decltype(bi)::value, decltype(ps)::value>),
+          dim3(W), dim3(64), 0, s, qp, kv, seq_lens, ws.cum_row, ws.part_o, ws.part_ml, batch,
+          num_q_heads, W, sl2);
       return 0;
     });
     SA_CHECK_LAUNCH("paged_decode_fp8");

@@ -547,3 +547,61 @@ def test_step_in_a_graph_and_on_another_stream():
         torch.randn(64, 64, device="cuda").sum()
         assert torch.equal(o, want[s]), s
     assert sl.tolist() == [x + steps for x in start.tolist()]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("run", [
+    lambda: test_attention(64, 64, 2, 1, True), lambda: test_attention(64, 128, 2, 3, False),
+    lambda: test_attention(128, 64, 2, 4, False), lambda: test_attention(128, 128, 1, 16, True),
+    lambda: test_attention_many_rows(), lambda: test_masked_places_hold_anything(64, 64),
+    lambda: test_masked_places_hold_anything(128, 128), lambda: test_no_rows_and_no_pages(),
+    lambda: test_other_index_types_and_strides_of_q(), lambda: test_rows_that_the_mask_leaves_empty(),
+    lambda: test_step_in_a_graph_and_on_another_stream()])
+def test_attention_behind_wide_tables(monkeypatch, run):
+    """The same checks with tables of at least 2304 keys, the rows' pages first:
+    wide tables have a kernel of their own."""
+    narrow = attend
+
+    def wide(q, c, table, lens, **kw):
+        pad = torch.full((table.shape[0], 36), -1, dtype=table.dtype, device=table.device)
+        return narrow(q, c, torch.cat([table, pad], 1), lens, **kw)
+
+    monkeypatch.setitem(globals(), "attend", wide)
+    run()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("b,H,D,ps,lens,gated", [
+    (1, 2, 64, 64, [1024], True), (2, 2, 128, 128, [1024, 1000], False), (1, 1, 128, 64, [961], True),
+    (2, 64, 64, 128, [2048, 1930], True), (2, 64, 128, 64, [2047, 1], False)])
+def test_attention_rows_as_long_as_a_short_table(b, H, D, ps, lens, gated):
+    """Several tiles a wave, closed and open ones, where one workgroup takes a row."""
+    L = max(lens)
+    width = (L + ps - 1) // ps
+    k, v, lg = tokens(b, H, L, D, gated, seed=21, spread=False)
+    table, c = make_cache(b, H, D, ps, width, gated, "cuda", fill=True)
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    build(k.cuda(), v.cuda(), None if lg is None else lg.cuda(), table, sl, c)
+    q = torch.randn(b, H, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
+    o = attend(q.cuda(), c, table, sl).cpu()
+    c = {name: None if t is None else t.cpu() for name, t in c.items()}
+    for r, n in enumerate(lens):
+        ids, full = table[r].long().cpu(), n // ps
+        for h in sorted({0, 1 % H, H // 2, H - 1}):
+            kk = (c["k_pages"][ids[:full], h].double() * c["k_scale"][ids[:full], h].double()[:, None, None]).reshape(-1, D)
+            vv = (c["v_pages"][ids[:full], h].double() * c["v_scale"][ids[:full], h].double()[:, None, None]).transpose(1, 2).reshape(-1, D)
+            kk = torch.cat([kk, c["k_tail"][r, h, :n - full * ps].double()])
+            vv = torch.cat([vv, c["v_tail"][r, h, :, :n - full * ps].t().double()])
+            on = torch.ones(n, dtype=torch.bool)
+            if gated:
+                on = lg[r, h, :n] > -INF
+                on[-1] = True
+            g = lg[r, h, :n][on] if gated else None
+            want = ref.attend(q[r, h], kk[on], vv[on], g)
+            A = ref.attend(q[r, h], kk[on], vv[on].abs(), g)
+            big = D ** -0.5 * (kk[on].abs() @ q[r, h].double().abs())
+            if gated:   # the newest key's gate does not count
+                big[:-1] += g[:-1].double().abs()
+            e = (D + 4) * 2.0 ** -24 * float(big.max())
+            err = (o[r, h].double() - want).abs()
+            assert (err <= (2.0 ** -8 + 2.5 * e) * A + 2.0 ** -8 * want.abs()).all(), (r, h)
