@@ -453,7 +453,9 @@ int sa_paged_kv_append(const void* k, const void* v, const float* log_gate,
  *   (batch, heads) f32: slot seq_lens[r] % page_size of the open block; a block
  *   that it fills is rounded into page page_table[r][seq_lens[r] / page_size];
  *   then seq_lens[r] += 1 on the device.  A page id outside the pool, or a slot
- *   behind max_pages, leaves the pages as they are.
+ *   behind max_pages, leaves the pages as they are, seq_lens[r] = -1 the whole
+ *   row.  Lengths and max_pages * page_size are below 2^27; while the call runs
+ *   the bits above mark who has read a length.
  * build: tokens t < min(seq_lens[r], seqlen) of row r; k, v bf16 with element
  *   strides sb (batch), st (token), sh (head), head_dim contiguous; log_gate
  *   f32 with strides gb, gh, gt.  Slots behind a row's tokens in its open block

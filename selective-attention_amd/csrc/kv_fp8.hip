@@ -33,6 +33,8 @@ __device__ __forceinline__ int block_exp(uint32_t top) {
 }
 __device__ __forceinline__ float pow2f(int e) { return __uint_as_float(static_cast<uint32_t>(e + 127) << 23); }
 
+using v2u = uint32_t __attribute__((ext_vector_type(2)));
+
 // magnitude bits of a finite bf16, 0 for infinities and NaN
 __device__ __forceinline__ uint32_t mag(uint32_t bits16) {
   const uint32_t a = bits16 & 0x7fffu;
@@ -63,48 +65,77 @@ __device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
   return v;
 }
 
-// One token per row.  One workgroup per row: the token into the open block
-// (and its gate into the page), and where that was the block's last slot, the
-// block's codes and scales, a wave per (head, keys or values) with its block in
-// registers between the maximum and the codes (128 x 128 blocks are read twice).
-// Bound by latency, one chain of length, page, tail and block: 64 rows, 8 heads of
-// 128, 7 us where no row closes a block, 14 where one or all of them do (between
-// events; 12 and 16 with the block read twice).
+// One token per row: the token into the open block (and its gate into the page),
+// and where that was the block's last slot, the block's codes and scales, a wave
+// per (head, keys or values) with its block in registers between the maximum and
+// the codes.  Four workgroups a row, since one moves a closing row's 256 KB (8
+// heads of 128) through its CU no faster than some 30 GB/s.  The length is read by
+// all four and advanced by one, whichever comes last: each sets its bit above
+// the length's 27 and so sees the bits set before, and the fourth stores the length
+// plus one, without the bits.  None waits for another.
+// Bound by latency, one chain of length, page and tail: 64 rows, 8 heads of 128,
+// 7 us where no row closes a block, 11 where one does, 13.5 where all do (between
+// events; 14.5 and 16.7 with one workgroup a row, and 64 rows of 16 heads, 128
+// tokens a block, all closing, 94 against 35).
+constexpr int kAppendParts = 4, kLenBits = 27;
 template <int D, int PS>
-__global__ __launch_bounds__(1024) void kv_fp8_append_kernel(
+__global__ __launch_bounds__(512) void kv_fp8_append_kernel(
     const bf16* __restrict__ k, const bf16* __restrict__ v, const float* __restrict__ log_gate,
     const int32_t* __restrict__ page_table, int32_t* __restrict__ seq_lens, int heads,
     int max_pages, int num_pages, uint8_t* __restrict__ k_pages, uint8_t* __restrict__ v_pages,
     float* __restrict__ k_scale, float* __restrict__ v_scale, bf16* k_tail, bf16* v_tail,
     float* gate_pages) {
-  constexpr int NV = PS * D / 8 / 64, NR = NV < 16 ? NV : 16;   // 16-byte pieces a lane; kept
-  const int row = blockIdx.x;
-  const int t = max(seq_lens[row], 0);
+  constexpr int NV = PS * D / 8 / 64;   // 16-byte pieces of a block a lane
+  const int row = blockIdx.x / kAppendParts, part = blockIdx.x % kAppendParts, tid = threadIdx.x;
+  const int n = heads * D;
+  const bf16 *kr = k + static_cast<long>(row) * n, *vr = v + static_cast<long>(row) * n;
+  // the loads that wait for no length
+  const int e0 = part * 512 + tid;
+  const bf16 k0 = e0 < n ? kr[e0] : bf16{}, v0 = e0 < n ? vr[e0] : bf16{};
+  __shared__ int len;
+  if (tid == 0) {
+    const int mine = 1 << (kLenBits + part);
+    constexpr int all = ((1 << kAppendParts) - 1) << kLenBits;
+    const int old = __hip_atomic_fetch_or(seq_lens + row, mine, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    len = old < 0 ? old : old & ~all;
+    if (old >= 0 && ((old | mine) & all) == all)
+      __hip_atomic_store(seq_lens + row, len + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  }
+  __syncthreads();
+  const int t = __builtin_amdgcn_readfirstlane(len);
+  if (t < 0) return;
   const int col = min(t / PS, max_pages - 1), s = t % PS;
   const int page = page_table[static_cast<long>(row) * max_pages + col];
+  const long tail0 = static_cast<long>(row) * heads * PS * D;
   // an invalid id, or a row past its table: the tail alone is written
   const bool ok = page >= 0 && page < num_pages && t / PS < max_pages;
-  const long tail0 = static_cast<long>(row) * heads * PS * D;
   const long page0 = static_cast<long>(ok ? page : 0) * heads;
-  for (int e = threadIdx.x; e < heads * D; e += blockDim.x) {
+  for (int e = e0; e < n; e += kAppendParts * 512) {
     const int h = e / D, d = e % D;
-    const long src = static_cast<long>(row) * heads * D + e;
     const long dst = tail0 + static_cast<long>(h) * PS * D;
-    k_tail[dst + s * D + d] = k[src];
-    v_tail[dst + d * PS + s] = v[src];
+    k_tail[dst + s * D + d] = e == e0 ? k0 : kr[e];
+    v_tail[dst + d * PS + s] = e == e0 ? v0 : vr[e];
     if (d == 0 && gate_pages && ok)
       gate_pages[(page0 + h) * PS + s] = log_gate[static_cast<long>(row) * heads + h];
   }
-  __syncthreads();   // the row's stores are visible to the whole workgroup
-  if (threadIdx.x == 0) seq_lens[row] = t + 1;
   if (s != PS - 1 || !ok) return;
-  const int lane = threadIdx.x & 63;
-  for (int it = threadIdx.x >> 6; it < 2 * heads; it += blockDim.x >> 6) {
+  // The block from the tail, its last token from k and v: the stores above may or
+  // may not be there yet, and nothing here depends on them (nor on that token's
+  // gate, which does not count).
+  const int lane = tid & 63;
+  for (int it = part + kAppendParts * __builtin_amdgcn_readfirstlane(tid >> 6); it < 2 * heads; it += kAppendParts * 8) {
     const int h = it >> 1;
     const bool val = it & 1;
-    const uint4* src = reinterpret_cast<const uint4*>((val ? v_tail : k_tail) + tail0 + static_cast<long>(h) * PS * D);
-    uint2* dst = reinterpret_cast<uint2*>((val ? v_pages : k_pages) + (page0 + h) * PS * D);
+    const __amdgpu_buffer_rsrc_t src = make_rsrc((val ? v_tail : k_tail) + tail0 + static_cast<long>(h) * PS * D);
+    const __amdgpu_buffer_rsrc_t dst = make_rsrc((val ? v_pages : k_pages) + (page0 + h) * PS * D);
+    auto load = [&](int i) __attribute__((always_inline)) {
+      return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(src, 16 * lane, 1024 * i, 0));
+    };
+    auto store = [&](int i, const uint2& c) __attribute__((always_inline)) {
+      __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(v2u, c), dst, 8 * lane, 512 * i, 0);
+    };
     const float* gr = gate_pages ? gate_pages + (page0 + h) * PS : nullptr;
+    const uint16_t* fresh = reinterpret_cast<const uint16_t*>((val ? vr : kr) + h * D);
     // dropped tokens are 0.  Values: a lane's pieces are all of the same eight
     // tokens (512 % PS = 0), one mask; keys: a piece is of one token.
     uint32_t keep[4] = {~0u, ~0u, ~0u, ~0u};
@@ -115,29 +146,36 @@ __global__ __launch_bounds__(1024) void kv_fp8_append_kernel(
         if (tok != PS - 1 && gr[tok] == -__builtin_inff()) keep[j >> 1] &= (j & 1) ? 0x0000ffffu : 0xffff0000u;
       }
     }
-    auto mask = [&](const uint4& x, int i) {
-      const int tok = 8 * i / D;
-      const bool dead = gr && !val && tok != PS - 1 && gr[tok] == -__builtin_inff();
-      return dead ? uint4{0u, 0u, 0u, 0u}
-                  : uint4{x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]};
-    };
-    uint4 x[NR];
+    const bool last = (8 * lane) % PS == PS - 8;   // values: the piece ends in the last token
+    auto piece = [&](uint4 x, int p) __attribute__((always_inline)) {
+      if (val) {
+        x = uint4{x.x & keep[0], x.y & keep[1], x.z & keep[2], x.w & keep[3]};
+        if (last) x.w = (x.w & 0xffffu) | static_cast<uint32_t>(fresh[8 * p / PS]) << 16;
+        return x;
+      }
+      const int tok = 8 * p / D;
+      if (tok == PS - 1) {
+        uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < NR; ++i) x[i] = src[lane + 64 * i];
+        for (int j = 0; j < 4; ++j)
+          w[j] = fresh[8 * p % D + 2 * j] | static_cast<uint32_t>(fresh[8 * p % D + 2 * j + 1]) << 16;
+        return uint4{w[0], w[1], w[2], w[3]};
+      }
+      return gr && gr[tok] == -__builtin_inff() ? uint4{0u, 0u, 0u, 0u} : x;
+    };
+    uint4 x[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) x[i] = load(i);
     uint32_t top = 0u;
 #pragma unroll
-    for (int i = 0; i < NR; ++i) {
-      x[i] = mask(x[i], lane + 64 * i);
+    for (int i = 0; i < NV; ++i) {
+      x[i] = piece(x[i], lane + 64 * i);
       top = max(top, mag_max(x[i]));
     }
-#pragma unroll 4
-    for (int i = NR; i < NV; ++i) top = max(top, mag_max(mask(src[lane + 64 * i], lane + 64 * i)));
     const int e = block_exp(wave_umax(top) << 16);
     const float inv = pow2f(-e);
 #pragma unroll
-    for (int i = 0; i < NR; ++i) dst[lane + 64 * i] = encode8(x[i], inv);
-#pragma unroll 4
-    for (int i = NR; i < NV; ++i) dst[lane + 64 * i] = encode8(mask(src[lane + 64 * i], lane + 64 * i), inv);
+    for (int i = 0; i < NV; ++i) store(i, encode8(x[i], inv));
     if (lane == 0) (val ? v_scale : k_scale)[page0 + h] = pow2f(e);
   }
 }
@@ -270,11 +308,13 @@ extern "C" int sa_paged_kv_append_fp8(const void* k, const void* v, const float*
                                      batch, heads, head_dim, page_size, max_pages, num_pages,
                                      k_pages, v_pages, k_scale, v_scale, k_tail, v_tail, gate_pages))
     return rc;
+  SA_CHECK_ARG(static_cast<long>(max_pages) * page_size < (1L << sa::kLenBits) && batch < (1 << 28),
+               "sa_paged_kv_append_fp8: table of %d pages x %d rows too large", max_pages, batch);
   if (batch == 0) return 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   sa::ProfScope prof_("kv_fp8_append", s);
   auto launch = [&](auto kern) {
-    hipLaunchKernelGGL(kern, dim3(batch), dim3(1024), 0, s, static_cast<const sa::bf16*>(k),
+    hipLaunchKernelGGL(kern, dim3(batch * sa::kAppendParts), dim3(512), 0, s, static_cast<const sa::bf16*>(k),
                        static_cast<const sa::bf16*>(v), log_gate, page_table, seq_lens, heads,
                        max_pages, num_pages, static_cast<uint8_t*>(k_pages),
                        static_cast<uint8_t*>(v_pages), k_scale, v_scale,

@@ -210,6 +210,16 @@ def test_append_and_build_refuse(what):
         build(k4, k4, None if lg is None else lg[..., None].expand(-1, -1, 5), table, lens, c)
 
 
+def test_append_refuses_tables_beyond_the_length_bits():
+    from selective_attention import _lib
+    lib = _lib.load()
+    at = 4096   # refused before any pointer is read
+    for pages, rows, rc in ((1 << 21, 0, 1), ((1 << 21) - 1, 0, 0), (1, 1 << 28, 1)):
+        assert lib.sa_paged_kv_append_fp8(at, at, None, at, at, rows, 1, 64, 64, pages, 1, at, at, at,
+                                          at, at, at, None, None) == rc
+    assert b"too large" in lib.sa_last_error()
+
+
 @pytest.mark.parametrize("what", ["heads", "group", "dtype", "D", "bias", "lens", "scale",
                                   "softmax", "cpu"])
 def test_attention_refuses(what):
@@ -319,6 +329,26 @@ def test_append_at_the_tables_end_and_bad_pages():
             same(c[name][ids].float(), keep[name][ids].float(), name)
     rows = refs(k, v, lg, [0, 0, 64], ps)
     check_cache(c, table, rows, [0, 0, 64])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("H,D,ps,gated", [(3, 64, 64, True), (1, 128, 128, False), (9, 64, 128, True)])
+def test_append_to_many_rows(H, D, ps, gated):
+    """Rows at every place of a block, some closing; a row of length -1 stays."""
+    b = 131
+    lens = [(17 * r) % (2 * ps) for r in range(b)]
+    lens[3], lens[50], lens[b - 1] = ps - 1, 2 * ps - 1, -1
+    k, v, lg = tokens(b, H, 2 * ps, D, gated, seed=22)
+    table, c = make_cache(b, H, D, ps, 2, gated, "cuda")
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    build(k.cuda(), v.cuda(), None if lg is None else lg.cuda(), table, sl, c)
+    keep = {n: None if t is None else t.clone() for n, t in c.items()}
+    r, i = torch.arange(b), torch.tensor(lens).clamp(min=0)
+    append(k[r, :, i].cuda(), v[r, :, i].cuda(), None if lg is None else lg[r, :, i].cuda(), table, sl, c)
+    assert sl.tolist() == [n + 1 if n >= 0 else -1 for n in lens]
+    same(c["k_tail"][b - 1], keep["k_tail"][b - 1], "tail")
+    same(c["v_tail"][b - 1], keep["v_tail"][b - 1], "tail")
+    check_cache(c, table, refs(k, v, lg, [n + 1 for n in lens], ps), [n + 1 for n in lens])
 
 
 @pytest.mark.gpu
