@@ -535,12 +535,16 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(
   if (asked && g_lp && (tg < 0 || tg >= V)) a = __builtin_nanf("");
   const float h = g_h ? g_h[row] : 0.0f;
   float all = a;
+  bool silent = !asked && h == 0.0f;   // zeros, whatever the row holds (a padded place, say)
   if (g_top)
-    for (int k = 0; k < top; ++k) all += g_top[row * top + k];
+    for (int k = 0; k < top; ++k) {
+      all += g_top[row * top + k];
+      silent = silent && g_top[row * top + k] == 0.0f;
+    }
   const float hl = h * kLn2, c = fmaf(h, H, all);   // a + sum b + h (log p + H) = hl log2 p + c
   auto grad = [&](float xv) {
     const float lp = fmaf(xv, kLog2e, n) - l2s;
-    return -fast_exp2(lp) * fmaf(hl, fmaxf(lp, kFloor), c);
+    return silent ? 0.0f : -fast_exp2(lp) * fmaf(hl, fmaxf(lp, kFloor), c);
   };
 #pragma unroll
   for (int q = 0; q < kGradP; ++q) {

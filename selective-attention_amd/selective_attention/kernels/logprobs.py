@@ -8,6 +8,7 @@ from .. import _lib
 from .common import act_dtype_code, call_on, require_one_device
 
 MAX_TOP = 64
+MAX_VOCAB = 1 << 28
 
 
 def _rows(logits):

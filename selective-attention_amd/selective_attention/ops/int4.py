@@ -75,6 +75,8 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool =
     N, K = weight.shape
     if N == 0 or K == 0:
         raise ValueError("quantize_int4: empty weight")
+    if not bool(torch.isfinite(weight).all()):
+        raise ValueError("quantize_int4: the weight holds infinities or NaN")
     w = F.pad(weight.detach().float(), (0, -K % group_size)).view(N, -1, group_size)
     if symmetric:
         s, zero = w.abs().amax(2) / 7.0, None

@@ -54,7 +54,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     Args:
         logits: (..., vocab) float32 or bfloat16; -inf rules a token out
         targets: (...) int32 or int64 token ids.  ignore_index: logprob 0 and no
-            gradient from it; any other id outside the vocabulary: NaN
+            gradient from it, whatever the row holds; any other id outside the
+            vocabulary: NaN
         top: alternatives a row, 0..64 and at most vocab; equal logits in the
             order of their ids
     Returns:
@@ -62,8 +63,9 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
         NaN.  Differentiable once in logits (logprob, entropy and top_logprobs);
         the gradient has the logits' dtype.
     """
-    if logits.dim() < 1 or logits.shape[-1] == 0:
-        raise ValueError(f"token_logprobs: logits need a vocabulary, got {tuple(logits.shape)}")
+    if logits.dim() < 1 or not 0 < logits.shape[-1] <= _k.MAX_VOCAB:
+        raise ValueError(f"token_logprobs: logits need a vocabulary of 1..{_k.MAX_VOCAB}, got "
+                         f"{tuple(logits.shape)}")
     if logits.dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"token_logprobs: logits must be float32 or bfloat16, got {logits.dtype}")
     if targets.dtype not in (torch.int32, torch.int64):

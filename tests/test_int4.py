@@ -131,6 +131,14 @@ def test_pack_refuses(what):
         pack_int4(codes, scales, z, **kw)
 
 
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_quantize_refuses_weights_that_are_no_numbers(bad):
+    w = torch.ones(16, 64)
+    w[3, 5] = bad
+    with pytest.raises(ValueError):
+        quantize_int4(w, 32)
+
+
 # --- the kernel ------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 2, 7, 16, 17, 32, 33, 64])

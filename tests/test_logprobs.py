@@ -57,6 +57,12 @@ def check(x, t, top, **kw):
 
 
 # --- refusals ------------------------------------------------------------------
+def test_refuses_rows_beyond_the_kernels_offsets():
+    x = torch.zeros(1, 1, dtype=torch.bfloat16).expand(1, (1 << 28) + 1)
+    with pytest.raises(ValueError, match="vocabulary"):
+        token_logprobs(x, torch.zeros(1, dtype=torch.int64))
+
+
 @pytest.mark.parametrize("what", ["dtype", "targets", "shape", "top", "vocab", "empty", "cpu"])
 def test_refuses(what):
     x, t = make(3, 50, torch.float32)
@@ -295,6 +301,24 @@ def test_targets_outside_give_no_number_and_double_backward_is_refused():
     import torch.autograd.forward_ad as fwd
     with pytest.raises(RuntimeError), fwd.dual_level():
         token_logprobs(fwd.make_dual(x.cuda(), torch.ones_like(x).cuda()), t.cuda())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_ignored_rows_take_no_gradient_whatever_they_hold(dtype):
+    """Padded places may hold anything: logprob 0 and a gradient of zeros, also where
+    other rows' entropy and alternatives are asked for."""
+    x, t = make(4, 203, dtype)
+    x[1, 7], x[2] = math.nan, -math.inf
+    t[1:3] = -100
+    leaf = x.cuda().requires_grad_(True)
+    out = token_logprobs(leaf, t.cuda(), top=3)
+    assert out.logprob[1:3].tolist() == [0.0, 0.0]
+    ones = torch.tensor([1.0, 0.0, 0.0, 1.0], device="cuda")
+    for outs, gs in (((out.logprob,), (torch.ones(4, device="cuda"),)),
+                     ((out.logprob, out.entropy, out.top_logprobs), (ones, ones, ones[:, None].expand(4, 3)))):
+        (d,) = torch.autograd.grad(outs, leaf, gs, retain_graph=True)
+        assert not d[1:3].any() and torch.isfinite(d).all() and d[0].any()
 
 
 @pytest.mark.gpu
