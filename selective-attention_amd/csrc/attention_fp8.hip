@@ -504,6 +504,7 @@ extern "C" int sa_paged_decode_fp8_fwd(
                  reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(k_tail) |
                  reinterpret_cast<uintptr_t>(v_tail)) & 15) == 0,
                "%s: q, the pages and the tails must be 16-byte aligned", who);
+  SA_CHECK_ARG(static_cast<long>(batch) * num_q_heads < (1L << 23), "%s: batch %d too large", who, batch);
   sa::DecodeWs ws;
   const size_t need = sa::decode_ws_layout(batch, num_q_heads, num_kv_heads, head_dim,
                                            sa::kDecodeMaxWaves, workspace, &ws);

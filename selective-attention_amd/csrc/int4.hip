@@ -471,7 +471,7 @@ extern "C" int sa_int4_dequant_bf16(const void* packed, const void* scales, cons
   SA_CHECK_ARG(packed && scales && out, "%s: null pointer", who);
   SA_CHECK_ARG((reinterpret_cast<uintptr_t>(packed) & 3) == 0, "%s: packed weights are not aligned", who);
   const long blocks = ((N + 15L) / 16) * ((K + 127L) / 128);
-  SA_CHECK_ARG(blocks < (1L << 31), "%s: weights too large", who);
+  SA_CHECK_ARG(blocks < (1L << 24), "%s: weights too large", who);   // (2^32 threads a grid)
   hipStream_t s = static_cast<hipStream_t>(stream);
   sa::ProfScope prof_("int4_dequant", s);
   hipLaunchKernelGGL(sa::int4_dequant_kernel, dim3(blocks), dim3(256), 0, s,

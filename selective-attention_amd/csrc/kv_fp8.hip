@@ -308,7 +308,7 @@ extern "C" int sa_paged_kv_append_fp8(const void* k, const void* v, const float*
                                      batch, heads, head_dim, page_size, max_pages, num_pages,
                                      k_pages, v_pages, k_scale, v_scale, k_tail, v_tail, gate_pages))
     return rc;
-  SA_CHECK_ARG(static_cast<long>(max_pages) * page_size < (1L << sa::kLenBits) && batch < (1 << 28),
+  SA_CHECK_ARG(static_cast<long>(max_pages) * page_size < (1L << sa::kLenBits) && batch < (1 << 21),
                "sa_paged_kv_append_fp8: table of %d pages x %d rows too large", max_pages, batch);
   if (batch == 0) return 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
@@ -346,7 +346,7 @@ extern "C" int sa_paged_kv_build_fp8(const void* k, const void* v, long sb, long
                "%s: k / v and their strides must keep 16-byte alignment", who);
   // page slots that can hold tokens
   const int cols = static_cast<int>(std::min<long>(max_pages, (static_cast<long>(seqlen) + page_size - 1) / page_size));
-  SA_CHECK_ARG(static_cast<long>(batch) * cols < (1L << 31), "%s: too many pages", who);
+  SA_CHECK_ARG(static_cast<long>(batch) * cols < (1L << 24), "%s: too many pages", who);   // (2^32 threads a grid)
   if (batch == 0 || cols == 0) return 0;
   hipStream_t s = static_cast<hipStream_t>(stream);
   sa::ProfScope prof_("kv_fp8_build", s);

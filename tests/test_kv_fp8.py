@@ -214,7 +214,7 @@ def test_append_refuses_tables_beyond_the_length_bits():
     from selective_attention import _lib
     lib = _lib.load()
     at = 4096   # refused before any pointer is read
-    for pages, rows, rc in ((1 << 21, 0, 1), ((1 << 21) - 1, 0, 0), (1, 1 << 28, 1)):
+    for pages, rows, rc in ((1 << 21, 0, 1), ((1 << 21) - 1, 0, 0), (1, 1 << 21, 1)):
         assert lib.sa_paged_kv_append_fp8(at, at, None, at, at, rows, 1, 64, 64, pages, 1, at, at, at,
                                           at, at, at, None, None) == rc
     assert b"too large" in lib.sa_last_error()

@@ -61,6 +61,10 @@ def test_refuses_rows_beyond_the_kernels_offsets():
     x = torch.zeros(1, 1, dtype=torch.bfloat16).expand(1, (1 << 28) + 1)
     with pytest.raises(ValueError, match="vocabulary"):
         token_logprobs(x, torch.zeros(1, dtype=torch.int64))
+    from selective_attention import _lib
+    lib, at = _lib.load(), 4096   # refused before any pointer is read
+    assert lib.sa_token_logprobs_fwd(1, at, 8, at, 1 << 23, 8, 0, -100, at, at, at, None, None, None, 0, None) == 1
+    assert b"bad sizes" in lib.sa_last_error()
 
 
 @pytest.mark.parametrize("what", ["dtype", "targets", "shape", "top", "vocab", "empty", "cpu"])
