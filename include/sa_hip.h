@@ -341,8 +341,8 @@ int sa_gemv_bf16_multi(const void* x, const void* xscale, int M, int K, int nseg
  * has none): y_i = x W_i^T + bias_i, i < nseg <= 4, all of the same x,
  *   W[n, k] = scale[n, k / group] (code[n, k] - zero[n, k / group]),
  * zero = 8 where there are no zeros, group in {32, 64, 128}.  x (M, K) bf16 with row
- * stride ldx (a multiple of 8 elements; columns K..ldx-1 hold zeros), 16-byte
- * aligned; with xscale (laid out as x, or NULL) the input is bf16(x * xscale).
+ * stride ldx >= K (elements; fastest on 16-byte boundaries, K and ldx multiples
+ * of 8); with xscale (laid out as x, or NULL) the input is bf16(x * xscale).
  * packed: (ceil(N / 16), ceil(K / 128), 64, 16) bytes, lane 16 g + c of a tile
  * being its row c, byte 4 j + i of it columns 32 j + 8 g + 2 i (low half) and
  * + 1 (high half).  scales, zeros: (ceil(N / 16), ceil(K / 128) 128 / group,

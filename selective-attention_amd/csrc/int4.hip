@@ -61,6 +61,10 @@ __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
   return pack_bf16x2(bf16lo_to_f32(a) * bf16lo_to_f32(b), bf16hi_to_f32(a) * bf16hi_to_f32(b));
 }
 
+// whether the pieces of eight columns stand on 16-byte boundaries and none passes K
+__device__ __forceinline__ bool whole_pieces(const bf16* x, int K, int ldx) {
+  return ((K | ldx) & 7) == 0 && (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+}
 // J blocks of 128 columns and 16 rows of x, those outside x as 0 (buffer loads,
 // whose range check answers for them without a branch), times xscale, rounded to
 // bf16, where that is given.  They are read along the rows (16 lanes a row, 4 rows
@@ -70,30 +74,59 @@ __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
 // 32 rows, 4096 -> 32000: 24.6 and 22).
 constexpr int kTurnRow = 17;   // uint4
 template <int J>
-__device__ __forceinline__ void load_x_rows(uint4 (&v)[J][4], const bf16* x, const bf16* xscale, int row0,
-                                            int k0, int M, int K, int ldx) {
-  const int lane = threadIdx.x & 63, bytes = M * ldx * 2;
-  const __amdgpu_buffer_rsrc_t rx =
-      __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(x), static_cast<short>(0), bytes, 0x00020000);
-  auto at = [&](int j, int i) {
-    const int row = row0 + 4 * i + (lane >> 4), k = k0 + 128 * j + 8 * (lane & 15);
-    return row < M && k < K ? (row * ldx + k) * 2 : bytes;
-  };
-#pragma unroll
-  for (int j = 0; j < J; ++j)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      v[j][i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rx, at(j, i), 0, 0));
-  if (xscale) {
-    const __amdgpu_buffer_rsrc_t rf =
-        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(xscale), static_cast<short>(0), bytes, 0x00020000);
+__device__ __forceinline__ void read_rows(uint4 (&v)[J][4], const bf16* x, int row0, int k0, int M, int K, int ldx) {
+  const int lane = threadIdx.x & 63;
+  if (whole_pieces(x, K, ldx)) {   // (uniform)
+    const int bytes = M * ldx * 2;
+    const __amdgpu_buffer_rsrc_t r =
+        __builtin_amdgcn_make_buffer_rsrc(const_cast<bf16*>(x), static_cast<short>(0), bytes, 0x00020000);
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const uint4 f = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rf, at(j, i), 0, 0));
+        const int row = row0 + 4 * i + (lane >> 4), k = k0 + 128 * j + 8 * (lane & 15);
+        const int at = row < M && k < K ? (row * ldx + k) * 2 : bytes;
+        v[j][i] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+      }
+    return;
+  }
+  // from the words that hold them: five, moved by half a word where a row starts in
+  // the middle of one, columns at and behind K as 0 (4 rows of 1023, 4383 outputs:
+  // 4.4 us, 4.0 of 1024; 32 of 4091, 32000 outputs: 27 and 22; a padded copy in
+  // front takes 10 us)
+  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 2);
+  const int bytes = (off + ((M - 1) * ldx + K) * 2 + 3) & ~3;
+  const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc(
+      const_cast<char*>(reinterpret_cast<const char*>(x) - off), static_cast<short>(0), bytes, 0x00020000);
+#pragma unroll
+  for (int j = 0; j < J; ++j)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = row0 + 4 * i + (lane >> 4), k = k0 + 128 * j + 8 * (lane & 15);
+      const int at = row < M && k < K ? off + (row * ldx + k) * 2 : bytes;
+      const uint4 a = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, at & ~3, 0, 0));
+      const uint32_t e = __builtin_amdgcn_raw_buffer_load_b32(r, (at & ~3) + 16, 0, 0);
+      const int sh = 8 * (at & 2), n = K - k;
+      uint32_t w[4] = {__builtin_amdgcn_alignbit(a.y, a.x, sh), __builtin_amdgcn_alignbit(a.z, a.y, sh),
+                       __builtin_amdgcn_alignbit(a.w, a.z, sh), __builtin_amdgcn_alignbit(e, a.w, sh)};
+#pragma unroll
+      for (int q = 0; q < 4; ++q) w[q] &= n > 2 * q + 1 ? ~0u : n > 2 * q ? 0xffffu : 0u;
+      v[j][i] = uint4{w[0], w[1], w[2], w[3]};
+    }
+}
+template <int J>
+__device__ __forceinline__ void load_x_rows(uint4 (&v)[J][4], const bf16* x, const bf16* xscale, int row0,
+                                            int k0, int M, int K, int ldx) {
+  read_rows(v, x, row0, k0, M, K, ldx);
+  if (xscale) {
+    uint4 f[J][4];
+    read_rows(f, xscale, row0, k0, M, K, ldx);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
         uint4& u = v[j][i];
-        u = uint4{mul_pair(u.x, f.x), mul_pair(u.y, f.y), mul_pair(u.z, f.z), mul_pair(u.w, f.w)};
+        u = uint4{mul_pair(u.x, f[j][i].x), mul_pair(u.y, f[j][i].y), mul_pair(u.z, f[j][i].z), mul_pair(u.w, f[j][i].w)};
       }
   }
 }
@@ -423,14 +456,13 @@ extern "C" int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int
   const char* who = "sa_int4_linear_bf16";
   SA_CHECK_ARG(M >= 1 && M <= 64 && K > 0 && K <= (1 << 22), "%s: M %d must be 1..64 and K %d 1..2^22",
                who, M, K);
-  SA_CHECK_ARG(ldx % 8 == 0 && ldx >= K && ldx <= (1 << 23), "%s: row stride %d must be a multiple of 8, at least K %d", who,
-               ldx, K);
+  SA_CHECK_ARG(ldx >= K && ldx <= (1 << 23), "%s: row stride %d must be at least K %d", who, ldx, K);
   SA_CHECK_ARG(sa::int4_group_ok(group), "%s: group %d not in {32, 64, 128}", who, group);
   SA_CHECK_ARG(nseg >= 1 && nseg <= sa::kInt4Segs, "%s: %d weight matrices, 1..%d allowed", who, nseg,
                sa::kInt4Segs);
   SA_CHECK_ARG(x && matrices, "%s: null pointer", who);
-  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xscale)) & 15) == 0,
-               "%s: x and xscale must be 16-byte aligned", who);
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xscale)) & 1) == 0,
+               "%s: x and xscale are not aligned to their type", who);
   sa::Int4Segs sg{};
   sg.nseg = nseg;
   const bool z = matrices[2] != 0;

@@ -12,6 +12,7 @@ from .common import call_on, require_device, require_one_device
 GROUPS = (32, 64, 128)
 MAX_ROWS = 64      # rows of one launch; more go through the widened weights
 MAX_MATRICES = 4
+MAX_STRIDE = 1 << 23
 
 
 def group_size(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor | None) -> int:
@@ -40,15 +41,14 @@ def group_size(packed: torch.Tensor, scales: torch.Tensor, zeros: torch.Tensor |
 
 
 def _rows(x: torch.Tensor, K: int) -> torch.Tensor:
-    """x (..., K) as (M, K) rows that the kernel reads: 16-byte aligned, the row
-    length padded with zeros to a multiple of 8."""
+    """x (..., K) as (M, K) rows of one stride; slices of longer rows as they lie."""
     if x.dim() != 2:
         x = x.reshape(-1, K)
-    if K % 8:
-        return torch.nn.functional.pad(x, (0, 8 - K % 8))
-    if not x.is_contiguous():
-        return x.contiguous()
-    return x if x.data_ptr() % 16 == 0 else x.clone()
+    return x if x.is_contiguous() or _strided(x, K) else x.contiguous()
+
+
+def _strided(x: torch.Tensor, K: int) -> bool:
+    return x.stride(1) == 1 and K <= x.stride(0) <= MAX_STRIDE
 
 
 def int4_linear_multi(x, weights, biases, sizes, G, xscale=None):
@@ -62,6 +62,12 @@ def int4_linear_multi(x, weights, biases, sizes, G, xscale=None):
     xr = _rows(x, K)
     xs = None if xscale is None else _rows(xscale, K)
     M = xr.shape[0]
+    if M == 1:
+        ld = K
+    else:
+        ld = xr.stride(0)
+        if xs is not None and xs.stride(0) != ld:
+            xr, xs, ld = xr.contiguous(), xs.contiguous(), K
     ys, words, kept = [], [], []
     for (packed, scales, zeros), b, N in zip(weights, biases, sizes):
         y = torch.empty((*x.shape[:-1], N), dtype=torch.bfloat16, device=x.device)
@@ -71,7 +77,7 @@ def int4_linear_multi(x, weights, biases, sizes, G, xscale=None):
         words += (packed.data_ptr(), scales.data_ptr(), 0 if zeros is None else zeros.data_ptr(),
                   0 if b is None else b.data_ptr(), y.data_ptr(), N)
         ys.append(y)
-    call_on(x, "sa_int4_linear_bf16", xr.data_ptr(), _lib.ptr(xs), M, K, xr.shape[1], G, n,
+    call_on(x, "sa_int4_linear_bf16", xr.data_ptr(), _lib.ptr(xs), M, K, ld, G, n,
             (ctypes.c_int64 * (6 * n))(*words), _lib.stream_of(x))
     return ys
 

@@ -207,6 +207,34 @@ def test_strides_and_alignment():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("M,N,K,G,zeros", [(1, 40, 999, 128, False), (20, 40, 1001, 64, True), (5, 50, 2047, 32, False),
+                                           (40, 33, 3999, 128, True), (3, 40, 4097, 64, False), (64, 20, 2050, 32, True),
+                                           (33, 24, 5002, 128, False), (2, 16, 1, 32, False), (7, 16, 1024, 64, False)])
+def test_rows_off_every_boundary(M, N, K, G, zeros):
+    """Odd lengths, strides and offsets; what stands beside the rows is not read
+    into them."""
+    codes, scales, z, b = make(N, K, G, zeros, seed=K, bias=True)
+    packed = pack_int4(codes, scales, z, G)
+    d, bias = dev(packed), b.cuda()
+    g = torch.Generator().manual_seed(M)
+    x, f = (torch.randn(M, K, generator=g).to(torch.bfloat16) for _ in range(2))
+    want = int4_linear(x.cuda(), *d, bias=bias, out_features=N)
+    check(want, x, packed, N, K, b)
+    for shift in (1, 2, 3, 8):
+        flat = torch.full((M * K + shift + 9,), float("nan"), dtype=torch.bfloat16, device="cuda")
+        flat[shift:shift + M * K] = x.cuda().flatten()
+        rows = flat[shift:shift + M * K].view(M, K)
+        assert torch.equal(int4_linear(rows, *d, bias=bias, out_features=N), want)
+        wide = torch.full((M, K + 2 * shift), float("nan"), dtype=torch.bfloat16, device="cuda")
+        wide[:, shift:shift + K] = x.cuda()
+        assert torch.equal(int4_linear(wide[:, shift:shift + K], *d, bias=bias, out_features=N), want)
+        y = int4_linear(rows, *d, bias=bias, out_features=N, xscale=f.cuda())
+        check(y, x, packed, N, K, b, f)
+        got = int4_linear(wide[:, shift:shift + K], *d, bias=bias, out_features=N, xscale=f.cuda())
+        assert torch.equal(got, y)
+
+
+@pytest.mark.gpu
 def test_what_is_no_number_stays_in_its_row():
     N, K, G = 32, 256, 128
     codes, scales, z, _ = make(N, K, G, True)
