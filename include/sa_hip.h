@@ -475,12 +475,14 @@ int sa_paged_kv_build_fp8(const void* k, const void* v, long sb, long st, long s
                           void* stream);
 
 /*
- * Paged GQA decode attention over that cache: sa_paged_decode_fwd's operation
- * and workspace (sa_paged_decode_workspace_size), the keys and values as the
- * codes stand for them.  q, o (batch, Hq, D) bf16; key_bias is gate_pages or
+ * Paged GQA decode attention over that cache: sa_paged_decode_fwd's operation,
+ * the keys and values as the codes stand for them.  workspace: of the size that
+ * sa_paged_decode_fp8_workspace_size says (0 bytes for short tables: NULL).  q, o (batch, Hq, D) bf16; key_bias is gate_pages or
  * NULL; a key whose bias is -inf (the newest apart) takes no part, whatever
  * its codes.  Page ids outside the pool contribute no keys.
  */
+size_t sa_paged_decode_fp8_workspace_size(int batch, int num_q_heads, int num_kv_heads,
+                                          int head_dim, int page_size, int max_pages);
 int sa_paged_decode_fp8_fwd(const void* q, const void* k_pages, const void* v_pages,
                             const float* k_scale, const float* v_scale, const void* k_tail,
                             const void* v_tail, const int32_t* page_table,

@@ -488,6 +488,14 @@ inline bool short_table(long keys, long pairs) { return keys <= 1024 || (keys <=
 }  // namespace
 }  // namespace sa
 
+extern "C" size_t sa_paged_decode_fp8_workspace_size(int batch, int num_q_heads, int num_kv_heads,
+                                                     int head_dim, int page_size, int max_pages) {
+  if (batch < 0 || num_kv_heads <= 0 || num_q_heads % num_kv_heads || max_pages < 0 ||
+      sa::short_table(static_cast<long>(max_pages) * page_size, static_cast<long>(batch) * num_kv_heads))
+    return 0;
+  return sa::decode_ws_layout(batch, num_q_heads, num_kv_heads, head_dim, sa::kDecodeMaxWaves, nullptr, nullptr);
+}
+
 extern "C" int sa_paged_decode_fp8_fwd(
     const void* q, const void* k_pages, const void* v_pages, const float* k_scale,
     const float* v_scale, const void* k_tail, const void* v_tail, const int32_t* page_table,
@@ -499,16 +507,16 @@ extern "C" int sa_paged_decode_fp8_fwd(
                                       key_bias, batch, num_q_heads, num_kv_heads, head_dim,
                                       page_size, max_pages, num_pages, o, who))
     return rc;
-  SA_CHECK_ARG(k_scale && v_scale && k_tail && v_tail && workspace, "%s: null pointer", who);
+  SA_CHECK_ARG(k_scale && v_scale && k_tail && v_tail, "%s: null pointer", who);
   SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k_pages) |
                  reinterpret_cast<uintptr_t>(v_pages) | reinterpret_cast<uintptr_t>(k_tail) |
                  reinterpret_cast<uintptr_t>(v_tail)) & 15) == 0,
                "%s: q, the pages and the tails must be 16-byte aligned", who);
   SA_CHECK_ARG(static_cast<long>(batch) * num_q_heads < (1L << 23), "%s: batch %d too large", who, batch);
-  sa::DecodeWs ws;
-  const size_t need = sa::decode_ws_layout(batch, num_q_heads, num_kv_heads, head_dim,
-                                           sa::kDecodeMaxWaves, workspace, &ws);
-  SA_CHECK_ARG(workspace_bytes >= need, "%s: workspace %zu B < %zu B", who, workspace_bytes, need);
+  const size_t need = sa_paged_decode_fp8_workspace_size(batch, num_q_heads, num_kv_heads, head_dim,
+                                                         page_size, max_pages);
+  SA_CHECK_ARG(workspace_bytes >= need && (workspace || need == 0), "%s: workspace %zu B < %zu B", who,
+               workspace_bytes, need);
   if (batch == 0) return 0;
   const float scale = softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(static_cast<float>(head_dim));
   const float sl2 = scale * sa::kLog2e;
@@ -531,6 +539,8 @@ extern "C" int sa_paged_decode_fp8_fwd(
     SA_CHECK_LAUNCH("paged_decode_fp8_short");
     return 0;
   }
+  sa::DecodeWs ws;
+  sa::decode_ws_layout(batch, num_q_heads, num_kv_heads, head_dim, sa::kDecodeMaxWaves, workspace, &ws);
   const int W = sa::with_sizes(head_dim, page_size, bias, [](auto d, auto bi, auto ps, int i) {
     return sa::decode_waves(
         sa::paged_decode_fp8_kernel<decltype(d)::value, decltype(bi)::value, decltype(ps)::value>, i);

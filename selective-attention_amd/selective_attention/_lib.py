@@ -34,6 +34,7 @@ SIGNATURES: dict[str, list] = {
                    _vp, _vp, _vp, _vp, _vp, _vp],
     "sa_ssd_bwd_workspace_size": [_i, _i, _i, _i, _i, _i, _i, _i],
     "sa_paged_decode_workspace_size": [_i, _i, _i, _i, _i],
+    "sa_paged_decode_fp8_workspace_size": [_i, _i, _i, _i, _i, _i],
     "sa_paged_decode_fwd": [_i, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _f,
                             _vp, _vp, _sz, _vp],
     "sa_paged_decode_noalloc_limit": [],
@@ -104,6 +105,7 @@ SIGNATURES: dict[str, list] = {
 RESTYPES = {"sa_last_error": ctypes.c_char_p, "sa_profile_enable": None, "sa_ssd_bwd_workspace_size": ctypes.c_size_t,
             "sa_ssd_bwd_gated_workspace_size": ctypes.c_size_t,
             "sa_paged_decode_workspace_size": ctypes.c_size_t,
+            "sa_paged_decode_fp8_workspace_size": ctypes.c_size_t,
             "sa_paged_decode_noalloc_limit": ctypes.c_size_t,
             "sa_token_logprobs_workspace_size": ctypes.c_size_t,
             "sa_ssm_conv_bwd_workspace_size": ctypes.c_size_t,

@@ -22,8 +22,8 @@ HEAD_DIMS = (64, 128)
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(b, Hq, Hkv, D, max_pages):
-    return _lib.load().sa_paged_decode_workspace_size(b, Hq, Hkv, D, max_pages)
+def _workspace_bytes(b, Hq, Hkv, D, ps, max_pages):
+    return _lib.load().sa_paged_decode_fp8_workspace_size(b, Hq, Hkv, D, ps, max_pages)
 
 
 def _check_cache(who, batch, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail, page_table,
@@ -102,14 +102,14 @@ def paged_decode_attn_fp8(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
     max_pages = pt.shape[1]
     if b == 0 or max_pages == 0:
         return torch.zeros_like(q)   # no row has a key
-    nbytes = _workspace_bytes(b, Hq, Hkv, D, max_pages)
-    ws = torch.empty((max(nbytes, 1),), dtype=torch.uint8, device=q.device)
+    nbytes = _workspace_bytes(b, Hq, Hkv, D, ps, max_pages)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=q.device) if nbytes else None
     o = torch.empty_like(q)
     scale = -1.0 if softmax_scale is None else float(softmax_scale)
     call_on(q, "sa_paged_decode_fp8_fwd", q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
             k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
             pt.data_ptr(), sl.data_ptr(), _lib.ptr(key_bias), b, Hq, Hkv, D, ps, max_pages, n,
-            scale, o.data_ptr(), ws.data_ptr(), nbytes, _lib.stream_of(q))
+            scale, o.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_of(q))
     return o
 
 

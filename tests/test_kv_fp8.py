@@ -210,6 +210,19 @@ def test_append_and_build_refuse(what):
         build(k4, k4, None if lg is None else lg[..., None].expand(-1, -1, 5), table, lens, c)
 
 
+def test_attention_refuses_a_workspace_too_small():
+    from selective_attention import _lib
+    lib = _lib.load()
+    assert lib.sa_paged_decode_fp8_workspace_size(1, 8, 8, 64, 64, 16) == 0    # 1024 keys: one launch
+    need = lib.sa_paged_decode_fp8_workspace_size(2, 8, 8, 64, 64, 17)
+    assert need == lib.sa_paged_decode_workspace_size(2, 8, 8, 64, 17) > 0
+    at = 4096   # refused before any pointer is read
+    for ws, nbytes in ((at, need - 1), (None, need)):
+        assert lib.sa_paged_decode_fp8_fwd(at, at, at, at, at, at, at, at, at, None, 2, 8, 8, 64, 64, 17, 9,
+                                           -1.0, at, ws, nbytes, None) == 1
+    assert b"workspace" in lib.sa_last_error()
+
+
 def test_append_refuses_tables_beyond_the_length_bits():
     from selective_attention import _lib
     lib = _lib.load()
