@@ -226,8 +226,10 @@ __device__ __forceinline__ void finish_row(const T* x, long row, long target, in
     const float h = kLn2 * (l2s - t / s);
     logprob[row] = lp;
     entropy[row] = h < 0.0f ? 0.0f : h;
-    stats[2 * row] = n;
-    stats[2 * row + 1] = l2s;
+    if (stats) {
+      stats[2 * row] = n;
+      stats[2 * row + 1] = l2s;
+    }
   }
   if (static_cast<int>(threadIdx.x) < top) {
     const uint64_t key = best[threadIdx.x];
@@ -659,7 +661,7 @@ extern "C" int sa_token_logprobs_fwd(int dtype, const void* logits, long ld, con
   const char* who = "sa_token_logprobs_fwd";
   if (const int rc = sa::logprobs_check(who, dtype, logits, ld, targets, rows, vocab, top)) return rc;
   if (rows == 0) return 0;
-  SA_CHECK_ARG(logprob && entropy && stats && (top == 0 || (top_ids && top_logprobs)), "%s: null pointer",
+  SA_CHECK_ARG(logprob && entropy && (top == 0 || (top_ids && top_logprobs)), "%s: null pointer",
                who);
   const size_t need = sa_token_logprobs_workspace_size(rows, vocab, top);
   SA_CHECK_ARG(need == 0 || (workspace && workspace_bytes >= need), "%s: workspace %zu B < %zu B", who,

@@ -2,6 +2,8 @@
 takes softmax and argmax of its logits, models/causal_lm.py:143-221)."""
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _lib
@@ -28,10 +30,15 @@ def _targets(t):
     return t.reshape(-1).to(torch.int64).contiguous()
 
 
-def token_logprobs_forward(logits, targets, top, ignore_index):
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(rows, V, top):
+    return _lib.load().sa_token_logprobs_workspace_size(rows, V, top)
+
+
+def token_logprobs_forward(logits, targets, top, ignore_index, with_stats=True):
     """logits (..., vocab) float32 or bfloat16, targets (...) integers -> (logprob
-    (...), entropy (...), stats (rows, 2), top_ids (..., top) int64, top_logprobs
-    (..., top) float32)."""
+    (...), entropy (...), stats (rows, 2) for the backward or None, top_ids
+    (..., top) int64, top_logprobs (..., top) float32)."""
     require_one_device(logits, targets)
     dev = logits.device
     x = _rows(logits)
@@ -40,17 +47,16 @@ def token_logprobs_forward(logits, targets, top, ignore_index):
     rows, V = x.shape
     tg = _targets(targets)
     shape = logits.shape[:-1]
-    f32 = dict(dtype=torch.float32, device=dev)
-    lp, H = torch.empty(shape, **f32), torch.empty(shape, **f32)
-    stats = torch.empty((rows, 2), **f32)
+    f32 = torch.float32
+    lp, H = torch.empty(shape, dtype=f32, device=dev), torch.empty(shape, dtype=f32, device=dev)
+    stats = torch.empty((rows, 2), dtype=f32, device=dev) if with_stats else None
     ids = torch.empty((*shape, top), dtype=torch.int64, device=dev)
-    tl = torch.empty((*shape, top), **f32)
-    nbytes = _lib.load().sa_token_logprobs_workspace_size(rows, V, top)
+    tl = torch.empty((*shape, top), dtype=f32, device=dev)
+    nbytes = _workspace_bytes(rows, V, top)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
-    call_on(x, "sa_token_logprobs_fwd", act_dtype_code(x.dtype), _lib.ptr(x), _stride(x),
-            _lib.ptr(tg), rows, V, top, int(ignore_index), _lib.ptr(lp), _lib.ptr(H),
-            _lib.ptr(stats), _lib.ptr(ids), _lib.ptr(tl), _lib.ptr(ws), nbytes,
-            _lib.stream_of(x))
+    call_on(x, "sa_token_logprobs_fwd", act_dtype_code(x.dtype), x.data_ptr(), _stride(x),
+            tg.data_ptr(), rows, V, top, ignore_index, lp.data_ptr(), H.data_ptr(),
+            _lib.ptr(stats), ids.data_ptr(), tl.data_ptr(), _lib.ptr(ws), nbytes, _lib.stream_of(x))
     return lp, H, stats, ids, tl
 
 

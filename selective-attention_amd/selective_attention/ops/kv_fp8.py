@@ -41,12 +41,14 @@ def paged_kv_append_fp8(k: torch.Tensor, v: torch.Tensor, log_gate: torch.Tensor
                         v_pages: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
                         k_tail: torch.Tensor, v_tail: torch.Tensor,
                         gate_pages: torch.Tensor | None) -> None:
-    check_ndim(k, 3, name="k")
-    check_ndim(k_pages, 4, name="k_pages")
-    b = k.shape[0]
-    check_shape(k, (b, k_pages.shape[1], k_pages.shape[3]), name="k")
-    check_shape(v, tuple(k.shape), name="v")
-    check_shape(log_gate, tuple(k.shape[:2]), name="log_gate", optional=True)
+    ks, ps = k.shape, k_pages.shape
+    if not (len(ks) == 3 and len(ps) == 4 and ks[1] == ps[1] and ks[2] == ps[3] and v.shape == ks
+            and (log_gate is None or log_gate.shape == ks[:2])):
+        check_ndim(k, 3, name="k")
+        check_ndim(k_pages, 4, name="k_pages")
+        check_shape(k, (ks[0], ps[1], ps[3]), name="k")
+        check_shape(v, tuple(ks), name="v")
+        check_shape(log_gate, tuple(ks[:2]), name="log_gate", optional=True)
     if (log_gate is None) != (gate_pages is None):
         raise ValueError("log_gate and gate_pages go together: give both or neither")
     _k.paged_kv_append_fp8(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, k_scale,

@@ -77,5 +77,5 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     top, ignore_index = int(top), int(ignore_index)
     if (torch.is_grad_enabled() and logits.requires_grad) or in_forward_mode():
         return TokenLogprobs(*TokenLogprobsFn.apply(logits, targets, top, ignore_index))
-    lp, H, _, ids, tl = _k.token_logprobs_forward(logits, targets, top, ignore_index)
+    lp, H, _, ids, tl = _k.token_logprobs_forward(logits, targets, top, ignore_index, False)
     return TokenLogprobs(lp, H, ids, tl)
