@@ -338,11 +338,11 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
 }
 
 // Short tables: one workgroup a (row, kv head), its waves taking the row's tiles in
-// turn and joining in LDS, so that no second launch and no workspace follow.  The
+// turn and joining in LDS (32 KB of sums O^T), so that no second launch and no workspace follow.  The
 // rows' own lengths stand on the device; the table's width, which bounds them, is
 // what the host can go by.
 template <int D>
-constexpr int kShortWaves = 512 / D;   // their sums O^T fill 32 KB: 16 columns of D fp32 each
+constexpr int kShortWaves = 512 / D;   // (half or twice as many: 16 rows of 1024 keys, D 64, 12.7 or 10.2 us; 9.9 so)
 template <int D, bool BIAS, int PS>
 __global__ __launch_bounds__(64 * kShortWaves<D>) void paged_decode_fp8_short_kernel(
     const bf16* __restrict__ q, const Fp8Cache kv, const int32_t* __restrict__ seq_lens,
