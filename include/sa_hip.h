@@ -363,8 +363,8 @@ int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zer
  * (rows, vocab) in `dtype` (f32 or bf16) with row stride ld (elements), targets
  * (rows) int64; all outputs f32 unless said:
  *   logprob (rows): log p of targets[r]; 0 at ignore_index, NaN for any other id
- *   outside the vocabulary.  entropy (rows): -sum p log p.  stats (rows, 2): n
- *   and log2 sum 2^(x log2(e) + n), for the backward, or NULL.  top_ids (rows,
+ *   outside the vocabulary.  entropy (rows): -sum p log p.  stats (rows, 2): m
+ *   = max x and log2 sum 2^((x - m) log2(e)), for the backward, or NULL.  top_ids (rows,
  *   top) int64 and top_logprobs (rows, top): the largest, ties to the lowest id;
  *   top 0..64 and <= vocab, both may be NULL for 0.  workspace: of the size that
  *   sa_token_logprobs_workspace_size says, 16-byte aligned (0 bytes: NULL).

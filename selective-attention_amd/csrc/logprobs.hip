@@ -1,13 +1,19 @@
 // Log probabilities of given tokens with the distribution's entropy, its largest
-// alternatives, and the gradient (gfx950).  For a row x of V logits, with a
-// reference n near -max x log2(e) and a_j = x_j c + n, c fp32's log2(e) (one fma,
-// exact but for its one rounding), s = sum_j 2^a_j, t = sum_j a_j 2^a_j:
+// alternatives, and the gradient (gfx950).  For a row x of V logits with the
+// largest m, a_j = (x_j - m) log2(e), s = sum_j 2^a_j, t = sum_j a_j 2^a_j:
 //
-//   log p_j = x_j - lse,  lse = (log2 s - n) / c  (this one in fp64; by c and not
-//   log2(e), so that a single large logit gives its own value),
+//   log p_j = (x_j - m) - ln 2 log2 s  (in fp64),
 //   H = -sum_j p_j log p_j = ln 2 (log2 s - t / s)
 //   d/dx_j  (a log p_i + h H + sum_k b_k log p_{i_k})
 //         = a [j = i] + sum_k b_k [j = i_k] - p_j (a + sum_k b_k + h (log p_j + H))
+//
+// The maximum is taken off in the logits' own unit: the difference is exact near
+// it and 0 at it, whatever the logits' size.  (One fma, x_j log2(e) + n with n =
+// -m log2(e) rounded, would save an instruction a logit, but carries n's rounding
+// into every exponent: up to 64 at m = 1e9, and at the type's lowest value n itself
+// is infinite, so that a mask of a large finite value over a whole piece made
+// its row NaN.  8192 x 32000 bf16, 20 alternatives: 115.3 us so, 117.9; without
+// alternatives, and in the gradient, level.)
 //
 // All sums in fp32.  Both directions are bound by the bytes of the logits: the
 // forward reads them once, the backward reads them and writes the gradient.
@@ -15,7 +21,7 @@
 // Forward: one workgroup a row, which stands in registers (64 logits a thread)
 // while its maximum, then the sums, then the alternatives are taken, so that no
 // running maximum rescales sums inside a piece; longer rows go in pieces joined
-// by their references.  bf16 logits stay packed and are widened anew in each
+// by their maxima.  bf16 logits stay packed and are widened anew in each
 // pass (the registers are made opaque in between, or the compiler keeps all 64
 // widened: 146 registers and 190 us for 8192 x 32000, against 63 and 95).
 //
@@ -37,8 +43,7 @@ constexpr int kList = 512;   // candidates of a piece
 // 2^a is 0 in fp32 from here down: a logit of -inf is taken as this in a 2^a,
 // which is then 0 and stays so under any factor
 constexpr float kFloor = -160.0f;
-constexpr float kLn2 = 0.6931471805599453f;
-constexpr double kInvLog2e = 1.0 / static_cast<double>(kLog2e);
+constexpr double kLn2 = 0.6931471805599453;
 
 constexpr uint32_t kOrderNan = 0xffffffffu, kOrderInf = 0xff800000u, kOrderLow = 0x007fffffu;   // NaN, +inf, -inf
 // floats in the order of their values as unsigned numbers above 0: -inf lowest,
@@ -186,20 +191,21 @@ __device__ __forceinline__ int block_scan(int c, int* wtot, int& total) {
   return pre;
 }
 
-// sums s, t of two sets of logits against their references n (+inf: none), joined
-// against the larger one
-__device__ __forceinline__ void join_sums(float& n, float& s, float& t, float n2, float s2, float t2) {
-  const float nn = fminf(n, n2);
+// sums s, t of two sets of logits against their maxima m (-inf: no finite logit,
+// s and t are 0 or NaN), joined against the larger one.  No sum is infinite, as
+// 2^a <= 1, so a factor of 0 leaves 0 or the NaN.
+__device__ __forceinline__ void join_sums(float& m, float& s, float& t, float m2, float s2, float t2) {
+  const float mm = fmaxf(m, m2);
   auto shift = [&](float from, float& ss, float& tt) {
-    if (from != nn && ss != 0.0f) {
-      const float dm = nn - from, f = fast_exp2(dm);
-      tt = fmaf(fmaxf(dm, kFloor), ss, tt) * f;
+    if (from != mm) {
+      const float da = (from - mm) * kLog2e, f = fast_exp2(da);
+      tt = fmaf(fmaxf(da, kFloor), ss, tt) * f;
       ss *= f;
     }
   };
-  shift(n, s, t);
-  shift(n2, s2, t2);
-  n = nn;
+  shift(m, s, t);
+  shift(m2, s2, t2);
+  m = mm;
   s += s2;
   t += t2;
 }
@@ -208,26 +214,25 @@ __device__ __forceinline__ void join_sums(float& n, float& s, float& t, float n2
 // more of a workgroup
 template <typename T>
 __device__ __forceinline__ void finish_row(const T* x, long row, long target, int V, int top, long ignore,
-                                           float n, float s, float t, const uint64_t* best,
+                                           float m, float s, float t, const uint64_t* best,
                                            float* logprob, float* entropy, float* stats,
                                            int64_t* top_ids, float* top_lp) {
-  if (n == __builtin_huge_valf()) s = __builtin_nanf("");   // no finite logit
+  if (m == -__builtin_huge_valf()) s = __builtin_nanf("");   // no finite logit
   const float l2s = log2f(s);
-  const double lse = kInvLog2e * (static_cast<double>(l2s) - static_cast<double>(n));
   // roundings keep on their side of 0 (and NaN stays)
   auto log_p = [&](float v) {
-    const float lp = static_cast<float>(static_cast<double>(v) - lse);
+    const float lp = static_cast<float>((static_cast<double>(v) - m) - kLn2 * l2s);
     return lp > 0.0f ? 0.0f : lp;
   };
   if (threadIdx.x == 0) {
     float lp = 0.0f;
     if (target != ignore)
       lp = target >= 0 && target < V ? log_p(to_f32(x[target])) : __builtin_nanf("");
-    const float h = kLn2 * (l2s - t / s);
+    const float h = static_cast<float>(kLn2) * (l2s - t / s);
     logprob[row] = lp;
     entropy[row] = h < 0.0f ? 0.0f : h;
     if (stats) {
-      stats[2 * row] = n;
+      stats[2 * row] = m;
       stats[2 * row + 1] = l2s;
     }
   }
@@ -243,7 +248,7 @@ __device__ __forceinline__ void finish_row(const T* x, long row, long target, in
 // SplitSums, then (rows, splits, top) keys, those behind a split's count not
 // written.
 struct SplitSums {
-  float n, s, t;
+  float m, s, t;
   int count;
 };
 
@@ -272,7 +277,7 @@ __global__ __launch_bounds__(NT, WPE) void token_logprobs_kernel(
 
   const __amdgpu_buffer_rsrc_t rsrc = row_rsrc(x, off, V);
 
-  float n = kInf, s = 0.0f, t = 0.0f;   // n: minus the reference; +inf before there is one
+  float m = -kInf, s = 0.0f, t = 0.0f;
   int nbest = 0;
   (void)nbest;
   const int step = SPLIT ? CH * static_cast<int>(gridDim.y) : CH;
@@ -324,13 +329,13 @@ __global__ __launch_bounds__(NT, WPE) void token_logprobs_kernel(
       mc = block_max<NW>(mx, red);
     }
     // a piece of -inf alone (or with NaN) is taken against 0: its terms are 0 (or NaN)
-    float nc = mc == -kInf ? 0.0f : -mc * kLog2e;
+    const float off_max = mc == -kInf ? 0.0f : mc;
     float sc = 0.0f, tc = 0.0f;
 #pragma unroll
     for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float a = fmaf(elem(raw[p], i), kLog2e, nc);
+        const float a = (elem(raw[p], i) - off_max) * kLog2e;
         const float e = fast_exp2(a);
         sc += e;
         tc = fmaf(fmaxf(a, kFloor), e, tc);
@@ -338,7 +343,7 @@ __global__ __launch_bounds__(NT, WPE) void token_logprobs_kernel(
 #pragma unroll
     for (int p = 0; p < P; ++p) opaque(raw[p]);
     block_sum2<NW>(sc, tc, red2);
-    join_sums(n, s, t, mc == -kInf ? kInf : nc, sc, tc);
+    join_sums(m, s, t, mc, sc, tc);
 
     if constexpr (TOP) {
       if constexpr (NW == 1) __syncthreads();   // bound, count (block_sum2's barrier elsewhere)
@@ -467,12 +472,12 @@ __global__ __launch_bounds__(NT, WPE) void token_logprobs_kernel(
   }
   if constexpr (SPLIT) {
     const long at = row * gridDim.y + blockIdx.y;
-    if (tid == 0) split[at] = SplitSums{n, s, t, nbest};
+    if (tid == 0) split[at] = SplitSums{m, s, t, nbest};
     if constexpr (TOP) {
       if (tid < nbest) split_keys[at * top + tid] = best[tid];
     }
   } else {
-    finish_row(x, row, targets[row], V, TOP ? top : 0, ignore, n, s, t, best, logprob, entropy, stats,
+    finish_row(x, row, targets[row], V, TOP ? top : 0, ignore, m, s, t, best, logprob, entropy, stats,
                top_ids, top_lp);
   }
 }
@@ -486,12 +491,12 @@ __global__ __launch_bounds__(64) void token_logprobs_join_kernel(
   __shared__ uint64_t list[2 * kMaxTop], best[kMaxTop];
   const long row = blockIdx.x;
   const int lane = threadIdx.x;
-  float n = __builtin_huge_valf(), s = 0.0f, t = 0.0f;
+  float m = -__builtin_huge_valf(), s = 0.0f, t = 0.0f;
   int nbest = 0;
   for (int p = 0; p < splits; ++p) {
     const long at = row * splits + p;
     const SplitSums q = split[at];
-    join_sums(n, s, t, q.n, q.s, q.t);
+    join_sums(m, s, t, q.m, q.s, q.t);
     if (top == 0) continue;
     if (lane < nbest) list[lane] = best[lane];
     if (lane < q.count) list[nbest + lane] = split_keys[at * top + lane];
@@ -505,7 +510,7 @@ __global__ __launch_bounds__(64) void token_logprobs_join_kernel(
     nbest = min(nl, top);
     __syncthreads();
   }
-  finish_row(logits + row * ld, row, targets[row], V, top, ignore, n, s, t, best, logprob, entropy, stats,
+  finish_row(logits + row * ld, row, targets[row], V, top, ignore, m, s, t, best, logprob, entropy, stats,
              top_ids, top_lp);
 }
 
@@ -530,7 +535,7 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(
   const int off = VEC ? static_cast<int>((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T)) : 0;
   const int base = static_cast<int>(blockIdx.y) * CH - off;
   const __amdgpu_buffer_rsrc_t rsrc = row_rsrc(x, off, V);
-  const float n = stats[2 * row], l2s = stats[2 * row + 1], H = entropy[row];
+  const float m = stats[2 * row], l2s = stats[2 * row + 1], H = entropy[row];
   const long tg = targets[row];
   const bool asked = tg != ignore;
   float a = asked && g_lp ? g_lp[row] : 0.0f;
@@ -543,9 +548,9 @@ __global__ __launch_bounds__(256) void token_logprobs_bwd_kernel(
       all += g_top[row * top + k];
       silent = silent && g_top[row * top + k] == 0.0f;
     }
-  const float hl = h * kLn2, c = fmaf(h, H, all);   // a + sum b + h (log p + H) = hl log2 p + c
+  const float hl = h * static_cast<float>(kLn2), c = fmaf(h, H, all);   // a + sum b + h (log p + H) = hl log2 p + c
   auto grad = [&](float xv) {
-    const float lp = fmaf(xv, kLog2e, n) - l2s;
+    const float lp = fmaf(xv - m, kLog2e, -l2s);
     return silent ? 0.0f : -fast_exp2(lp) * fmaf(hl, fmaxf(lp, kFloor), c);
   };
 #pragma unroll

@@ -52,7 +52,8 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
                    ignore_index: int = -100) -> TokenLogprobs:
     """
     Args:
-        logits: (..., vocab) float32 or bfloat16; -inf rules a token out
+        logits: (..., vocab) float32 or bfloat16 of any finite size; -inf rules a
+            token out
         targets: (...) int32 or int64 token ids.  ignore_index: logprob 0 and no
             gradient from it, whatever the row holds; any other id outside the
             vocabulary: NaN

@@ -354,3 +354,125 @@ def test_graph_of_forward_and_backward():
         torch.randn(64, 64, device="cuda").sum()
         for a, b in zip(got, w):
             assert torch.equal(a, b)
+
+
+# --- finite logits of any size ---------------------------------------------------
+def shifted(x):
+    """x in float64 less each row's maximum: the same distribution.  Beside 1e30 the
+    logarithm of a sum is below float64's own step."""
+    x = x.double()
+    return x - x.amax(1, keepdim=True)
+
+
+def near_shifted(out, x, t, top):
+    """The results for x against those for shifted(x), rounded to fp32 (differences
+    of two logits may pass its range)."""
+    lp, H, ids, tl = ref.forward(shifted(x), t, top)
+    near(out.logprob, lp.float(), "logprob")
+    near(out.entropy, H, "entropy", E_H)
+    assert torch.equal(out.top_ids.cpu(), ids)
+    near(out.top_logprobs, tl.float(), "top_logprobs")
+
+
+def masked_rows(V, dtype, mask):
+    """Rows where all but ten tokens hold `mask`, the ten first, last, in the
+    middle and spread over the row, and one where every token does."""
+    low = torch.finfo(dtype).min if mask == "lowest" else mask
+    x = torch.full((5, V), low, dtype=torch.float64)
+    g = torch.Generator().manual_seed(V)
+    keep = [torch.arange(10), torch.arange(V - 10, V), torch.arange(V // 2, V // 2 + 10),
+            torch.randperm(V, generator=g)[:10]]
+    for r, j in enumerate(keep):
+        x[r, j] = torch.randn(10, generator=g).double() * 3
+    t = torch.tensor([int(j[3]) for j in keep] + [V // 3])
+    return x.to(dtype), t
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e10, -1e30, "lowest"])
+@pytest.mark.parametrize("V,rows,top", [(5000, 1, 0), (5000, 600, 20), (40000, 1, 20), (40000, 600, 0),
+                                        (40000, 600, 20), (131072, 1, 0), (131072, 1, 20), (131072, 600, 20)])
+def test_finite_masks(V, rows, top, mask, dtype):
+    """Masks of a large finite value, over whole pieces of a row and over all of it
+    (then the row is uniform): what -inf in their place gives, and -log V."""
+    x, t = masked_rows(V, dtype, mask)
+    if rows == 1:
+        for r in range(5):
+            near_shifted(token_logprobs(x[r:r + 1].cuda(), t[r:r + 1].cuda(), top=top), x[r:r + 1], t[r:r + 1], top)
+        return
+    of = torch.arange(rows) % 5
+    out = token_logprobs(x.cuda()[of.cuda()], t[of].cuda(), top=top)
+    for a, name in zip(out, out._fields):
+        want = a[:5]
+        for i in range(5, rows, 5):   # rows stand at different places to a 16-byte boundary
+            if name == "top_ids":
+                assert torch.equal(a[i:i + 5], want)
+            else:
+                near(a[i:i + 5], want.cpu(), name, 2 * (E_H if name == "entropy" else E_LP))
+    near_shifted(type(out)(*(a[:5] for a in out)), x, t, top)
+
+
+def grad_near(x, t, top):
+    g = torch.Generator().manual_seed(7)
+    rows = x.shape[0]
+    up = [torch.randn(rows, generator=g), torch.randn(rows, generator=g),
+          torch.randn(rows, top, generator=g) if top else None]
+    leaf = x.cuda().requires_grad_(True)
+    out = token_logprobs(leaf, t.cuda(), top=top)
+    pairs = [(o, u.cuda()) for o, u in zip((out.logprob, out.entropy, out.top_logprobs), up) if u is not None]
+    (dx,) = torch.autograd.grad([p[0] for p in pairs], leaf, [p[1] for p in pairs])
+    z = shifted(x)
+    want = ref.backward(z, t, *up, top=top)
+    size = sum(float(u.abs().max()) * (u.shape[-1] if u.dim() > 1 else 1) for u in up if u is not None)
+    half = 2.0 ** -8 if x.dtype == torch.bfloat16 else 2.0 ** -24
+    own = torch.zeros_like(z).scatter_(1, t[:, None], 1.0).scatter_(1, ref.forward(z, t, top)[2], 1.0)
+    tol = E_P * size * torch.softmax(z, 1) + 4 * 2.0 ** -24 * size * own
+    err = (dx.double().cpu() - want).abs()
+    assert (err <= tol + half * want.abs() + 1e-38).all(), float((err - tol - half * want.abs()).max())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mask", [-1e10, -1e30, "lowest"])
+@pytest.mark.parametrize("V,top", [(5000, 0), (40000, 20), (131072, 3)])
+def test_gradient_of_finite_masks(V, top, mask, dtype):
+    grad_near(*masked_rows(V, dtype, mask), top)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("V", [500, 70001])
+def test_logits_of_any_finite_size(V, dtype):
+    """Three equal largest logits of any size, in different pieces where the row
+    has several: each has probability 1 / 3, the others none.  And logits from
+    one end of the type's range to the other."""
+    sizes = [1e7, 1e8, 5e9, -5e9, 1e20, 1e30, -1e30, 3e38, -3e38]
+    x = torch.tensor(sizes, dtype=torch.float64)[:, None].expand(-1, V).clone()
+    x -= 0.125 * x.abs()
+    for j in (7, V // 2, V - 1):
+        x[:, j] = torch.tensor(sizes, dtype=torch.float64)
+    x = x.to(dtype)
+    t = torch.full((len(sizes),), 7)
+    t[1::2] = 8
+    for n in (1, len(sizes)):
+        near_shifted(token_logprobs(x[:n].cuda(), t[:n].cuda(), top=2), x[:n], t[:n], 2)
+    grad_near(x, t, 2)
+    ends = torch.full((2, V), -3e38, dtype=torch.float64)
+    ends[:, V - 3] = 3e38
+    ends, t = ends.to(dtype), torch.tensor([V - 3, 0])
+    near_shifted(token_logprobs(ends.cuda(), t.cuda(), top=1), ends, t, 1)
+
+
+@pytest.mark.gpu
+def test_distributions_far_from_zero():
+    """Rows moved by a number that keeps every difference exact: the distribution of
+    the row around zero."""
+    g = torch.Generator().manual_seed(3)
+    near0 = torch.randint(-64, 65, (4, 33000), generator=g).double() / 8
+    t = torch.randint(0, 33000, (4,), generator=g)
+    for by in (2.0 ** 17, -2.0 ** 17, 2.0 ** 20 - 8):     # steps of 2^-7 to 2^-4 there
+        x = (near0 + by).float()
+        assert torch.equal(x.double() - by, near0)
+        near_shifted(token_logprobs(x.cuda(), t.cuda(), top=5), x, t, 5)
+        grad_near(x, t, 5)
