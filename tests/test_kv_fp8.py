@@ -648,3 +648,68 @@ def test_attention_rows_as_long_as_a_short_table(b, H, D, ps, lens, gated):
             e = (D + 4) * 2.0 ** -24 * float(big.max())
             err = (o[r, h].double() - want).abs()
             assert (err <= (2.0 ** -8 + 2.5 * e) * A + 2.0 ** -8 * want.abs()).all(), (r, h)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("D,ps,gated", [(64, 64, True), (64, 128, False), (128, 64, False), (128, 128, True)])
+def test_attention_keeps_its_weights(D, ps, gated, wide):
+    """Outputs that are small differences of large sums: as many values of 1 as of
+    -1, under weights e^s of scores s in steps of 2^-7.  A weight stands in the
+    products as two bf16 numbers, which is off by 2^-16 of it; s by 2.5 e A as in
+    check_attention, e^s by 2^-21, the sums over the keys by (n / 32 + 40) 2^-24
+    (n at most 600): below (2^-15 + 2.5 e) A together, and one rounding to bf16."""
+    lens, H = [2, 10, 64, 70, 128, 256, 600], 2
+    b, L = len(lens), max(lens)
+    g = torch.Generator().manual_seed(D)
+    k = torch.zeros(b, H, L, D)
+    k[..., 0] = torch.randint(0, 16, (b, H, L), generator=g).float()   # exact in e4m3
+    q = torch.zeros(b, H, D, dtype=torch.bfloat16)
+    q[..., 0] = 1.0
+    v = torch.empty(b, H, L, D)
+    for r, n in enumerate(lens):
+        sign = torch.ones(H, D, n)
+        sign[..., n // 2:] = -1.0
+        at = torch.rand(H, D, n, generator=g).argsort(-1)
+        v[r, :, :n] = sign.gather(-1, at).transpose(1, 2)
+    k, v, lg = k.to(torch.bfloat16), v.to(torch.bfloat16), torch.zeros(b, H, L) if gated else None
+    width = (L + ps - 1) // ps
+    table, c = make_cache(b, H, D, ps, width, gated, "cuda")
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    build(k.cuda(), v.cuda(), None if lg is None else lg.cuda(), table, sl, c)
+    if wide:
+        table = torch.cat([table, torch.full((b, 36), -1, dtype=torch.int32, device="cuda")], 1)
+    sc = 2.0 ** -7
+    o = attend(q.cuda(), c, table, sl, softmax_scale=sc).double().cpu()
+    e = (D + 4) * 2.0 ** -24 * sc * 15
+    for r, cr in enumerate(refs(k, v, lg, lens, ps)):
+        for h in range(H):
+            kk, vv = cr[h].keys_values()
+            want = ref.attend(q[r, h], kk, vv, None, sc)
+            err = (o[r, h] - want).abs()      # A = 1
+            assert (err <= 2.0 ** -15 + 2.5 * e + 2.0 ** -8 * want.abs()).all(), (lens[r], h, float(err.max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("wide", [False, True])
+def test_infinite_values_of_an_open_block(D, wide):
+    """They stand as they are until the block is rounded: the output has them, in
+    their own dimension alone, and NaN where both signs meet."""
+    H, ps, n = 2, 64, 90
+    k, v, _ = tokens(1, H, n, D, False, seed=14, spread=False)
+    clean_v = v.clone()
+    v[0, 0, 70, 3], v[0, 0, 80, 5], v[0, 0, 64, 9], v[0, 0, 89, 9] = INF, -INF, INF, -INF
+    q = torch.randn(1, H, D, generator=torch.Generator().manual_seed(5)).to(torch.bfloat16)
+    sl = torch.full((1,), n, dtype=torch.int32, device="cuda")
+    out = []
+    for values in (clean_v, v):
+        table, c = make_cache(1, H, D, ps, 2, False, "cuda")
+        build(k.cuda(), values.cuda(), None, table, sl, c)
+        if wide:
+            table = torch.cat([table, torch.full((1, 36), -1, dtype=torch.int32, device="cuda")], 1)
+        out.append(attend(q.cuda(), c, table, sl).float().cpu())
+    clean, o = out
+    assert o[0, 0, 3] == INF and o[0, 0, 5] == -INF and torch.isnan(o[0, 0, 9])
+    rest = [d for d in range(D) if d not in (3, 5, 9)]
+    assert torch.equal(o[0, 0, rest], clean[0, 0, rest]) and torch.equal(o[0, 1], clean[0, 1])
