@@ -12,9 +12,11 @@
 //   sum_k x (c - z) = 16 (sum_k x (1 + c / 16) - (1 + z / 16) sum_k x)
 //
 // both sums on the matrix cores (16x16x32, the weights as the A operand, x as
-// B; sum_k x as the product with ones, once for all tiles of a wave).  The
-// difference costs at most three to four bits of fp32's 24, so a result is
-// off by about 2^-20 of sum |x w| before its one rounding to bf16.
+// B; sum_k x as the product with ones, once for all tiles of a wave).  Both are
+// rounded on their own, so a result is off by at most (K / 32 + 36) 2^-24 times 16
+// (1.94 + 1.94) sum_k s |x_k| before its one rounding to bf16: a share of s |x|,
+// not of |x w|, which codes at the zero point do not make smaller.  A group without
+// a weight has s = 0 and adds exactly nothing.
 //
 // Packed weights: tiles of 16 rows and 128 columns, (N / 16, K / 128, 64, 16)
 // bytes, so that one 16-byte load a lane is a tile.  Lane 16 g + c holds row c;

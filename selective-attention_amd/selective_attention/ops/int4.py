@@ -68,7 +68,8 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool =
     """weight (out_features, in_features) -> (packed, scales, zeros or None), each
     group rounded to the nearest code: symmetric, scale = max|w| / 7 around
     code 8; else scale = (max - min) / 15 over the group's range with 0 in it and
-    zero points.  The codes are chosen for the scale as bfloat16 keeps it."""
+    zero points.  The codes are chosen for the scale as bfloat16 keeps it; a group
+    of zeros has the scale 0 and so adds exactly nothing."""
     check_ndim(weight, 2, name="weight")
     if group_size not in _k.GROUPS:
         raise ValueError(f"group_size {group_size} must be one of {_k.GROUPS}")
@@ -84,10 +85,10 @@ def quantize_int4(weight: torch.Tensor, group_size: int = 128, symmetric: bool =
         lo, hi = w.amin(2).clamp(max=0.0), w.amax(2).clamp(min=0.0)
         s = (hi - lo) / 15.0
     s = s.to(torch.bfloat16)
-    s = torch.where(s > 0, s, torch.ones_like(s))
+    by = torch.where(s > 0, s, torch.ones_like(s)).float()
     if not symmetric:
-        zero = torch.round(-lo / s.float()).clamp(0, 15)
-    q = torch.round(w / s.float()[..., None]) + (8.0 if zero is None else zero[..., None])
+        zero = torch.round(-lo / by).clamp(0, 15)
+    q = torch.round(w / by[..., None]) + (8.0 if zero is None else zero[..., None])
     codes = q.clamp(0, 15).to(torch.uint8).reshape(N, -1)[:, :K]
     return pack_int4(codes, s, zero, group_size)
 

@@ -339,3 +339,40 @@ def test_layer_matches_linear_on_its_own_weights():
         assert torch.equal(mixed[0], y)
         assert torch.equal(mixed[1], lin(x.cuda()))
     assert (w - lin.weight.double().cpu()).abs().max() <= 0.55 * q.scales.double().abs().max()
+
+
+# --- groups without a weight -------------------------------------------------------
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("G", [32, 64, 128])
+def test_quantize_gives_a_group_of_zeros_the_scale_zero(G, symmetric):
+    w = torch.randn(20, 300, generator=torch.Generator().manual_seed(2))
+    w[3] = 0.0
+    w[:, G:2 * G] = 0.0
+    packed = quantize_int4(w, G, symmetric)
+    s = packed[1].float().transpose(1, 2).reshape(-1, packed[1].shape[1])[:20, :(300 + G - 1) // G]
+    zero = torch.zeros_like(s, dtype=torch.bool)
+    zero[3], zero[:, 1] = True, True
+    assert not s[zero].any() and (s[~zero] > 0).all()
+    assert not ref.weight(*packed, 20, 300)[w == 0].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("symmetric", [True, False])
+@pytest.mark.parametrize("M,K,G", [(1, 256, 128), (7, 1000, 32), (20, 2055, 64), (64, 4300, 128), (80, 512, 64)])
+def test_groups_of_zeros_add_nothing(M, K, G, symmetric):
+    """A weight's rows and groups of zeros beside large activations: exactly nothing."""
+    g = torch.Generator().manual_seed(K)
+    w = torch.randn(40, K, generator=g) * 0.02
+    w[[0, 17, 39]] = 0.0
+    w[:, G:2 * G] = 0.0
+    b = torch.randn(40, generator=g).to(torch.bfloat16)
+    x = torch.randn(M, K, generator=g).to(torch.bfloat16)
+    packed = quantize_int4(w, G, symmetric)
+    d = dev(packed)
+    base = int4_linear(x.cuda(), *d, bias=b.cuda(), out_features=40)
+    x[:, G:2 * G] *= 10000.0
+    y = int4_linear(x.cuda(), *d, bias=b.cuda(), out_features=40)
+    assert torch.equal(y, base)
+    x *= 10000.0
+    y = int4_linear(x.cuda(), *d, bias=b.cuda(), out_features=40).cpu()
+    assert torch.equal(y[:, [0, 17, 39]], b[[0, 17, 39]].expand(M, 3))
