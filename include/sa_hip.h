@@ -383,8 +383,6 @@ int sa_token_logprobs_bwd(int dtype, const void* logits, long ld, const int64_t*
                           const float* g_entropy, const float* g_top, void* dlogits, long ldd,
                           void* stream);
 
-
-
 /*
  * SwiGLU's gated product (modules/feed_forward.py:10-11): out = bf16(a *
  * bf16(silu(c))), n bf16 elements (n % 8 == 0, 16-byte aligned).

@@ -929,17 +929,6 @@ int decode_plan_launch(const int32_t* seq_lens, int batch, int page_size, int ma
   return 0;
 }
 
-// merge of the segments that a W-wave stream-K decode left in ws
-int decode_merge_launch(int batch, int num_q_heads, int num_kv_heads, int head_dim, void* o,
-                        const DecodeWs& ws, int W, hipStream_t s) {
-  sa::ProfScope prof_("paged_decode_merge", s);
-  hipLaunchKernelGGL(sa::paged_decode_merge_kernel, dim3(batch * num_q_heads), dim3(64), 0, s,
-                     ws.part_o, ws.part_ml, ws.cum_row, static_cast<sa::bf16*>(o), batch,
-                     num_q_heads, num_kv_heads, head_dim, W);
-  SA_CHECK_LAUNCH("paged_decode_merge");
-  return 0;
-}
-
 // plan (more than 64 rows), stream-K decode and merge on workspace `ws` with W waves
 int decode_launch(const void* q, const void* k_pages, const void* v_pages,
                   const int32_t* page_table, const int32_t* seq_lens, const float* key_bias,
@@ -964,7 +953,12 @@ int decode_launch(const void* q, const void* k_pages, const void* v_pages,
       key_bias ? launch(sa::paged_decode_kernel<64, true>) : launch(sa::paged_decode_kernel<64, false>);
     SA_CHECK_LAUNCH("paged_decode");
   }
-  return decode_merge_launch(batch, num_q_heads, num_kv_heads, head_dim, o, ws, W, s);
+  sa::ProfScope prof_("paged_decode_merge", s);
+  hipLaunchKernelGGL(sa::paged_decode_merge_kernel, dim3(batch * num_q_heads), dim3(64), 0, s,
+                     ws.part_o, ws.part_ml, ws.cum_row, static_cast<sa::bf16*>(o), batch,
+                     num_q_heads, num_kv_heads, head_dim, W);
+  SA_CHECK_LAUNCH("paged_decode_merge");
+  return 0;
 }
 
 }  // namespace sa

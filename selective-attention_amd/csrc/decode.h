@@ -101,8 +101,6 @@ inline int decode_waves(K kern, int variant) {
 
 int decode_plan_launch(const int32_t* seq_lens, int batch, int page_size, int max_pages,
                        const DecodeWs& ws, hipStream_t s);
-int decode_merge_launch(int batch, int num_q_heads, int num_kv_heads, int head_dim, void* o,
-                        const DecodeWs& ws, int W, hipStream_t s);
 int decode_check(int dtype, const void* q, const void* k_pages, const void* v_pages,
                  const int32_t* page_table, const int32_t* seq_lens, const float* key_bias,
                  int batch, int num_q_heads, int num_kv_heads, int head_dim, int page_size,

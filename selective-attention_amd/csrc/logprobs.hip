@@ -638,7 +638,7 @@ void launch_logprobs(const void* logits, long ld, const int64_t* targets, long r
 int logprobs_check(const char* who, int dtype, const void* logits, long ld, const int64_t* targets,
                    long rows, int V, int top) {
   SA_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype %d", who, dtype);
-  // (2^32 threads a grid, 256 a row)
+  // (2^32 threads a grid, up to 512 a row)
   SA_CHECK_ARG(rows >= 0 && rows < (1L << 23) && V > 0 && V <= (1 << 28) && ld >= V,
                "%s: bad sizes rows=%ld vocab=%d row stride=%ld", who, rows, V, ld);
   SA_CHECK_ARG(top >= 0 && top <= kMaxTop && top <= V, "%s: top %d must be 0..%d and at most the vocab %d",
