@@ -434,7 +434,7 @@ void int4_stream(const void* x, const void* xscale, Int4Segs& sg, int M, int K, 
 
 template <int G, bool Z>
 void int4_rows(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int ldx, hipStream_t s) {
-  const int kb = (K + 127) / 128;
+  const int kb = (K + 127) / 128;   // (int4_streams)
   auto stream = [&](auto kw) {
     constexpr int KW = decltype(kw)::value;
     M <= 16 ? int4_stream<1, G, Z, KW>(x, xscale, sg, M, K, ldx, s)
@@ -448,6 +448,8 @@ void int4_rows(const void* x, const void* xscale, Int4Segs& sg, int M, int K, in
   else int4_go<4, G, Z, 2, 8>(x, xscale, sg, M, K, ldx, s);
 }
 
+// whether int4_rows streams the tiles past x, else it goes tile by tile
+bool int4_streams(int K, int G) { return K <= (G > 32 ? 4096 : 2048); }
 bool int4_group_ok(int G) { return G == 32 || G == 64 || G == 128; }
 
 }  // namespace
@@ -468,6 +470,8 @@ extern "C" int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int
   sa::Int4Segs sg{};
   sg.nseg = nseg;
   const bool z = matrices[2] != 0;
+  // tile by tile a workgroup of 512 threads takes two (2^32 threads a grid)
+  const long max_tiles = sa::int4_streams(K, group) ? 1L << 27 : (1L << 24) - 2 * sa::kInt4Segs;
   long tiles = 0;
   for (int i = 0; i < nseg; ++i) {
     const int64_t* m = matrices + 6 * i;   // packed, scales, zeros, bias, y, N
@@ -476,7 +480,7 @@ extern "C" int sa_int4_linear_bf16(const void* x, const void* xscale, int M, int
     SA_CHECK_ARG((m[2] != 0) == z, "%s: zero points for all weight matrices or for none", who);
     SA_CHECK_ARG((m[0] & 15) == 0 && ((m[1] | m[2]) & 7) == 0, "%s: weight matrix %d is not aligned", who, i);
     tiles += (m[5] + 15) / 16;
-    SA_CHECK_ARG(tiles < (1 << 27), "%s: too many columns", who);
+    SA_CHECK_ARG(tiles < max_tiles, "%s: too many columns", who);
     sg.W[i] = reinterpret_cast<const uint4*>(m[0]);
     sg.scale[i] = reinterpret_cast<const sa::bf16*>(m[1]);
     sg.zero[i] = reinterpret_cast<const sa::bf16*>(m[2]);

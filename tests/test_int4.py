@@ -376,3 +376,18 @@ def test_groups_of_zeros_add_nothing(M, K, G, symmetric):
     x *= 10000.0
     y = int4_linear(x.cuda(), *d, bias=b.cuda(), out_features=40).cpu()
     assert torch.equal(y[:, [0, 17, 39]], b[[0, 17, 39]].expand(M, 3))
+
+
+def test_linear_refuses_grids_beyond_the_launch():
+    """Tile by tile (K of more than 4096) two tiles are a workgroup of 512 threads, and
+    a launch has fewer than 2^32; the kernel that streams its tiles has no such limit."""
+    import ctypes
+
+    from selective_attention import _lib
+    lib, at = _lib.load(), 4096   # refused before any pointer is read
+    words = [at, at, 0, 0, at, 1 << 26] * 4
+    rc = lib.sa_int4_linear_bf16(at, None, 1, 4352, 4352, 128, 4, (ctypes.c_int64 * 24)(*words), None)
+    assert rc == 1 and b"too many columns" in lib.sa_last_error()
+    words = [at, at, 0, 0, at, 1 << 30] * 4
+    rc = lib.sa_int4_linear_bf16(at, None, 1, 128, 128, 128, 4, (ctypes.c_int64 * 24)(*words), None)
+    assert rc == 1 and b"too many columns" in lib.sa_last_error()
