@@ -48,8 +48,8 @@ __device__ __forceinline__ v8bf widen8(uint32_t lo, uint32_t hi, float scale) {
 // 16 bytes of a buffer at a lane's and a constant offset.  NT: non-temporal, the
 // line is not kept.  The codes are read once a step, and without it the caches'
 // own traffic costs a tenth: 64 rows of 1 to 32 thousand keys, 8 heads of 128,
-// 456 us; 410 with it, 5.9 TB/s.  Only where a tile takes whole lines: at 128 keys a
-// page the two tiles of a V^T row share its line (5.1 TB/s without, 4.2 with).
+// 435 us; 386 with it, 6.3 TB/s.  Only where a tile takes whole lines: at 128 keys a
+// page the two tiles of a V^T row share its line (5.3 TB/s without, 4.3 with).
 template <bool NT>
 __device__ __forceinline__ uint4 buf_load16(__amdgpu_buffer_rsrc_t r, unsigned off) {
   return __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(r, off, 0, NT ? 2 : 0));
@@ -371,7 +371,7 @@ __global__ __launch_bounds__(64, 2) void paged_decode_fp8_kernel(
 // rows' own lengths stand on the device; the table's width, which bounds them, is
 // what the host can go by.
 template <int D>
-constexpr int kShortWaves = 512 / D;   // (half or twice as many: 16 rows of 1024 keys, D 64, 12.7 or 10.2 us; 9.9 so)
+constexpr int kShortWaves = 512 / D;   // (half or twice as many: 16 rows of 1024 keys, D 64, 11.8 or 15.7 us; 10.2 so)
 template <int D, bool BIAS, int PS>
 __global__ __launch_bounds__(64 * kShortWaves<D>) void paged_decode_fp8_short_kernel(
     const bf16* __restrict__ q, const Fp8Cache kv, const int32_t* __restrict__ seq_lens,
@@ -427,7 +427,7 @@ __global__ __launch_bounds__(64 * kShortWaves<D>) void paged_decode_fp8_short_ke
 // waves, each a quarter of the segments with eight loads in flight (attention of 1
 // row of 32000 keys, 8 heads of 128, 256 segments a head: 42 us with one wave a
 // head, as the bf16 cache's merge has it, 24 so; 4 rows of 6600, 16 heads of 64:
-// 22.9 and 20).
+// 3 us less, 21.3).
 template <int D>
 __global__ __launch_bounds__(256) void paged_decode_fp8_merge_kernel(
     const float* __restrict__ part_o, const float* __restrict__ part_ml,
@@ -509,9 +509,9 @@ auto with_sizes(int head_dim, int page_size, bool bias, F f) {
 // Whether the one-launch kernel takes a call, by the table's width in keys and the
 // number of (row, kv head) pairs.  Measured, GPU time of one and of two launches in
 // us (rows of half to all of the width, gated heads of 64 / ungated of 128): one
-// row, 16 / 8 heads, 256 keys 4.1, 8.3 / 4.7, 8.1; 1024 keys 6.9, 8.8 / 9.9, 9.2
-// (a launch costs the host some 4 us besides); 2048 keys 12.6, 10.0 / 16.7, 8.8.
-// 16 rows, 2048 keys 15.3, 20.8 / 19.6, 22.6; 4096 keys 25.3, 29.4 / 35.5, 31.7.
+// row, 16 / 8 heads, 256 keys 4.2, 8.5 / 4.5, 8.1; 1024 keys 7.5, 8.9 / 8.4, 9.1
+// (a launch costs the host some 4 us besides); 2048 keys 13.5, 10.1 / 17.0, 9.2.
+// 16 rows, 2048 keys 15.7, 21.6 / 19.5, 23.2; 4096 keys 26.3, 30.5 / 34.2, 32.7.
 inline bool short_table(long keys, long pairs) { return keys <= 1024 || (keys <= 2048 && pairs >= 128); }
 
 }  // namespace

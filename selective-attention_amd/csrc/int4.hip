@@ -72,8 +72,8 @@ __device__ __forceinline__ bool whole_pieces(const bf16* x, int K, int ldx) {
 // bf16, where that is given.  They are read along the rows (16 lanes a row, 4 rows
 // a load) and turned into operand order in the wave's own LDS (16 rows of 272
 // bytes): loads in operand order take 64 bytes from each of 16 rows, which at K =
-// 4096 lie in one channel of the L2 (64 rows, 4096 -> 4096: 13.3 us, turned 10.4;
-// 32 rows, 4096 -> 32000: 24.6 and 22).
+// 4096 lie in one channel of the L2 (64 rows, 4096 -> 4096: 13.8 us, turned 10.0;
+// 32 rows, 4096 -> 32000: 25.0 and 21.3).
 constexpr int kTurnRow = 17;   // uint4
 template <int J>
 __device__ __forceinline__ void read_rows(uint4 (&v)[J][4], const bf16* x, int row0, int k0, int M, int K, int ldx) {
@@ -94,7 +94,7 @@ __device__ __forceinline__ void read_rows(uint4 (&v)[J][4], const bf16* x, int r
   }
   // from the words that hold them: five, moved by half a word where a row starts in
   // the middle of one, columns at and behind K as 0 (4 rows of 1023, 4383 outputs:
-  // 4.4 us, 4.0 of 1024; 32 of 4091, 32000 outputs: 27 and 22; a padded copy in
+  // 4.0 us, 3.6 of 1024; 32 of 4091, 32000 outputs: 25 and 21; a padded copy in
   // front takes 10 us)
   const int off = static_cast<int>(reinterpret_cast<uintptr_t>(x) & 2);
   const int bytes = (off + ((M - 1) * ldx + K) * 2 + 3) & ~3;
@@ -252,8 +252,8 @@ __global__ __launch_bounds__(64 * NW) void int4_linear_kernel(const bf16* __rest
 // of its KW blocks in registers, in operand order and with the groups' sums, and
 // the workgroup goes through the tiles t, t + gridDim.x, ..., so that only the
 // weights are streamed: x is read and put in order once a workgroup, not once a
-// tile (4096 -> 32000, 8 rows: 25.7 us by tiles, 16.2 here; 32 rows: 36.4 and 22;
-// the weights' bytes at 6 TB/s are 11.4 us).  The next tile's codes and factors are
+// tile (4096 -> 32000, group 128, 8 rows: 17.3 us by tiles, 15.8 here; 32 rows: 31.3
+// and 21.3; the weights' bytes at 6 TB/s are 11.4 us).  The next tile's codes and factors are
 // in flight while this one's are multiplied (two in flight: no faster); the eight
 // waves' sums meet in one of two LDS buffers, one barrier a tile.
 template <int CT, int G, bool Z, int KW>
@@ -426,12 +426,20 @@ void int4_stream(const void* x, const void* xscale, Int4Segs& sg, int M, int K, 
     sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? (sg.N[i] + 15) / 16 : 0);
   const int parts = (M + 16 * CT - 1) / (16 * CT);
   // one workgroup a CU where its registers leave room for no second one (KW = 4),
-  // else two (1024 -> 32000, 4 rows: 8.3 and 6.8 us; 4096 -> 32000: 16.3 and 19)
+  // else two (1024 -> 32000, 4 rows: 8.3 and 6.8 us; 4096 -> 32000: 15.7 and 18.9)
   const int grid = std::min(sg.blk0[kInt4Segs], (KW == 4 ? 256 : 512) / parts);
   hipLaunchKernelGGL((int4_stream_kernel<CT, G, Z, KW>), dim3(grid, parts), dim3(512), 0, s,
                      static_cast<const bf16*>(x), static_cast<const bf16*>(xscale), sg, M, K, ldx);
 }
 
+// By K and the group, in us, by tiles and streamed.  Up to 2048 columns the stream: 1024
+// -> 32000, 4 rows 8.1, 6.8; 1024 -> 1024, 1 row 3.3, 2.9; 1024 -> 4384, 4 rows,
+// group 64, 3.8, 4.0.  Up to 4096 too, where group 128 gains at whole K (4096 -> 4096, 1
+// row 6.8, 5.2; 4096 -> 32000, 1 row 17.2, 15.7, 32 rows 31.3, 21.3, 64 rows, in two
+// parts that each read the weights, 47.6, 34.5) and loses where waves have no block
+// (2560 -> 32000, 1 row 12.7, 15.2; 32 rows 22.6, 20.6).  Group 64 holds twice the
+// factors and spills up to 19 registers there: 4096 -> 4096, 1 row 7.3, 6.1; 4096 ->
+// 32000, 1 row 18.5, 19.1, 64 rows 51, 63; 2176 -> 32000, 1 row 12.2, 18.4.
 template <int G, bool Z>
 void int4_rows(const void* x, const void* xscale, Int4Segs& sg, int M, int K, int ldx, hipStream_t s) {
   const int kb = (K + 127) / 128;   // (int4_streams)

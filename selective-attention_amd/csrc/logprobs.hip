@@ -23,7 +23,8 @@
 // running maximum rescales sums inside a piece; longer rows go in pieces joined
 // by their maxima.  bf16 logits stay packed and are widened anew in each
 // pass (the registers are made opaque in between, or the compiler keeps all 64
-// widened: 146 registers and 190 us for 8192 x 32000, against 63 and 95).
+// widened: 8192 x 32000 with 20 alternatives 176 us, against 120; without
+// alternatives level, 94).
 //
 // Alternatives, k of them in the order of (value, lowest index first).  Among
 // the 64 maxima of 64 disjoint groups of the piece's logits the k-th largest,
@@ -627,7 +628,7 @@ void launch_logprobs(const void* logits, long ld, const int64_t* targets, long r
     go(token_logprobs_kernel<T, 64, 8, TOP, kW, false>, 64);
   } else if (V <= 256 * 64 || (TOP && rows >= kFewRows)) {
     // with alternatives the barriers of four waves cost less than those of eight:
-    // 8192 x 32000, 20 of them, 126 us in two pieces, 144 in one (90 without any:
+    // 8192 x 32000, 20 of them, 120 us in two pieces, 139 in one (94 without any:
     // the bytes); 4 rows, 8 of them, take 11 us and 9
     go(token_logprobs_kernel<T, 256, 8, TOP, kW, false>, 256);
   } else {

@@ -132,8 +132,9 @@ def paged_kv_append_fp8(k, v, log_gate, page_table, seq_lens, k_pages, v_pages, 
     """One token per row: k, v (batch, kv_heads, head_dim) into the rows' open
     blocks at slot seq_lens[row] % page_size, log_gate (batch, kv_heads) into the
     page's gates (both None for a cache without gates); a block that this fills
-    is rounded into its page.  seq_lens (batch,) int32 advances in place; a row
-    of length -1 is left as it is."""
+    is rounded into its page.  seq_lens (batch,) int32, below 2^27, advances in
+    place; a row of length -1 is left as it is.  While the call runs the lengths
+    carry marks in their bits 27 to 30: a reader on another stream waits for it."""
     who = "paged_kv_append_fp8"
     b, H, D = k.shape
     n, _, ps, _ = _check_cache(who, b, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,

@@ -105,8 +105,9 @@ class CausalLM(nn.Module):
         """Log probability of each token after the first given those before it, with
         the entropy and `top` alternatives at its place: TokenLogprobs of
         (batch_size, seq_len - 1[, top]).  Tokens at or past a length have logprob
-        0 and pass no gradient; in training, minus the sum over the others'
-        number is the language model's loss."""
+        0, which passes no gradient (entropy and alternatives there are of the
+        padded place); in training, minus the sum over the others' number is
+        the language model's loss."""
         b, L = input_ids.shape
         logits = self.forward(input_ids, lengths, attn_gate_thresholds)
         # targets one place to the left, the last place without one: the logits'

@@ -5,8 +5,15 @@
 with codes 0..15, zero = 8 where no zero points are given, and groups of 32, 64
 or 128 columns.  pack_int4 and quantize_int4 lay a weight out once; int4_linear
 takes it as it lies.  Up to 64 rows (decode steps) one kernel reads the codes
-and keeps the group's factors in fp32; more rows, and rows that take a
-gradient, go through the weights widened to bfloat16 and a plain matrix product.
+and keeps the group's factors in fp32: W is exact, and the output's rounding the
+only one to fewer bits.  More rows, and rows that take a gradient, go through the
+weights widened to bfloat16 and a plain matrix product: every W[n, k] is rounded
+there, by up to 2^-8 of it, so that a row's result moves by up to 2^-8 sum_k
+|x_k W[n, k]| where a 65th row comes to stand beside it.
+
+x is taken to be finite.  A row with an infinity gives NaN in every output up to 64
+rows (the kernel takes the difference of two sums of x), infinities or NaN above;
+the rows beside it stand.
 
 New ops (the reference's layers are nn.Linear in the model's dtype,
 modules/feed_forward.py:4-11).

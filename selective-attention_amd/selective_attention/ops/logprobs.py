@@ -53,7 +53,10 @@ def token_logprobs(logits: torch.Tensor, targets: torch.Tensor, top: int = 0,
     """
     Args:
         logits: (..., vocab) float32 or bfloat16 of any finite size; -inf rules a
-            token out
+            token out.  Read in place where the vocabulary is dense and one stride
+            leads from row to row; others (logits[:, :-1] of a batch) are copied,
+            in the forward and again in the backward: shift the targets and
+            ignore the last place instead, as CausalLM.score does
         targets: (...) int32 or int64 token ids.  ignore_index: logprob 0 and no
             gradient from it, whatever the row holds; any other id outside the
             vocabulary: NaN
