@@ -12,8 +12,8 @@
 // -m log2(e) rounded, would save an instruction a logit, but carries n's rounding
 // into every exponent: up to 64 at m = 1e9, and at the type's lowest value n itself
 // is infinite, so that a mask of a large finite value over a whole piece made
-// its row NaN.  8192 x 32000 bf16, 20 alternatives: 115.3 us so, 117.9; without
-// alternatives, and in the gradient, level.)
+// its row NaN.  8192 x 32000 bf16: 86 us so, 91 now; 20 alternatives 122 and 126;
+// forward and gradient 282 and 284.)
 //
 // All sums in fp32.  Both directions are bound by the bytes of the logits: the
 // forward reads them once, the backward reads them and writes the gradient.
@@ -23,8 +23,8 @@
 // running maximum rescales sums inside a piece; longer rows go in pieces joined
 // by their maxima.  bf16 logits stay packed and are widened anew in each
 // pass (the registers are made opaque in between, or the compiler keeps all 64
-// widened: 8192 x 32000 with 20 alternatives 176 us, against 120; without
-// alternatives level, 94).
+// widened: 8192 x 32000 with 20 alternatives 176 us, against 126; without
+// alternatives level, 91).
 //
 // Alternatives, k of them in the order of (value, lowest index first).  Among
 // the 64 maxima of 64 disjoint groups of the piece's logits the k-th largest,
@@ -628,8 +628,8 @@ void launch_logprobs(const void* logits, long ld, const int64_t* targets, long r
     go(token_logprobs_kernel<T, 64, 8, TOP, kW, false>, 64);
   } else if (V <= 256 * 64 || (TOP && rows >= kFewRows)) {
     // with alternatives the barriers of four waves cost less than those of eight:
-    // 8192 x 32000, 20 of them, 120 us in two pieces, 139 in one (94 without any:
-    // the bytes); 4 rows, 8 of them, take 11 us and 9
+    // 8192 x 32000, 20 of them, 120 us in two pieces, 139 in one (91 without any:
+    // 86 are the bytes); 4 rows, 8 of them, take 11 us and 9
     go(token_logprobs_kernel<T, 256, 8, TOP, kW, false>, 256);
   } else {
     go(token_logprobs_kernel<T, 512, 8, TOP, 4, false>, 512);
