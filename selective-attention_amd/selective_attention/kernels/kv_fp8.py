@@ -84,7 +84,8 @@ def paged_decode_attn_fp8(q, k_pages, v_pages, k_scale, v_scale, k_tail, v_tail,
         softmax_scale: head_dim ** -0.5 when None
         key_bias: (num_pages, num_kv_heads, page_size) float32 or None: added to
             every key's score except the newest (position seq_len - 1); a key at
-            -inf takes no part, whatever it holds
+            -inf takes no part, whatever it holds (nor does one below some -2e38,
+            whose score in powers of two passes float32)
 
     Returns:
         o: (batch, num_q_heads, head_dim) bfloat16; a row without keys gets zeros.
