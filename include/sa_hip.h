@@ -358,6 +358,44 @@ int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zer
                          int group, void* out, void* stream);
 
 /*
+ * Rows in 8 bits, the inputs of sa_fp8_linear (the reference has none).  For each
+ * block of 128 columns of a row v of `dim` columns, e4m3 codes c and one scale s = 2^e,
+ * the smallest power of two with max|v| <= 448 s (1 for a block of zeros, at least
+ * 2^-126); c is v / s rounded to nearest, v not rounded before.  Infinities and
+ * NaN give NaN codes, the scale goes by what is finite.  kb = ceil(dim / 128):
+ *   codes (rows, 128 kb), 16-byte aligned, zeros behind dim;
+ *   scales (rows, 4 ceil(kb / 4)) e8m0 bytes, 2^(byte - 127), 127 behind block kb - 1.
+ * sa_rows_fp8: v = x, x * gate (gate not NULL), or with `silu` (bfloat16)
+ * x * gate / (1 + e^-gate); x, gate (rows, dim) of `dtype` with row strides ldx, ldg
+ * (elements; fastest on 16-byte boundaries and dim a multiple of 8).
+ * sa_rms_norm_fp8: v = t / sqrt(mean(t^2) + eps) (1 + weight), t = x (row stride ldx), or
+ * x + residual in `dtype`, stored to sum (both contiguous, both NULL or neither);
+ * weight (dim) float32; dim at most 65536.
+ */
+int sa_rows_fp8(int dtype, const void* x, const void* gate, int silu, int64_t rows, int dim,
+                int64_t ldx, int64_t ldg, void* codes, void* scales, void* stream);
+int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, const float* weight,
+                    int64_t rows, int dim, int64_t ldx, float eps, void* sum, void* codes,
+                    void* scales, void* stream);
+
+/*
+ * Linear layers in 8 bits (the reference has none): y_i = x W_i^T + bias_i, i < nseg
+ * <= 4, all of the same M rows x in 8 bits (codes, scales as above, K columns):
+ *   W[n, k] = 2^(e[n / 128, k / 128] - 127) c[n, k].
+ * packed: (ceil(N / 16), ceil(K / 128), 8, 16, 16) e4m3 bytes, piece j of a tile being
+ * columns 16 j .. + 15 of its 16 rows, zeros in the padding, 16-byte aligned; scales
+ * (ceil(N / 128), 4 ceil(K / 512)) e8m0 bytes e.  bias (N) bf16 or NULL, y (M, N) bf16.
+ * matrices: five words each, the addresses of packed, scales, bias (0: none) and y,
+ * and N.
+ */
+int sa_fp8_linear(const void* codes, const void* scales, int64_t M, int K, int nseg,
+                  const int64_t* matrices, void* stream);
+
+/* The weights that such a packed matrix stands for, in bf16: out (N, K). */
+int sa_fp8_dequant_bf16(const void* packed, const void* scales, int N, int K, void* out,
+                        void* stream);
+
+/*
  * Log probabilities of given tokens (no kernel in the reference, which takes
  * softmax and argmax of its logits, models/causal_lm.py:143-221).  logits
  * (rows, vocab) in `dtype` (f32 or bf16) with row stride ld (elements), targets

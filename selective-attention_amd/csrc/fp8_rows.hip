@@ -1,0 +1,362 @@
+// Rows in 8 bits: the inputs of the 8-bit linear layers (fp8_linear.hip, gfx950).
+//
+//   rows       v = x, or x * gate
+//   silu_mul   v = a c / (1 + e^-c)                          (SwiGLU's product)
+//   rms_norm   t = x + r in x's type (r optional), v = t / sqrt(mean t^2 + eps) (1 + w)
+//
+// and of each row of v, for each block of 128 columns, the e4m3 codes of v / s
+// with s = 2^e the smallest power of two that max|v| <= 448 s holds for (1 for a
+// block of zeros).  A float's relative step does not depend on its exponent, so a
+// power of two loses nothing against max|v| / 448 but a part of the subnormal
+// codes, and the matrix cores take it as it is: one e8m0 byte, 2^(byte - 127).
+// Infinities and NaN give NaN codes; the scale goes by what is finite.
+//
+// Outputs: codes (rows, 128 kb) with zeros behind dim, scales (rows, 4 ceil(kb / 4))
+// with 127 (2^0) behind block kb - 1: the products read them a word at a time.
+//
+// Rounding: v is computed to within a few 2^-48 (rows, rms_norm; silu_mul 2 2^-24)
+// and rounded to fp32 to odd, so that the one rounding that counts, to e4m3, is that
+// of v itself: rounding to nearest twice would send values next to a tie the wrong way.
+//
+// Streams of memory: 16 lanes a block, 8 columns a lane, the maximum over 16 lanes
+// by four lane exchanges.
+#include "common.h"
+#include "prof.h"
+
+#include <type_traits>
+
+namespace sa {
+namespace {
+
+constexpr int kQBlock = 128;
+
+// y + lo (|lo| at most half an ulp of y) rounded to odd: y where lo is 0 or y is
+// odd, else its neighbour towards lo, which is odd.  A y of 0, infinity or NaN stays
+__device__ __forceinline__ float to_odd(float y, float lo) {
+  const uint32_t b = __float_as_uint(y);
+  const int step = (static_cast<int>(b ^ __float_as_uint(lo)) >> 31) | 1;
+  return __uint_as_float(lo != 0.0f && fabsf(lo) < fabsf(y) && (b & 1u) == 0u ? b + step : b);
+}
+
+// e8m0 byte of the scale of a block with the largest finite magnitude top
+__device__ __forceinline__ uint32_t scale_byte(float top) {
+  const uint32_t b = __float_as_uint(top);
+  // 448 = 1.75 2^8: the mantissa decides between 2^(E - 8) and the next one
+  const int e = static_cast<int>(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return b == 0u ? 127u : static_cast<uint32_t>(max(e, 1));
+}
+
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
+  return v;
+}
+
+// the block's scale and the lane's eight codes; all 16 lanes of the block are here
+__device__ __forceinline__ uint2 encode_block(const float (&v)[8], uint32_t& byte) {
+  float top = 0.0f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float m = fabsf(v[i]);
+    top = fmaxf(top, m < __builtin_inff() ? m : 0.0f);
+  }
+  byte = scale_byte(max16(top));
+  const float inv = __uint_as_float((254u - byte) << 23);   // 2^(127 - byte); byte is 1..247
+  uint32_t r[2];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    float q[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = fmaf(0.0f, v[4 * h + i], v[4 * h + i] * inv);   // (an infinity: NaN)
+    int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
+    p = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], p, true);
+    r[h] = static_cast<uint32_t>(p);
+  }
+  return uint2{r[0], r[1]};
+}
+
+// where a lane's codes and, by the block's first lane, its scale go
+struct RowsOut {
+  uint8_t* codes;
+  uint8_t* scales;
+  int kb, words;   // blocks and words of scales a row
+};
+__device__ __forceinline__ void put_block(const RowsOut& o, long row, int b, int l16, const uint2& c, uint32_t byte) {
+  *reinterpret_cast<uint2*>(o.codes + (row * o.kb + b) * kQBlock + 8 * l16) = c;
+  uint8_t* s = o.scales + row * 4 * o.words;
+  if (l16 == 0) s[b] = static_cast<uint8_t>(byte);
+  else if (b == o.kb - 1 && l16 < 4 * o.words - b) s[b + l16] = 127;
+}
+
+// eight columns of a row from k on, those at or behind dim as 0.  VEC: dim is a
+// multiple of 8 and rows start on 16-byte boundaries
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(float (&v)[8], const T* row, int k, int dim) {
+  if constexpr (VEC) {
+    if (k < dim) {
+      if constexpr (sizeof(T) == 2) {
+        const uint4 q = *reinterpret_cast<const uint4*>(row + k);
+        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          v[2 * i] = bf16lo_to_f32(u[i]);
+          v[2 * i + 1] = bf16hi_to_f32(u[i]);
+        }
+      } else {
+        const float4 a = *reinterpret_cast<const float4*>(row + k), b = *reinterpret_cast<const float4*>(row + k + 4);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < dim ? to_f32(row[k + i]) : 0.0f;
+  }
+}
+
+// v = x, x * gate, or x * silu(gate); 16 lanes a block, blocks in order
+enum { kPlain = 0, kGated = 1, kSilu = 2 };
+template <typename T, bool VEC, int MODE>
+__global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, const T* __restrict__ gate, long ldx,
+                                                   long ldg, int dim, uint32_t blocks, const RowsOut o) {
+  const int l16 = threadIdx.x & 15;
+  const uint32_t q = blockIdx.x * 16u + (threadIdx.x >> 4);
+  if (q >= blocks) return;   // (16 lanes at a time)
+  const uint32_t row = q / static_cast<uint32_t>(o.kb);
+  const int b = static_cast<int>(q - row * o.kb), k = kQBlock * b + 8 * l16;
+  float v[8];
+  load8<T, VEC>(v, x + row * ldx, k, dim);
+  if constexpr (MODE != kPlain) {
+    float c[8];
+    load8<T, VEC>(c, gate + row * ldg, k, dim);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if constexpr (MODE == kGated) {
+        const float y = v[i] * c[i];
+        v[i] = to_odd(y, fmaf(v[i], c[i], -y));   // (exact for bf16)
+      } else {
+        // e^-c by the transcendental unit (2^t, 1 ulp), with what t's rounding leaves
+        const float t = -c[i] * kLog2e, dt = fmaf(-c[i], kLog2e, -t) + -c[i] * 1.925963033500642e-8f;
+        const float e = fast_exp2(t), d = 1.0f + fmaf(e, dt * 0.6931471805599453f, e);
+        float r = __builtin_amdgcn_rcpf(d);
+        r = fmaf(fmaf(-d, r, 1.0f), r, r);
+        r = d < __builtin_inff() ? r : 0.0f;   // (c below -88: 0, as with e^-c infinite; no NaN of inf - inf)
+        v[i] = v[i] * c[i] * r;   // (a c is exact)
+      }
+    }
+  }
+  uint32_t byte;
+  const uint2 c = encode_block(v, byte);
+  put_block(o, row, b, l16, c, byte);
+}
+
+// 1 / sqrt(ss / dim + eps) as hi + lo: fp32's own, then a Newton step in fp64
+__device__ __forceinline__ void rstd_of(double ss, int dim, float eps, float& hi, float& lo) {
+  const double m = ss / dim + static_cast<double>(eps);
+  const float r = 1.0f / sqrtf(static_cast<float>(m));
+  const double rd = r, r2 = rd * (1.5 - 0.5 * m * rd * rd);
+  const bool fine = r > 0.0f && r < __builtin_inff();   // else a sum beyond fp32 (0), or of zeros with eps 0
+  hi = fine ? static_cast<float>(r2) : r;
+  lo = fine ? static_cast<float>(r2 - static_cast<double>(hi)) : 0.0f;
+}
+
+// A row stays in registers between its sum of squares and its codes: W waves a row
+// and V pieces of 8 columns a lane (W = 1: four rows a workgroup).  The squares
+// are summed by four in fp32 and then in fp64, which costs two additions for
+// eight columns and leaves the sum exact to a few 2^-28.
+template <typename T, bool VEC, bool RES, int V, int W>
+__global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
+    const T* __restrict__ x, const T* __restrict__ res, const float* __restrict__ weight, long rows, long ldx,
+    int dim, float eps, T* __restrict__ sum, const RowsOut o) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const long row = W == 1 ? blockIdx.x * 4L + (tid >> 6) : static_cast<long>(blockIdx.x);
+  const int t = W == 1 ? lane : tid, l16 = tid & 15;
+  if (W == 1 && row >= rows) return;   // (whole waves; no barrier below for W = 1)
+  float v[V][8];
+  double ss = 0.0;
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int k = 8 * (t + 64 * W * j);
+    load8<T, VEC>(v[j], x + row * ldx, k, dim);
+    if constexpr (RES) {
+      float r[8];
+      load8<T, VEC>(r, res + row * dim, k, dim);
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        if constexpr (sizeof(T) == 2) {
+          const uint32_t p = pack_bf16x2(v[j][i] + r[i], v[j][i + 1] + r[i + 1]);
+          v[j][i] = bf16lo_to_f32(p);
+          v[j][i + 1] = bf16hi_to_f32(p);
+        } else {
+          v[j][i] += r[i];
+          v[j][i + 1] += r[i + 1];
+        }
+      }
+      T* out = sum + row * dim + k;
+      if constexpr (VEC) {
+        if (k < dim) {
+          if constexpr (sizeof(T) == 2) {
+            *reinterpret_cast<uint4*>(out) = uint4{pack_bf16x2(v[j][0], v[j][1]), pack_bf16x2(v[j][2], v[j][3]),
+                                                   pack_bf16x2(v[j][4], v[j][5]), pack_bf16x2(v[j][6], v[j][7])};
+          } else {
+            reinterpret_cast<float4*>(out)[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
+            reinterpret_cast<float4*>(out)[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < dim) out[i] = from_f32<T>(v[j][i]);
+      }
+    }
+    float s0 = 0.0f, s1 = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      s0 = fmaf(v[j][i], v[j][i], s0);
+      s1 = fmaf(v[j][4 + i], v[j][4 + i], s1);
+    }
+    ss += static_cast<double>(s0) + static_cast<double>(s1);
+  }
+#pragma unroll
+  for (int s = 32; s > 0; s >>= 1) ss += __shfl_xor(ss, s, 64);
+  if constexpr (W > 1) {
+    __shared__ double part[W];
+    if (lane == 0) part[tid >> 6] = ss;
+    __syncthreads();
+    ss = 0.0;
+#pragma unroll
+    for (int i = 0; i < W; ++i) ss += part[i];
+  }
+  float hi, lo;
+  rstd_of(ss, dim, eps, hi, lo);
+#pragma unroll
+  for (int j = 0; j < V; ++j) {
+    const int p = t + 64 * W * j, k = 8 * p, b = p >> 4;
+    float w[8];
+    load8<float, VEC>(w, weight, k, dim);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // (p + e) (g + gl) with p + e = v rstd and g + gl = 1 + w
+      const float g = 1.0f + w[i], gl = w[i] - (g - 1.0f);
+      const float q = v[j][i] * hi, e = fmaf(v[j][i], hi, -q) + v[j][i] * lo;
+      const float c = fmaf(e, g, q * gl), y = fmaf(q, g, c);
+      v[j][i] = k + (VEC ? 0 : i) < dim ? to_odd(y, fmaf(q, g, -y) + c) : 0.0f;
+    }
+    if (b < o.kb) {   // (16 lanes at a time)
+      uint32_t byte;
+      const uint2 c = encode_block(v[j], byte);
+      put_block(o, row, b, l16, c, byte);
+    }
+  }
+}
+
+RowsOut rows_out(void* codes, void* scales, int dim) {
+  const int kb = (dim + kQBlock - 1) / kQBlock;
+  return RowsOut{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), kb, (kb + 3) / 4};
+}
+bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+template <typename T>
+void rows_go(int mode, const void* x, const void* gate, long ldx, long ldg, int dim, uint32_t blocks, const RowsOut& o,
+             hipStream_t s) {
+  constexpr long kAlign = 16 / sizeof(T);
+  const bool vec = dim % 8 == 0 && ldx % kAlign == 0 && on16(x) && (mode == kPlain || (ldg % kAlign == 0 && on16(gate)));
+  auto go = [&](auto kern) {
+    hipLaunchKernelGGL(kern, dim3((blocks + 15) / 16), dim3(256), 0, s, static_cast<const T*>(x),
+                       static_cast<const T*>(gate), ldx, ldg, dim, blocks, o);
+  };
+  if (mode == kPlain) vec ? go(rows_kernel<T, true, kPlain>) : go(rows_kernel<T, false, kPlain>);
+  else if (mode == kGated) vec ? go(rows_kernel<T, true, kGated>) : go(rows_kernel<T, false, kGated>);
+  else if constexpr (sizeof(T) == 2) vec ? go(rows_kernel<T, true, kSilu>) : go(rows_kernel<T, false, kSilu>);
+}
+
+template <typename T, bool VEC, bool RES>
+void norm_go(const void* x, const void* res, const float* w, long rows, long ldx, int dim, float eps, void* sum,
+             const RowsOut& o, hipStream_t s) {
+  auto go = [&](auto kern, int waves) {
+    const long grid = waves == 1 ? (rows + 3) / 4 : rows;
+    hipLaunchKernelGGL(kern, dim3(grid), dim3(waves == 1 ? 256 : 64 * waves), 0, s, static_cast<const T*>(x),
+                       static_cast<const T*>(res), w, rows, ldx, dim, eps, static_cast<T*>(sum), o);
+  };
+  if (dim <= 512) go(rms_norm_fp8_kernel<T, VEC, RES, 1, 1>, 1);
+  else if (dim <= 1024) go(rms_norm_fp8_kernel<T, VEC, RES, 2, 1>, 1);
+  else if (dim <= 2048) go(rms_norm_fp8_kernel<T, VEC, RES, 1, 4>, 4);
+  else if (dim <= 4096) go(rms_norm_fp8_kernel<T, VEC, RES, 2, 4>, 4);
+  else if (dim <= 8192) go(rms_norm_fp8_kernel<T, VEC, RES, 4, 4>, 4);
+  else if (dim <= 16384) go(rms_norm_fp8_kernel<T, VEC, RES, 2, 16>, 16);
+  else go(rms_norm_fp8_kernel<T, VEC, RES, 8, 16>, 16);
+}
+constexpr int kMaxNormDim = 65536;
+
+int rows_check(const char* who, int dtype, long rows, int dim, const void* codes, const void* scales) {
+  SA_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype code %d", who, dtype);
+  SA_CHECK_ARG(rows >= 0 && dim > 0 && dim <= (1 << 26), "%s: bad sizes rows=%ld dim=%d", who, rows, dim);
+  SA_CHECK_ARG(rows * ((dim + kQBlock - 1L) / kQBlock) < (1L << 28), "%s: %ld rows of %d columns are too many", who,
+               rows, dim);   // (2^32 threads a grid)
+  SA_CHECK_ARG(rows == 0 || (codes && scales), "%s: null pointer", who);
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 3)) == 0,
+               "%s: codes or scales are not aligned", who);
+  return 0;
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" int sa_rows_fp8(int dtype, const void* x, const void* gate, int silu, int64_t rows, int dim, int64_t ldx,
+                           int64_t ldg, void* codes, void* scales, void* stream) {
+  const char* who = silu ? "sa_rows_fp8 (silu)" : "sa_rows_fp8";
+  if (const int rc = sa::rows_check(who, dtype, rows, dim, codes, scales)) return rc;
+  if (rows == 0) return 0;
+  SA_CHECK_ARG(x && (gate || !silu), "%s: null pointer", who);
+  SA_CHECK_ARG(!silu || dtype == sa::kBF16, "%s: bfloat16 alone", who);
+  SA_CHECK_ARG(ldx >= dim && (!gate || ldg >= dim), "%s: row strides %ld, %ld below dim %d", who,
+               static_cast<long>(ldx), static_cast<long>(ldg), dim);
+  const uintptr_t size = dtype == sa::kF32 ? 4 : 2;
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(gate)) & (size - 1)) == 0,
+               "%s: inputs are not aligned to their type", who);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  sa::ProfScope prof_(silu ? "silu_mul_fp8" : "rows_fp8", s);
+  const sa::RowsOut o = sa::rows_out(codes, scales, dim);
+  const uint32_t blocks = static_cast<uint32_t>(rows * o.kb);
+  const int mode = silu ? sa::kSilu : gate ? sa::kGated : sa::kPlain;
+  if (dtype == sa::kF32) sa::rows_go<float>(mode, x, gate, ldx, ldg, dim, blocks, o, s);
+  else sa::rows_go<sa::bf16>(mode, x, gate, ldx, ldg, dim, blocks, o, s);
+  SA_CHECK_LAUNCH(who);
+  return 0;
+}
+
+extern "C" int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, const float* weight, int64_t rows,
+                               int dim, int64_t ldx, float eps, void* sum, void* codes, void* scales, void* stream) {
+  const char* who = "sa_rms_norm_fp8";
+  if (const int rc = sa::rows_check(who, dtype, rows, dim, codes, scales)) return rc;
+  if (rows == 0) return 0;
+  SA_CHECK_ARG(dim <= sa::kMaxNormDim, "%s: dim %d above %d", who, dim, sa::kMaxNormDim);
+  SA_CHECK_ARG(rows < (1L << 22) || (dim <= 1024 && rows < (1L << 26)), "%s: %ld rows of %d columns are too many", who,
+               static_cast<long>(rows), dim);   // (2^32 threads a grid)
+  SA_CHECK_ARG(x && weight && (!residual == !sum), "%s: null pointer, or one of residual and sum without the other", who);
+  SA_CHECK_ARG(ldx >= dim, "%s: row stride %ld below dim %d", who, static_cast<long>(ldx), dim);
+  const uintptr_t size = dtype == sa::kF32 ? 4 : 2;
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(residual) |
+                 reinterpret_cast<uintptr_t>(sum)) & (size - 1)) == 0 && (reinterpret_cast<uintptr_t>(weight) & 3) == 0,
+               "%s: inputs are not aligned to their type", who);
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  sa::ProfScope prof_("rms_norm_fp8", s);
+  const sa::RowsOut o = sa::rows_out(codes, scales, dim);
+  auto go = [&](auto tag) {
+    using T = decltype(tag);
+    const bool vec = dim % 8 == 0 && ldx % (16 / static_cast<long>(sizeof(T))) == 0 && sa::on16(x) &&
+                     sa::on16(residual) && sa::on16(sum) && sa::on16(weight);
+    if (residual) {
+      vec ? sa::norm_go<T, true, true>(x, residual, weight, rows, ldx, dim, eps, sum, o, s)
+          : sa::norm_go<T, false, true>(x, residual, weight, rows, ldx, dim, eps, sum, o, s);
+    } else {
+      vec ? sa::norm_go<T, true, false>(x, residual, weight, rows, ldx, dim, eps, sum, o, s)
+          : sa::norm_go<T, false, false>(x, residual, weight, rows, ldx, dim, eps, sum, o, s);
+    }
+  };
+  dtype == sa::kF32 ? go(float{}) : go(sa::bf16{});
+  SA_CHECK_LAUNCH(who);
+  return 0;
+}

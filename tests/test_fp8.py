@@ -1,0 +1,679 @@
+"""8-bit linear layers and the rows that enter them (ops/fp8.py) against
+oracle/fp8.py in float64.
+
+Rows: quantize_rows_fp8 and rms_norm_fp8 round a value known to some 2^-45 of itself
+(products of two fp32 or bf16 numbers are taken with their remainder, the norm's
+factor in two words) to odd and then to e4m3, so the codes and scales are the
+oracle's own, bit for bit; the inputs here are random, no exact norm lies within
+2^-40 of a tie.  silu_mul_fp8's value has seven fp32 roundings (e^-c 1 ulp and the
+remainder's product, the sum, a reciprocal with one correction, two products): it
+is off by at most 8 2^-24 of itself, so a code by half a step and that.
+
+Products: codes and scales are exact.  The matrix cores take the products of 8
+columns, 8 i to 8 i + 7, together: aligned to the largest of their exponent sums and cut
+below 2^-13 of it (a product 2^-13 of the largest counts, one of 2^-14 does not), so
+each of the other seven is off by less than 2^-13 of the largest, 7 2^-13 of the
+magnitudes' sum A over all groups at most.  K / 8 such sums are added in fp32, each
+addition off by at most 2^-23 of A, the waves' sums by eight more, and the result is
+rounded once to bf16, 2^-8 of it at most.  Where all products of a group lie within
+2^13 of each other and no sum passes 2^24 of the last bit, nothing is lost but that
+last rounding: whole numbers give the oracle's own result.
+"""
+import math
+
+import pytest
+import torch
+
+from oracle import fp8 as ref
+from selective_attention.ops import (Fp8Rows, dequantize_fp8, fp8_linear, fp8_linear_multi, pack_fp8,
+                                     quantize_fp8, quantize_rows_fp8, rms_norm_fp8, silu_mul_fp8)
+
+E4, E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def rand(*shape, seed=0, dtype=torch.bfloat16, big=True):
+    g = torch.Generator().manual_seed(seed)
+    x = torch.randn(*shape, generator=g)
+    if big and len(shape) > 1:   # columns of unlike size
+        x = x * torch.exp(2.0 * torch.randn(shape[-1], generator=g))
+    return x.to(dtype)
+
+
+def make_rows(M, K, seed=0):
+    """Rows in 8 bits made by the oracle, on the CPU."""
+    codes, scales = ref.rows(rand(M, K, seed=seed))
+    return Fp8Rows(codes.to(E4), (torch.log2(scales) + 127).to(torch.uint8).view(E8), K)
+
+
+def on(r: Fp8Rows) -> Fp8Rows:
+    return Fp8Rows(r.codes.cuda(), r.scales.cuda(), r.features)
+
+
+def same_rows(r: Fp8Rows, v: torch.Tensor):
+    codes, scales = ref.rows(v.reshape(-1, v.shape[-1]))
+    assert r.shape == v.shape
+    assert r.codes.dtype == E4 and r.scales.dtype == E8
+    assert torch.equal(r.scales.cpu().double().reshape(scales.shape), scales)
+    got = r.codes.cpu().double().reshape(codes.shape)
+    assert torch.equal(torch.isnan(got), torch.isnan(codes))
+    assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(codes))
+
+
+def check_linear(y, rows, packed, scales, N, bias=None):
+    K = rows.codes.shape[-1]
+    w = torch.nn.functional.pad(ref.weight(packed, scales, N, 128 * packed.shape[1]), (0, 0))
+    want, A = ref.linear(ref.values(rows.codes.reshape(-1, K), rows.scales.reshape(-1, rows.scales.shape[-1]), K),
+                         w, bias)
+    tol = 7 * 2.0 ** -13 * A + (K / 8 + 8) * 2.0 ** -23 * A + 2.0 ** -8 * want.abs() + 2.0 ** -133
+    err = (y.double().cpu().reshape(want.shape) - want).abs()
+    assert (err <= tol).all(), (float((err - tol).max()), float(err.max()))
+
+
+# --- layout and rounding, on the CPU ---------------------------------------------
+@pytest.mark.parametrize("N,K", [(16, 128), (33, 100), (1, 1), (130, 300)])
+def test_pack_keeps_codes_and_scales(N, K):
+    g = torch.Generator().manual_seed(3)
+    codes = torch.randn(N, K, generator=g).to(E4)
+    nb, kb = (N + 127) // 128, (K + 127) // 128
+    e = torch.randint(-126, 128, (nb, kb), generator=g)
+    byte = (e + 127).to(torch.uint8)
+    for scales in (byte, byte.view(E8), torch.exp2(e.double()), torch.exp2(e.float())):
+        packed, s = pack_fp8(codes, scales)
+        assert packed.shape == ((N + 15) // 16, kb, 8, 16, 16) and s.shape == (nb, (kb + 3) // 4 * 4)
+        assert torch.equal(ref.unpack(packed, N, K), codes.double())
+        assert torch.equal(s.view(torch.uint8)[:, :kb], byte)
+        assert (s.view(torch.uint8)[:, kb:] == 127).all()
+    whole = ref.unpack(packed, packed.shape[0] * 16, kb * 128)
+    assert not whole[N:].any() and not whole[:, K:].any()
+
+
+@pytest.mark.parametrize("N,K", [(128, 128), (200, 300), (5, 129)])
+def test_quantize_rounds_to_the_nearest_code(N, K):
+    w = rand(N, K, seed=1, dtype=torch.float32)
+    w[3] = 0.0
+    packed, scales = quantize_fp8(w)
+    s = torch.exp2(scales.view(torch.uint8).double() - 127)[torch.arange(N) // 128][:, torch.arange(K) // 128]
+    assert torch.equal(ref.unpack(packed, N, K), ref.e4m3(w.double() / s))
+    for i in range(0, N, 128):
+        for j in range(0, K, 128):
+            top = w[i:i + 128, j:j + 128].abs().max().double()
+            assert ref.scale_of(top[None])[0] == s[i, j]
+
+
+def test_quantize_borders_and_zeros():
+    """448 2^e keeps the scale, the next number doubles it; a block of zeros has 1."""
+    w = torch.zeros(128, 512)
+    w[0, 0], w[0, 128], w[0, 256] = 448 * 2.0 ** -9, math.nextafter(448.0, 1e9), 1e-45
+    w[0, 128] = torch.nextafter(torch.tensor(448.0), torch.tensor(1e9))
+    byte = quantize_fp8(w)[1].view(torch.uint8)
+    assert byte.tolist() == [[127 - 9, 128, 1, 127]]
+
+
+@pytest.mark.parametrize("what", ["type", "nan", "scales", "power", "range", "zero", "int", "empty"])
+def test_pack_refuses(what):
+    codes, scales = torch.zeros(130, 128).to(E4), torch.ones(2, 1)
+    if what == "type":
+        codes = codes.view(torch.uint8)
+    elif what == "nan":
+        codes.view(torch.uint8)[7, 7] = 0x7f
+    elif what == "scales":
+        scales = scales[:1]
+    elif what == "power":
+        scales[1] = 0.75
+    elif what == "range":
+        scales = torch.full((2, 1), 255, dtype=torch.uint8)
+    elif what == "zero":
+        scales[0] = 0.0
+    elif what == "int":
+        scales = scales.int()
+    elif what == "empty":
+        codes = codes[:0]
+    with pytest.raises((ValueError, TypeError)):
+        pack_fp8(codes, scales)
+
+
+@pytest.mark.parametrize("value", [math.inf, math.nan])
+def test_quantize_refuses_what_is_not_finite(value):
+    w = torch.zeros(4, 4)
+    w[1, 2] = value
+    with pytest.raises(ValueError):
+        quantize_fp8(w)
+    with pytest.raises(ValueError):
+        quantize_fp8(w[:0])
+
+
+@pytest.mark.parametrize("what", ["dtype", "features", "outs", "packed", "layout", "scales", "scale type", "bias",
+                                  "bias type", "xscale", "rows xscale", "codes", "rows scales", "count", "cpu",
+                                  "rows cpu", "no features"])
+def test_linear_refuses(what):
+    packed, scales = quantize_fp8(rand(32, 256, dtype=torch.float32))
+    x, kw = torch.zeros(2, 256, dtype=torch.bfloat16), dict(out_features=32)
+    if what == "dtype":
+        x = x.float()
+    elif what == "features":
+        x = x[:, :128]
+    elif what == "outs":
+        kw = dict(out_features=48)
+    elif what == "packed":
+        packed = packed.view(torch.int8)
+    elif what == "layout":
+        packed = packed.transpose(2, 3)
+    elif what == "scales":
+        scales = scales[:, :2]
+    elif what == "scale type":
+        scales = scales.float()
+    elif what == "bias":
+        kw["bias"] = torch.zeros(31, dtype=torch.bfloat16)
+    elif what == "bias type":
+        kw["bias"] = torch.zeros(32)
+    elif what == "xscale":
+        kw["xscale"] = x[:1]
+    elif what == "rows xscale":
+        x, kw["xscale"] = make_rows(2, 256), x
+    elif what == "codes":
+        x = Fp8Rows(make_rows(2, 256).codes.float(), make_rows(2, 256).scales)
+    elif what == "rows scales":
+        x = Fp8Rows(make_rows(2, 256).codes, make_rows(2, 256).scales[:1])
+    elif what == "rows cpu":
+        x = make_rows(2, 256)
+    elif what == "no features":
+        x = x[:, :0]
+    with pytest.raises((ValueError, TypeError)):
+        if what == "count":
+            fp8_linear_multi(x, [(packed, scales)] * 5, [None] * 5, [32] * 5)
+        else:
+            fp8_linear(x, packed, scales, **kw)
+
+
+@pytest.mark.parametrize("what", ["norm weight", "norm residual", "norm eps", "norm dtype", "norm wide", "norm cpu",
+                                  "norm grad", "silu dtype", "silu shape", "silu grad", "rows dtype", "rows gate",
+                                  "rows grad", "rows none", "rows cpu"])
+def test_rows_refuse(what):
+    x, w = torch.zeros(2, 8), torch.zeros(8)
+    h = x.to(torch.bfloat16)
+    calls = {
+        "norm weight": lambda: rms_norm_fp8(x, w[:7]), "norm residual": lambda: rms_norm_fp8(x, w, residual=h),
+        "norm eps": lambda: rms_norm_fp8(x, w, -1.0), "norm dtype": lambda: rms_norm_fp8(x.double().cuda() if torch.cuda.is_available() else x.int(), w),
+        "norm wide": lambda: rms_norm_fp8(torch.zeros(1, 65537), torch.zeros(65537)),
+        "norm cpu": lambda: rms_norm_fp8(x, w), "norm grad": lambda: rms_norm_fp8(x, w.requires_grad_()),
+        "silu dtype": lambda: silu_mul_fp8(x, x), "silu shape": lambda: silu_mul_fp8(h, h[:1]),
+        "silu grad": lambda: silu_mul_fp8(h.requires_grad_(), h), "rows dtype": lambda: quantize_rows_fp8(x.half()),
+        "rows gate": lambda: quantize_rows_fp8(x, h), "rows grad": lambda: quantize_rows_fp8(x.requires_grad_()),
+        "rows none": lambda: quantize_rows_fp8(x[:, :0]), "rows cpu": lambda: quantize_rows_fp8(x),
+    }
+    with pytest.raises((ValueError, TypeError, RuntimeError)):
+        calls[what]()
+
+
+# --- rows on the GPU ---------------------------------------------------------------
+SHAPES = [(1, 1), (3, 127), (2, 128), (5, 130), (1, 512), (4, 1000), (7, 1024), (3, 2056), (65, 4096), (2, 4100),
+          (3, 8200), (2, 16384), (1, 20000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_quantize_rows(shape, gated, dtype):
+    x = rand(*shape, seed=5, dtype=dtype)
+    gate = torch.sigmoid(rand(*shape, seed=6, dtype=torch.float32, big=False)).to(dtype) if gated else None
+    r = quantize_rows_fp8(x.cuda(), None if gate is None else gate.cuda())
+    same_rows(r, x.double() if gate is None else x.double() * gate.double())
+
+
+@pytest.mark.gpu
+def test_quantize_rows_borders():
+    """Ties, both ends of a block's range, subnormal codes, zeros, and blocks at fp32's ends."""
+    x = torch.zeros(6, 256)
+    ties = torch.arange(8, 16, dtype=torch.float32)
+    x[0, 0], x[0, 1:9], x[0, 9:17] = 448.0, ties + 0.5, -(ties + 0.5) * 2.0 ** -8
+    x[1, 0], x[1, 130] = 448.0, float(torch.nextafter(torch.tensor(448.0), torch.tensor(1e9)))
+    x[2, 0], x[2, 1:65] = 1.0, torch.arange(64, dtype=torch.float32) * 2.0 ** -18
+    x[3, 5], x[3, 200] = 1e-45, 2.0 ** -130
+    x[4, 5], x[4, 6] = 3.4e38, -1e30
+    x[5, 1], x[5, 2] = 447.99997, 16.499998
+    same_rows(quantize_rows_fp8(x.cuda()), x)
+    same_rows(quantize_rows_fp8(x.to(torch.bfloat16).cuda()), x.to(torch.bfloat16).double())
+
+
+@pytest.mark.gpu
+def test_quantize_rows_next_to_ties():
+    """fp32 products whose rounding to fp32 is a tie of e4m3: the remainder decides."""
+    a = torch.full((1, 128), 448.0)
+    b = torch.ones(1, 128)
+    # (1 + 2^-4 + 2^-12) (1 - 2^-12 + ..): exact products around 1.0625, the tie of 1 and 1.125
+    for i in range(1, 120):
+        u = 1.0625 * (1.0 + i * 2.0 ** -20)
+        a[0, i] = torch.tensor(u)
+        b[0, i] = torch.tensor(1.0625) / a[0, i]
+    exact = a.double() * b.double()
+    near = (exact - 1.0625).abs()[0, 1:120]
+    assert (near[near > 0] < 2.0 ** -23).any()
+    same_rows(quantize_rows_fp8(a.cuda(), b.cuda()), exact)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rows_that_are_not_finite(dtype):
+    x = rand(6, 300, seed=8, dtype=dtype)
+    x[1, 7], x[2, 140], x[3, 299] = math.inf, -math.inf, math.nan
+    x[4, 128:256] = math.inf
+    same_rows(quantize_rows_fp8(x.cuda()), x.double())
+    one = torch.ones_like(x)
+    same_rows(quantize_rows_fp8(x.cuda(), one.cuda()), x.double())
+    same_rows(quantize_rows_fp8(one.cuda(), x.cuda()), x.double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", ["rows", "gated", "silu", "norm"])
+def test_rows_of_a_stride(fn):
+    """Slices of longer rows, on and off 16-byte boundaries, views and expanded rows."""
+    wide = rand(9, 600, seed=9)
+    other = rand(9, 600, seed=10, big=False)
+    w = 0.1 * rand(256, seed=1, dtype=torch.float32)
+    for a, b in ((0, 0), (8, 16), (3, 8), (1, 1)):
+        x, c = wide[:, a:a + 256], other[:, b:b + 256]
+        xg, cg = wide.cuda()[:, a:a + 256], other.cuda()[:, b:b + 256]
+        if fn == "rows":
+            same_rows(quantize_rows_fp8(xg), x.double())
+        elif fn == "gated":
+            same_rows(quantize_rows_fp8(xg, cg), x.double() * c.double())
+        elif fn == "silu":
+            check_silu(silu_mul_fp8(xg, cg), x, c)
+        else:
+            same_rows(rms_norm_fp8(xg, w.cuda(), 1e-6), ref.rms_norm(x, w, 1e-6)[1])
+            t, v = ref.rms_norm(x, w, 1e-6, c)
+            got, r = rms_norm_fp8(xg, w.cuda(), 1e-6, residual=cg)
+            assert torch.equal(got.cpu(), t)
+            same_rows(r, v)
+    if fn == "rows":
+        x3 = wide[:8].view(2, 4, 600).transpose(0, 1)
+        same_rows(quantize_rows_fp8(wide[:8].cuda().view(2, 4, 600).transpose(0, 1)), x3.double())
+        same_rows(quantize_rows_fp8(wide[:1].cuda().expand(5, 600)), wide[:1].expand(5, 600).double())
+        same_rows(quantize_rows_fp8(wide[0].cuda()), wide[0].double())
+
+
+def check_silu(r, a, c):
+    a, c = a.double(), c.double()
+    v = (a * c * torch.sigmoid(c)).reshape(-1, a.shape[-1])
+    K = v.shape[1]
+    kb = (K + 127) // 128
+    got = r.codes.cpu().double().reshape(v.shape[0], -1)
+    s = r.scales.cpu().double().reshape(v.shape[0], -1)
+    v = torch.nn.functional.pad(v, (0, 128 * kb - K))
+    top = v.abs().view(-1, kb, 128).amax(2)
+    off = 8 * 2.0 ** -24
+    lo, hi = ref.scale_of(top * (1 - off)), ref.scale_of(top * (1 + off))
+    assert ((s[:, :kb] >= lo) & (s[:, :kb] <= hi)).all() and (s[:, kb:] == 1).all()
+    u = v / s[:, :kb].repeat_interleave(128, 1)
+    tol = ref.half_step(u.abs() * (1 + off)) + off * u.abs()
+    assert ((got - u).abs() <= tol).all() and not got[:, K:].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", SHAPES)
+def test_silu_mul(shape):
+    a, c = rand(*shape, seed=11), (3 * rand(*shape, seed=12, big=False)).to(torch.bfloat16)
+    check_silu(silu_mul_fp8(a.cuda(), c.cuda()), a, c)
+
+
+@pytest.mark.gpu
+def test_silu_mul_ends():
+    """Far gates, where e^-c leaves fp32; infinities and NaN."""
+    c = torch.linspace(-120, 120, 256).to(torch.bfloat16)[None].repeat(2, 1)
+    a = torch.ones_like(c)
+    a[0, :128] = 2.0 ** -100
+    r = silu_mul_fp8(a.cuda(), c.cuda())
+    keep = c.double() > -86          # (below, e^-c may pass fp32's range and the product is 0)
+    v = torch.where(keep, a.double() * c.double() * torch.sigmoid(c.double()), 0.0)
+    got = torch.where(keep, r.dequantize().cpu().double(), 0.0)
+    s = r.scales.cpu().double()[:, :2].repeat_interleave(128, 1)
+    assert ((got - v).abs() <= s * (ref.half_step(v / s) + 1e-6 * (v / s).abs())).all()
+    assert torch.isfinite(r.codes.float()).all()
+    bad = torch.tensor([[math.inf, -math.inf, math.nan, 1.0]]).to(torch.bfloat16)
+    fine = torch.ones_like(bad)
+    for x, y in ((bad, fine), (fine, bad)):
+        assert torch.isnan(silu_mul_fp8(x.cuda(), y.cuda()).codes.float().cpu()[0, :4]).tolist() == [True, True, True, False]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("shape", SHAPES + [(1, 65536), (2, 33000)])
+def test_rms_norm(shape, residual, dtype):
+    x, w = rand(*shape, seed=13, dtype=dtype), 0.3 * rand(shape[-1], seed=14, dtype=torch.float32)
+    res = rand(*shape, seed=15, dtype=dtype) if residual else None
+    t, v = ref.rms_norm(x, w, 1e-6, res)
+    got = rms_norm_fp8(x.cuda(), w.cuda(), 1e-6, residual=None if res is None else res.cuda())
+    if residual:
+        assert torch.equal(got[0].cpu(), t)
+        got = got[1]
+    same_rows(got, v)
+
+
+@pytest.mark.gpu
+def test_rms_norm_of_odd_rows():
+    """A row of zeros, tiny and large rows, one with an infinity or a NaN; its neighbours stand."""
+    x = rand(6, 640, seed=16, dtype=torch.float32)
+    w = 0.2 * rand(640, seed=17, dtype=torch.float32)
+    x[0] = 0.0
+    x[1] *= 1e-20
+    x[2] *= 1e15
+    x[3, 5] = math.nan
+    r = rms_norm_fp8(x.cuda(), w.cuda(), 1e-6)
+    keep = [0, 1, 2, 4, 5]
+    v = ref.rms_norm(x, w, 1e-6)[1]
+    for i in keep:
+        same_rows(Fp8Rows(r.codes[i:i + 1], r.scales[i:i + 1]), v[i:i + 1])
+    assert torch.isnan(r.codes[3].float()).all()
+    x[4, 9] = math.inf               # the factor is 0: zeros, and NaN where 0 meets the infinity
+    r = rms_norm_fp8(x.cuda(), w.cuda(), 1e-6)
+    want = torch.zeros(640)
+    want[9] = math.nan
+    assert torch.equal(torch.isnan(r.codes[4].float()).cpu(), torch.isnan(want))
+    assert not torch.nan_to_num(r.codes[4].float()).any()
+    same_rows(Fp8Rows(r.codes[5:], r.scales[5:]), v[5:])
+    r = rms_norm_fp8(torch.full((1, 256), 3e38).cuda(), torch.ones(256).cuda(), 0.0)    # squares beyond fp32
+    assert not r.codes.float().any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("fn", [lambda x: quantize_rows_fp8(x), lambda x: silu_mul_fp8(x, x),
+                                lambda x: rms_norm_fp8(x, torch.zeros(200, device="cuda"))])
+def test_no_rows(fn):
+    r = fn(torch.zeros(0, 3, 200, dtype=torch.bfloat16, device="cuda"))
+    assert r.shape == (0, 3, 200) and r.codes.shape == (0, 3, 256) and r.scales.shape == (0, 3, 4)
+    packed = tuple(t.cuda() for t in quantize_fp8(rand(40, 200, dtype=torch.float32)))
+    assert fp8_linear(r, *packed, out_features=40).shape == (0, 3, 40)
+
+
+# --- products ------------------------------------------------------------------------
+def weight(N, K, seed=20):
+    w = rand(N, K, seed=seed, dtype=torch.float32) / K ** 0.5
+    return quantize_fp8(w)
+
+
+SIZES = [(1, 1, 1), (1, 128, 16), (2, 1000, 17), (3, 130, 300), (15, 512, 64), (16, 1024, 129), (17, 640, 100),
+         (31, 4096, 48), (33, 2050, 65), (64, 1024, 4384), (65, 384, 130), (100, 129, 257), (128, 256, 128),
+         (130, 1024, 140), (255, 2048, 255), (300, 700, 600), (513, 1152, 520), (1000, 128, 1000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_linear(M, K, N, bias):
+    rows, (packed, scales) = make_rows(M, K, seed=M), weight(N, K)
+    b = rand(N, seed=2) if bias else None
+    y = fp8_linear(on(rows), packed.cuda(), scales.cuda(), None if b is None else b.cuda(), out_features=N)
+    assert y.shape == (M, N) and y.dtype == torch.bfloat16
+    check_linear(y, rows, packed, scales, N, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_linear_of_whole_numbers(M, K, N):
+    """Sums that fp32 holds: the result is the exact one, rounded once."""
+    g = torch.Generator().manual_seed(M + N)
+    x, w = torch.randint(-4, 5, (M, K), generator=g).float(), torch.randint(-4, 5, (N, K), generator=g).float()
+    kb = (K + 127) // 128
+    xs = torch.randint(127, 130, (M, (kb + 3) // 4 * 4), generator=g).to(torch.uint8)
+    rows = Fp8Rows(torch.nn.functional.pad(x, (0, -K % 128)).to(E4), xs.view(E8), K)
+    packed, scales = pack_fp8(w.to(E4), torch.randint(126, 129, ((N + 127) // 128, kb), generator=g).to(torch.uint8))
+    b = torch.randint(-8, 9, (N,), generator=g).to(torch.bfloat16)
+    y = fp8_linear(on(rows), packed.cuda(), scales.cuda(), b.cuda(), out_features=N)
+    want, _ = ref.linear(ref.values(rows.codes, rows.scales, K), ref.weight(packed, scales, N, K), b)
+    assert torch.equal(y.cpu().double(), want.to(torch.bfloat16).double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 40, 300])
+def test_linear_cuts_within_eight_columns_alone(M):
+    """Large terms that cancel leave what stands outside their groups of eight columns,
+    down to 2^-20 of them, also in other blocks: 2^16 + 2^-4 has 21 bits, fp32 holds 24
+    (of 2^-13, 2^-29 of 2^16, it could hold none)."""
+    K, N = 640, 16
+    x, w = torch.zeros(M, K), torch.ones(N, K)
+    x[:, 0], x[:, 88] = 256.0, -256.0
+    for i, k in enumerate((8, 40, 64, 96, 127, 128, 300, 639)):
+        x[:, k] = 2.0 ** (i - 4)
+    scales = torch.full((M, 8), 127, dtype=torch.uint8).view(E8)
+    sel = torch.zeros(K, dtype=torch.bool)
+    sel[0] = sel[88] = True
+    packed, ws = pack_fp8(torch.where(sel, 256 * w, w).to(E4), torch.ones(1, 5))
+    y = fp8_linear(Fp8Rows(x.to(E4).cuda(), scales.cuda()), packed.cuda(), ws.cuda(), out_features=N)
+    assert (y.cpu().double() == 255 * 2.0 ** -4).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 40, 200])
+def test_linear_of_tensors_and_gates(M):
+    K, N = 333, 77
+    packed, scales = weight(N, K)
+    x, gate = rand(2, M, K, seed=3), torch.sigmoid(rand(2, M, K, seed=4, big=False))
+    for g in (None, gate):
+        v = x.double() if g is None else x.double() * g.double()
+        codes, s = ref.rows(v.reshape(-1, K))
+        rows = Fp8Rows(codes.to(E4), (torch.log2(s) + 127).to(torch.uint8).view(E8), K)
+        y = fp8_linear(x.cuda(), packed.cuda(), scales.cuda(), out_features=N, xscale=None if g is None else g.cuda())
+        assert y.shape == (2, M, N)
+        check_linear(y, rows, packed, scales, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 20, 300])
+def test_linear_multi(M):
+    K, sizes = 600, [128, 1, 300, 513]
+    ws = [weight(N, K, seed=N) for N in sizes]
+    bs = [None, rand(1, seed=1), rand(300, seed=2), None]
+    rows = make_rows(M, K)
+    ys = fp8_linear_multi(on(rows), [(p.cuda(), s.cuda()) for p, s in ws], [None if b is None else b.cuda() for b in bs],
+                          sizes)
+    for y, w, b, N in zip(ys, ws, bs, sizes):
+        assert y.is_contiguous()
+        check_linear(y, rows, *w, N, b)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 64, 257])
+def test_linear_scales(M):
+    """Every block with a scale of its own, far apart."""
+    g = torch.Generator().manual_seed(4)
+    K, N = 1300, 400
+    rows = make_rows(M, K)
+    rows.scales = torch.randint(90, 160, rows.scales.shape, generator=g).to(torch.uint8).view(E8)
+    codes = torch.randn(N, K, generator=g).to(E4)
+    packed, scales = pack_fp8(codes, torch.randint(90, 160, (4, 11), generator=g).to(torch.uint8))
+    y = fp8_linear(on(rows), packed.cuda(), scales.cuda(), out_features=N)
+    check_linear(y, rows, packed, scales, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [4, 70, 300])
+def test_linear_keeps_nan_in_its_row(M):
+    K, N = 500, 200
+    x = rand(M, K, seed=7)
+    x[1, 130] = math.inf
+    x[M - 1, 3] = math.nan
+    packed, scales = (t.cuda() for t in weight(N, K))
+    y = fp8_linear(x.cuda(), packed, scales, out_features=N)
+    bad = torch.zeros(M, dtype=torch.bool)
+    bad[1] = bad[M - 1] = True
+    assert torch.equal(torch.isnan(y).all(1).cpu(), bad) and torch.equal(torch.isnan(y).any(1).cpu(), bad)
+    x[1, 130] = x[M - 1, 3] = 0.0
+    z = fp8_linear(x.cuda(), packed, scales, out_features=N)
+    assert torch.equal(y.cpu()[~bad], z.cpu()[~bad])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [4, 90])
+def test_linear_of_views(M):
+    """Rows and scales that are slices are copied; uint8 scales are taken as they are."""
+    K, N = 256, 96
+    rows, (packed, scales) = make_rows(2 * M, K), weight(N, K)
+    cut = Fp8Rows(on(rows).codes[::2], on(rows).scales.view(torch.uint8)[::2])
+    y = fp8_linear(cut, packed.cuda(), scales.view(torch.uint8).cuda(), out_features=N)
+    check_linear(y, Fp8Rows(rows.codes[::2], rows.scales.view(torch.uint8)[::2].contiguous()), packed, scales, N)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("N,K", [(1, 1), (40, 200), (128, 128), (300, 515)])
+def test_dequantize(N, K):
+    packed, scales = weight(N, K)
+    got = dequantize_fp8(packed.cuda(), scales.cuda(), N, K)
+    assert got.dtype == torch.bfloat16 and torch.equal(got.cpu().double(), ref.weight(packed, scales, N, K))
+    with pytest.raises(ValueError):
+        dequantize_fp8(packed.cuda(), scales.cuda(), N + 16, K)
+
+
+# --- gradients -------------------------------------------------------------------------
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [3, 100])
+def test_gradients_are_the_formulas(M):
+    K, N = 300, 70
+    packed, scales = weight(N, K)
+    w = ref.weight(packed, scales, N, K)
+    x, gate = rand(M, K, seed=1, big=False).cuda().requires_grad_(), torch.sigmoid(rand(M, K, seed=2, big=False)).cuda().requires_grad_()
+    b, dy = rand(N, seed=3).cuda().requires_grad_(), rand(M, N, seed=4, big=False)
+    y = fp8_linear(x, packed.cuda(), scales.cuda(), b, out_features=N)
+    with torch.no_grad():
+        assert torch.equal(y, fp8_linear(x, packed.cuda(), scales.cuda(), b, out_features=N))
+    dx, db = torch.autograd.grad(y, (x, b), dy.cuda())
+    want, A = ref.linear(dy.double(), w.t())
+    # N products summed in fp32 and one rounding; the bias M
+    assert ((dx.cpu().double() - want).abs() <= (N + 8) * 2.0 ** -23 * A + 2.0 ** -8 * want.abs()).all()
+    want = dy.double().sum(0)
+    assert ((db.cpu().double() - want).abs() <= (M + 8) * 2.0 ** -23 * dy.double().abs().sum(0) + 2.0 ** -8 * want.abs()).all()
+    y = fp8_linear(x, packed.cuda(), scales.cuda(), out_features=N, xscale=gate)
+    dxs = torch.autograd.grad(y, (x, gate), dy.cuda())
+    want, A = ref.linear(dy.double(), w.t())
+    for got, f in zip(dxs, (gate, x)):
+        f = f.detach().cpu().double()
+        # the product's gradient is rounded before and after it meets the other factor
+        tol = ((N + 8) * 2.0 ** -23 * A + 2.0 ** -8 * want.abs()) * (1 + 2.0 ** -8) * f.abs() + 2.0 ** -8 * (want * f).abs()
+        assert ((got.cpu().double() - want * f).abs() <= tol).all()
+    rows = make_rows(M, K)
+    y = fp8_linear(on(rows), packed.cuda(), scales.cuda(), b, out_features=N)
+    (db,) = torch.autograd.grad(y, b, dy.cuda())
+    want = dy.double().sum(0)
+    assert ((db.cpu().double() - want).abs() <= (M + 8) * 2.0 ** -23 * dy.double().abs().sum(0) + 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.gpu
+def test_gradient_is_the_difference():
+    """Where x and x + d are both codes (whole numbers to 8, 448 in each block so that
+    the scale is 1), the layer is linear in x and its difference is the gradient's:
+    weights of whole numbers keep every sum exact."""
+    K, N = 256, 32
+    g = torch.Generator().manual_seed(0)
+    x = torch.randint(-4, 5, (2, K), generator=g).float()
+    x[:, 0] = x[:, 128] = 448.0
+    codes = torch.randint(-2, 3, (N, K), generator=g).float()
+    codes[:, 0] = codes[:, 128] = 0.0
+    packed, scales = (t.cuda() for t in pack_fp8(codes.to(E4), torch.ones(1, 2)))
+    d = torch.randint(-4, 5, (2, K), generator=g).float()
+    d[:, 0] = d[:, 128] = 0.0
+    xg = x.to(torch.bfloat16).cuda().requires_grad_()
+    y = fp8_linear(xg, packed, scales, out_features=N)
+    dy = torch.randint(-1, 2, (2, N), generator=g).to(torch.bfloat16)
+    (dx,) = torch.autograd.grad(y, xg, dy.cuda())
+    # the outputs' own rounding to bf16 is kept out by taking the difference of their exact values
+    w = codes.double()
+    diff = (((x + d).double() @ w.t() - x.double() @ w.t()) * dy.double()).sum()
+    assert torch.equal(y.detach().cpu().double(), (x.double() @ w.t()).to(torch.bfloat16).double())
+    y2 = fp8_linear((x + d).to(torch.bfloat16).cuda(), packed, scales, out_features=N)
+    assert torch.equal(y2.cpu().double(), ((x + d).double() @ w.t()).to(torch.bfloat16).double())
+    assert (dx.cpu().double() * d.double()).sum() == diff
+
+
+@pytest.mark.gpu
+def test_forward_mode_is_refused():
+    import torch.autograd.forward_ad as fwd
+    packed, scales = (t.cuda() for t in weight(16, 128))
+    x = torch.ones(1, 128, dtype=torch.bfloat16, device="cuda")
+    with fwd.dual_level():
+        dual = fwd.make_dual(x, x)
+        for call in (lambda: fp8_linear(dual, packed, scales), lambda: quantize_rows_fp8(dual),
+                     lambda: silu_mul_fp8(dual, dual), lambda: rms_norm_fp8(dual, torch.zeros(128, device="cuda"))):
+            with pytest.raises((RuntimeError, NotImplementedError)):
+                call()
+
+
+# --- a run of them, streams and graphs ---------------------------------------------------
+def chain(x, res, w, ws, bs):
+    """A pre-norm SwiGLU layer in 8 bits."""
+    t, n = rms_norm_fp8(x, w, 1e-6, residual=res)
+    a, c = fp8_linear_multi(n, ws[:2], bs[:2], [384, 384])
+    return t + fp8_linear(silu_mul_fp8(a, c), *ws[2], bs[2], out_features=256)
+
+
+def chain_inputs(M, seed=0):
+    x, res = rand(M, 256, seed=seed).cuda(), rand(M, 256, seed=seed + 1).cuda()
+    w = 0.1 * rand(256, seed=2, dtype=torch.float32).cuda()
+    ws = [tuple(t.cuda() for t in weight(n, k, seed=i)) for i, (n, k) in enumerate(((384, 256), (384, 256), (256, 384)))]
+    bs = [rand(n, seed=9, big=False).cuda() for n in (384, 384, 256)]
+    return x, res, w, ws, bs
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [1, 6, 80, 700])
+def test_a_run_of_them(M):
+    """Each step against the oracle on the step's own inputs."""
+    x, res, w, ws, bs = chain_inputs(M)
+    t, n = rms_norm_fp8(x, w, 1e-6, residual=res)
+    want, v = ref.rms_norm(x.cpu(), w.cpu(), 1e-6, res.cpu())
+    assert torch.equal(t.cpu(), want)
+    same_rows(n, v)
+    a, c = fp8_linear_multi(n, ws[:2], bs[:2], [384, 384])
+    for y, p, b in ((a, ws[0], bs[0]), (c, ws[1], bs[1])):
+        check_linear(y, n, *p, 384, b.cpu())
+    r = silu_mul_fp8(a, c)
+    check_silu(r, a.cpu(), c.cpu())
+    y = fp8_linear(r, *ws[2], bs[2], out_features=256)
+    check_linear(y, r, *ws[2], 256, bs[2].cpu())
+    assert torch.equal(chain(x, res, w, ws, bs), t + y)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [2, 300])
+def test_captured_on_another_stream(M):
+    """Two graphs of the run, replayed with eager work between, on new inputs."""
+    ins = [chain_inputs(M, seed=s) for s in (0, 40)]
+    eager = [chain(*i) for i in ins]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        assert all(torch.equal(chain(*i), e) for i, e in zip(ins, eager))
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for i in ins:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(chain(*i))
+        graphs.append(g)
+    for turn in range(3):
+        for k in (0, 1):
+            x = rand(M, 256, seed=100 + turn + 10 * k).cuda()
+            ins[k][0].copy_(x)
+            graphs[k].replay()
+            want = chain(*ins[k])
+            torch.cuda.synchronize()
+            assert torch.equal(outs[k], want)
+
+
+@pytest.mark.gpu
+def test_offsets_past_32_bits():
+    """Rows and outputs behind 2^32 bytes."""
+    M, K, N = (1 << 25) // 2 + 5, 256, 128
+    x = torch.zeros(M, K, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = rand(3, K, seed=1).cuda()
+    packed, scales = weight(N, K)
+    r = quantize_rows_fp8(x)
+    same_rows(Fp8Rows(r.codes[-3:], r.scales[-3:], K), x[-3:].cpu().double())
+    del x
+    y = fp8_linear(Fp8Rows(r.codes[:1 << 24], r.scales[:1 << 24]), packed.cuda(), scales.cuda(), out_features=N)
+    assert not y[-1].any()
+    y = fp8_linear(Fp8Rows(r.codes[5:], r.scales[5:]), packed.cuda(), scales.cuda(), out_features=N)
+    check_linear(y[-3:], Fp8Rows(r.codes[-3:], r.scales[-3:]), packed, scales, N)
+    assert not y[:-3].any()
+    with pytest.raises(RuntimeError):
+        fp8_linear(r, packed.cuda(), scales.cuda(), out_features=N)
