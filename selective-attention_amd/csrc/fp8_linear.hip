@@ -121,146 +121,226 @@ __device__ __forceinline__ v16f mfma_fp8(const v8i& a, const v8i& b, const v16f&
 __device__ __forceinline__ v8i lds_frag(const uint8_t* p, const uint8_t* q) {
   return join16(*reinterpret_cast<const uint4*>(p), *reinterpret_cast<const uint4*>(q));
 }
+// (memory is not moved past it)
 __device__ __forceinline__ void lds_barrier() {
   asm volatile("" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+using yes = std::integral_constant<bool, true>;
+using no = std::integral_constant<bool, false>;
+
+// What a workgroup of a tile kernel computes: columns n0 .. of matrix seg for rows m0 ..
+struct Fp8Tile {
+  int seg, n0, m0;
+};
+// Tiles in the order of the XCDs, a part of the list each, so that an L2 serves
+// neighbours; in it, `high` rows of tiles at a time
+template <int BN, int BM>
+__device__ __forceinline__ Fp8Tile tile_of(const Fp8Segs& sg, int mtiles) {
+  const int ntiles = sg.blk0[kFp8Segs], total = ntiles * mtiles, xcd = blockIdx.x & 7;
+  const int id = xcd * (total >> 3) + min(xcd, total & 7) + (blockIdx.x >> 3);
+  const int band = id / (4 * ntiles), left = id - band * 4 * ntiles, high = min(4, mtiles - 4 * band);
+  const int nt = left / high;
+  Fp8Tile t{0, 0, (4 * band + left % high) * BM};
+#pragma unroll
+  for (int i = 1; i < kFp8Segs; ++i) t.seg += (i < sg.nseg && nt >= sg.blk0[i]) ? 1 : 0;
+  t.n0 = (nt - sg.blk0[t.seg]) * BN;
+  return t;
+}
+
+// The scales of a wave's 32 SN columns and 32 SM rows, a word for four blocks: the
+// rows' a lane each, the weight's one for the wave (columns of one block of 128)
+template <int SM>
+struct Fp8Scales {
+  const uint32_t *w, *x;
+  uint32_t at[SM], sx[SM], nx[SM], sw, nw;
+  int words;
+  __device__ __forceinline__ Fp8Scales(const Fp8Segs& sg, const uint8_t* xs, const Fp8Tile& t, int n, int m, int M,
+                                       int words_) : words(words_) {
+    w = reinterpret_cast<const uint32_t*>(sg.scale[t.seg]) + static_cast<long>(min(n, sg.N[t.seg] - 1) >> 7) * words;
+    x = reinterpret_cast<const uint32_t*>(xs) + static_cast<long>(t.m0) * words;
+#pragma unroll
+    for (int j = 0; j < SM; ++j)
+      at[j] = static_cast<uint32_t>(min(m - t.m0 + 32 * j + static_cast<int>(threadIdx.x & 31), M - 1 - t.m0)) * words;
+    load(0);
+  }
+  __device__ __forceinline__ void load(int g) {   // the next word
+    nw = w[g];
+#pragma unroll
+    for (int j = 0; j < SM; ++j) nx[j] = x[at[j] + g];
+  }
+  __device__ __forceinline__ void take() {
+    sw = nw;
+#pragma unroll
+    for (int j = 0; j < SM; ++j) sx[j] = nx[j];
+  }
+  // from block t to the next: the low byte is block t + 1's
+  __device__ __forceinline__ void step(int t) {
+    if ((t & 3) == 3) return take();
+    sw >>= 8;
+#pragma unroll
+    for (int j = 0; j < SM; ++j) sx[j] >>= 8;
+  }
+  // a word two blocks ahead of its use
+  __device__ __forceinline__ void ahead(int t) {
+    if ((t & 3) == 1) load(min((t >> 2) + 1, words - 1));
+  }
+};
+
+// The wave's 32 SM rows and 32 SN columns of y, through its own part of LDS (32 rows
+// of kCols columns at a time) so that they leave as whole pieces of 2 kCols bytes.  They
+// pass the caches by: nothing here reads them again, and the next tiles' operands
+// stay (32768 rows, 1024 -> 4096: 165 us, so 142).
+template <int SN, int SM>
+struct Fp8Out {
+  static constexpr int kCols = SN > 1 ? 64 : 32, kPitch = 2 * kCols + 16, kBytes = 32 * kPitch;
+  static __device__ __forceinline__ void store(const v16f (&acc)[SN][SM], uint8_t* ys, const float* bias, bf16* y0,
+                                               int nw, int mw, int N, int M) {
+    const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    bf16* y = y0 + static_cast<long>(mw) * N + nw;
+    const bool whole = (N & 7) == 0 && (reinterpret_cast<uintptr_t>(y0) & 15) == 0;
+    constexpr int kSq = kCols / 32, kLanes = kCols / 8;
+#pragma unroll
+    for (int j = 0; j < SM; ++j)
+#pragma unroll
+      for (int i0 = 0; i0 < SN; i0 += kSq) {
+        // lane (c, h) holds columns 8 q + 4 h + e of square i for row c
+#pragma unroll
+        for (int i = 0; i < kSq; ++i)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const v16f& a = acc[i0 + i][j];
+            const float4 b = *reinterpret_cast<const float4*>(bias + 32 * (i0 + i) + 8 * q + 4 * h);
+            *reinterpret_cast<uint2*>(ys + c * kPitch + (32 * i + 8 * q + 4 * h) * 2) =
+                uint2{pack_bf16x2(a[4 * q] + b.x, a[4 * q + 1] + b.y), pack_bf16x2(a[4 * q + 2] + b.z, a[4 * q + 3] + b.w)};
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if (whole) {
+#pragma unroll
+          for (int r = 0; r < 32; r += 64 / kLanes) {
+            const int row = r + lane / kLanes, n = 32 * i0 + 8 * (lane % kLanes);
+            const v4f v = *reinterpret_cast<const v4f*>(ys + row * kPitch + 16 * (lane % kLanes));
+            if (mw + 32 * j + row < M && nw + n < N)
+              __builtin_nontemporal_store(v, reinterpret_cast<v4f*>(y + static_cast<long>(32 * j + row) * N + n));
+          }
+        } else {
+          // rows start anywhere: words of two columns where both are the wave's, else one
+          constexpr int kPairs = kCols / 2;
+#pragma unroll 4
+          for (int r = 0; r < 32; r += 64 / kPairs) {
+            const int row = r + lane / kPairs, left = N - nw - 32 * i0;   // columns of y from here on
+            bf16* to = y + static_cast<long>(32 * j + row) * N + 32 * i0;
+            const bf16* from = reinterpret_cast<const bf16*>(ys + row * kPitch);
+            const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(to) >> 1) & 1, n = 2 * (lane % kPairs) + odd;
+            if (mw + 32 * j + row < M) {
+              if (n + 1 < min(kCols, left))
+                *reinterpret_cast<uint32_t*>(to + n) = from[n].x | static_cast<uint32_t>(from[n + 1].x) << 16;
+              else if (n < min(kCols, left))
+                to[n] = from[n];
+              if (odd && n == 1 && left > 0) to[0] = from[0];
+            }
+          }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+  }
+};
 
 // A workgroup of four waves (2 by 2) computes 64 SN columns of y for 64 SM rows of x;
 // a wave SN by SM squares of 32 (W as the first operand, so that a lane holds four
 // neighbouring columns of one row).  A step is one block of 128 columns of K, in LDS in
 // two stages that DMA fills: W as it is packed, x as rows of 128 bytes whose pieces of
-// 16 are permuted by row (piece p of row r at p ^ (r & 7)), so that eight lanes read
-// all banks.  Operands are held for half a step (64 columns): while the matrix cores
-// take one half, the next is read, also over the steps' border, so that a step needs
-// one barrier, in its middle: there this step's stage has been read by all and the
-// next one has landed.
+// 16 are permuted by row (piece p of row r at p ^ (r / 2 & 7)), so that sixteen lanes
+// read all banks.  Operands are held for half a step (64 columns): while the matrix
+// cores take one half, the next is read, also over the steps' border, so that a step
+// needs one barrier, in its middle: there this step's stage has been read by all and
+// the next one has landed.  For large products, 256 by 256 with one wave a SIMD (its
+// sums fill half of the registers): of all shapes it reads LDS the least.
 template <int SN, int SM>
-__global__ __launch_bounds__(256, SN * SM > 4 ? 1 : 2) void fp8_tile_kernel(const uint8_t* __restrict__ x,
-                                                                          const uint8_t* __restrict__ xs,
-                                                                          const Fp8Segs sg, int M, int kb_n,
-                                                                          int mtiles) {
+__global__ __launch_bounds__(256, 1) void fp8_large_kernel(const uint8_t* __restrict__ x,
+                                                           const uint8_t* __restrict__ xs, const Fp8Segs sg, int M,
+                                                           int kb_n, int mtiles) {
   constexpr int BN = 64 * SN, BM = 64 * SM, kW = BN * 128, kStage = (BN + BM) * 128;
-  constexpr int kPitch = 64 * SN + 16;                    // bytes of a row of y in LDS
-  static_assert(4 * 32 * kPitch <= 2 * kStage, "y fits the stages");
+  using Out = Fp8Out<SN, SM>;
+  static_assert(4 * Out::kBytes <= 2 * kStage, "y fits the stages");
   __shared__ __align__(16) uint8_t smem[2 * kStage + 4 * BN];
   float* bias_lds = reinterpret_cast<float*>(smem + 2 * kStage);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
   const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid & 1, wm = wid >> 1;
-
-  // tiles in order of the XCDs, a part of the list each; in it, four rows of tiles at a time
-  const int ntiles = sg.blk0[kFp8Segs], total = ntiles * mtiles;
-  int id = blockIdx.x;
-  {
-    const int per = total >> 3, more = total & 7, xcd = id & 7;
-    id = xcd * per + min(xcd, more) + (id >> 3);
-  }
-  const int band = id / (4 * ntiles), left = id - band * 4 * ntiles, high = min(4, mtiles - 4 * band);
-  const int mt = 4 * band + left % high, nt = left / high;
-  int seg = 0;
-#pragma unroll
-  for (int i = 1; i < kFp8Segs; ++i) seg += (i < sg.nseg && nt >= sg.blk0[i]) ? 1 : 0;
-  const int N = sg.N[seg], tiles = (N + 15) >> 4, words = (kb_n + 3) >> 2;
-  const int n0 = (nt - sg.blk0[seg]) * BN, m0 = mt * BM;
-  const bf16* bias = sg.bias[seg];
+  const Fp8Tile tile = tile_of<BN, BM>(sg, mtiles);
+  const int N = sg.N[tile.seg], n0 = tile.n0, m0 = tile.m0, nw = n0 + wn * 32 * SN, mw = m0 + wm * 32 * SM;
+  const bf16* bias = sg.bias[tile.seg];
   if (tid < BN) bias_lds[tid] = bias && n0 + tid < N ? to_f32(bias[n0 + tid]) : 0.0f;
 
-  // DMA: 1 KB an instruction; a wave takes SN * 2 of W and SM * 2 of x
+  // DMA: 1 KB an instruction; a wave takes SN * 2 of W (a tile's half each) and SM * 2 of x
+  // (eight rows); what lies behind the last tile or row is the last again and not stored
   const uint32_t ls = lds_addr(smem);
-  const uint8_t* wbase = sg.W[seg] + static_cast<long>(n0 >> 4) * kb_n * 2048;
+  const uint8_t* wbase = sg.W[tile.seg] + static_cast<long>(n0 >> 4) * kb_n * 2048;
   const uint8_t* xbase = x + static_cast<long>(m0) * kb_n * 128;
   uint32_t woff[2 * SN], xoff[2 * SM];
 #pragma unroll
   for (int i = 0; i < 2 * SN; ++i) {
-    const int q = wid * 2 * SN + i, t = min(q >> 1, tiles - 1 - (n0 >> 4));   // (behind the last: not stored)
+    const int q = wid * 2 * SN + i, t = min(q >> 1, ((N + 15) >> 4) - 1 - (n0 >> 4));
     woff[i] = static_cast<uint32_t>(t) * kb_n * 2048 + (q & 1) * 1024 + lane * 16;
   }
 #pragma unroll
   for (int i = 0; i < 2 * SM; ++i) {
     const int r = min((wid * 2 * SM + i) * 8 + (lane >> 3), M - 1 - m0);
-    xoff[i] = static_cast<uint32_t>(r) * kb_n * 128 + ((lane & 7) ^ (lane >> 3)) * 16;
+    xoff[i] = static_cast<uint32_t>(r) * kb_n * 128 + ((lane & 7) ^ ((lane >> 4) + 4 * (i & 1))) * 16;
   }
-  auto dma_w = [&](int i, int t, uint32_t stage) __attribute__((always_inline)) {
-    dma_lds16(wbase + static_cast<long>(t) * 2048, woff[i], stage + ((wid * 2 * SN + i) << 10));
+  auto dma = [&](int i, int t, uint32_t stage) __attribute__((always_inline)) {
+    if (i < 2 * SN) dma_lds16(wbase + static_cast<long>(t) * 2048, woff[i], stage + ((wid * 2 * SN + i) << 10));
+    else if (i < 2 * (SN + SM))
+      dma_lds16(xbase + static_cast<long>(t) * 128, xoff[i - 2 * SN], stage + kW + ((wid * 2 * SM + i - 2 * SN) << 10));
   };
-  auto dma_x = [&](int i, int t, uint32_t stage) __attribute__((always_inline)) {
-    dma_lds16(xbase + static_cast<long>(t) * 128, xoff[i], stage + kW + ((wid * 2 * SM + i) << 10));
-  };
-  // scales, a word for four blocks: the rows' a lane each, the weight's one for the wave
-  const uint8_t* wsp = sg.scale[seg] + static_cast<long>(min((n0 + wn * 32 * SN) >> 7, (N - 1) >> 7)) * 4 * words;
-  uint32_t sx[SM], nsx[SM], sw, nsw;
-  const uint8_t* xsp[SM];
+  auto dma_all = [&](int t, uint32_t stage) __attribute__((always_inline)) {
 #pragma unroll
-  for (int j = 0; j < SM; ++j) xsp[j] = xs + static_cast<long>(min(m0 + (wm * SM + j) * 32 + c, M - 1)) * 4 * words;
-  auto load_scales = [&](int g) __attribute__((always_inline)) {
-    nsw = *reinterpret_cast<const uint32_t*>(wsp + 4 * g);
-#pragma unroll
-    for (int j = 0; j < SM; ++j) nsx[j] = *reinterpret_cast<const uint32_t*>(xsp[j] + 4 * g);
-  };
-  auto take_scales = [&]() __attribute__((always_inline)) {
-    sw = nsw;
-#pragma unroll
-    for (int j = 0; j < SM; ++j) sx[j] = nsx[j];
+    for (int i = 0; i < 2 * (SN + SM); ++i) dma(i, t, stage);
   };
 
   // operands' places in a stage: piece 4 half + 2 h + i of a row
   const int wa = wn * SN * 4096 + (c >> 4) * 2048 + h * 512 + (c & 15) * 16;
   int xa[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) xa[i] = kW + wm * SM * 4096 + c * 128 + ((((i >> 1) * 4 + 2 * h + (i & 1)) ^ (c & 7)) * 16);
+  for (int i = 0; i < 4; ++i)
+    xa[i] = kW + wm * SM * 4096 + c * 128 + ((((i >> 1) * 4 + 2 * h + (i & 1)) ^ ((c >> 1) & 7)) * 16);
   v8i fw[2][SN], fx[2][SM];
-  auto read_w = [&](int half, int s, int stage) __attribute__((always_inline)) {
-    const uint8_t* p = smem + stage + wa + s * 4096 + half * 1024;
-    fw[half][s] = lds_frag(p, p + 256);
-  };
-  auto read_x = [&](int half, int s, int stage) __attribute__((always_inline)) {
-    const uint8_t* p = smem + stage + s * 4096;
-    fx[half][s] = lds_frag(p + xa[2 * half], p + xa[2 * half + 1]);
-  };
   // operand r in the order in which the products need them: one of W, those of x, the rest of W
   auto read_frag = [&](int half, int r, int stage) __attribute__((always_inline)) {
-    if (r == 0) read_w(half, 0, stage);
-    else if (r <= SM) read_x(half, r - 1, stage);
-    else if (r < SN + SM) read_w(half, r - SM, stage);
+    if (r == 0 || (r > SM && r < SN + SM)) {
+      const int s = r == 0 ? 0 : r - SM;
+      const uint8_t* p = smem + stage + wa + s * 4096 + half * 1024;
+      fw[half][s] = lds_frag(p, p + 256);
+    } else if (r <= SM) {
+      const uint8_t* p = smem + stage + (r - 1) * 4096;
+      fx[half][r - 1] = lds_frag(p + xa[2 * half], p + xa[2 * half + 1]);
+    }
   };
-  constexpr int kReads = SN * SM >= 8 ? 1 : 2, kDma = (2 * (SN + SM) + SN * SM - 1) / (SN * SM);
-  static_assert(kReads * SN * SM >= SN + SM, "all operands are read");
-  v16f acc[SN][SM];
-#pragma unroll
-  for (int i = 0; i < SN; ++i)
-#pragma unroll
-    for (int j = 0; j < SM; ++j)
-#pragma unroll
-      for (int e = 0; e < 16; ++e) acc[i][j][e] = 0.0f;
+  constexpr int kSlots = SN * SM, kReads = (SN + SM + kSlots - 1) / kSlots, kDma = (2 * (SN + SM) + kSlots - 1) / kSlots;
 
-#pragma unroll
-  for (int i = 0; i < 2 * SN; ++i) dma_w(i, 0, ls);
-#pragma unroll
-  for (int i = 0; i < 2 * SM; ++i) dma_x(i, 0, ls);
-  load_scales(0);
+  v16f acc[SN][SM] = {};
+  dma_all(0, ls);
+  Fp8Scales<SM> sc(sg, xs, tile, nw, mw, M, (kb_n + 3) >> 2);
   __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<0>());
   lds_barrier();
-  take_scales();
-  if (kb_n > 1) {
-#pragma unroll
-    for (int i = 0; i < 2 * SN; ++i) dma_w(i, 1, ls + kStage);
-#pragma unroll
-    for (int i = 0; i < 2 * SM; ++i) dma_x(i, 1, ls + kStage);
-  }
+  sc.take();
+  if (kb_n > 1) dma_all(1, ls + kStage);
 #pragma unroll
   for (int r = 0; r < SN + SM; ++r) read_frag(0, r, 0);
 
-  // step t: MORE: a step t + 2 follows, NEXT: a step t + 1
+  // step t: a step t + 1 follows (NEXT), a step t + 2 (MORE)
   auto step = [&](int t, auto next, auto more) __attribute__((always_inline)) {
     constexpr bool NEXT = decltype(next)::value, MORE = decltype(more)::value;
     const int cur = (t & 1) * kStage, oth = kStage - cur;
-    if (NEXT && (t & 3) == 1) load_scales(min((t >> 2) + 1, words - 1));
+    if (NEXT) sc.ahead(t);
     // (the order is kept as written: reads and DMA go out between the products)
 #pragma unroll
-    for (int k = 0; k < SN * SM; ++k) {
+    for (int k = 0; k < kSlots; ++k) {
       const int i = k / SM, j = k % SM;
-      acc[i][j] = mfma_fp8(fw[0][i], fx[0][j], acc[i][j], sw, sx[j]);
+      acc[i][j] = mfma_fp8(fw[0][i], fx[0][j], acc[i][j], sc.sw, sc.sx[j]);
 #pragma unroll
       for (int r = k * kReads; r < (k + 1) * kReads; ++r) read_frag(1, r, cur);
       __builtin_amdgcn_sched_barrier(0);
@@ -270,79 +350,192 @@ __global__ __launch_bounds__(256, SN * SM > 4 ? 1 : 2) void fp8_tile_kernel(cons
       lds_barrier();   // this stage is read by all, the next one has landed
     }
 #pragma unroll
-    for (int k = 0; k < SN * SM; ++k) {
+    for (int k = 0; k < kSlots; ++k) {
       const int i = k / SM, j = k % SM;
-      acc[i][j] = mfma_fp8(fw[1][i], fx[1][j], acc[i][j], sw, sx[j]);
+      acc[i][j] = mfma_fp8(fw[1][i], fx[1][j], acc[i][j], sc.sw, sc.sx[j]);
       if constexpr (NEXT) {
 #pragma unroll
         for (int r = k * kReads; r < (k + 1) * kReads; ++r) read_frag(0, r, oth);
       }
       if constexpr (MORE) {
 #pragma unroll
-        for (int d = k * kDma; d < (k + 1) * kDma; ++d) {
-          if (d < 2 * SN) dma_w(d, t + 2, ls + cur);
-          else if (d < 2 * (SN + SM)) dma_x(d - 2 * SN, t + 2, ls + cur);
-        }
+        for (int d = k * kDma; d < (k + 1) * kDma; ++d) dma(d, t + 2, ls + cur);
       }
       __builtin_amdgcn_sched_barrier(0);
     }
-    if constexpr (NEXT) {
-      if ((t & 3) == 3) {
-        take_scales();
-      } else {
-        sw >>= 8;
-#pragma unroll
-        for (int j = 0; j < SM; ++j) sx[j] >>= 8;
-      }
-    }
+    if constexpr (NEXT) sc.step(t);
   };
-  using yes = std::integral_constant<bool, true>;
-  using no = std::integral_constant<bool, false>;
   int t = 0;
   for (; t + 2 < kb_n; ++t) step(t, yes{}, yes{});
   if (t + 1 < kb_n) step(t++, yes{}, no{});
   step(t, no{}, no{});
 
-  // rows of y through LDS, 32 at a time, the wave's own: whole pieces of 64 SN columns
   __builtin_amdgcn_s_waitcnt(kLgkmWait0);
   lds_barrier();
-  uint8_t* ys = smem + wid * 32 * kPitch;
-  bf16* y = sg.y[seg];
-  const int nw = n0 + wn * 32 * SN;
-  const bool whole = (N & 7) == 0 && (reinterpret_cast<uintptr_t>(y) & 15) == 0;
+  Out::store(acc, smem + wid * Out::kBytes, bias_lds + wn * 32 * SN, sg.y[tile.seg], nw, mw, N, M);
+}
+
+// keeps a product where it is written, between the reads and DMA around it
+__device__ __forceinline__ void pin(v16f& c) { asm volatile("" : "+a"(c)::"memory"); }
+
+// The same for fewer rows and columns than fill the card with such tiles.  A step is half a block, in a ring of R stages, R - 1 on their way
+// while one is multiplied: a tile alone on its CU waits for nothing but memory's first
+// answer if the ring is deep, several on a CU cover each other and leave room for fewer stages.
+// x lies in rows of 64 bytes, piece p of row r at p ^ (r / 4 & 3).  The scales' words
+// come with each stage (a load into a register would make the compiler wait for all DMA
+// before its use).
+template <int SN, int SM, int R, int OCC>
+__global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __restrict__ x,
+                                                            const uint8_t* __restrict__ xs, const Fp8Segs sg, int M,
+                                                            int kb_n, int mtiles) {
+  constexpr int BN = 64 * SN, BM = 64 * SM, kW = BN * 64, kOps = (BN + BM) * 64, kStage = kOps + 1024;
+  constexpr int kParts = (BN + BM) / 16, kDmas = (kParts + 3) / 4 + 1;   // DMA instructions of operands, and all of a wave
+  static_assert(BM <= 128 && BN <= 256, "a stage's scales: two waves' rows, one's columns");
+  static_assert((R - 1) * kDmas < 63, "vmcnt counts them");
+  using Out = Fp8Out<SN, SM>;
+  static_assert(4 * Out::kBytes <= R * kStage, "y fits the stages");
+  __shared__ __align__(16) uint8_t smem[R * kStage + 4 * BN];
+  float* bias_lds = reinterpret_cast<float*>(smem + R * kStage);
+  const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
+  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid & 1, wm = wid >> 1;
+  const Fp8Tile tile = tile_of<BN, BM>(sg, mtiles);
+  const int N = sg.N[tile.seg], n0 = tile.n0, m0 = tile.m0, nw = n0 + wn * 32 * SN, mw = m0 + wm * 32 * SM;
+  const bf16* bias = sg.bias[tile.seg];
+  if (tid < BN) bias_lds[tid] = bias && n0 + tid < N ? to_f32(bias[n0 + tid]) : 0.0f;
+
+  // part q of a stage: half a tile of W, or sixteen rows of x; wave w takes w, w + 4, ..
+  // (a part too many is the last again, at the same place)
+  const uint32_t ls = lds_addr(smem);
+  const uint8_t* d_w = sg.W[tile.seg] + static_cast<long>(n0 >> 4) * kb_n * 2048;
+  const uint8_t* d_x = x + static_cast<long>(m0) * kb_n * 128;
+  uint32_t off[kDmas];
 #pragma unroll
-  for (int j = 0; j < SM; ++j) {
-    // lane (c, h) holds columns 8 q + 4 h + e of square i for row c
+  for (int i = 0; i < kDmas - 1; ++i) {
+    const int q = min(wid + 4 * i, kParts - 1);
+    off[i] = q < BN / 16 ? static_cast<uint32_t>(min(q, ((N + 15) >> 4) - 1 - (n0 >> 4))) * kb_n * 2048 + lane * 16
+                         : static_cast<uint32_t>(min((q - BN / 16) * 16 + (lane >> 2), M - 1 - m0)) * kb_n * 128 +
+                               ((lane & 3) ^ (lane >> 4)) * 16;
+  }
+  // words of scales: waves 0 and 1 of 64 rows each, 2 and 3 of the groups of 32 columns
+  const int words = (kb_n + 3) >> 2;
+  const uint8_t* d_s;
+  if (wid < 2) {
+    d_s = xs + static_cast<long>(m0) * 4 * words;
+    off[kDmas - 1] = static_cast<uint32_t>(min(64 * wid + lane, M - 1 - m0)) * 4 * words;
+  } else {
+    d_s = sg.scale[tile.seg] + static_cast<long>(n0 >> 7) * 4 * words;
+    off[kDmas - 1] = static_cast<uint32_t>((min(n0 + 32 * min(lane, BN / 32 - 1), N - 1) >> 7) - (n0 >> 7)) * 4 * words;
+  }
+  int d_u = 0;
+  auto dma = [&](int i, uint32_t stage) __attribute__((always_inline)) {
+    const int q = min(wid + 4 * i, kParts - 1);
+    if (i < kDmas - 1) dma_lds16(q < BN / 16 ? d_w : d_x, off[i], stage + (q << 10));
+    else if (i == kDmas - 1) dma_lds4(d_s, off[i], stage + kOps + (wid << 8));
+  };
+  auto advance = [&]() __attribute__((always_inline)) {
+    d_w += 1024;
+    d_x += 64;
+    d_s += (d_u & 7) == 7 ? 4 : 0;
+    ++d_u;
+  };
+
+  const int wa = wn * SN * 2048 + (c >> 4) * 1024 + h * 512 + (c & 15) * 16;
+  int xa[2];
 #pragma unroll
-    for (int i = 0; i < SN; ++i)
+  for (int i = 0; i < 2; ++i) xa[i] = kW + wm * SM * 2048 + c * 64 + (((2 * h + i) ^ ((c >> 2) & 3)) * 16);
+  const int sxa = kOps + (wm * SM * 32 + c) * 4, swa = kOps + 512 + wn * SN * 4;
+  v8i fw[2][SN], fx[2][SM];
+  uint32_t sw[2], sx[2][SM];
+  auto read_frag = [&](int half, int r, int stage) __attribute__((always_inline)) {
+    if (r == 0) {
+      sw[half] = *reinterpret_cast<const uint32_t*>(smem + stage + swa);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 b = *reinterpret_cast<const float4*>(bias_lds + wn * 32 * SN + 32 * i + 8 * q + 4 * h);
-        *reinterpret_cast<uint2*>(ys + c * kPitch + (32 * i + 8 * q + 4 * h) * 2) =
-            uint2{pack_bf16x2(acc[i][j][4 * q] + b.x, acc[i][j][4 * q + 1] + b.y),
-                  pack_bf16x2(acc[i][j][4 * q + 2] + b.z, acc[i][j][4 * q + 3] + b.w)};
-      }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    const int mw = m0 + (wm * SM + j) * 32;
-    if (whole) {
-      constexpr int kLanes = 4 * SN;
+      for (int j = 0; j < SM; ++j) sx[half][j] = *reinterpret_cast<const uint32_t*>(smem + stage + sxa + 128 * j);
+    }
+    if (r == 0 || (r > SM && r < SN + SM)) {
+      const int s = r == 0 ? 0 : r - SM;
+      const uint8_t* p = smem + stage + wa + s * 2048;
+      fw[half][s] = lds_frag(p, p + 256);
+    } else if (r <= SM) {
+      const uint8_t* p = smem + stage + (r - 1) * 2048;
+      fx[half][r - 1] = lds_frag(p + xa[0], p + xa[1]);
+    }
+  };
+  // all but the newest n stages of DMA have landed, and the wave's reads
+  auto landed = [&](int n) __attribute__((always_inline)) {
+    switch (n) {
+#define SA_FP8_WAIT(k) \
+  case k: \
+    if constexpr (k < R - 1) __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<(k < R - 1 ? k : 0) * kDmas>()); \
+    break;
+      SA_FP8_WAIT(1) SA_FP8_WAIT(2) SA_FP8_WAIT(3) SA_FP8_WAIT(4) SA_FP8_WAIT(5) SA_FP8_WAIT(6) SA_FP8_WAIT(7)
+      SA_FP8_WAIT(8) SA_FP8_WAIT(9) SA_FP8_WAIT(10)
+#undef SA_FP8_WAIT
+      default: __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<0>());
+    }
+  };
+  static_assert(R >= 3 && R <= 12, "landed counts to R - 2");
+
+  const int U = 2 * kb_n, filled = min(U, R);
+  v16f acc[SN][SM] = {};
+  for (int s = 0; s < filled; ++s) {
 #pragma unroll
-      for (int r = 0; r < 32; r += 64 / kLanes) {
-        const int row = r + lane / kLanes, n = nw + 8 * (lane % kLanes);
-        const uint4 v = *reinterpret_cast<const uint4*>(ys + row * kPitch + 16 * (lane % kLanes));
-        if (mw + row < M && n < N) *reinterpret_cast<uint4*>(y + static_cast<long>(mw + row) * N + n) = v;
-      }
-    } else {
-      for (int e = lane; e < 32 * 32 * SN; e += 64) {
-        const int row = e / (32 * SN), k = e % (32 * SN);
-        if (mw + row < M && nw + k < N)
-          y[static_cast<long>(mw + row) * N + nw + k] = *reinterpret_cast<const bf16*>(ys + row * kPitch + 2 * k);
+    for (int i = 0; i < kDmas; ++i) dma(i, ls + s * kStage);
+    advance();
+  }
+  landed(filled - 2);   // (at least two)
+  lds_barrier();
+#pragma unroll
+  for (int r = 0; r < SN + SM; ++r) read_frag(0, r, 0);
+  __builtin_amdgcn_s_waitcnt(kLgkmWait0);
+  lds_barrier();
+
+  // half-step u on stage cur, whose operands are in registers and which all have read:
+  // those of u + 1 are read, stage cur takes half-step u + R
+  int cur = 0, u = 0;
+  auto half_step = [&](auto half, auto more) __attribute__((always_inline)) {
+    constexpr int HF = decltype(half)::value;
+    constexpr bool MORE = decltype(more)::value;
+    const int shift = (u >> 1 & 3) * 8;   // the block's byte
+    const int oth = cur == (R - 1) * kStage ? 0 : cur + kStage;
+    constexpr int kSlots = SN * SM, kReads = (SN + SM + kSlots - 1) / kSlots, kPer = (kDmas + kSlots - 1) / kSlots;
+#pragma unroll
+    for (int k = 0; k < kSlots; ++k) {
+      const int i = k / SM, j = k % SM;
+      acc[i][j] = mfma_fp8(fw[HF][i], fx[HF][j], acc[i][j], sw[HF] >> shift, sx[HF][j] >> shift);
+      pin(acc[i][j]);
+#pragma unroll
+      for (int r = k * kReads; r < (k + 1) * kReads; ++r) read_frag(HF ^ 1, r, oth);   // (of the last: not used)
+      if constexpr (MORE) {
+#pragma unroll
+        for (int d = k * kPer; d < (k + 1) * kPer; ++d) dma(d, ls + cur);
       }
     }
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
+    if constexpr (MORE) {
+      advance();
+      __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<(R - 2) * kDmas>());
+    } else {
+      landed(U - 3 - u);
+    }
+    lds_barrier();
+    cur = oth;
+    ++u;
+  };
+  using h0 = std::integral_constant<int, 0>;
+  using h1 = std::integral_constant<int, 1>;
+  while (u + 1 + R < U) {
+    half_step(h0{}, yes{});
+    half_step(h1{}, yes{});
   }
+  if (R % 2 == 1 && u + R < U) {
+    half_step(h0{}, yes{});
+    half_step(h1{}, no{});
+  }
+  while (u < U) {
+    half_step(h0{}, no{});
+    half_step(h1{}, no{});
+  }
+  Out::store(acc, smem + wid * Out::kBytes, bias_lds + wn * 32 * SN, sg.y[tile.seg], nw, mw, N, M);
 }
 
 // the weights in bf16, (N, K) row-major; a code times its scale is a bf16 number
@@ -368,23 +561,93 @@ __global__ __launch_bounds__(128) void fp8_dequant_kernel(const uint8_t* __restr
   }
 }
 
+// tiles of BN columns, all matrices after each other
+void cut_tiles(Fp8Segs& sg, int BN) {
+  sg.blk0[0] = 0;
+  for (int i = 0; i < kFp8Segs; ++i) sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? (sg.N[i] + BN - 1) / BN : 0);
+}
 template <int CT, int R, int NW>
 void fp8_few(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
-  sg.blk0[0] = 0;
-  for (int i = 0; i < kFp8Segs; ++i)
-    sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? ((sg.N[i] + 15) / 16 + R - 1) / R : 0);
+  cut_tiles(sg, 16 * R);
+  ProfScope prof_("fp8_few", s);
   hipLaunchKernelGGL((fp8_few_kernel<CT, R, NW>), dim3(sg.blk0[kFp8Segs] * ((M + 16 * CT - 1) / (16 * CT))),
                      dim3(64 * NW), 0, s, static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb);
 }
 
 template <int SN, int SM>
-void fp8_tile(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
-  sg.blk0[0] = 0;
-  for (int i = 0; i < kFp8Segs; ++i)
-    sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? (sg.N[i] + 64 * SN - 1) / (64 * SN) : 0);
+void fp8_large(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
+  cut_tiles(sg, 64 * SN);
   const int mtiles = (M + 64 * SM - 1) / (64 * SM);
-  hipLaunchKernelGGL((fp8_tile_kernel<SN, SM>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256), 0, s,
+  ProfScope prof_("fp8_large", s);
+  hipLaunchKernelGGL((fp8_large_kernel<SN, SM>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
+}
+template <int SN, int SM, int R, int OCC>
+void fp8_ring(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
+  cut_tiles(sg, 64 * SN);
+  const int mtiles = (M + 64 * SM - 1) / (64 * SM);
+  ProfScope prof_("fp8_ring", s);
+  hipLaunchKernelGGL((fp8_ring_kernel<SN, SM, R, OCC>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256), 0, s,
+                     static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
+}
+
+// The kernel by the sizes.  Up to 64 rows and 12288 columns the waves share K
+// (fp8_few): 16 rows 1024 -> 4384 4.1 us (tiles of 64 by 64: 5.6), 32 rows 4096 -> 4096 7.6
+// (11.5), 64 rows 11008 -> 4096 18.6 (26.8); two tiles a workgroup, which read x once, from
+// 17 rows on, and for wide matrices also below (16 rows, 4096 -> 32000: 32.6, so 24.9).
+// Wider ones, from 17 rows on, go in tiles (32 rows, 4096 -> 32000: 41, tiles 25.5), as do
+// more rows, by the least estimate in us of
+//   tiles <= 256      first(kb), that of one tile on each CU
+//   more              again + (tiles / 256, between itself and its ceiling) each(kb)
+// fitted to 27 products of 65 to 32768 rows, K 1024 to 8192, N 1024 to 32000: the choice
+// was never more than 9 % behind the best.
+struct Fp8Shape {
+  int bn, bm;
+  float first0, first1, again, each0, each1;
+};
+constexpr Fp8Shape kFp8Shapes[] = {
+    {256, 256, 8.0f, 1.06f, 8.0f, 5.0f, 1.48f},   // fp8_large: a full card is bound by power, from one tile a CU on
+    {256, 128, 4.0f, 0.93f, 5.3f, 1.3f, 0.87f},
+    {128, 128, 3.0f, 0.60f, 2.9f, 0.5f, 0.58f},
+    {128, 64, 3.0f, 0.40f, 4.0f, -0.2f, 0.39f},
+    {64, 64, 3.0f, 0.30f, 4.0f, -0.2f, 0.255f},
+};
+int fp8_shape(const Fp8Segs& sg, int M, int kb, float* per_cu) {
+  int best = 0;
+  float least = 0.0f;
+  for (int i = 0; i < 5; ++i) {
+    const Fp8Shape& p = kFp8Shapes[i];
+    long tiles = 0;
+    for (int k = 0; k < sg.nseg; ++k) tiles += (sg.N[k] + p.bn - 1) / p.bn;
+    tiles *= (M + p.bm - 1) / p.bm;
+    const float r = static_cast<float>(tiles) / 256.0f, each = p.each0 + p.each1 * static_cast<float>(kb);
+    float us = p.first0 + p.first1 * static_cast<float>(kb);
+    if (r > 1.0f) us = p.again + 0.5f * (r + static_cast<float>((tiles + 255) / 256)) * each;
+    else if (i == 0) us = std::max(us, r * (each + 2.0f));
+    if (i == 0 || us < least) {
+      least = us;
+      best = i;
+      *per_cu = r;
+    }
+  }
+  return best;
+}
+
+void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
+  long N = 0;
+  for (int i = 0; i < sg.nseg; ++i) N += sg.N[i];
+  if (M <= 16) return N <= 12288 ? fp8_few<1, 1, 8>(x, xs, sg, M, kb, s) : fp8_few<1, 2, 8>(x, xs, sg, M, kb, s);
+  if (M <= 64 && N <= 12288)
+    return M <= 32 ? fp8_few<1, 2, 8>(x, xs, sg, M, kb, s) : fp8_few<2, 2, 8>(x, xs, sg, M, kb, s);
+  // few tiles a CU get deep rings, more of them room beside each other
+  float per_cu = 0.0f;
+  switch (fp8_shape(sg, M, kb, &per_cu)) {
+    case 0: return fp8_large<4, 4>(x, xs, sg, M, kb, s);
+    case 1: return fp8_ring<4, 2, 3, 2>(x, xs, sg, M, kb, s);
+    case 2: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
+    case 3: return per_cu <= 2.0f ? fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 1, 3, 4>(x, xs, sg, M, kb, s);
+    default: return per_cu <= 2.0f ? fp8_ring<1, 1, 8, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
+  }
 }
 
 }  // namespace
@@ -408,29 +671,18 @@ extern "C" int sa_fp8_linear(const void* codes, const void* scales, int64_t M, i
                  who, i, static_cast<long>(m[4]));
     SA_CHECK_ARG((m[0] & 15) == 0 && (m[1] & 3) == 0 && ((m[2] | m[3]) & 1) == 0, "%s: weight matrix %d is not aligned",
                  who, i);
-    tiles += (m[4] + 15) / 16;
+    tiles += (m[4] + 63) / 64;
     sg.W[i] = reinterpret_cast<const uint8_t*>(m[0]);
     sg.scale[i] = reinterpret_cast<const uint8_t*>(m[1]);
     sg.bias[i] = reinterpret_cast<const sa::bf16*>(m[2]);
     sg.y[i] = reinterpret_cast<sa::bf16*>(m[3]);
     sg.N[i] = static_cast<int>(m[4]);
   }
-  SA_CHECK_ARG(tiles * ((M + 63) / 64) < (1L << 23), "%s: %ld rows and %ld columns are too many", who,
-               static_cast<long>(M), 16 * tiles);   // (2^32 threads a grid)
+  SA_CHECK_ARG(tiles * ((M + 63) / 64) < (1L << 24), "%s: %ld rows and %ld columns are too many", who,
+               static_cast<long>(M), 64 * tiles);   // (2^32 threads a grid)
   hipStream_t s = static_cast<hipStream_t>(stream);
-  sa::ProfScope prof_("fp8_linear", s);
   const int kb = (K + 127) / 128, m = static_cast<int>(M);
-  if (m <= 16) sa::fp8_few<1, 1, 8>(codes, scales, sg, m, kb, s);
-  else if (m <= 32) sa::fp8_few<2, 1, 8>(codes, scales, sg, m, kb, s);
-  else if (m <= 64) sa::fp8_few<4, 2, 8>(codes, scales, sg, m, kb, s);
-  else {
-    long big = 0;   // tiles of 256 by 256
-    for (int i = 0; i < nseg; ++i) big += (sg.N[i] + 255) / 256;
-    big *= (m + 255) / 256;
-    if (big >= 200) sa::fp8_tile<4, 4>(codes, scales, sg, m, kb, s);
-    else if (big >= 60) sa::fp8_tile<2, 2>(codes, scales, sg, m, kb, s);
-    else sa::fp8_tile<1, 1>(codes, scales, sg, m, kb, s);
-  }
+  sa::fp8_go(codes, scales, sg, m, kb, s);
   SA_CHECK_LAUNCH(who);
   return 0;
 }

@@ -425,6 +425,61 @@ def test_linear_of_whole_numbers(M, K, N):
     assert torch.equal(y.cpu().double(), want.to(torch.bfloat16).double())
 
 
+# (M, K, [N_i]), the kernel: few rows, tiles of each shape, odd borders, long K, many rows
+TILES = [(16, 1024, [20000], "few"), (32, 11008, [500], "few"), (64, 700, [12287], "few"), (17, 256, [12289], "ring"),
+         (64, 4096, [32000], "ring"), (66, 33000, [70], "ring"), (257, 16384, [300], "ring"), (500, 2050, [4383], "ring"),
+         (1111, 1030, [4383], "ring"), (2001, 1024, [4384], "ring"), (2047, 4096, [4096], "ring"), (2047, 4096, [4100], "large"),
+         (700, 4200, [1111], "ring"), (70000, 128, [64], "ring"), (8100, 1024, [4384], "ring"),
+         (4100, 1408, [4097], "ring"), (8192, 2100, [4104], "ring"), (4095, 4096, [4095], "large"),
+         (300, 640, [128, 1, 1000, 333], "ring"), (4096, 2048, [1111, 2000, 77, 900], "ring"), (2040, 6000, [2000, 1027, 77, 900], "large"),
+         (3000, 1, [5000], "ring"), (5000, 130, [5001], "ring")]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M,K,sizes,kernel", TILES)
+def test_linear_tiles(M, K, sizes, kernel):
+    """Whole numbers as above, against float64 on the GPU; every kernel and its borders."""
+    from selective_attention.profiling import kernel_timer
+    g = torch.Generator(device="cuda").manual_seed(M + K)
+    draw = lambda lo, hi, *s: torch.randint(lo, hi, s, generator=g, device="cuda")  # noqa: E731
+    kb, K8 = (K + 127) // 128, -K % 128
+    x = draw(-3, 4, M, K).float()
+    xs = draw(127, 129, M, (kb + 3) // 4 * 4).to(torch.uint8)
+    rows = Fp8Rows(torch.nn.functional.pad(x, (0, K8)).to(E4), xs.view(E8), K)
+    xv = x.double() * torch.exp2(xs.double() - 127)[:, torch.arange(K, device="cuda") // 128]
+    ws, bs, want = [], [], []
+    for N in sizes:
+        w, s = draw(-3, 4, N, K).float(), draw(126, 129, (N + 127) // 128, kb).to(torch.uint8)
+        ws.append(pack_fp8(w.to(E4), s))
+        bs.append(draw(-8, 9, N).to(torch.bfloat16) if N % 2 else None)
+        at = torch.arange(N, device="cuda")[:, None] // 128, torch.arange(K, device="cuda")[None] // 128
+        y = torch.matmul(xv, (w.double() * torch.exp2(s.double() - 127)[at]).t().contiguous())
+        want.append(y if bs[-1] is None else y + bs[-1].double())
+    with kernel_timer() as kt:
+        ys = fp8_linear_multi(rows, ws, bs, sizes)
+    assert list(kt.stats) == ["fp8_" + kernel]
+    for y, v in zip(ys, want):
+        assert torch.equal(y, v.to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+def test_linear_results_next_to_others():
+    """Outputs stop at their matrix's last row and column."""
+    for M, K, N in ((5, 256, 33), (70, 256, 65), (300, 384, 129), (4100, 1408, 4097), (4095, 4096, 4095)):
+        packed, scales = (t.cuda() for t in weight(N, K))
+        x = make_rows(M, K) if M < 1000 else Fp8Rows(torch.ones(M, K).to(E4), torch.full((M, (K + 511) // 512 * 4), 127, dtype=torch.uint8).view(E8))
+        x = on(x)
+        pool = torch.full((M * N + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
+        from selective_attention.kernels.fp8 import linear_multi
+        want = linear_multi(x.codes, x.scales, (M,), K, [(packed, scales)], [None], [N])[0]
+        import ctypes
+        from selective_attention import _lib
+        words = (ctypes.c_int64 * 5)(packed.data_ptr(), scales.data_ptr(), 0, pool.data_ptr() + 2 * 1025, N)
+        _lib.call("sa_fp8_linear", x.codes.data_ptr(), x.scales.data_ptr(), M, K, 1, words, _lib.stream_of(pool))
+        assert torch.equal(pool[1025:1025 + M * N].view(M, N), want)     # (rows off every boundary)
+        assert (pool[:1025] == 7).all() and (pool[1025 + M * N:] == 7).all()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 40, 300])
 def test_linear_cuts_within_eight_columns_alone(M):
