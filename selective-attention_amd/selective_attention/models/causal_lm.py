@@ -19,7 +19,7 @@ import torch
 import torch.nn as nn
 
 from ..inference import CausalBlockCache, GenerationConfig, InferenceState
-from ..modules.layers import Int4Linear, Linear, quantize_linears
+from ..modules.layers import Fp8Linear, Int4Linear, Linear, quantize_linears, quantize_linears_fp8
 from ..modules import CausalBlock, RMSNorm
 from ..ops.logprobs import TokenLogprobs, token_logprobs
 from ._graph import graph_decode
@@ -86,6 +86,15 @@ class CausalLM(nn.Module):
             self.lm_head = Int4Linear.from_linear(self.lm_head, group_size, symmetric)
         return self
 
+    def quantize_fp8(self) -> "CausalLM":
+        """Every linear layer and the head to 8 bits (Fp8Linear), in place, for inference in
+        bfloat16: the norms and SwiGLU's product then leave in 8 bits too, and the
+        products run at twice bfloat16's rate.  The embedding keeps its own table."""
+        quantize_linears_fp8(self.layers)
+        if isinstance(self.lm_head, nn.Linear):
+            self.lm_head = Fp8Linear.from_linear(self.lm_head)
+        return self
+
     def _hidden(self, input_ids, lengths=None, attn_gate_thresholds=None, cache=None):
         h = self.embedding(input_ids)
         for i, layer in enumerate(self.layers):
@@ -98,7 +107,8 @@ class CausalLM(nn.Module):
                 attn_gate_thresholds: torch.Tensor | List | None = None,
                 cache: list | None = None, analysis_cfg=None, stats=None):
         """input_ids (batch_size, seq_len) -> logits (batch_size, seq_len, vocab_size)."""
-        return self.lm_head(self.norm(self._hidden(input_ids, lengths, attn_gate_thresholds, cache)))
+        h = self._hidden(input_ids, lengths, attn_gate_thresholds, cache)
+        return self.lm_head(self.norm(h, self.lm_head))
 
     def score(self, input_ids: torch.Tensor, lengths: torch.Tensor | None = None,
               attn_gate_thresholds: torch.Tensor | List | None = None, top: int = 0) -> TokenLogprobs:
@@ -128,7 +138,7 @@ class CausalLM(nn.Module):
         pend = None
         for i, layer in enumerate(self.layers):
             h, pend = layer.step(h, cache[i], state, gen_cfg, pending=pend, defer_add=True)
-        return self.lm_head(self.norm.add_forward(h, pend)[1])
+        return self.lm_head(self.norm.add_forward(h, pend, self.lm_head)[1])
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, gen_cfg: GenerationConfig, analysis_cfg=None,
@@ -155,7 +165,7 @@ class CausalLM(nn.Module):
         state = InferenceState(lengths.clone())
         h = self._hidden(input_ids, lengths, gen_cfg.attn_gate_thresholds, cache)
         # logits of each row's last token only (the rows the reference keeps)
-        logits = self.lm_head(self.norm(h[torch.arange(b, device=dev), lengths - 1]))
+        logits = self.lm_head(self.norm(h[torch.arange(b, device=dev), lengths - 1], self.lm_head))
         seq_ids = torch.full((b, L + new), gen_cfg.pad_token_id, dtype=input_ids.dtype, device=dev)
         seq_ids[:, :L] = input_ids
         lps = None if logprobs is None else _LogprobLog(b, max(new, 0), logprobs, dev)

@@ -23,7 +23,7 @@ import torch.nn as nn
 
 from ..ops.attention import attn_varlen, paged_decode_attn
 from ..ops.selective_mha import ScoreStdFn, cross_attention_train
-from .layers import Linear
+from .layers import Linear, all_fp8, project
 from .selective_attention import _threshold
 
 
@@ -45,13 +45,23 @@ class CrossSelectiveMHA(nn.Module):
         self.register_buffer("score_std_ema", torch.zeros(self.num_heads))
         nn.init.constant_(self.select_gate_proj.bias, 2.0)
 
+    @property
+    def takes_rows(self) -> bool:
+        """Whether the input (not the context) may come in 8 bits (RMSNorm.forward)."""
+        return all_fp8(self.q_proj) and not self.training
+
     def _context(self, context, context_lengths, threshold, prefill):
         """Keys and values as (b * Lc, H, D) bf16 rows, the bias as (H, b * Lc)
         float32 and the key offsets (b + 1,) int32."""
         b, Lc, _ = context.shape
         dev = context.device
         H, D = self.num_heads, self.head_dim
-        gate = torch.sigmoid(self.select_gate_proj(context)).float().transpose(1, 2)   # (b, H, Lc)
+        layers = [self.select_gate_proj, self.k_proj, self.v_proj]
+        if all_fp8(*layers):     # one launch, the context rounded and read once
+            gate, k, v = project(context, layers)
+        else:
+            gate, k, v = self.select_gate_proj(context), None, None
+        gate = torch.sigmoid(gate).float().transpose(1, 2)   # (b, H, Lc)
         first = torch.arange(Lc, device=dev) == 0
         if prefill:
             gate = torch.where(first[None, None, :], torch.ones_like(gate), gate)
@@ -63,8 +73,10 @@ class CrossSelectiveMHA(nn.Module):
             kept &= (gate >= thr[None, :, None]) | first[None, None, :]
         lg = torch.log(gate) * self.score_std_ema.float()[None, :, None] * self.log_gate_penalty
         lg = torch.where(kept, lg, torch.full_like(lg, float("-inf")))
-        k = self.k_proj(context).to(torch.bfloat16).reshape(b * Lc, H, D)
-        v = self.v_proj(context).to(torch.bfloat16).reshape(b * Lc, H, D)
+        if k is None:
+            k, v = self.k_proj(context), self.v_proj(context)
+        k = k.to(torch.bfloat16).reshape(b * Lc, H, D)
+        v = v.to(torch.bfloat16).reshape(b * Lc, H, D)
         cu_k = torch.arange(b + 1, dtype=torch.int32, device=dev) * Lc
         return k, v, lg.transpose(0, 1).reshape(H, b * Lc).contiguous(), cu_k
 

@@ -9,9 +9,11 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from ..kernels.fp8 import MAX_NORM_DIM
 from ..kernels.int4 import MAX_MATRICES
 from ..kernels.lm_ops import (add_rms_norm, add_rms_norm_supported, gemv, gemv_multi,
                               gemv_supported, rms_norm, rope_qk, silu_mul)
+from ..ops.fp8 import (fp8_linear, fp8_linear_multi, quantize_fp8, rms_norm_fp8, silu_mul_fp8)
 from ..ops.int4 import int4_linear, int4_linear_multi, quantize_int4
 
 
@@ -105,22 +107,94 @@ class Int4Linear(nn.Module):
                 f"bias={self.bias is not None}, group_size={self.group_size}, symmetric={self.symmetric}")
 
 
-def quantize_linears(module: nn.Module, group_size: int = 128, symmetric: bool = True) -> nn.Module:
-    """Replace every linear layer inside `module` by its Int4Linear, in place."""
+class Fp8Linear(nn.Module):
+    """A linear layer whose weight is kept in 8 bits with a scale for each 128 by 128
+    (ops/fp8.py), for inference: bfloat16 rows, which it rounds to 8 bits, or
+    Fp8Rows that the op before it made; no weight gradient.  Buffers: packed, scales
+    (e8m0 bytes), bias in bfloat16 whatever the module is cast to."""
+
+    takes_rows = True
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, device=None):
+        super().__init__()
+        self.in_features, self.out_features = in_features, out_features
+        nt, kb = (out_features + 15) // 16, (in_features + 127) // 128
+        self.register_buffer("packed", torch.zeros(nt, kb, 8, 16, 16, dtype=torch.uint8, device=device))
+        self.register_buffer("scales", torch.full(((out_features + 127) // 128, (kb + 3) // 4 * 4), 127,
+                                                  dtype=torch.uint8, device=device))
+        self.register_buffer("bias", torch.zeros(out_features, dtype=torch.bfloat16, device=device) if bias else None)
+
+    @classmethod
+    def from_linear(cls, lin: nn.Linear) -> "Fp8Linear":
+        """lin's weight rounded to its nearest codes (quantize_fp8)."""
+        q = cls(lin.in_features, lin.out_features, lin.bias is not None, lin.weight.device)
+        q.packed, scales = quantize_fp8(lin.weight)
+        q.scales = scales.view(torch.uint8)
+        if lin.bias is not None:
+            q.bias = lin.bias.detach().to(torch.bfloat16)
+        return q
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = self.bias
+        super()._apply(fn, *args, **kwargs)
+        if kept is not None and self.bias.dtype != torch.bfloat16:   # moved, not cast
+            self.bias = kept.to(self.bias.device)
+        return self
+
+    def weights(self):
+        return self.packed, self.scales
+
+    def forward(self, x) -> torch.Tensor:
+        return fp8_linear(x, self.packed, self.scales, self.bias, self.out_features)
+
+    def split_forward(self, x, sizes) -> list:
+        """torch.split(self(x), sizes, dim=-1), each piece a contiguous tensor; one
+        launch of several matrices where the pieces are whole blocks of 128."""
+        if len(sizes) <= MAX_MATRICES and min(sizes) > 0 and all(n % 128 == 0 for n in sizes[:-1]):
+            w = zip(torch.split(self.packed, [(n + 15) // 16 for n in sizes]),
+                    torch.split(self.scales, [(n + 127) // 128 for n in sizes]))
+            bs = [None] * len(sizes) if self.bias is None else torch.split(self.bias, sizes)
+            return fp8_linear_multi(x, list(w), bs, sizes)
+        return [p.contiguous() for p in torch.split(self(x), sizes, dim=-1)]
+
+    def extra_repr(self) -> str:
+        return f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}"
+
+
+def _replace_linears(module: nn.Module, make) -> nn.Module:
     for name, child in module.named_children():
         if isinstance(child, nn.Linear):
-            setattr(module, name, Int4Linear.from_linear(child, group_size, symmetric))
+            setattr(module, name, make(child))
         else:
-            quantize_linears(child, group_size, symmetric)
+            _replace_linears(child, make)
     return module
+
+
+def quantize_linears(module: nn.Module, group_size: int = 128, symmetric: bool = True) -> nn.Module:
+    """Replace every linear layer inside `module` by its Int4Linear, in place."""
+    return _replace_linears(module, lambda lin: Int4Linear.from_linear(lin, group_size, symmetric))
+
+
+def quantize_linears_fp8(module: nn.Module) -> nn.Module:
+    """Replace every linear layer inside `module` by its Fp8Linear, in place."""
+    return _replace_linears(module, Fp8Linear.from_linear)
+
+
+def all_fp8(*linears) -> bool:
+    return all(isinstance(lin, Fp8Linear) for lin in linears)
 
 
 def project(x: torch.Tensor, linears, xscale: torch.Tensor | None = None) -> list:
     """[lin(x * xscale if xscale is given else x) for lin in linears]: one
     multi-GEMV launch on the decode shape (at most 4 layers), where the
     product x * xscale is taken in bf16 as torch does; 4-bit layers of one kind
-    likewise."""
-    if all(isinstance(lin, Int4Linear) for lin in linears):
+    likewise; 8-bit layers for any rows (also Fp8Rows, without xscale), with the
+    product rounded to 8 bits alone."""
+    if all_fp8(*linears):
+        if len(linears) <= MAX_MATRICES:
+            return fp8_linear_multi(x, [lin.weights() for lin in linears], [lin.bias for lin in linears],
+                                    [lin.out_features for lin in linears], xscale)
+    elif all(isinstance(lin, Int4Linear) for lin in linears):
         if len(linears) <= MAX_MATRICES and len({(lin.group_size, lin.symmetric) for lin in linears}) == 1:
             return int4_linear_multi(x, [lin.weights() for lin in linears],
                                      [lin.bias for lin in linears],
@@ -145,7 +219,19 @@ class RMSNorm(nn.Module):
             shape = (dim,) if num_groups is None else (num_groups, dim)
             self.weight = nn.Parameter(torch.zeros(shape))
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    def _rows_for(self, layer, x: torch.Tensor, y: torch.Tensor | None = None) -> bool:
+        """Whether `layer` takes the norm of x (+ y) in 8 bits, and the kernel may give it."""
+        return (layer is not None and getattr(layer, "takes_rows", False) and self.elementwise_affine
+                and self.weight.dim() == 1 and x.is_cuda and x.dtype == torch.bfloat16
+                and x.shape[-1] <= MAX_NORM_DIM
+                and not (torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad
+                                                      or (y is not None and y.requires_grad))))
+
+    def forward(self, x: torch.Tensor, layer: nn.Module | None = None):
+        """The norm of x; in 8 bits (Fp8Rows) where the layer behind it, when it is
+        named, takes such rows in inference."""
+        if self._rows_for(layer, x):
+            return rms_norm_fp8(x, self.weight, self.eps)
         if (self.elementwise_affine and x.is_cuda and x.is_contiguous()
                 and x.dtype in (torch.float32, torch.bfloat16)
                 and not (torch.is_grad_enabled() and (x.requires_grad or self.weight.requires_grad))):
@@ -156,15 +242,18 @@ class RMSNorm(nn.Module):
             out = out * (1.0 + self.weight.float())
         return out.type_as(x)
 
-    def add_forward(self, x: torch.Tensor, y: torch.Tensor):
-        """(x + y, self(x + y)): a pre-norm block's residual add and its next
-        norm, in one kernel in inference for bf16 rows of 512k <= 4096 elements."""
+    def add_forward(self, x: torch.Tensor, y: torch.Tensor, layer: nn.Module | None = None):
+        """(x + y, self(x + y, layer)): a pre-norm block's residual add and its next
+        norm, in one kernel in inference for bf16 rows of 512k <= 4096 elements, and
+        for those that leave in 8 bits."""
+        if y.dtype == x.dtype and y.shape == x.shape and self._rows_for(layer, x, y):
+            return rms_norm_fp8(x, self.weight, self.eps, residual=y)
         if (self.elementwise_affine and add_rms_norm_supported(x, self.weight)
                 and not (torch.is_grad_enabled()
                          and (x.requires_grad or y.requires_grad or self.weight.requires_grad))):
             return add_rms_norm(x, y, self.weight, self.eps)
         s = x + y
-        return s, self(s)
+        return s, self(s, layer)
 
 
 def _rotate_half(x: torch.Tensor) -> torch.Tensor:
@@ -229,8 +318,15 @@ class SwiGLU(nn.Module):
         self.w2 = Linear(dim, hidden_dim)
         self.out = Linear(hidden_dim, dim)
 
-    def forward(self, x: torch.Tensor) -> torch.Tensor:
+    @property
+    def takes_rows(self) -> bool:
+        return all_fp8(self.w1, self.w2)
+
+    def forward(self, x) -> torch.Tensor:
         a, c = project(x, [self.w1, self.w2])
+        if (isinstance(self.out, Fp8Linear) and a.is_cuda and a.dtype == c.dtype == torch.bfloat16
+                and not (torch.is_grad_enabled() and (a.requires_grad or c.requires_grad))):
+            return self.out(silu_mul_fp8(a, c))      # one kernel, rows in 8 bits
         if (a.is_cuda and a.dtype == torch.bfloat16 and c.dtype == torch.bfloat16
                 and a.numel() % 8 == 0
                 and not (torch.is_grad_enabled() and (a.requires_grad or c.requires_grad))):

@@ -29,7 +29,7 @@ import torch.nn as nn
 from ..kernels.lm_ops import mha_gates, mha_prompt_gates
 from ..ops.attention import attn_varlen
 from ..ops.selective_mha import ScoreStdFn, gated_attention_train, selective_mha_prefill
-from .layers import Linear, RoPE, project
+from .layers import Linear, RoPE, all_fp8, project
 
 
 def _threshold(thr, num_heads: int, device):
@@ -93,6 +93,16 @@ class SelectiveMHA(nn.Module):
         self.register_buffer("score_std_ema", torch.zeros(self.num_heads))
         nn.init.constant_(self.gate_proj.bias, 2.0)
 
+    @property
+    def takes_rows(self) -> bool:
+        """Whether the input may come in 8 bits (RMSNorm.forward)."""
+        return all_fp8(self.gate_proj, self.q_proj, self.k_proj, self.v_proj) and not self.training
+
+    def _gated_out(self, out, out_gate):
+        if all_fp8(self.out_proj):   # the product is rounded to 8 bits alone
+            return project(out, [self.out_proj], xscale=out_gate)[0]
+        return self.out_proj(out * out_gate)
+
     def _gates(self, hidden_states):
         gate = torch.sigmoid(self.gate_proj(hidden_states))
         return torch.split(gate, [self.num_heads, self.dim], dim=-1)
@@ -123,7 +133,10 @@ class SelectiveMHA(nn.Module):
         dev = hidden_states.device
         H, D = self.num_heads, self.head_dim
         thr = _threshold(attn_gate_threshold, H, dev)
-        g = self.gate_proj(hidden_states)
+        if self.takes_rows:      # one launch, the input read once
+            g, q, k, v = project(hidden_states, [self.gate_proj, self.q_proj, self.k_proj, self.v_proj])
+        else:
+            g, q, k, v = self.gate_proj(hidden_states), None, None, None
         if _one_kernel_gates(g, thr, lengths):
             # sigmoid, split, threshold, lengths and log-gate in one kernel
             log_gate, out_gate, kept = mha_prompt_gates(
@@ -140,28 +153,30 @@ class SelectiveMHA(nn.Module):
                 kept &= (torch.arange(L, device=dev)[None, :] < lens[:, None])[:, None, :]
             log_gate = self._log_gate(select_gate, kept)
             kept = kept.any()
-        v = self.v_proj(hidden_states)
+        if v is None:
+            v = self.v_proj(hidden_states)
         any_kept = _later_bool(kept)
         # with every key dropped each query attends only itself (:208-209): told
         # after the launches where these cannot refuse, before them elsewhere
         if not (kept.is_cuda and D in (64, 128) and b * L > 0) and not any_kept():
-            return self.out_proj(v * out_gate)
-        q, k = self.rope.rotate_qk(self.q_proj(hidden_states).view(b, L, H, D),
-                                   self.k_proj(hidden_states).view(b, L, H, D), None, L)
+            return self._gated_out(v, out_gate)
+        if q is None:
+            q, k = self.q_proj(hidden_states), self.k_proj(hidden_states)
+        q, k = self.rope.rotate_qk(q.view(b, L, H, D), k.view(b, L, H, D), None, L)
         q, k = q.transpose(1, 2), k.transpose(1, 2)                   # (b, H, L, D) views
         vh = v.view(b, L, H, D).to(torch.bfloat16).transpose(1, 2)
         if self.is_causal:
             out = selective_mha_prefill(q, k, vh, log_gate, lengths)
             if not any_kept():
-                return self.out_proj(v * out_gate)
+                return self._gated_out(v, out_gate)
             if cache is not None:
                 cache.build_kv(k, vh, log_gate, lengths)
             out = out.transpose(1, 2).reshape(b, L, self.dim)
         else:
             out = self._bidirectional(q, k, vh, log_gate, lengths)
             if not any_kept():
-                return self.out_proj(v * out_gate)
-        return self.out_proj(out.to(hidden_states.dtype) * out_gate)
+                return self._gated_out(v, out_gate)
+        return self._gated_out(out.to(hidden_states.dtype), out_gate)
 
     def _train_forward(self, hidden_states, lengths):
         """The reference's training forward (:197-277): no threshold, the

@@ -18,7 +18,7 @@ import torch.nn as nn
 
 from ..kernels.ssm_io import ssm_conv_forward
 from ..kernels.ssu import ssu_gated_forward
-from .layers import Linear
+from .layers import Linear, all_fp8
 from ..ops import SSDScanGatedFn, SSMConvFn, SSMGateFn, SSUFn, ssm_conv_step
 
 
@@ -64,6 +64,11 @@ class SSM(nn.Module):
 
         self.out_proj = Linear(self.inner_dim, model_dim)
         self.dropout = nn.Dropout(dropout_rate)
+
+    @property
+    def takes_rows(self) -> bool:
+        """Whether the input may come in 8 bits (RMSNorm.forward)."""
+        return all_fp8(self.in_proj) and not self.training
 
     def _A(self) -> torch.Tensor:
         """A = -exp(A_log) in fp32; in inference computed once per value of
