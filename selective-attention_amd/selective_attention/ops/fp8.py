@@ -72,33 +72,43 @@ class Fp8Rows:
         return f"Fp8Rows(shape={tuple(self.shape)}, device={self.device})"
 
 
-def _no_gradient(who: str, *ts):
-    if in_forward_mode() or (torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)):
+def _check_rows(who: str, x: torch.Tensor, other: torch.Tensor | None, name: str) -> int:
+    """The features of x, and of `other`, which has its shape and dtype."""
+    shape = x.shape
+    if not shape or shape[-1] == 0:
+        raise ValueError(f"{who}: x must have features, got shape {tuple(shape)}")
+    if other is not None and (other.shape != shape or other.dtype != x.dtype):
+        raise ValueError(f"{who}: {name} must be {tuple(shape)} {x.dtype}, got {tuple(other.shape)} {other.dtype}")
+    return shape[-1]
+
+
+def _no_gradient(who: str, x: torch.Tensor, *others):
+    wanted = False
+    if torch.is_grad_enabled():
+        wanted = x.requires_grad
+        for t in others:
+            wanted = wanted or (t is not None and t.requires_grad)
+    if wanted or in_forward_mode():
         raise RuntimeError(f"{who}: codes have no gradient; pass fp8_linear the rows in bfloat16 instead, "
                            "or call it under torch.no_grad()")
 
 
-def _check_rows(who: str, x: torch.Tensor, other: torch.Tensor | None, name: str):
-    if x.dim() == 0 or x.shape[-1] == 0:
-        raise ValueError(f"{who}: x must have features, got shape {tuple(x.shape)}")
-    if other is not None and (other.shape != x.shape or other.dtype != x.dtype):
-        raise ValueError(f"{who}: {name} must be {tuple(x.shape)} {x.dtype}, got {tuple(other.shape)} {other.dtype}")
-
-
 def quantize_rows_fp8(x: torch.Tensor, xscale: torch.Tensor | None = None) -> Fp8Rows:
     """x (..., features) float32 or bfloat16, or x * xscale (of x's shape and dtype), in 8 bits."""
-    _check_rows("quantize_rows_fp8", x, xscale, "xscale")
+    dim = _check_rows("quantize_rows_fp8", x, xscale, "xscale")
     _no_gradient("quantize_rows_fp8", x, xscale)
-    return Fp8Rows(*_k.quantize_rows(x, xscale), x.shape[-1])
+    codes, scales = _k.quantize_rows(x, xscale)
+    return Fp8Rows(codes, scales, dim)
 
 
 def silu_mul_fp8(a: torch.Tensor, c: torch.Tensor) -> Fp8Rows:
     """a * silu(c) of bfloat16 tensors of one shape (..., features), in 8 bits."""
-    _check_rows("silu_mul_fp8", a, c, "c")
+    dim = _check_rows("silu_mul_fp8", a, c, "c")
     if a.dtype != torch.bfloat16:
         raise TypeError(f"silu_mul_fp8: a and c must be bfloat16, got {a.dtype}")
     _no_gradient("silu_mul_fp8", a, c)
-    return Fp8Rows(*_k.quantize_rows(a, c, True), a.shape[-1])
+    codes, scales = _k.quantize_rows(a, c, True)
+    return Fp8Rows(codes, scales, dim)
 
 
 def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
@@ -107,9 +117,9 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
     dtype: Fp8Rows, with a residual (t, Fp8Rows).  x, residual (..., features) float32
     or bfloat16, weight (features,).  The squares are summed in fp32's range: a row
     whose sum passes it gives zeros."""
-    _check_rows("rms_norm_fp8", x, residual, "residual")
-    dim = x.shape[-1]
-    check_shape(weight, (dim,), name="weight")
+    dim = _check_rows("rms_norm_fp8", x, residual, "residual")
+    if weight.shape != (dim,):
+        check_shape(weight, (dim,), name="weight")
     if dim > _k.MAX_NORM_DIM:
         raise ValueError(f"rms_norm_fp8: {dim} features, at most {_k.MAX_NORM_DIM}")
     eps = float(eps)
@@ -186,17 +196,15 @@ def quantize_fp8(weight: torch.Tensor):
 
 def _weight(packed: torch.Tensor, scales: torch.Tensor, N: int, K: int):
     """Checks a packed weight against its sizes."""
-    shape = packed.shape
-    if len(shape) != 5 or shape[2:] != (8, 16, 16) or packed.dtype != torch.uint8:
-        raise ValueError(f"fp8: packed must be (tiles, blocks, 8, 16, 16) uint8, got {tuple(shape)} {packed.dtype}")
-    if shape[0] == 0 or shape[0] != (N + 15) // 16 or shape[1] != (K + 127) // 128:
-        raise ValueError(f"fp8: packed {tuple(shape)} holds {16 * shape[0]} rows and {128 * shape[1]} columns "
-                         f"(padded), not {N} and {K}")
-    if scales.shape != ((N + 127) // 128, (K + 511) // 512 * 4):
-        raise ValueError(f"fp8: scales must be {((N + 127) // 128, (K + 511) // 512 * 4)}, got {tuple(scales.shape)}")
+    tiles, blocks = (N + 15) >> 4, (K + 127) >> 7
+    if packed.shape != (tiles, blocks, 8, 16, 16) or packed.dtype != torch.uint8 or not tiles:
+        raise ValueError(f"fp8: packed must be (tiles, blocks, 8, 16, 16) uint8, {(tiles, blocks, 8, 16, 16)} for {N} "
+                         f"out_features and {K} in_features, got {tuple(packed.shape)} {packed.dtype}")
+    if scales.shape != ((N + 127) >> 7, (blocks + 3) >> 2 << 2):
+        raise ValueError(f"fp8: scales must be {((N + 127) >> 7, (blocks + 3) >> 2 << 2)}, got {tuple(scales.shape)}")
     if scales.dtype not in _BYTES:
         raise TypeError(f"fp8: scales must be {SCALES} or its bytes, got {scales.dtype}")
-    if not (packed.is_contiguous() and scales.is_contiguous()) or packed.data_ptr() % 16 or scales.data_ptr() % 4:
+    if not (packed.is_contiguous() and scales.is_contiguous()) or packed.data_ptr() & 15 or scales.data_ptr() & 3:
         raise ValueError("fp8: packed and scales must be contiguous on 16- and 4-byte boundaries")
 
 
@@ -212,6 +220,23 @@ def dequantize_fp8(packed: torch.Tensor, scales: torch.Tensor, out_features: int
     return _k.dequantize(packed, scales, N, K)
 
 
+def _rows(x: Fp8Rows):
+    """(features, codes, scales) of rows, checked; slices are copied."""
+    K, codes, scales = x.features, x.codes, x.scales
+    shape, s = codes.shape, scales.shape
+    Kp = (K + 127) >> 7 << 7
+    if codes.dtype != CODES or not Kp or shape[-1] != Kp:
+        raise ValueError(f"fp8_linear: codes must be (..., {Kp}) {CODES}, got {tuple(shape)} {codes.dtype}")
+    if s[:-1] != shape[:-1] or s[-1] != (Kp + 511) >> 9 << 2 or scales.dtype not in _BYTES:
+        raise ValueError(f"fp8_linear: scales must be (..., {(Kp + 511) >> 9 << 2}) {SCALES} beside codes "
+                         f"{tuple(shape)}, got {tuple(s)} {scales.dtype}")
+    if not codes.is_contiguous() or codes.data_ptr() & 15:
+        codes = codes.clone(memory_format=torch.contiguous_format)
+    if not scales.is_contiguous() or scales.data_ptr() & 3:
+        scales = scales.clone(memory_format=torch.contiguous_format)
+    return K, codes, scales
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     """x W^T + bias; the gradient passes the rows' rounding as it is."""
 
@@ -221,8 +246,7 @@ class _Fp8LinearFn(torch.autograd.Function):
             rows = _k.quantize_rows(x, None)
         ctx.save_for_backward(packed, scales)
         ctx.N, ctx.K = N, None if x is None else x.shape[-1]
-        lead = rows[0].shape[:-1]
-        return _k.linear_multi(*rows, lead, rows[0].shape[-1], [(packed, scales)], [bias], [N])[0]
+        return _k.linear_multi(*rows, [(packed, scales)], [bias], [N])[0]
 
     @staticmethod
     def backward(ctx, dy):
@@ -244,36 +268,26 @@ def fp8_linear_multi(x, weights, biases, sizes, xscale: torch.Tensor | None = No
     if not 1 <= n <= MAX_MATRICES or len(biases) != n or len(sizes) != n:
         raise ValueError(f"fp8_linear_multi: 1..{MAX_MATRICES} weights with as many biases and sizes, "
                          f"got {n}, {len(biases)}, {len(sizes)}")
-    is_rows = isinstance(x, Fp8Rows)
+    is_rows = type(x) is Fp8Rows
     if is_rows:
         if xscale is not None:
             raise ValueError("fp8_linear: xscale goes with x as a tensor, not with rows in 8 bits")
-        codes, scales = x.codes, x.scales
-        K, Kp = x.features, codes.shape[-1]
-        if codes.dtype != CODES or Kp != (K + 127) // 128 * 128 or Kp == 0:
-            raise ValueError(f"fp8_linear: codes must be (..., {(K + 127) // 128 * 128}) {CODES}, "
-                             f"got {tuple(codes.shape)} {codes.dtype}")
-        if scales.shape[:-1] != codes.shape[:-1] or scales.shape[-1] != (Kp + 511) // 512 * 4 or scales.dtype not in _BYTES:
-            raise ValueError(f"fp8_linear: scales must be (..., {(Kp + 511) // 512 * 4}) {SCALES} beside codes "
-                             f"{tuple(codes.shape)}, got {tuple(scales.shape)} {scales.dtype}")
-        if not codes.is_contiguous() or codes.data_ptr() % 16:
-            codes = codes.clone(memory_format=torch.contiguous_format)
-        if not scales.is_contiguous() or scales.data_ptr() % 4:
-            scales = scales.clone(memory_format=torch.contiguous_format)
+        K, codes, scales = _rows(x)
+        grad = False
     else:
-        _check_rows("fp8_linear", x, xscale, "xscale")
+        K = _check_rows("fp8_linear", x, xscale, "xscale")
         if x.dtype != torch.bfloat16:
             raise TypeError(f"fp8_linear: x must be bfloat16 or Fp8Rows, got {x.dtype}")
-        K = x.shape[-1]
+        grad = x.requires_grad or (xscale is not None and xscale.requires_grad)
     for (packed, ws), b, N in zip(weights, biases, sizes):
         _weight(packed, ws, N, K)
         if b is not None:
-            check_shape(b, (N,), name="bias")
+            if b.shape != (N,):
+                check_shape(b, (N,), name="bias")
             if b.dtype != torch.bfloat16:
                 raise TypeError(f"fp8_linear: bias must be bfloat16, got {b.dtype}")
-    if in_forward_mode() or (torch.is_grad_enabled() and (
-            (not is_rows and (x.requires_grad or (xscale is not None and xscale.requires_grad)))
-            or any(b is not None and b.requires_grad for b in biases))):
+            grad = grad or b.requires_grad
+    if (grad and torch.is_grad_enabled()) or in_forward_mode():
         if not is_rows and xscale is not None:
             x = x * xscale
         rows = (codes, scales) if is_rows else None
@@ -281,7 +295,7 @@ def fp8_linear_multi(x, weights, biases, sizes, xscale: torch.Tensor | None = No
                 for w, b, N in zip(weights, biases, sizes)]
     if not is_rows:
         codes, scales = _k.quantize_rows(x, xscale)
-    return _k.linear_multi(codes, scales, codes.shape[:-1], codes.shape[-1], weights, biases, sizes)
+    return _k.linear_multi(codes, scales, weights, biases, sizes)
 
 
 def fp8_linear(x, packed: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,

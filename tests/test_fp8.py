@@ -471,7 +471,7 @@ def test_linear_results_next_to_others():
         x = on(x)
         pool = torch.full((M * N + 4096,), 7.0, dtype=torch.bfloat16, device="cuda")
         from selective_attention.kernels.fp8 import linear_multi
-        want = linear_multi(x.codes, x.scales, (M,), K, [(packed, scales)], [None], [N])[0]
+        want = linear_multi(x.codes, x.scales, [(packed, scales)], [None], [N])[0]
         import ctypes
         from selective_attention import _lib
         words = (ctypes.c_int64 * 5)(packed.data_ptr(), scales.data_ptr(), 0, pool.data_ptr() + 2 * 1025, N)
