@@ -48,8 +48,10 @@ __device__ __forceinline__ v4f mfma_fp8(const v8i& a, const v8i& b, const v4f& c
 }
 
 // A workgroup of NW waves computes R tiles of 16 columns of y for 16 CT rows of x;
-// the waves take the blocks of K in turn and their sums meet in LDS.  Lane 16 g + c
-// holds columns 16 g .. + 15 and 64 + 16 g .. of a block, of row c.
+// the waves take the blocks of K in turn and their sums meet in LDS.  Operands go
+// from memory to registers, the next block's while this one's are multiplied: no wave
+// has what another needs.  Lane 16 g + c holds columns 16 g .. + 15 and 64 + 16 g .. of a
+// block, of row c.
 template <int CT, int R, int NW>
 __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const uint8_t* __restrict__ x,
                                                           const uint8_t* __restrict__ xs, const Fp8Segs sg, int M,
@@ -63,35 +65,65 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const uint8_t* __restr
   for (int i = 1; i < kFp8Segs; ++i) seg += (i < sg.nseg && bid >= sg.blk0[i]) ? 1 : 0;
   const int N = sg.N[seg], tiles = (N + 15) >> 4, words = (kb_n + 3) >> 2;
   const int t0 = (bid - sg.blk0[seg]) * R;
-  const uint8_t* W = sg.W[seg];
-  const uint8_t* S = sg.scale[seg];
+  // (rows and tiles behind the last are the last again, not stored)
+  const uint4* wp[R];
+  const uint4* xp[CT];
+  const uint8_t* sxp[CT];
+#pragma unroll
+  for (int r = 0; r < R; ++r)
+    wp[r] = reinterpret_cast<const uint4*>(sg.W[seg] + static_cast<long>(min(t0 + r, tiles - 1)) * kb_n * 2048) + lane;
+#pragma unroll
+  for (int t = 0; t < CT; ++t) {
+    const long row = min(m0 + 16 * t + c, M - 1);
+    xp[t] = reinterpret_cast<const uint4*>(x + row * kb_n * 128) + g;
+    sxp[t] = xs + row * 4 * words;
+  }
+  const uint8_t* swp[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) swp[r] = sg.scale[seg] + static_cast<long>(min(t0 + r, tiles - 1) >> 3) * 4 * words;
 
+  struct Block {
+    uint4 w[R][2], x[CT][2];
+    uint32_t sw[R], sx[CT];
+  };
+  auto load = [&](int kb, Block& q) __attribute__((always_inline)) {
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      q.w[r][0] = wp[r][kb * 128];
+      q.w[r][1] = wp[r][kb * 128 + 64];
+      q.sw[r] = swp[r][kb];
+    }
+#pragma unroll
+    for (int t = 0; t < CT; ++t) {
+      q.x[t][0] = xp[t][kb * 8];
+      q.x[t][1] = xp[t][kb * 8 + 4];
+      q.sx[t] = sxp[t][kb];
+    }
+  };
   v4f acc[R][CT];
 #pragma unroll
   for (int r = 0; r < R; ++r)
 #pragma unroll
     for (int t = 0; t < CT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
-  for (int kb = wid; kb < kb_n; kb += NW) {
-    v8i w[R], xf[CT];
-    uint32_t sw[R], sx[CT];
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int t = min(t0 + r, tiles - 1);   // (behind the last: not stored)
-      const uint4* p = reinterpret_cast<const uint4*>(W + (static_cast<long>(t) * kb_n + kb) * 2048) + lane;
-      w[r] = join16(p[0], p[64]);
-      sw[r] = S[static_cast<long>(t >> 3) * 4 * words + kb];
-    }
-#pragma unroll
-    for (int t = 0; t < CT; ++t) {
-      const long row = min(m0 + 16 * t + c, M - 1);
-      const uint4* p = reinterpret_cast<const uint4*>(x + (row * kb_n + kb) * 128) + g;
-      xf[t] = join16(p[0], p[4]);
-      sx[t] = xs[row * 4 * words + kb];
-    }
+  auto multiply = [&](const Block& q) __attribute__((always_inline)) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
 #pragma unroll
-      for (int t = 0; t < CT; ++t) acc[r][t] = mfma_fp8(w[r], xf[t], acc[r][t], sw[r], sx[t]);
+      for (int t = 0; t < CT; ++t)
+        acc[r][t] = mfma_fp8(join16(q.w[r][0], q.w[r][1]), join16(q.x[t][0], q.x[t][1]), acc[r][t], q.sw[r], q.sx[t]);
+  };
+  // (two copies of the body, so that no register of a load in flight is moved)
+  Block q0, q1;
+  int kb = wid;
+  if (kb < kb_n) load(kb, q0);
+  while (kb < kb_n) {
+    if (kb + NW < kb_n) load(kb + NW, q1);
+    multiply(q0);
+    kb += NW;
+    if (kb >= kb_n) break;
+    if (kb + NW < kb_n) load(kb + NW, q0);
+    multiply(q1);
+    kb += NW;
   }
   // lane (c, g) holds columns 4 g + e of the tile for row 16 t + c of x
 #pragma unroll
@@ -192,6 +224,7 @@ struct Fp8Scales {
 // of kCols columns at a time) so that they leave as whole pieces of 2 kCols bytes.  They
 // pass the caches by: nothing here reads them again, and the next tiles' operands
 // stay (32768 rows, 1024 -> 4096: 165 us, so 142).
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(2)));   // 16 bytes at any even address
 template <int SN, int SM>
 struct Fp8Out {
   static constexpr int kCols = SN > 1 ? 64 : 32, kPitch = 2 * kCols + 16, kBytes = 32 * kPitch;
@@ -199,7 +232,6 @@ struct Fp8Out {
                                                int nw, int mw, int N, int M) {
     const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     bf16* y = y0 + static_cast<long>(mw) * N + nw;
-    const bool whole = (N & 7) == 0 && (reinterpret_cast<uintptr_t>(y0) & 15) == 0;
     constexpr int kSq = kCols / 32, kLanes = kCols / 8;
 #pragma unroll
     for (int j = 0; j < SM; ++j)
@@ -217,30 +249,16 @@ struct Fp8Out {
           }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-        if (whole) {
 #pragma unroll
-          for (int r = 0; r < 32; r += 64 / kLanes) {
-            const int row = r + lane / kLanes, n = 32 * i0 + 8 * (lane % kLanes);
-            const v4f v = *reinterpret_cast<const v4f*>(ys + row * kPitch + 16 * (lane % kLanes));
-            if (mw + 32 * j + row < M && nw + n < N)
-              __builtin_nontemporal_store(v, reinterpret_cast<v4f*>(y + static_cast<long>(32 * j + row) * N + n));
-          }
-        } else {
-          // rows start anywhere: words of two columns where both are the wave's, else one
-          constexpr int kPairs = kCols / 2;
-#pragma unroll 4
-          for (int r = 0; r < 32; r += 64 / kPairs) {
-            const int row = r + lane / kPairs, left = N - nw - 32 * i0;   // columns of y from here on
-            bf16* to = y + static_cast<long>(32 * j + row) * N + 32 * i0;
-            const bf16* from = reinterpret_cast<const bf16*>(ys + row * kPitch);
-            const int odd = static_cast<int>(reinterpret_cast<uintptr_t>(to) >> 1) & 1, n = 2 * (lane % kPairs) + odd;
-            if (mw + 32 * j + row < M) {
-              if (n + 1 < min(kCols, left))
-                *reinterpret_cast<uint32_t*>(to + n) = from[n].x | static_cast<uint32_t>(from[n + 1].x) << 16;
-              else if (n < min(kCols, left))
-                to[n] = from[n];
-              if (odd && n == 1 && left > 0) to[0] = from[0];
-            }
+        for (int r = 0; r < 32; r += 64 / kLanes) {
+          const int row = r + lane / kLanes, n = 32 * i0 + 8 * (lane % kLanes), left = mw + 32 * j + row < M ? N - nw - n : 0;
+          bf16* to = y + static_cast<long>(32 * j + row) * N + n;
+          const uint8_t* from = ys + row * kPitch + 16 * (lane % kLanes);
+          if (left >= 8) {
+            __builtin_nontemporal_store(*reinterpret_cast<const v4f*>(from), reinterpret_cast<v4f_any*>(to));
+          } else {   // the matrix's last columns
+#pragma unroll 1
+            for (int e = 0; e < left; ++e) to[e] = *reinterpret_cast<const bf16*>(from + 2 * e);
           }
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -591,40 +609,52 @@ void fp8_ring(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStre
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
 }
 
-// The kernel by the sizes.  Up to 64 rows and 12288 columns the waves share K
-// (fp8_few): 16 rows 1024 -> 4384 4.1 us (tiles of 64 by 64: 5.6), 32 rows 4096 -> 4096 7.6
-// (11.5), 64 rows 11008 -> 4096 18.6 (26.8); two tiles a workgroup, which read x once, from
-// 17 rows on, and for wide matrices also below (16 rows, 4096 -> 32000: 32.6, so 24.9).
-// Wider ones, from 17 rows on, go in tiles (32 rows, 4096 -> 32000: 41, tiles 25.5), as do
-// more rows, by the least estimate in us of
-//   tiles <= 256      first(kb), that of one tile on each CU
+// The kernel by the sizes: the least estimate in us, of kb blocks of K, of
+//   tiles <= 256      first(kb), one tile on each CU
 //   more              again + (tiles / 256, between itself and its ceiling) each(kb)
-// fitted to 27 products of 65 to 32768 rows, K 1024 to 8192, N 1024 to 32000: the choice
-// was never more than 9 % behind the best.
+// fitted to 60 products of 1 to 32768 rows, K 1024 to 11008, N 1024 to 32000; the choice
+// was at most 12 % behind the best of all (linear8 in us, tiles of fp8_few, fp8_ring and
+// fp8_large as rows x columns):
+//   1 row, 1024 -> 1024       16 x 16 3.4   16 x 64 3.7    64 x 64 5.3
+//   64 rows, 4096 -> 4096     16 x 16 15.3  16 x 64 8.1    64 x 64 11.7
+//   200 rows, 8192 -> 1024    16 x 16 25.6  16 x 64 12.6   64 x 64 21.9
+//   32 rows, 4096 -> 32000    16 x 32 42.8  64 x 64 30.3   64 x 128 25.5
+//   500 rows, 1024 -> 4384    32 x 64 24.5  64 x 64 8.2    128 x 128 8.3   256 x 256 16.6
+//   4000 rows, 1024 -> 4384   64 x 64 36    128 x 128 25.8 128 x 256 28.4  256 x 256 34.6
+//   8192 rows, 4096 -> 4096   128 x 128 156 256 x 256 105
 struct Fp8Shape {
-  int bn, bm;
+  int bm, bn;
   float first0, first1, again, each0, each1;
 };
+constexpr int kFp8Few = 4;   // shapes of fp8_few, then tiles
 constexpr Fp8Shape kFp8Shapes[] = {
-    {256, 256, 8.0f, 1.06f, 8.0f, 5.0f, 1.48f},   // fp8_large: a full card is bound by power, from one tile a CU on
-    {256, 128, 4.0f, 0.93f, 5.3f, 1.3f, 0.87f},
-    {128, 128, 3.0f, 0.60f, 2.9f, 0.5f, 0.58f},
-    {128, 64, 3.0f, 0.40f, 4.0f, -0.2f, 0.39f},
+    {16, 16, 2.6f, 0.106f, 1.5f, 0.8f, 0.0725f},
+    {16, 32, 2.5f, 0.119f, 1.5f, 1.0f, 0.115f},
+    {16, 64, 2.8f, 0.146f, 1.5f, 4.4f, 0.0625f},
+    {32, 64, 3.9f, 0.2125f, 1.6f, 1.9f, 0.2375f},
     {64, 64, 3.0f, 0.30f, 4.0f, -0.2f, 0.255f},
+    {64, 128, 3.0f, 0.40f, 4.0f, -0.2f, 0.39f},
+    {128, 128, 3.0f, 0.60f, 2.9f, 0.5f, 0.58f},
+    {128, 256, 4.0f, 0.93f, 5.3f, 1.3f, 0.87f},
+    {256, 256, 8.0f, 1.06f, 8.0f, 5.0f, 1.48f},   // (full of such tiles the card is bound by power)
 };
 int fp8_shape(const Fp8Segs& sg, int M, int kb, float* per_cu) {
+  constexpr int kShapes = sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]);
   int best = 0;
   float least = 0.0f;
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < kShapes; ++i) {
     const Fp8Shape& p = kFp8Shapes[i];
     long tiles = 0;
     for (int k = 0; k < sg.nseg; ++k) tiles += (sg.N[k] + p.bn - 1) / p.bn;
     tiles *= (M + p.bm - 1) / p.bm;
-    const float r = static_cast<float>(tiles) / 256.0f, each = p.each0 + p.each1 * static_cast<float>(kb);
-    float us = p.first0 + p.first1 * static_cast<float>(kb);
-    if (r > 1.0f) us = p.again + 0.5f * (r + static_cast<float>((tiles + 255) / 256)) * each;
-    else if (i == 0) us = std::max(us, r * (each + 2.0f));
-    if (i == 0 || us < least) {
+    if (tiles >= 1 << 23) continue;   // (2^32 threads a grid, of up to 512 a tile)
+    if ((i == 2 || i == 3) && tiles > 256) continue;   // (1 row, 4096 -> 32000: 16 x 64 25.6, 64 x 128 24.7)
+    const float r = static_cast<float>(tiles) / 256.0f, k = static_cast<float>(kb), each = p.each0 + p.each1 * k;
+    float us = p.first0 + p.first1 * k;
+    if (i < kFp8Few) us = std::max(us, p.again + r * each);
+    else if (r > 1.0f) us = p.again + 0.5f * (r + static_cast<float>((tiles + 255) / 256)) * each;
+    else if (i == kShapes - 1) us = std::max(us, r * (each + 2.0f));
+    if (least == 0.0f || us < least) {
       least = us;
       best = i;
       *per_cu = r;
@@ -634,19 +664,18 @@ int fp8_shape(const Fp8Segs& sg, int M, int kb, float* per_cu) {
 }
 
 void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
-  long N = 0;
-  for (int i = 0; i < sg.nseg; ++i) N += sg.N[i];
-  if (M <= 16) return N <= 12288 ? fp8_few<1, 1, 8>(x, xs, sg, M, kb, s) : fp8_few<1, 2, 8>(x, xs, sg, M, kb, s);
-  if (M <= 64 && N <= 12288)
-    return M <= 32 ? fp8_few<1, 2, 8>(x, xs, sg, M, kb, s) : fp8_few<2, 2, 8>(x, xs, sg, M, kb, s);
   // few tiles a CU get deep rings, more of them room beside each other
   float per_cu = 0.0f;
   switch (fp8_shape(sg, M, kb, &per_cu)) {
-    case 0: return fp8_large<4, 4>(x, xs, sg, M, kb, s);
-    case 1: return fp8_ring<4, 2, 3, 2>(x, xs, sg, M, kb, s);
-    case 2: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
-    case 3: return per_cu <= 2.0f ? fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 1, 3, 4>(x, xs, sg, M, kb, s);
-    default: return per_cu <= 2.0f ? fp8_ring<1, 1, 8, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
+    case 0: return fp8_few<1, 1, 8>(x, xs, sg, M, kb, s);
+    case 1: return fp8_few<1, 2, 8>(x, xs, sg, M, kb, s);
+    case 2: return fp8_few<1, 4, 8>(x, xs, sg, M, kb, s);
+    case 3: return fp8_few<2, 4, 8>(x, xs, sg, M, kb, s);
+    case 4: return per_cu <= 2.0f ? fp8_ring<1, 1, 8, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
+    case 5: return per_cu <= 2.0f ? fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 1, 3, 4>(x, xs, sg, M, kb, s);
+    case 6: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
+    case 7: return fp8_ring<4, 2, 3, 2>(x, xs, sg, M, kb, s);
+    default: return fp8_large<4, 4>(x, xs, sg, M, kb, s);
   }
 }
 
@@ -678,8 +707,8 @@ extern "C" int sa_fp8_linear(const void* codes, const void* scales, int64_t M, i
     sg.y[i] = reinterpret_cast<sa::bf16*>(m[3]);
     sg.N[i] = static_cast<int>(m[4]);
   }
-  SA_CHECK_ARG(tiles * ((M + 63) / 64) < (1L << 24), "%s: %ld rows and %ld columns are too many", who,
-               static_cast<long>(M), 64 * tiles);   // (2^32 threads a grid)
+  SA_CHECK_ARG(tiles * ((M + 63) / 64) < (1L << 23), "%s: %ld rows and %ld columns are too many", who,
+               static_cast<long>(M), 64 * tiles);   // (tiles of 64 by 64 and more always fit a grid)
   hipStream_t s = static_cast<hipStream_t>(stream);
   const int kb = (K + 127) / 128, m = static_cast<int>(M);
   sa::fp8_go(codes, scales, sg, m, kb, s);

@@ -289,6 +289,7 @@ void norm_go(const void* x, const void* res, const float* w, long rows, long ldx
   else go(rms_norm_fp8_kernel<T, VEC, RES, 8, 16>, 16);
 }
 constexpr int kMaxNormDim = 65536;
+int norm_waves(int dim) { return dim <= 1024 ? 1 : dim <= 8192 ? 4 : 16; }   // (as norm_go)
 
 int rows_check(const char* who, int dtype, long rows, int dim, const void* codes, const void* scales) {
   SA_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype code %d", who, dtype);
@@ -333,7 +334,7 @@ extern "C" int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, c
   if (const int rc = sa::rows_check(who, dtype, rows, dim, codes, scales)) return rc;
   if (rows == 0) return 0;
   SA_CHECK_ARG(dim <= sa::kMaxNormDim, "%s: dim %d above %d", who, dim, sa::kMaxNormDim);
-  SA_CHECK_ARG(rows < (1L << 22) || (dim <= 1024 && rows < (1L << 26)), "%s: %ld rows of %d columns are too many", who,
+  SA_CHECK_ARG(rows * 64 * sa::norm_waves(dim) < (1L << 32), "%s: %ld rows of %d columns are too many", who,
                static_cast<long>(rows), dim);   // (2^32 threads a grid)
   SA_CHECK_ARG(x && weight && (!residual == !sum), "%s: null pointer, or one of residual and sum without the other", who);
   SA_CHECK_ARG(ldx >= dim, "%s: row stride %ld below dim %d", who, static_cast<long>(ldx), dim);

@@ -426,8 +426,9 @@ def test_linear_of_whole_numbers(M, K, N):
 
 
 # (M, K, [N_i]), the kernel: few rows, tiles of each shape, odd borders, long K, many rows
-TILES = [(16, 1024, [20000], "few"), (32, 11008, [500], "few"), (64, 700, [12287], "few"), (17, 256, [12289], "ring"),
-         (64, 4096, [32000], "ring"), (66, 33000, [70], "ring"), (257, 16384, [300], "ring"), (500, 2050, [4383], "ring"),
+TILES = [(61, 4000, [4090], "few"), (120, 3970, [1800, 1, 1000, 1090], "few"), (30, 900, [1, 4000], "few"),
+         (16, 1024, [20000], "few"), (32, 11008, [500], "few"), (64, 700, [12287], "ring"), (17, 256, [12289], "ring"),
+         (64, 4096, [32000], "ring"), (66, 33000, [70], "few"), (257, 16384, [300], "few"), (500, 2050, [4383], "ring"),
          (1111, 1030, [4383], "ring"), (2001, 1024, [4384], "ring"), (2047, 4096, [4096], "ring"), (2047, 4096, [4100], "large"),
          (700, 4200, [1111], "ring"), (70000, 128, [64], "ring"), (8100, 1024, [4384], "ring"),
          (4100, 1408, [4097], "ring"), (8192, 2100, [4104], "ring"), (4095, 4096, [4095], "large"),
