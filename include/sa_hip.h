@@ -391,6 +391,14 @@ int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, const float*
 int sa_fp8_linear(const void* codes, const void* scales, int64_t M, int K, int nseg,
                   const int64_t* matrices, void* stream);
 
+/*
+ * The same for 1 to 16 rows x (M, K) bf16 with row stride ldx (elements; fastest on
+ * 16-byte boundaries, K a multiple of 8), or x * xscale (stride ldg) where xscale is not
+ * NULL, which the kernel rounds as sa_rows_fp8 does.
+ */
+int sa_fp8_linear_bf16(const void* x, const void* xscale, int M, int K, int64_t ldx, int64_t ldg,
+                       int nseg, const int64_t* matrices, void* stream);
+
 /* The weights that such a packed matrix stands for, in bf16: out (N, K). */
 int sa_fp8_dequant_bf16(const void* packed, const void* scales, int N, int K, void* out,
                         void* stream);

@@ -16,7 +16,7 @@
 // bytes: in a tile, 16 columns of its 16 rows after each other, so that 16 lanes
 // read 256 bytes in a row both from memory and from LDS.  N and K are padded with
 // zeros to whole tiles.  Scales: (N / 128, 4 ceil(K / 512)) bytes.
-#include "common.h"
+#include "fp8.h"
 #include "prof.h"
 
 #include <algorithm>
@@ -52,10 +52,47 @@ __device__ __forceinline__ v4f mfma_fp8(const v8i& a, const v8i& b, const v4f& c
 // from memory to registers, the next block's while this one's are multiplied: no wave
 // has what another needs.  Lane 16 g + c holds columns 16 g .. + 15 and 64 + 16 g .. of a
 // block, of row c.
-template <int CT, int R, int NW>
-__global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const uint8_t* __restrict__ x,
-                                                          const uint8_t* __restrict__ xs, const Fp8Segs sg, int M,
-                                                          int kb_n) {
+// X: the rows are codes with scales (kCodes), or bfloat16 that each wave rounds for
+// itself, block by block (kBf16; kGated: times the gate): the four lanes of a row have
+// a block's columns between them, so its scale costs two lane exchanges, and up to 16
+// rows save the launch that would make the codes (4 rows, 1024 -> 4384: 17.4 us a call
+// with it).
+enum { kCodes = 0, kBf16 = 1, kGated = 2 };
+struct Fp8X {
+  const void *x, *other;   // codes and scales, or rows and gate
+  int64_t ldx, ldg;        // of rows in bfloat16
+  int K;
+  bool vec;                // these stand on 16-byte boundaries, K is a multiple of 8
+};
+// sixteen columns of a row from k on, those at or behind K as 0
+__device__ __forceinline__ void load16(uint4 (&q)[2], const bf16* row, int k, int K, bool vec) {
+  if (vec) {   // (uniform)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) q[i] = ld16(row + k + 8 * i, k + 8 * i < K);
+  } else {
+    uint32_t w[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t lo = k + 2 * i < K ? row[k + 2 * i].x : 0u, hi = k + 2 * i + 1 < K ? row[k + 2 * i + 1].x : 0u;
+      w[i] = lo | hi << 16;
+    }
+    q[0] = uint4{w[0], w[1], w[2], w[3]};
+    q[1] = uint4{w[4], w[5], w[6], w[7]};
+  }
+}
+__device__ __forceinline__ void widen16(float* v, const uint4 (&q)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[8 * i + 2 * e] = bf16lo_to_f32(u[e]);
+      v[8 * i + 2 * e + 1] = bf16hi_to_f32(u[e]);
+    }
+  }
+}
+template <int CT, int R, int NW, int X>
+__global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const Fp8X in, const Fp8Segs sg, int M, int kb_n) {
   __shared__ float part[NW * R * CT * 256];
   const int tid = threadIdx.x, lane = tid & 63, wid = tid >> 6, c = lane & 15, g = lane >> 4;
   const int across = sg.blk0[kFp8Segs];   // workgroups a row of tiles
@@ -69,21 +106,27 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const uint8_t* __restr
   const uint4* wp[R];
   const uint4* xp[CT];
   const uint8_t* sxp[CT];
+  const bf16 *xr[CT], *gr[CT];
 #pragma unroll
   for (int r = 0; r < R; ++r)
     wp[r] = reinterpret_cast<const uint4*>(sg.W[seg] + static_cast<long>(min(t0 + r, tiles - 1)) * kb_n * 2048) + lane;
 #pragma unroll
   for (int t = 0; t < CT; ++t) {
     const long row = min(m0 + 16 * t + c, M - 1);
-    xp[t] = reinterpret_cast<const uint4*>(x + row * kb_n * 128) + g;
-    sxp[t] = xs + row * 4 * words;
+    if constexpr (X == kCodes) {
+      xp[t] = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(in.x) + row * kb_n * 128) + g;
+      sxp[t] = static_cast<const uint8_t*>(in.other) + row * 4 * words;
+    } else {
+      xr[t] = static_cast<const bf16*>(in.x) + row * in.ldx;
+      if constexpr (X == kGated) gr[t] = static_cast<const bf16*>(in.other) + row * in.ldg;
+    }
   }
   const uint8_t* swp[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) swp[r] = sg.scale[seg] + static_cast<long>(min(t0 + r, tiles - 1) >> 3) * 4 * words;
 
   struct Block {
-    uint4 w[R][2], x[CT][2];
+    uint4 w[R][2], x[CT][X == kCodes ? 1 : 2][2], gate[X == kGated ? CT : 1][2][2];
     uint32_t sw[R], sx[CT];
   };
   auto load = [&](int kb, Block& q) __attribute__((always_inline)) {
@@ -95,9 +138,17 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const uint8_t* __restr
     }
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
-      q.x[t][0] = xp[t][kb * 8];
-      q.x[t][1] = xp[t][kb * 8 + 4];
-      q.sx[t] = sxp[t][kb];
+      if constexpr (X == kCodes) {
+        q.x[t][0][0] = xp[t][kb * 8];
+        q.x[t][0][1] = xp[t][kb * 8 + 4];
+        q.sx[t] = sxp[t][kb];
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          load16(q.x[t][i], xr[t], 128 * kb + 64 * i + 16 * g, in.K, in.vec);
+          if constexpr (X == kGated) load16(q.gate[t][i], gr[t], 128 * kb + 64 * i + 16 * g, in.K, in.vec);
+        }
+      }
     }
   };
   v4f acc[R][CT];
@@ -107,10 +158,34 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const uint8_t* __restr
     for (int t = 0; t < CT; ++t) acc[r][t] = v4f{0.f, 0.f, 0.f, 0.f};
   auto multiply = [&](const Block& q) __attribute__((always_inline)) {
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int t = 0; t < CT; ++t) {
+      v8i xf;
+      uint32_t sx;
+      if constexpr (X == kCodes) {
+        xf = join16(q.x[t][0][0], q.x[t][0][1]);
+        sx = q.sx[t];
+      } else {
+        float v[32], top = 0.0f;
 #pragma unroll
-      for (int t = 0; t < CT; ++t)
-        acc[r][t] = mfma_fp8(join16(q.w[r][0], q.w[r][1]), join16(q.x[t][0], q.x[t][1]), acc[r][t], q.sw[r], q.sx[t]);
+        for (int i = 0; i < 2; ++i) widen16(v + 16 * i, q.x[t][i]);
+        if constexpr (X == kGated) {
+          float f[32];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) widen16(f + 16 * i, q.gate[t][i]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] *= f[i];   // (exact)
+        }
+#pragma unroll
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, finite_abs(v[i]));
+        top = fmaxf(top, __shfl_xor(top, 16, 64));
+        sx = scale_byte(fmaxf(top, __shfl_xor(top, 32, 64)));
+        const float inv = scale_inverse(sx);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) xf[i] = static_cast<int>(encode4(v + 4 * i, inv));
+      }
+#pragma unroll
+      for (int r = 0; r < R; ++r) acc[r][t] = mfma_fp8(join16(q.w[r][0], q.w[r][1]), xf, acc[r][t], q.sw[r], sx);
+    }
   };
   // (two copies of the body, so that no register of a load in flight is moved)
   Block q0, q1;
@@ -584,14 +659,13 @@ void cut_tiles(Fp8Segs& sg, int BN) {
   sg.blk0[0] = 0;
   for (int i = 0; i < kFp8Segs; ++i) sg.blk0[i + 1] = sg.blk0[i] + (i < sg.nseg ? (sg.N[i] + BN - 1) / BN : 0);
 }
-template <int CT, int R, int NW>
-void fp8_few(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
+template <int CT, int R, int NW, int X>
+void fp8_few(const Fp8X& in, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   cut_tiles(sg, 16 * R);
   ProfScope prof_("fp8_few", s);
-  hipLaunchKernelGGL((fp8_few_kernel<CT, R, NW>), dim3(sg.blk0[kFp8Segs] * ((M + 16 * CT - 1) / (16 * CT))),
-                     dim3(64 * NW), 0, s, static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb);
+  hipLaunchKernelGGL((fp8_few_kernel<CT, R, NW, X>), dim3(sg.blk0[kFp8Segs] * ((M + 16 * CT - 1) / (16 * CT))),
+                     dim3(64 * NW), 0, s, in, sg, M, kb);
 }
-
 template <int SN, int SM>
 void fp8_large(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   cut_tiles(sg, 64 * SN);
@@ -638,11 +712,11 @@ constexpr Fp8Shape kFp8Shapes[] = {
     {128, 256, 4.0f, 0.93f, 5.3f, 1.3f, 0.87f},
     {256, 256, 8.0f, 1.06f, 8.0f, 5.0f, 1.48f},   // (full of such tiles the card is bound by power)
 };
-int fp8_shape(const Fp8Segs& sg, int M, int kb, float* per_cu) {
+int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   // of the first `shapes`
   constexpr int kShapes = sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]);
   int best = 0;
   float least = 0.0f;
-  for (int i = 0; i < kShapes; ++i) {
+  for (int i = 0; i < shapes; ++i) {
     const Fp8Shape& p = kFp8Shapes[i];
     long tiles = 0;
     for (int k = 0; k < sg.nseg; ++k) tiles += (sg.N[k] + p.bn - 1) / p.bn;
@@ -664,13 +738,14 @@ int fp8_shape(const Fp8Segs& sg, int M, int kb, float* per_cu) {
 }
 
 void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
+  const Fp8X in{x, xs, 0, 0, 0, false};
   // few tiles a CU get deep rings, more of them room beside each other
   float per_cu = 0.0f;
-  switch (fp8_shape(sg, M, kb, &per_cu)) {
-    case 0: return fp8_few<1, 1, 8>(x, xs, sg, M, kb, s);
-    case 1: return fp8_few<1, 2, 8>(x, xs, sg, M, kb, s);
-    case 2: return fp8_few<1, 4, 8>(x, xs, sg, M, kb, s);
-    case 3: return fp8_few<2, 4, 8>(x, xs, sg, M, kb, s);
+  switch (fp8_shape(sg, M, kb, sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]), &per_cu)) {
+    case 0: return fp8_few<1, 1, 8, kCodes>(in, sg, M, kb, s);
+    case 1: return fp8_few<1, 2, 8, kCodes>(in, sg, M, kb, s);
+    case 2: return fp8_few<1, 4, 8, kCodes>(in, sg, M, kb, s);
+    case 3: return fp8_few<2, 4, 8, kCodes>(in, sg, M, kb, s);
     case 4: return per_cu <= 2.0f ? fp8_ring<1, 1, 8, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
     case 5: return per_cu <= 2.0f ? fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 1, 3, 4>(x, xs, sg, M, kb, s);
     case 6: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
@@ -679,19 +754,17 @@ void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream
   }
 }
 
-}  // namespace
-}  // namespace sa
+// up to 16 rows in bfloat16
+template <int X>
+void fp8_go_bf16(const Fp8X& in, Fp8Segs& sg, int M, int kb, hipStream_t s) {
+  float per_cu = 0.0f;
+  if (fp8_shape(sg, M, kb, 2, &per_cu) == 0) fp8_few<1, 1, 8, X>(in, sg, M, kb, s);
+  else fp8_few<1, 2, 8, X>(in, sg, M, kb, s);
+}
 
-extern "C" int sa_fp8_linear(const void* codes, const void* scales, int64_t M, int K, int nseg,
-                             const int64_t* matrices, void* stream) {
-  const char* who = "sa_fp8_linear";
-  SA_CHECK_ARG(M >= 1 && M <= (1 << 24) && K > 0 && K <= (1 << 22), "%s: M %ld must be 1..2^24 and K %d 1..2^22", who,
-               static_cast<long>(M), K);
-  SA_CHECK_ARG(nseg >= 1 && nseg <= sa::kFp8Segs, "%s: %d weight matrices, 1..%d allowed", who, nseg, sa::kFp8Segs);
-  SA_CHECK_ARG(codes && scales && matrices, "%s: null pointer", who);
-  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 3)) == 0,
-               "%s: codes or scales of x are not aligned", who);
-  sa::Fp8Segs sg{};
+// the weights of a call, checked
+int fp8_matrices(const char* who, Fp8Segs& sg, int64_t M, int nseg, const int64_t* matrices) {
+  SA_CHECK_ARG(nseg >= 1 && nseg <= kFp8Segs && matrices, "%s: %d weight matrices, 1..%d allowed", who, nseg, kFp8Segs);
   sg.nseg = nseg;
   long tiles = 0;
   for (int i = 0; i < nseg; ++i) {
@@ -703,15 +776,48 @@ extern "C" int sa_fp8_linear(const void* codes, const void* scales, int64_t M, i
     tiles += (m[4] + 63) / 64;
     sg.W[i] = reinterpret_cast<const uint8_t*>(m[0]);
     sg.scale[i] = reinterpret_cast<const uint8_t*>(m[1]);
-    sg.bias[i] = reinterpret_cast<const sa::bf16*>(m[2]);
-    sg.y[i] = reinterpret_cast<sa::bf16*>(m[3]);
+    sg.bias[i] = reinterpret_cast<const bf16*>(m[2]);
+    sg.y[i] = reinterpret_cast<bf16*>(m[3]);
     sg.N[i] = static_cast<int>(m[4]);
   }
   SA_CHECK_ARG(tiles * ((M + 63) / 64) < (1L << 23), "%s: %ld rows and %ld columns are too many", who,
                static_cast<long>(M), 64 * tiles);   // (tiles of 64 by 64 and more always fit a grid)
+  return 0;
+}
+
+}  // namespace
+}  // namespace sa
+
+extern "C" int sa_fp8_linear(const void* codes, const void* scales, int64_t M, int K, int nseg,
+                             const int64_t* matrices, void* stream) {
+  const char* who = "sa_fp8_linear";
+  SA_CHECK_ARG(M >= 1 && M <= (1 << 24) && K > 0 && K <= (1 << 22), "%s: M %ld must be 1..2^24 and K %d 1..2^22", who,
+               static_cast<long>(M), K);
+  SA_CHECK_ARG(codes && scales, "%s: null pointer", who);
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 3)) == 0,
+               "%s: codes or scales of x are not aligned", who);
+  sa::Fp8Segs sg{};
+  if (const int rc = sa::fp8_matrices(who, sg, M, nseg, matrices)) return rc;
+  sa::fp8_go(codes, scales, sg, static_cast<int>(M), (K + 127) / 128, static_cast<hipStream_t>(stream));
+  SA_CHECK_LAUNCH(who);
+  return 0;
+}
+
+extern "C" int sa_fp8_linear_bf16(const void* x, const void* xscale, int M, int K, int64_t ldx, int64_t ldg, int nseg,
+                                  const int64_t* matrices, void* stream) {
+  const char* who = "sa_fp8_linear_bf16";
+  SA_CHECK_ARG(M >= 1 && M <= 16 && K > 0 && K <= (1 << 22), "%s: M %d must be 1..16 and K %d 1..2^22", who, M, K);
+  SA_CHECK_ARG(x, "%s: null pointer", who);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(xscale);
+  SA_CHECK_ARG((at & 1) == 0, "%s: x and xscale are not aligned to their type", who);
+  SA_CHECK_ARG(M == 1 || (ldx >= K && (!xscale || ldg >= K)), "%s: row strides %ld, %ld below K %d", who,
+               static_cast<long>(ldx), static_cast<long>(ldg), K);
+  sa::Fp8Segs sg{};
+  if (const int rc = sa::fp8_matrices(who, sg, M, nseg, matrices)) return rc;
+  const sa::Fp8X in{x, xscale, ldx, ldg, K, (at & 15) == 0 && ((ldx | ldg | K) & 7) == 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
-  const int kb = (K + 127) / 128, m = static_cast<int>(M);
-  sa::fp8_go(codes, scales, sg, m, kb, s);
+  xscale ? sa::fp8_go_bf16<sa::kGated>(in, sg, M, (K + 127) / 128, s)
+         : sa::fp8_go_bf16<sa::kBf16>(in, sg, M, (K + 127) / 128, s);
   SA_CHECK_LAUNCH(who);
   return 0;
 }

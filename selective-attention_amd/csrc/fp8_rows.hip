@@ -20,31 +20,13 @@
 //
 // Streams of memory: 16 lanes a block, 8 columns a lane, the maximum over 16 lanes
 // by four lane exchanges.
-#include "common.h"
+#include "fp8.h"
 #include "prof.h"
 
 #include <type_traits>
 
 namespace sa {
 namespace {
-
-constexpr int kQBlock = 128;
-
-// y + lo (|lo| at most half an ulp of y) rounded to odd: y where lo is 0 or y is
-// odd, else its neighbour towards lo, which is odd.  A y of 0, infinity or NaN stays
-__device__ __forceinline__ float to_odd(float y, float lo) {
-  const uint32_t b = __float_as_uint(y);
-  const int step = (static_cast<int>(b ^ __float_as_uint(lo)) >> 31) | 1;
-  return __uint_as_float(lo != 0.0f && fabsf(lo) < fabsf(y) && (b & 1u) == 0u ? b + step : b);
-}
-
-// e8m0 byte of the scale of a block with the largest finite magnitude top
-__device__ __forceinline__ uint32_t scale_byte(float top) {
-  const uint32_t b = __float_as_uint(top);
-  // 448 = 1.75 2^8: the mantissa decides between 2^(E - 8) and the next one
-  const int e = static_cast<int>(b >> 23) - 8 + ((b & 0x7fffffu) > 0x600000u ? 1 : 0);
-  return b == 0u ? 127u : static_cast<uint32_t>(max(e, 1));
-}
 
 __device__ __forceinline__ float max16(float v) {
 #pragma unroll
@@ -56,23 +38,10 @@ __device__ __forceinline__ float max16(float v) {
 __device__ __forceinline__ uint2 encode_block(const float (&v)[8], uint32_t& byte) {
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float m = fabsf(v[i]);
-    top = fmaxf(top, m < __builtin_inff() ? m : 0.0f);
-  }
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
   byte = scale_byte(max16(top));
-  const float inv = __uint_as_float((254u - byte) << 23);   // 2^(127 - byte); byte is 1..247
-  uint32_t r[2];
-#pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    float q[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) q[i] = fmaf(0.0f, v[4 * h + i], v[4 * h + i] * inv);   // (an infinity: NaN)
-    int p = __builtin_amdgcn_cvt_pk_fp8_f32(q[0], q[1], 0, false);
-    p = __builtin_amdgcn_cvt_pk_fp8_f32(q[2], q[3], p, true);
-    r[h] = static_cast<uint32_t>(p);
-  }
-  return uint2{r[0], r[1]};
+  const float inv = scale_inverse(byte);
+  return uint2{encode4(v, inv), encode4(v + 4, inv)};
 }
 
 // where a lane's codes and, by the block's first lane, its scale go

@@ -78,6 +78,7 @@ SIGNATURES: dict[str, list] = {
     "sa_rows_fp8": [_i, _vp, _vp, _i, _i64, _i, _i64, _i64, _vp, _vp, _vp],
     "sa_rms_norm_fp8": [_i, _vp, _vp, _vp, _i64, _i, _i64, _f, _vp, _vp, _vp, _vp],
     "sa_fp8_linear": [_vp, _vp, _i64, _i, _i, ctypes.POINTER(_i64), _vp],
+    "sa_fp8_linear_bf16": [_vp, _vp, _i, _i, _i64, _i64, _i, ctypes.POINTER(_i64), _vp],
     "sa_fp8_dequant_bf16": [_vp, _vp, _i, _i, _vp, _vp],
     "sa_token_logprobs_workspace_size": [_i64, _i, _i],
     "sa_token_logprobs_fwd": [_i, _vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp,

@@ -13,6 +13,7 @@ from .common import act_dtype_code, call_on, require_device
 CODES, SCALES = torch.float8_e4m3fn, torch.float8_e8m0fnu
 MAX_MATRICES = 4
 MAX_NORM_DIM = 65536
+FEW_ROWS = 16     # bfloat16 rows that the product itself rounds
 
 
 def blocks_of(n: int) -> int:
@@ -80,24 +81,46 @@ def rms_norm(x: torch.Tensor, residual: torch.Tensor | None, weight: torch.Tenso
 _WORDS = [ctypes.c_int64 * (5 * n) for n in range(MAX_MATRICES + 1)]
 
 
-def linear_multi(codes, scales, weights, biases, sizes):
-    """codes, scales of rows (..., 128 blocks); weights [(packed, scales)], biases [(N_i,)
-    bf16 or None], sizes [N_i] -> [(..., N_i) bf16], one launch."""
-    _one_device(codes, scales)
-    lead, Kp = codes.shape[:-1], codes.shape[-1]
+def _matrices(x, lead, weights, biases, sizes):
+    """([y_i], the words of the call, what it keeps alive)."""
     ys, words, kept = [], [], []
     for (packed, ws), b, N in zip(weights, biases, sizes):
-        _one_device(codes, packed, ws, b)
-        y = codes.new_empty((*lead, N), dtype=torch.bfloat16)
+        _one_device(x, packed, ws, b)
+        y = x.new_empty((*lead, N), dtype=torch.bfloat16)
         if b is not None and not b.is_contiguous():
             b = b.contiguous()
             kept.append(b)
         words += (packed.data_ptr(), ws.data_ptr(), 0 if b is None else b.data_ptr(), y.data_ptr(), N)
         ys.append(y)
+    return ys, _WORDS[len(ys)](*words), kept
+
+
+def linear_multi(codes, scales, weights, biases, sizes):
+    """codes, scales of rows (..., 128 blocks); weights [(packed, scales)], biases [(N_i,)
+    bf16 or None], sizes [N_i] -> [(..., N_i) bf16], one launch."""
+    _one_device(codes, scales)
+    Kp = codes.shape[-1]
+    ys, words, _kept = _matrices(codes, codes.shape[:-1], weights, biases, sizes)
     rows = codes.numel() // Kp
     if rows:
-        call_on(codes, "sa_fp8_linear", codes.data_ptr(), scales.data_ptr(), rows, Kp, len(ys),
-                _WORDS[len(ys)](*words), _lib.stream_of(codes))
+        call_on(codes, "sa_fp8_linear", codes.data_ptr(), scales.data_ptr(), rows, Kp, len(ys), words,
+                _lib.stream_of(codes))
+    return ys
+
+
+def linear_multi_bf16(x, xscale, weights, biases, sizes):
+    """The same of x, or x * xscale, (..., K) bf16: up to 16 rows in one launch, more
+    through their codes."""
+    K = x.shape[-1]
+    rows = x.numel() // K
+    if not 0 < rows <= FEW_ROWS:
+        return linear_multi(*quantize_rows(x, xscale), weights, biases, sizes)
+    _one_device(x, xscale)
+    ys, words, _kept = _matrices(x, x.shape[:-1], weights, biases, sizes)
+    xr, ldx = _strided(x, K)
+    gr, ldg = (None, K) if xscale is None else _strided(xscale, K)
+    call_on(x, "sa_fp8_linear_bf16", xr.data_ptr(), None if gr is None else gr.data_ptr(), rows, K, ldx, ldg, len(ys),
+            words, _lib.stream_of(x))
     return ys
 
 

@@ -242,10 +242,10 @@ class _Fp8LinearFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, rows, bias, packed, scales, N):
-        if rows is None:
-            rows = _k.quantize_rows(x, None)
         ctx.save_for_backward(packed, scales)
         ctx.N, ctx.K = N, None if x is None else x.shape[-1]
+        if rows is None:
+            return _k.linear_multi_bf16(x, None, [(packed, scales)], [bias], [N])[0]
         return _k.linear_multi(*rows, [(packed, scales)], [bias], [N])[0]
 
     @staticmethod
@@ -293,9 +293,9 @@ def fp8_linear_multi(x, weights, biases, sizes, xscale: torch.Tensor | None = No
         rows = (codes, scales) if is_rows else None
         return [_Fp8LinearFn.apply(None if is_rows else x, rows, b, *w, N)
                 for w, b, N in zip(weights, biases, sizes)]
-    if not is_rows:
-        codes, scales = _k.quantize_rows(x, xscale)
-    return _k.linear_multi(codes, scales, weights, biases, sizes)
+    if is_rows:
+        return _k.linear_multi(codes, scales, weights, biases, sizes)
+    return _k.linear_multi_bf16(x, xscale, weights, biases, sizes)
 
 
 def fp8_linear(x, packed: torch.Tensor, scales: torch.Tensor, bias: torch.Tensor | None = None,

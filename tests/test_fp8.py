@@ -516,6 +516,27 @@ def test_linear_of_tensors_and_gates(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("M,K", [(1, 1), (1, 1024), (5, 333), (16, 130), (16, 4104), (9, 2048), (17, 500)])
+def test_few_rows_are_rounded_as_by_the_rows_op(M, K, gated):
+    """Up to 16 bf16 rows go through one launch that rounds them itself: the same codes
+    and, at these widths, the same order of sums; on and off 16-byte boundaries, with what
+    is not finite, several matrices and a bias."""
+    wide, other = rand(M, K + 24, seed=M), torch.sigmoid(rand(M, K + 24, seed=3, big=False))
+    if M > 2:
+        wide[1, K // 2 + 8], wide[2, 8] = math.inf, math.nan
+        wide[0] = 0.0
+    ws = [tuple(t.cuda() for t in weight(n, K, seed=n)) for n in (64, 1, 300)]
+    bs = [rand(64, seed=1).cuda(), None, rand(300, seed=2).cuda()]
+    for a, b in ((0, 0), (8, 16), (3, 8), (1, 2)):
+        x, g = wide.cuda()[:, a:a + K], other.cuda()[:, b:b + K] if gated else None
+        want = fp8_linear_multi(quantize_rows_fp8(x, g), ws, bs, [64, 1, 300])
+        for y, v in zip(fp8_linear_multi(x, ws, bs, [64, 1, 300], g), want):
+            assert torch.equal(torch.isnan(y), torch.isnan(v))
+            assert torch.equal(torch.nan_to_num(y), torch.nan_to_num(v))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_linear_multi(M):
     K, sizes = 600, [128, 1, 300, 513]
