@@ -367,7 +367,7 @@ int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zer
  *   scales (rows, 4 ceil(kb / 4)) e8m0 bytes, 2^(byte - 127), 127 behind block kb - 1.
  * sa_rows_fp8: v = x, x * gate (gate not NULL), or with `silu` (bfloat16)
  * x * gate / (1 + e^-gate); x, gate (rows, dim) of `dtype` with row strides ldx, ldg
- * (elements; fastest on 16-byte boundaries and dim a multiple of 8).
+ * (elements).
  * sa_rms_norm_fp8: v = t / sqrt(mean(t^2) + eps) (1 + weight), t = x (row stride ldx), or
  * x + residual in `dtype`, stored to sum (both contiguous, both NULL or neither);
  * weight (dim) float32; dim at most 65536.
@@ -392,9 +392,8 @@ int sa_fp8_linear(const void* codes, const void* scales, int64_t M, int K, int n
                   const int64_t* matrices, void* stream);
 
 /*
- * The same for 1 to 16 rows x (M, K) bf16 with row stride ldx (elements; fastest on
- * 16-byte boundaries, K a multiple of 8), or x * xscale (stride ldg) where xscale is not
- * NULL, which the kernel rounds as sa_rows_fp8 does.
+ * The same for 1 to 16 rows x (M, K) bf16 with row stride ldx (elements), or x * xscale
+ * (stride ldg) where xscale is not NULL, which the kernel rounds as sa_rows_fp8 does.
  */
 int sa_fp8_linear_bf16(const void* x, const void* xscale, int M, int K, int64_t ldx, int64_t ldg,
                        int nseg, const int64_t* matrices, void* stream);

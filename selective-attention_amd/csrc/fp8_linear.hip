@@ -62,22 +62,26 @@ struct Fp8X {
   const void *x, *other;   // codes and scales, or rows and gate
   int64_t ldx, ldg;        // of rows in bfloat16
   int K;
-  bool vec;                // these stand on 16-byte boundaries, K is a multiple of 8
 };
-// sixteen columns of a row from k on, those at or behind K as 0
-__device__ __forceinline__ void load16(uint4 (&q)[2], const bf16* row, int k, int K, bool vec) {
-  if (vec) {   // (uniform)
+// sixteen columns of a row from k on, those at or behind K as 0 (pieces of eight at any
+// address, the row's last by elements)
+typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void load16(uint4 (&q)[2], const bf16* row, int k, int K) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) q[i] = ld16(row + k + 8 * i, k + 8 * i < K);
-  } else {
-    uint32_t w[8];
+  for (int i = 0; i < 2; ++i) {
+    const int at = k + 8 * i;
+    q[i] = uint4{0u, 0u, 0u, 0u};
+    if (at + 8 <= K) {
+      q[i] = __builtin_bit_cast(uint4, *reinterpret_cast<const v4u_any*>(row + at));
+    } else if (at < K) {
+      uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t lo = k + 2 * i < K ? row[k + 2 * i].x : 0u, hi = k + 2 * i + 1 < K ? row[k + 2 * i + 1].x : 0u;
-      w[i] = lo | hi << 16;
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t lo = at + 2 * e < K ? row[at + 2 * e].x : 0u, hi = at + 2 * e + 1 < K ? row[at + 2 * e + 1].x : 0u;
+        w[e] = lo | hi << 16;
+      }
+      q[i] = uint4{w[0], w[1], w[2], w[3]};
     }
-    q[0] = uint4{w[0], w[1], w[2], w[3]};
-    q[1] = uint4{w[4], w[5], w[6], w[7]};
   }
 }
 __device__ __forceinline__ void widen16(float* v, const uint4 (&q)[2]) {
@@ -145,8 +149,8 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const Fp8X in, const F
       } else {
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-          load16(q.x[t][i], xr[t], 128 * kb + 64 * i + 16 * g, in.K, in.vec);
-          if constexpr (X == kGated) load16(q.gate[t][i], gr[t], 128 * kb + 64 * i + 16 * g, in.K, in.vec);
+          load16(q.x[t][i], xr[t], 128 * kb + 64 * i + 16 * g, in.K);
+          if constexpr (X == kGated) load16(q.gate[t][i], gr[t], 128 * kb + 64 * i + 16 * g, in.K);
         }
       }
     }
@@ -165,6 +169,7 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const Fp8X in, const F
         xf = join16(q.x[t][0][0], q.x[t][0][1]);
         sx = q.sx[t];
       } else {
+        // (infinities apart, the codes come straight from the bf16 words, or the products)
         float v[32], top = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i) widen16(v + 16 * i, q.x[t][i]);
@@ -176,12 +181,30 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const Fp8X in, const F
           for (int i = 0; i < 32; ++i) v[i] *= f[i];   // (exact)
         }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) top = fmaxf(top, finite_abs(v[i]));
+        for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));   // (a NaN is passed over)
+        const bool rare = __any(top == __builtin_inff());
+        if (rare) {
+          top = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            v[i] = no_infinity(v[i]);
+            top = fmaxf(top, fabsf(v[i]));
+          }
+        }
         top = fmaxf(top, __shfl_xor(top, 16, 64));
         sx = scale_byte(fmaxf(top, __shfl_xor(top, 32, 64)));
-        const float inv = scale_inverse(sx);
+        const float scale = scale_value(sx);
+        if (X == kGated || rare) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) xf[i] = static_cast<int>(encode4(v + 4 * i, inv));
+          for (int i = 0; i < 8; ++i) xf[i] = static_cast<int>(encode4(v + 4 * i, scale));
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const uint4& u = q.x[t][i >> 1][i & 1];
+            xf[2 * i] = static_cast<int>(encode4(u.x, u.y, scale));
+            xf[2 * i + 1] = static_cast<int>(encode4(u.z, u.w, scale));
+          }
+        }
       }
 #pragma unroll
       for (int r = 0; r < R; ++r) acc[r][t] = mfma_fp8(join16(q.w[r][0], q.w[r][1]), xf, acc[r][t], q.sw[r], sx);
@@ -738,7 +761,7 @@ int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   /
 }
 
 void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
-  const Fp8X in{x, xs, 0, 0, 0, false};
+  const Fp8X in{x, xs, 0, 0, 0};
   // few tiles a CU get deep rings, more of them room beside each other
   float per_cu = 0.0f;
   switch (fp8_shape(sg, M, kb, sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]), &per_cu)) {
@@ -814,7 +837,7 @@ extern "C" int sa_fp8_linear_bf16(const void* x, const void* xscale, int M, int 
                static_cast<long>(ldx), static_cast<long>(ldg), K);
   sa::Fp8Segs sg{};
   if (const int rc = sa::fp8_matrices(who, sg, M, nseg, matrices)) return rc;
-  const sa::Fp8X in{x, xscale, ldx, ldg, K, (at & 15) == 0 && ((ldx | ldg | K) & 7) == 0};
+  const sa::Fp8X in{x, xscale, ldx, ldg, K};
   hipStream_t s = static_cast<hipStream_t>(stream);
   xscale ? sa::fp8_go_bf16<sa::kGated>(in, sg, M, (K + 127) / 128, s)
          : sa::fp8_go_bf16<sa::kBf16>(in, sg, M, (K + 127) / 128, s);

@@ -28,20 +28,22 @@
 namespace sa {
 namespace {
 
-__device__ __forceinline__ float max16(float v) {
-#pragma unroll
-  for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o, 64));
-  return v;
-}
-
 // the block's scale and the lane's eight codes; all 16 lanes of the block are here
-__device__ __forceinline__ uint2 encode_block(const float (&v)[8], uint32_t& byte) {
+__device__ __forceinline__ uint2 encode_block(float (&v)[8], uint32_t& byte) {
   float top = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = fmaxf(top, finite_abs(v[i]));
+  for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));   // (a NaN is passed over)
+  if (__any(top == __builtin_inff())) {
+    top = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      v[i] = no_infinity(v[i]);
+      top = fmaxf(top, fabsf(v[i]));
+    }
+  }
   byte = scale_byte(max16(top));
-  const float inv = scale_inverse(byte);
-  return uint2{encode4(v, inv), encode4(v + 4, inv)};
+  const float scale = scale_value(byte);
+  return uint2{encode4(v, scale), encode4(v + 4, scale)};
 }
 
 // where a lane's codes and, by the block's first lane, its scale go
@@ -57,37 +59,54 @@ __device__ __forceinline__ void put_block(const RowsOut& o, long row, int b, int
   else if (b == o.kb - 1 && l16 < 4 * o.words - b) s[b + l16] = 127;
 }
 
-// eight columns of a row from k on, those at or behind dim as 0.  VEC: dim is a
-// multiple of 8 and rows start on 16-byte boundaries
-template <typename T, bool VEC>
+// eight columns of a row from k on, those at or behind dim as 0: a whole piece by 16-byte
+// accesses at any address (16-byte boundaries are no faster; one element at a time took
+// 3 to 4 times as long), the row's last by elements
+typedef uint32_t v4u_any __attribute__((ext_vector_type(4), aligned(2)));
+typedef float v4f_any __attribute__((ext_vector_type(4), aligned(4)));
+template <typename T>
 __device__ __forceinline__ void load8(float (&v)[8], const T* row, int k, int dim) {
-  if constexpr (VEC) {
-    if (k < dim) {
-      if constexpr (sizeof(T) == 2) {
-        const uint4 q = *reinterpret_cast<const uint4*>(row + k);
-        const uint32_t u[4] = {q.x, q.y, q.z, q.w};
+  if (k + 8 <= dim) {
+    if constexpr (sizeof(T) == 2) {
+      const v4u_any q = *reinterpret_cast<const v4u_any*>(row + k);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          v[2 * i] = bf16lo_to_f32(u[i]);
-          v[2 * i + 1] = bf16hi_to_f32(u[i]);
-        }
-      } else {
-        const float4 a = *reinterpret_cast<const float4*>(row + k), b = *reinterpret_cast<const float4*>(row + k + 4);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+      for (int i = 0; i < 4; ++i) {
+        v[2 * i] = bf16lo_to_f32(q[i]);
+        v[2 * i + 1] = bf16hi_to_f32(q[i]);
       }
-      return;
-    }
+    } else {
+      const v4f_any a = *reinterpret_cast<const v4f_any*>(row + k), b = *reinterpret_cast<const v4f_any*>(row + k + 4);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+      for (int i = 0; i < 4; ++i) {
+        v[i] = a[i];
+        v[4 + i] = b[i];
+      }
+    }
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = k + i < dim ? to_f32(row[k + i]) : 0.0f;
   }
 }
+template <typename T>
+__device__ __forceinline__ void store8(T* row, int k, int dim, const float (&v)[8]) {
+  if (k + 8 <= dim) {
+    if constexpr (sizeof(T) == 2) {
+      *reinterpret_cast<v4u_any*>(row + k) = v4u_any{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
+                                                     pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    } else {
+      *reinterpret_cast<v4f_any*>(row + k) = v4f_any{v[0], v[1], v[2], v[3]};
+      *reinterpret_cast<v4f_any*>(row + k + 4) = v4f_any{v[4], v[5], v[6], v[7]};
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (k + i < dim) row[k + i] = from_f32<T>(v[i]);
+  }
+}
 
 // v = x, x * gate, or x * silu(gate); 16 lanes a block, blocks in order
 enum { kPlain = 0, kGated = 1, kSilu = 2 };
-template <typename T, bool VEC, int MODE>
+template <typename T, int MODE>
 __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, const T* __restrict__ gate, long ldx,
                                                    long ldg, int dim, uint32_t blocks, const RowsOut o) {
   const int l16 = threadIdx.x & 15;
@@ -96,10 +115,10 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
   const uint32_t row = q / static_cast<uint32_t>(o.kb);
   const int b = static_cast<int>(q - row * o.kb), k = kQBlock * b + 8 * l16;
   float v[8];
-  load8<T, VEC>(v, x + row * ldx, k, dim);
+  load8<T>(v, x + row * ldx, k, dim);
   if constexpr (MODE != kPlain) {
     float c[8];
-    load8<T, VEC>(c, gate + row * ldg, k, dim);
+    load8<T>(c, gate + row * ldg, k, dim);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       if constexpr (MODE == kGated) {
@@ -121,37 +140,37 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
   put_block(o, row, b, l16, c, byte);
 }
 
-// 1 / sqrt(ss / dim + eps) as hi + lo: fp32's own, then a Newton step in fp64
-__device__ __forceinline__ void rstd_of(double ss, int dim, float eps, float& hi, float& lo) {
-  const double m = ss / dim + static_cast<double>(eps);
-  const float r = 1.0f / sqrtf(static_cast<float>(m));
-  const double rd = r, r2 = rd * (1.5 - 0.5 * m * rd * rd);
-  const bool fine = r > 0.0f && r < __builtin_inff();   // else a sum beyond fp32 (0), or of zeros with eps 0
-  hi = fine ? static_cast<float>(r2) : r;
-  lo = fine ? static_cast<float>(r2 - static_cast<double>(hi)) : 0.0f;
+// 1 / sqrt(ss inv_dim + eps) as hi + lo: the unit's estimate in fp64 (2^-23 off at
+// most) and one Newton step; 0 for a row with an infinity
+__device__ __forceinline__ void rstd_of(double ss, double inv_dim, float eps, float& hi, float& lo) {
+  const double m = fma(ss, inv_dim, static_cast<double>(eps)), e = __builtin_amdgcn_rsq(m);
+  const double r = m == static_cast<double>(__builtin_inff()) ? 0.0 : e * fma(-0.5 * m, e * e, 1.5);
+  hi = static_cast<float>(r);
+  lo = static_cast<float>(r - static_cast<double>(hi));
 }
 
 // A row stays in registers between its sum of squares and its codes: W waves a row
-// and V pieces of 8 columns a lane (W = 1: four rows a workgroup).  The squares
-// are summed by four in fp32 and then in fp64, which costs two additions for
-// eight columns and leaves the sum exact to a few 2^-28.
-template <typename T, bool VEC, bool RES, int V, int W>
+// and V pieces of 8 columns a lane (W = 1: four rows a workgroup).  The squares are
+// summed in fp64, at fp32's rate but for the widening: in fp32 the row's factor is off
+// by 2^-26, and one code in some 10^7 falls on the wrong side of its tie.
+template <typename T, bool RES, int V, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
     const T* __restrict__ x, const T* __restrict__ res, const float* __restrict__ weight, long rows, long ldx,
-    int dim, float eps, T* __restrict__ sum, const RowsOut o) {
+    int dim, double inv_dim, float eps, T* __restrict__ sum, const RowsOut o) {
   const int tid = threadIdx.x, lane = tid & 63;
   const long row = W == 1 ? blockIdx.x * 4L + (tid >> 6) : static_cast<long>(blockIdx.x);
   const int t = W == 1 ? lane : tid, l16 = tid & 15;
   if (W == 1 && row >= rows) return;   // (whole waves; no barrier below for W = 1)
-  float v[V][8];
-  double ss = 0.0;
+  float v[V][8], w[V][8];
+  double ss = 0.0, s1 = 0.0;
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int k = 8 * (t + 64 * W * j);
-    load8<T, VEC>(v[j], x + row * ldx, k, dim);
+    load8<T>(v[j], x + row * ldx, k, dim);
+    if constexpr (V <= 2) load8<float>(w[j], weight, k, dim);   // (with the row: one latency)
     if constexpr (RES) {
       float r[8];
-      load8<T, VEC>(r, res + row * dim, k, dim);
+      load8<T>(r, res + row * dim, k, dim);
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         if constexpr (sizeof(T) == 2) {
@@ -163,33 +182,16 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
           v[j][i + 1] += r[i + 1];
         }
       }
-      T* out = sum + row * dim + k;
-      if constexpr (VEC) {
-        if (k < dim) {
-          if constexpr (sizeof(T) == 2) {
-            *reinterpret_cast<uint4*>(out) = uint4{pack_bf16x2(v[j][0], v[j][1]), pack_bf16x2(v[j][2], v[j][3]),
-                                                   pack_bf16x2(v[j][4], v[j][5]), pack_bf16x2(v[j][6], v[j][7])};
-          } else {
-            reinterpret_cast<float4*>(out)[0] = make_float4(v[j][0], v[j][1], v[j][2], v[j][3]);
-            reinterpret_cast<float4*>(out)[1] = make_float4(v[j][4], v[j][5], v[j][6], v[j][7]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          if (k + i < dim) out[i] = from_f32<T>(v[j][i]);
-      }
+      store8<T>(sum + row * dim, k, dim, v[j]);
     }
-    float s0 = 0.0f, s1 = 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      s0 = fmaf(v[j][i], v[j][i], s0);
-      s1 = fmaf(v[j][4 + i], v[j][4 + i], s1);
+    for (int i = 0; i < 8; i += 2) {
+      const double a = v[j][i], b = v[j][i + 1];
+      ss = fma(a, a, ss);
+      s1 = fma(b, b, s1);
     }
-    ss += static_cast<double>(s0) + static_cast<double>(s1);
   }
-#pragma unroll
-  for (int s = 32; s > 0; s >>= 1) ss += __shfl_xor(ss, s, 64);
+  ss = wave_sum64(ss + s1);
   if constexpr (W > 1) {
     __shared__ double part[W];
     if (lane == 0) part[tid >> 6] = ss;
@@ -199,19 +201,18 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
     for (int i = 0; i < W; ++i) ss += part[i];
   }
   float hi, lo;
-  rstd_of(ss, dim, eps, hi, lo);
+  rstd_of(ss, inv_dim, eps, hi, lo);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int p = t + 64 * W * j, k = 8 * p, b = p >> 4;
-    float w[8];
-    load8<float, VEC>(w, weight, k, dim);
+    if constexpr (V > 2) load8<float>(w[j], weight, k, dim);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       // (p + e) (g + gl) with p + e = v rstd and g + gl = 1 + w
-      const float g = 1.0f + w[i], gl = w[i] - (g - 1.0f);
+      const float g = 1.0f + w[j][i], gl = w[j][i] - (g - 1.0f);
       const float q = v[j][i] * hi, e = fmaf(v[j][i], hi, -q) + v[j][i] * lo;
       const float c = fmaf(e, g, q * gl), y = fmaf(q, g, c);
-      v[j][i] = k + (VEC ? 0 : i) < dim ? to_odd(y, fmaf(q, g, -y) + c) : 0.0f;
+      v[j][i] = k + i < dim ? to_odd(y, fmaf(q, g, -y) + c) : 0.0f;
     }
     if (b < o.kb) {   // (16 lanes at a time)
       uint32_t byte;
@@ -225,37 +226,38 @@ RowsOut rows_out(void* codes, void* scales, int dim) {
   const int kb = (dim + kQBlock - 1) / kQBlock;
   return RowsOut{static_cast<uint8_t*>(codes), static_cast<uint8_t*>(scales), kb, (kb + 3) / 4};
 }
-bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 template <typename T>
 void rows_go(int mode, const void* x, const void* gate, long ldx, long ldg, int dim, uint32_t blocks, const RowsOut& o,
              hipStream_t s) {
-  constexpr long kAlign = 16 / sizeof(T);
-  const bool vec = dim % 8 == 0 && ldx % kAlign == 0 && on16(x) && (mode == kPlain || (ldg % kAlign == 0 && on16(gate)));
   auto go = [&](auto kern) {
     hipLaunchKernelGGL(kern, dim3((blocks + 15) / 16), dim3(256), 0, s, static_cast<const T*>(x),
                        static_cast<const T*>(gate), ldx, ldg, dim, blocks, o);
   };
-  if (mode == kPlain) vec ? go(rows_kernel<T, true, kPlain>) : go(rows_kernel<T, false, kPlain>);
-  else if (mode == kGated) vec ? go(rows_kernel<T, true, kGated>) : go(rows_kernel<T, false, kGated>);
-  else if constexpr (sizeof(T) == 2) vec ? go(rows_kernel<T, true, kSilu>) : go(rows_kernel<T, false, kSilu>);
+  if (mode == kPlain) go(rows_kernel<T, kPlain>);
+  else if (mode == kGated) go(rows_kernel<T, kGated>);
+  else if constexpr (sizeof(T) == 2) go(rows_kernel<T, kSilu>);
 }
 
-template <typename T, bool VEC, bool RES>
+constexpr long kFewRows = 512;
+template <typename T, bool RES>
 void norm_go(const void* x, const void* res, const float* w, long rows, long ldx, int dim, float eps, void* sum,
              const RowsOut& o, hipStream_t s) {
   auto go = [&](auto kern, int waves) {
     const long grid = waves == 1 ? (rows + 3) / 4 : rows;
     hipLaunchKernelGGL(kern, dim3(grid), dim3(waves == 1 ? 256 : 64 * waves), 0, s, static_cast<const T*>(x),
-                       static_cast<const T*>(res), w, rows, ldx, dim, eps, static_cast<T*>(sum), o);
+                       static_cast<const T*>(res), w, rows, ldx, dim, 1.0 / dim, eps, static_cast<T*>(sum), o);
   };
-  if (dim <= 512) go(rms_norm_fp8_kernel<T, VEC, RES, 1, 1>, 1);
-  else if (dim <= 1024) go(rms_norm_fp8_kernel<T, VEC, RES, 2, 1>, 1);
-  else if (dim <= 2048) go(rms_norm_fp8_kernel<T, VEC, RES, 1, 4>, 4);
-  else if (dim <= 4096) go(rms_norm_fp8_kernel<T, VEC, RES, 2, 4>, 4);
-  else if (dim <= 8192) go(rms_norm_fp8_kernel<T, VEC, RES, 4, 4>, 4);
-  else if (dim <= 16384) go(rms_norm_fp8_kernel<T, VEC, RES, 2, 16>, 16);
-  else go(rms_norm_fp8_kernel<T, VEC, RES, 8, 16>, 16);
+  // few rows are bound by one row's latency, and take more waves for it
+  const bool few = rows <= kFewRows;
+  if (dim <= 512) go(rms_norm_fp8_kernel<T, RES, 1, 1>, 1);
+  else if (dim <= 1024 && !few) go(rms_norm_fp8_kernel<T, RES, 2, 1>, 1);
+  else if (dim <= 2048) go(rms_norm_fp8_kernel<T, RES, 1, 4>, 4);
+  else if (dim <= 8192 && few) go(rms_norm_fp8_kernel<T, RES, 1, 16>, 16);
+  else if (dim <= 4096) go(rms_norm_fp8_kernel<T, RES, 2, 4>, 4);
+  else if (dim <= 8192) go(rms_norm_fp8_kernel<T, RES, 4, 4>, 4);
+  else if (dim <= 16384) go(rms_norm_fp8_kernel<T, RES, 2, 16>, 16);
+  else go(rms_norm_fp8_kernel<T, RES, 8, 16>, 16);
 }
 constexpr int kMaxNormDim = 65536;
 int norm_waves(int dim) { return dim <= 1024 ? 1 : dim <= 8192 ? 4 : 16; }   // (as norm_go)
@@ -316,15 +318,8 @@ extern "C" int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, c
   const sa::RowsOut o = sa::rows_out(codes, scales, dim);
   auto go = [&](auto tag) {
     using T = decltype(tag);
-    const bool vec = dim % 8 == 0 && ldx % (16 / static_cast<long>(sizeof(T))) == 0 && sa::on16(x) &&
-                     sa::on16(residual) && sa::on16(sum) && sa::on16(weight);
-    if (residual) {
-      vec ? sa::norm_go<T, true, true>(x, residual, weight, rows, ldx, dim, eps, sum, o, s)
-          : sa::norm_go<T, false, true>(x, residual, weight, rows, ldx, dim, eps, sum, o, s);
-    } else {
-      vec ? sa::norm_go<T, true, false>(x, residual, weight, rows, ldx, dim, eps, sum, o, s)
-          : sa::norm_go<T, false, false>(x, residual, weight, rows, ldx, dim, eps, sum, o, s);
-    }
+    residual ? sa::norm_go<T, true>(x, residual, weight, rows, ldx, dim, eps, sum, o, s)
+             : sa::norm_go<T, false>(x, residual, weight, rows, ldx, dim, eps, sum, o, s);
   };
   dtype == sa::kF32 ? go(float{}) : go(sa::bf16{});
   SA_CHECK_LAUNCH(who);

@@ -115,8 +115,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: torch.Tensor, eps: float = 1e-6,
                  residual: torch.Tensor | None = None):
     """t rsqrt(mean(t^2) + eps) (1 + weight) in 8 bits, t = x, or x + residual in x's
     dtype: Fp8Rows, with a residual (t, Fp8Rows).  x, residual (..., features) float32
-    or bfloat16, weight (features,).  The squares are summed in fp32's range: a row
-    whose sum passes it gives zeros."""
+    or bfloat16, weight (features,)."""
     dim = _check_rows("rms_norm_fp8", x, residual, "residual")
     if weight.shape != (dim,):
         check_shape(weight, (dim,), name="weight")
