@@ -14,7 +14,7 @@
 // Outputs: codes (rows, 128 kb) with zeros behind dim, scales (rows, 4 ceil(kb / 4))
 // with 127 (2^0) behind block kb - 1: the products read them a word at a time.
 //
-// Rounding: v is computed to within a few 2^-48 (rows, rms_norm; silu_mul 2 2^-24)
+// Rounding: v is computed to within a few 2^-48 (rows, rms_norm; silu_mul 8 2^-24)
 // and rounded to fp32 to odd, so that the one rounding that counts, to e4m3, is that
 // of v itself: rounding to nearest twice would send values next to a tie the wrong way.
 //
@@ -131,7 +131,7 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
         float r = __builtin_amdgcn_rcpf(d);
         r = fmaf(fmaf(-d, r, 1.0f), r, r);
         r = d < __builtin_inff() ? r : 0.0f;   // (c below -88: 0, as with e^-c infinite; no NaN of inf - inf)
-        v[i] = v[i] * c[i] * r;   // (a c is exact)
+        v[i] = v[i] * r * c[i];   // (a c may pass fp32's range where the result does not)
       }
     }
   }

@@ -337,6 +337,18 @@ def test_silu_mul_ends():
 
 
 @pytest.mark.gpu
+def test_silu_mul_where_a_c_passes_fp32():
+    """a c beyond fp32's range, a silu(c) within it; and far gates, whose product is 0."""
+    c = -torch.linspace(0.25, 86, 256).to(torch.bfloat16)[None].repeat(2, 1)
+    a = torch.full_like(c, 2.0 ** 127)
+    a[1] = -a[1]
+    check_silu(silu_mul_fp8(a.cuda(), c.cuda()), a, c)
+    far = torch.full_like(c, -2.0 ** 100)
+    r = silu_mul_fp8(a.cuda(), far.cuda())
+    assert not r.codes.float().any() and (r.scales.float() == 1).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("shape", SHAPES + [(1, 65536), (2, 33000), (513, 1000), (600, 1024), (530, 1999),
