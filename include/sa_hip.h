@@ -403,6 +403,14 @@ int sa_fp8_dequant_bf16(const void* packed, const void* scales, int N, int K, vo
                         void* stream);
 
 /*
+ * The bias's gradient: out (N) bf16 = the sums over the rows of x (M, N) bf16, in fp32
+ * and always in the same order.  workspace: what the function before gives (0: NULL).
+ */
+size_t sa_colsum_bf16_workspace_size(int64_t M, int N);
+int sa_colsum_bf16(const void* x, int64_t M, int N, void* out, void* workspace,
+                   size_t workspace_size, void* stream);
+
+/*
  * Log probabilities of given tokens (no kernel in the reference, which takes
  * softmax and argmax of its logits, models/causal_lm.py:143-221).  logits
  * (rows, vocab) in `dtype` (f32 or bf16) with row stride ld (elements), targets

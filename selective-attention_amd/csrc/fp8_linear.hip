@@ -12,6 +12,10 @@
 // for random numbers by 2^-18 to 2^-20 of it, far below that rounding; the form
 // without the cut, bf16 operands, has half the rate.
 //
+// Three kernels by size (kFp8Shapes): few rows, where the weights' stream and its
+// latency count; a ring of half-steps for what does not fill the card with large tiles;
+// and those.
+//
 // Packed weights: tiles of 16 rows and 128 columns, (N / 16, K / 128, 8, 16, 16)
 // bytes: in a tile, 16 columns of its 16 rows after each other, so that 16 lanes
 // read 256 bytes in a row both from memory and from LDS.  N and K are padded with
@@ -374,7 +378,10 @@ struct Fp8Out {
 // cores take one half, the next is read, also over the steps' border, so that a step
 // needs one barrier, in its middle: there this step's stage has been read by all and
 // the next one has landed.  For large products, 256 by 256 with one wave a SIMD (its
-// sums fill half of the registers): of all shapes it reads LDS the least.
+// sums fill half of the registers): of all shapes it reads LDS the least.  8192 x 8192 x
+// 8192 412 us, 2670 TFLOP/s, with the matrix cores busy in 73 % of the cycles at 1.6 to
+// 1.75 GHz: full of such tiles the card lowers its clock, so that fewer idle cycles do
+// not end it sooner (bank conflicts cut to a tenth: the same time).
 template <int SN, int SM>
 __global__ __launch_bounds__(256, 1) void fp8_large_kernel(const uint8_t* __restrict__ x,
                                                            const uint8_t* __restrict__ xs, const Fp8Segs sg, int M,
@@ -494,9 +501,10 @@ __global__ __launch_bounds__(256, 1) void fp8_large_kernel(const uint8_t* __rest
 // keeps a product where it is written, between the reads and DMA around it
 __device__ __forceinline__ void pin(v16f& c) { asm volatile("" : "+a"(c)::"memory"); }
 
-// The same for fewer rows and columns than fill the card with such tiles.  A step is half a block, in a ring of R stages, R - 1 on their way
-// while one is multiplied: a tile alone on its CU waits for nothing but memory's first
-// answer if the ring is deep, several on a CU cover each other and leave room for fewer stages.
+// The same for fewer rows and columns than fill the card with such tiles.  A step is
+// half a block, in a ring of R stages, R - 1 on their way while one is multiplied: a
+// tile alone on its CU waits for nothing but memory's first answer if the ring is deep,
+// several on a CU cover each other and leave room for fewer stages.
 // x lies in rows of 64 bytes, piece p of row r at p ^ (r / 4 & 3).  The scales' words
 // come with each stage (a load into a register would make the compiler wait for all DMA
 // before its use).
@@ -655,7 +663,8 @@ __global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __res
 }
 
 // the weights in bf16, (N, K) row-major; a code times its scale is a bf16 number
-// (but for scales below 2^-117).  One workgroup a tile and block.
+// (but for scales below 2^-117).  One workgroup a tile and block: 16384 x 16384 143 us,
+// 5.6 TB/s (stores of single elements 497).
 __global__ __launch_bounds__(128) void fp8_dequant_kernel(const uint8_t* __restrict__ W,
                                                           const uint8_t* __restrict__ scale, bf16* __restrict__ out,
                                                           int N, int K, int kb_n) {
@@ -669,12 +678,65 @@ __global__ __launch_bounds__(128) void fp8_dequant_kernel(const uint8_t* __restr
     if (n >= N) continue;
     const uint32_t u[2] = {q.x, q.y};
     bf16* o = out + static_cast<long>(n) * K + k;
+    float v[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float v = __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(u[e >> 2] >> (8 * (e & 3))), 0);
-      if (k + e < K) o[e] = from_f32<bf16>(ldexpf(v, static_cast<int>(byte) - 127));
+    for (int e = 0; e < 8; ++e)
+      v[e] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(static_cast<int>(u[e >> 2] >> (8 * (e & 3))), 0), static_cast<int>(byte) - 127);
+    if (k + 8 <= K) {
+      *reinterpret_cast<v4u_any*>(o) =
+          v4u_any{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (k + e < K) o[e] = from_f32<bf16>(v[e]);
     }
   }
+}
+
+// The bias's gradient: sums over the rows of x (rows, N), in fp32.  A workgroup takes 64
+// columns of `chunk` rows, eight columns a thread (128 bytes of a row, a line) and every
+// 32nd row, whose sums meet in LDS; more chunks than one go to a second pass over their
+// sums, in order.  32768 x 4096 46 us, 5.8 TB/s; 32768 x 1024 15.5, where 256 columns a
+// workgroup and 256 chunks took 47 in the second pass; 4095 columns 119, no row on a line.
+constexpr int kSumCols = 64, kSumRows = 32;
+template <typename TI, typename TO>
+__global__ __launch_bounds__(256) void colsum_kernel(const TI* __restrict__ x, TO* __restrict__ out, long rows, int N,
+                                                     int chunk) {
+  __shared__ float part[kSumRows][kSumCols];
+  const int c = threadIdx.x & 7, g = threadIdx.x >> 3, n = blockIdx.x * kSumCols + 8 * c;
+  const long r0 = static_cast<long>(blockIdx.y) * chunk, r1 = min(rows, r0 + chunk);
+  float acc[8] = {};
+  if (sizeof(TI) == 2 && n + 8 <= N) {
+#pragma unroll 8
+    for (long r = r0 + g; r < r1; r += kSumRows) {
+      const v4u_any q = *reinterpret_cast<const v4u_any*>(x + r * N + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        acc[2 * i] += bf16lo_to_f32(q[i]);
+        acc[2 * i + 1] += bf16hi_to_f32(q[i]);
+      }
+    }
+  } else {
+    for (long r = r0 + g; r < r1; r += kSumRows)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (n + i < N) acc[i] += to_f32(x[r * N + n + i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) part[g][8 * c + i] = acc[i];
+  __syncthreads();
+  const int t = threadIdx.x, col = blockIdx.x * kSumCols + t;
+  if (t >= kSumCols || col >= N) return;
+  float v = 0.0f;
+#pragma unroll
+  for (int i = 0; i < kSumRows; ++i) v += part[i][t];
+  out[static_cast<long>(blockIdx.y) * N + col] = from_f32<TO>(v);
+}
+// rows of a chunk: 64 chunks at most, which the second pass reads in two steps, and
+// enough for the card
+int colsum_chunk(long M, int N) {
+  const long across = (N + kSumCols - 1L) / kSumCols, want = std::min(64L, std::max(1L, 4096 / across));
+  return static_cast<int>(std::max((M + want - 1) / want, 4L * kSumRows));
 }
 
 // tiles of BN columns, all matrices after each other
@@ -856,6 +918,42 @@ extern "C" int sa_fp8_dequant_bf16(const void* packed, const void* scales, int N
   sa::ProfScope prof_("fp8_dequant", s);
   hipLaunchKernelGGL(sa::fp8_dequant_kernel, dim3(blocks), dim3(128), 0, s, static_cast<const uint8_t*>(packed),
                      static_cast<const uint8_t*>(scales), static_cast<sa::bf16*>(out), N, K, static_cast<int>(kb));
+  SA_CHECK_LAUNCH(who);
+  return 0;
+}
+
+extern "C" size_t sa_colsum_bf16_workspace_size(int64_t M, int N) {
+  if (M < 1 || N < 1) return 0;
+  const long chunk = sa::colsum_chunk(M, N), chunks = (M + chunk - 1) / chunk;
+  return chunks > 1 ? static_cast<size_t>(chunks) * N * sizeof(float) : 0;
+}
+
+extern "C" int sa_colsum_bf16(const void* x, int64_t M, int N, void* out, void* workspace, size_t workspace_size,
+                              void* stream) {
+  const char* who = "sa_colsum_bf16";
+  SA_CHECK_ARG(M >= 1 && M <= (1L << 31) && N >= 1 && N <= (1 << 24), "%s: bad sizes M=%ld N=%d", who,
+               static_cast<long>(M), N);
+  SA_CHECK_ARG(x && out, "%s: null pointer", who);
+  SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 1) == 0 &&
+                   (reinterpret_cast<uintptr_t>(workspace) & 3) == 0,
+               "%s: a tensor is not aligned to its type", who);
+  const size_t need = sa_colsum_bf16_workspace_size(M, N);
+  SA_CHECK_ARG(need == 0 || (workspace && workspace_size >= need), "%s: workspace of %zu bytes, %zu needed", who,
+               workspace ? workspace_size : 0, need);
+  const int chunk = sa::colsum_chunk(M, N);
+  const int chunks = static_cast<int>((M + chunk - 1) / chunk), across = (N + sa::kSumCols - 1) / sa::kSumCols;
+  hipStream_t s = static_cast<hipStream_t>(stream);
+  sa::ProfScope prof_("colsum", s);
+  const auto* in = static_cast<const sa::bf16*>(x);
+  auto* o = static_cast<sa::bf16*>(out);
+  auto* ws = static_cast<float*>(workspace);
+  if (chunks == 1) {
+    hipLaunchKernelGGL((sa::colsum_kernel<sa::bf16, sa::bf16>), dim3(across), dim3(256), 0, s, in, o, M, N, chunk);
+  } else {
+    hipLaunchKernelGGL((sa::colsum_kernel<sa::bf16, float>), dim3(across, chunks), dim3(256), 0, s, in, ws, M, N, chunk);
+    hipLaunchKernelGGL((sa::colsum_kernel<float, sa::bf16>), dim3(across), dim3(256), 0, s, ws, o,
+                       static_cast<long>(chunks), N, chunks);
+  }
   SA_CHECK_LAUNCH(who);
   return 0;
 }

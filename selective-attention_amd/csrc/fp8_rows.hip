@@ -18,8 +18,11 @@
 // and rounded to fp32 to odd, so that the one rounding that counts, to e4m3, is that
 // of v itself: rounding to nearest twice would send values next to a tie the wrong way.
 //
-// Streams of memory: 16 lanes a block, 8 columns a lane, the maximum over 16 lanes
-// by four lane exchanges.
+// Streams of memory: 16 lanes a block, 8 columns a lane, so that a block's maximum is
+// four rotations within a row of lanes and its codes leave as 128 bytes.  Large calls
+// run at the rate of a copy (5.1 TB/s): silu_mul 32768 x 4096 120 us, 5.6 TB/s; norm
+// with residual 32768 x 1024 46.7 us, 5.0; rows 8191 x 2056 10.3 us, 4.9.  Few rows are
+// one latency after another: 4 rows 2.3 to 3.4 us, and the call's host time above that.
 #include "fp8.h"
 #include "prof.h"
 
@@ -248,7 +251,9 @@ void norm_go(const void* x, const void* res, const float* w, long rows, long ldx
     hipLaunchKernelGGL(kern, dim3(grid), dim3(waves == 1 ? 256 : 64 * waves), 0, s, static_cast<const T*>(x),
                        static_cast<const T*>(res), w, rows, ldx, dim, 1.0 / dim, eps, static_cast<T*>(sum), o);
   };
-  // few rows are bound by one row's latency, and take more waves for it
+  // few rows are bound by one row's latency, and take more waves for it: with fewer 1 row
+  // of 1024 takes 3.5 us, so 2.7, 1 of 8192 6.4 and 3.8, 512 of 1024 4.9 and 4.0, 512 of 4096
+  // 6.3 and 6.5; more rows fill the card either way, and one wave a row needs no barrier
   const bool few = rows <= kFewRows;
   if (dim <= 512) go(rms_norm_fp8_kernel<T, RES, 1, 1>, 1);
   else if (dim <= 1024 && !few) go(rms_norm_fp8_kernel<T, RES, 2, 1>, 1);

@@ -80,6 +80,8 @@ SIGNATURES: dict[str, list] = {
     "sa_fp8_linear": [_vp, _vp, _i64, _i, _i, ctypes.POINTER(_i64), _vp],
     "sa_fp8_linear_bf16": [_vp, _vp, _i, _i, _i64, _i64, _i, ctypes.POINTER(_i64), _vp],
     "sa_fp8_dequant_bf16": [_vp, _vp, _i, _i, _vp, _vp],
+    "sa_colsum_bf16_workspace_size": [_i64, _i],
+    "sa_colsum_bf16": [_vp, _i64, _i, _vp, _vp, _sz, _vp],
     "sa_token_logprobs_workspace_size": [_i64, _i, _i],
     "sa_token_logprobs_fwd": [_i, _vp, _i64, _vp, _i64, _i, _i, _i64, _vp, _vp, _vp, _vp, _vp, _vp,
                               _sz, _vp],
@@ -113,6 +115,7 @@ RESTYPES = {"sa_last_error": ctypes.c_char_p, "sa_profile_enable": None, "sa_ssd
             "sa_paged_decode_fp8_workspace_size": ctypes.c_size_t,
             "sa_paged_decode_noalloc_limit": ctypes.c_size_t,
             "sa_token_logprobs_workspace_size": ctypes.c_size_t,
+            "sa_colsum_bf16_workspace_size": ctypes.c_size_t,
             "sa_ssm_conv_bwd_workspace_size": ctypes.c_size_t,
             "sa_ssm_gate_bwd_workspace_size": ctypes.c_size_t,
             "sa_score_stats_workspace_size": ctypes.c_size_t,

@@ -131,3 +131,18 @@ def dequantize(packed, scales, N: int, K: int):
     call_on(packed, "sa_fp8_dequant_bf16", packed.data_ptr(), scales.data_ptr(), N, K, out.data_ptr(),
             _lib.stream_of(packed))
     return out
+
+
+def column_sums(x: torch.Tensor):
+    """(N,) bf16: the sums over all rows of x (..., N) bf16, in fp32."""
+    require_device(x)
+    N = x.shape[-1]
+    x = x.contiguous()
+    M = x.numel() // N
+    if not M:
+        return x.new_zeros(N)
+    out = x.new_empty(N)
+    need = _lib.load().sa_colsum_bf16_workspace_size(M, N)
+    ws = x.new_empty(need, dtype=torch.uint8) if need else None
+    call_on(x, "sa_colsum_bf16", x.data_ptr(), M, N, out.data_ptr(), _lib.ptr(ws), need, _lib.stream_of(x))
+    return out

@@ -14,7 +14,8 @@ become NaN codes, which make their row's outputs NaN and no other's.  fp8_linear
 takes such Fp8Rows, or a bfloat16 tensor that it rounds itself; a row's outputs do
 not depend on the rows beside it, but for the order of fp32 sums.  It is
 differentiable in x (a tensor) and bias: the gradient passes the rounding as it
-is, dx = dy W with W the weights that the codes stand for, in bfloat16.
+is, dx = dy W with W the weights that the codes stand for, in bfloat16 (x times xscale
+is then rounded to bfloat16 before its codes).
 
 New ops (the reference's layers are nn.Linear in the model's dtype,
 modules/feed_forward.py:4-11, behind modules/rms_norm.py:4-44).
@@ -35,8 +36,8 @@ _BYTES = (SCALES, torch.uint8)
 class Fp8Rows:
     """Rows in 8 bits: codes (..., 128 blocks) float8_e4m3fn, zeros behind the last
     feature, and scales (..., 4 ceil(blocks / 4)) float8_e8m0fnu (or its bytes, uint8),
-    of which those behind the last block are not used.  shape and dtype are those of
-    the tensor that the rows stand for."""
+    of which those behind the last block are not used.  shape is that of the tensor
+    that the rows stand for, dtype bfloat16, that of the layers."""
 
     __slots__ = ("codes", "scales", "features")
 
@@ -254,7 +255,7 @@ class _Fp8LinearFn(torch.autograd.Function):
             w = _k.dequantize(*ctx.saved_tensors, ctx.N, ctx.K)
             dx = (dy.reshape(-1, ctx.N) @ w).view(*dy.shape[:-1], ctx.K)
         if ctx.needs_input_grad[2]:
-            db = dy.float().reshape(-1, ctx.N).sum(0).to(torch.bfloat16)
+            db = _k.column_sums(dy)
         return dx, None, db, None, None, None
 
 

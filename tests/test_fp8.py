@@ -649,6 +649,54 @@ def test_gradients_are_the_formulas(M):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(1, 1), (7, 33), (64, 300), (65, 256), (3, 700, 257), (20000, 300), (70000, 5), (300, 70000)])
+def test_bias_gradient(shape):
+    """M numbers summed in fp32 (each addition off by half an ulp of at most the
+    magnitudes' sum), rounded once."""
+    N, M = shape[-1], math.prod(shape[:-1])
+    packed, scales = (t.cuda() for t in weight(N, 1))
+    b, dy = torch.zeros(N, dtype=torch.bfloat16, device="cuda").requires_grad_(), rand(*shape, seed=4, big=False)
+    x = torch.ones(*shape[:-1], 1, dtype=torch.bfloat16, device="cuda")
+    y = fp8_linear(x, packed, scales, b, out_features=N)
+    (db,) = torch.autograd.grad(y, b, dy.cuda(), retain_graph=True)
+    d = dy.double().reshape(M, N)
+    want = d.sum(0)
+    assert ((db.cpu().double() - want).abs() <= M * 2.0 ** -24 * d.abs().sum(0) + 2.0 ** -8 * want.abs()).all()
+    assert torch.equal(db, torch.autograd.grad(y, b, dy.cuda(), retain_graph=True)[0])
+    (db,) = torch.autograd.grad(y.sum(), b)      # (a gradient of one number in all places)
+    assert torch.equal(db, torch.full_like(db, M))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [12, 6000])
+def test_gradients_captured(M):
+    """A captured forward and backward, replayed on new inputs with eager work between."""
+    K, N = 256, 384
+    packed, scales = (t.cuda() for t in weight(N, K))
+    x, b, dy = rand(M, K, big=False).cuda().requires_grad_(), rand(N, big=False).cuda().requires_grad_(), rand(M, N, seed=1).cuda()
+
+    def run(x, b, dy):
+        return torch.autograd.grad(fp8_linear(x, packed, scales, b, out_features=N), (x, b), dy)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(x, b, dy)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out = run(x, b, dy)
+    for turn in range(4):
+        with torch.no_grad():
+            x.copy_(rand(M, K, seed=10 + turn, big=False))
+            dy.copy_(rand(M, N, seed=20 + turn))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(x.detach().clone().requires_grad_(), b.detach().clone().requires_grad_(), dy.clone())
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, w) for o, w in zip(out, want))
+
+
+@pytest.mark.gpu
 def test_gradient_is_the_difference():
     """Where x and x + d are both codes (whole numbers to 8, 448 in each block so that
     the scale is 1), the layer is linear in x and its difference is the gradient's:
