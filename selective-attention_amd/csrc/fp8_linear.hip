@@ -505,36 +505,46 @@ __device__ __forceinline__ void pin(v16f& c) { asm volatile("" : "+a"(c)::"memor
 // half a block, in a ring of R stages, R - 1 on their way while one is multiplied: a
 // tile alone on its CU waits for nothing but memory's first answer if the ring is deep,
 // several on a CU cover each other and leave room for fewer stages.
-// x lies in rows of 64 bytes, piece p of row r at p ^ (r / 4 & 3).  The scales' words
-// come with each stage (a load into a register would make the compiler wait for all DMA
-// before its use).
-template <int SN, int SM, int R, int OCC>
-__global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __restrict__ x,
-                                                            const uint8_t* __restrict__ xs, const Fp8Segs sg, int M,
-                                                            int kb_n, int mtiles) {
-  constexpr int BN = 64 * SN, BM = 64 * SM, kW = BN * 64, kOps = (BN + BM) * 64, kStage = kOps + 1024;
-  constexpr int kParts = (BN + BM) / 16, kDmas = (kParts + 3) / 4 + 1;   // DMA instructions of operands, and all of a wave
-  static_assert(BM <= 128 && BN <= 256, "a stage's scales: two waves' rows, one's columns");
-  static_assert((R - 1) * kDmas < 63, "vmcnt counts them");
+// x lies in rows of 64 bytes, piece p of row r at p ^ (r / 4 & 3).  The scales' words come
+// with every eighth half-step, into two places in turn (a load into a register would make
+// the compiler wait for all DMA before its use; with every half-step they took more of
+// the cache's time than the operands, each row's word being a line of its own: 1000 rows,
+// 11008 -> 4096 59 us, so 47).
+// KS = 2: eight waves, a ring and one half of K for each four, whose sums meet in LDS:
+// small tiles wait less than their operands take (512 rows, 4096 -> 1024: 12.4 us, so 11.1).
+template <int SN, int SM, int R, int OCC, int KS>
+__global__ __launch_bounds__(256 * KS, OCC * KS) void fp8_ring_kernel(const uint8_t* __restrict__ x,
+                                                                      const uint8_t* __restrict__ xs, const Fp8Segs sg,
+                                                                      int M, int kb_n, int mtiles) {
+  constexpr int BN = 64 * SN, BM = 64 * SM, kW = BN * 64, kStage = (BN + BM) * 64;
+  constexpr int kScales = R * kStage, kRing = kScales + 2048, kSums = SN * SM * 4096;   // (a wave's sums, in bytes)
+  constexpr int kParts = (BN + BM) / 16, kDmas = (kParts + 3) / 4;   // DMA instructions of a stage, and of a wave
+  static_assert(BM <= 128 && BN <= 256, "a word's scales: two waves' rows, one's columns");
+  static_assert(R >= 3 && R <= 8, "the word after the next comes when the last half-step of this one has been read");
+  static_assert((R - 1) * kDmas + 1 < 63, "vmcnt counts them");
   using Out = Fp8Out<SN, SM>;
   static_assert(4 * Out::kBytes <= R * kStage, "y fits the stages");
-  __shared__ __align__(16) uint8_t smem[R * kStage + 4 * BN];
-  float* bias_lds = reinterpret_cast<float*>(smem + R * kStage);
+  static_assert(KS == 1 || (KS == 2 && 4 * kSums <= KS * kRing && Out::kBytes <= kSums), "sums and y fit the rings");
+  __shared__ __align__(16) uint8_t smem[KS * kRing + 4 * BN];
+  float* bias_lds = reinterpret_cast<float*>(smem + KS * kRing);
   const int tid = threadIdx.x, lane = tid & 63, c = lane & 31, h = lane >> 5;
-  const int wid = __builtin_amdgcn_readfirstlane(tid >> 6), wn = wid & 1, wm = wid >> 1;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), part = wave >> 2, wid = wave & 3, wn = wid & 1, wm = wid >> 1;
   const Fp8Tile tile = tile_of<BN, BM>(sg, mtiles);
   const int N = sg.N[tile.seg], n0 = tile.n0, m0 = tile.m0, nw = n0 + wn * 32 * SN, mw = m0 + wm * 32 * SM;
   const bf16* bias = sg.bias[tile.seg];
   if (tid < BN) bias_lds[tid] = bias && n0 + tid < N ? to_f32(bias[n0 + tid]) : 0.0f;
 
-  // part q of a stage: half a tile of W, or sixteen rows of x; wave w takes w, w + 4, ..
-  // (a part too many is the last again, at the same place)
-  const uint32_t ls = lds_addr(smem);
+  // the half-steps u0 to U - 1 of this part of the waves
+  const int most = 2 * ((kb_n + KS - 1) / KS), u0 = part * most, U = min(u0 + most, 2 * kb_n);
+  // piece q of a stage: half a tile of W, or sixteen rows of x; wave w takes w, w + 4, ..
+  // (a piece too many is the last again, at the same place)
+  uint8_t* ring = smem + part * kRing;
+  const uint32_t ls = lds_addr(ring);
   const uint8_t* d_w = sg.W[tile.seg] + static_cast<long>(n0 >> 4) * kb_n * 2048;
   const uint8_t* d_x = x + static_cast<long>(m0) * kb_n * 128;
-  uint32_t off[kDmas];
+  uint32_t off[kDmas], s_off;
 #pragma unroll
-  for (int i = 0; i < kDmas - 1; ++i) {
+  for (int i = 0; i < kDmas; ++i) {
     const int q = min(wid + 4 * i, kParts - 1);
     off[i] = q < BN / 16 ? static_cast<uint32_t>(min(q, ((N + 15) >> 4) - 1 - (n0 >> 4))) * kb_n * 2048 + lane * 16
                          : static_cast<uint32_t>(min((q - BN / 16) * 16 + (lane >> 2), M - 1 - m0)) * kb_n * 128 +
@@ -545,21 +555,24 @@ __global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __res
   const uint8_t* d_s;
   if (wid < 2) {
     d_s = xs + static_cast<long>(m0) * 4 * words;
-    off[kDmas - 1] = static_cast<uint32_t>(min(64 * wid + lane, M - 1 - m0)) * 4 * words;
+    s_off = static_cast<uint32_t>(min(64 * wid + lane, M - 1 - m0)) * 4 * words;
   } else {
     d_s = sg.scale[tile.seg] + static_cast<long>(n0 >> 7) * 4 * words;
-    off[kDmas - 1] = static_cast<uint32_t>((min(n0 + 32 * min(lane, BN / 32 - 1), N - 1) >> 7) - (n0 >> 7)) * 4 * words;
+    s_off = static_cast<uint32_t>((min(n0 + 32 * min(lane, BN / 32 - 1), N - 1) >> 7) - (n0 >> 7)) * 4 * words;
   }
-  int d_u = 0;
+  d_w += static_cast<long>(u0) * 1024;
+  d_x += static_cast<long>(u0) * 64;
+  int d_u = u0;
+  auto word_at = [&](int u) __attribute__((always_inline)) { return ((u >> 3) & 1) * 1024; };
   auto dma = [&](int i, uint32_t stage) __attribute__((always_inline)) {
     const int q = min(wid + 4 * i, kParts - 1);
-    if (i < kDmas - 1) dma_lds16(q < BN / 16 ? d_w : d_x, off[i], stage + (q << 10));
-    else if (i == kDmas - 1) dma_lds4(d_s, off[i], stage + kOps + (wid << 8));
+    if (i == 0 && ((d_u & 7) == 0 || (KS > 1 && d_u == u0)))
+      dma_lds4(d_s + (d_u >> 3) * 4, s_off, ls + kScales + word_at(d_u) + (wid << 8));
+    if (i < kDmas) dma_lds16(q < BN / 16 ? d_w : d_x, off[i], stage + (q << 10));
   };
   auto advance = [&]() __attribute__((always_inline)) {
     d_w += 1024;
     d_x += 64;
-    d_s += (d_u & 7) == 7 ? 4 : 0;
     ++d_u;
   };
 
@@ -567,40 +580,39 @@ __global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __res
   int xa[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i) xa[i] = kW + wm * SM * 2048 + c * 64 + (((2 * h + i) ^ ((c >> 2) & 3)) * 16);
-  const int sxa = kOps + (wm * SM * 32 + c) * 4, swa = kOps + 512 + wn * SN * 4;
+  const int sxa = kScales + (wm * SM * 32 + c) * 4, swa = kScales + 512 + wn * SN * 4;
   v8i fw[2][SN], fx[2][SM];
   uint32_t sw[2], sx[2][SM];
-  auto read_frag = [&](int half, int r, int stage) __attribute__((always_inline)) {
+  auto read_frag = [&](int half, int r, int stage, int word) __attribute__((always_inline)) {
     if (r == 0) {
-      sw[half] = *reinterpret_cast<const uint32_t*>(smem + stage + swa);
+      sw[half] = *reinterpret_cast<const uint32_t*>(ring + word + swa);
 #pragma unroll
-      for (int j = 0; j < SM; ++j) sx[half][j] = *reinterpret_cast<const uint32_t*>(smem + stage + sxa + 128 * j);
+      for (int j = 0; j < SM; ++j) sx[half][j] = *reinterpret_cast<const uint32_t*>(ring + word + sxa + 128 * j);
     }
     if (r == 0 || (r > SM && r < SN + SM)) {
       const int s = r == 0 ? 0 : r - SM;
-      const uint8_t* p = smem + stage + wa + s * 2048;
+      const uint8_t* p = ring + stage + wa + s * 2048;
       fw[half][s] = lds_frag(p, p + 256);
     } else if (r <= SM) {
-      const uint8_t* p = smem + stage + (r - 1) * 2048;
+      const uint8_t* p = ring + stage + (r - 1) * 2048;
       fx[half][r - 1] = lds_frag(p + xa[0], p + xa[1]);
     }
   };
-  // all but the newest n stages of DMA have landed, and the wave's reads
+  // all but the newest n stages of DMA have landed, and the wave's reads (a scales' word
+  // among the newest, not counted, lets one piece less be on its way)
   auto landed = [&](int n) __attribute__((always_inline)) {
     switch (n) {
 #define SA_FP8_WAIT(k) \
   case k: \
     if constexpr (k < R - 1) __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<(k < R - 1 ? k : 0) * kDmas>()); \
     break;
-      SA_FP8_WAIT(1) SA_FP8_WAIT(2) SA_FP8_WAIT(3) SA_FP8_WAIT(4) SA_FP8_WAIT(5) SA_FP8_WAIT(6) SA_FP8_WAIT(7)
-      SA_FP8_WAIT(8) SA_FP8_WAIT(9) SA_FP8_WAIT(10)
+      SA_FP8_WAIT(1) SA_FP8_WAIT(2) SA_FP8_WAIT(3) SA_FP8_WAIT(4) SA_FP8_WAIT(5) SA_FP8_WAIT(6)
 #undef SA_FP8_WAIT
       default: __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<0>());
     }
   };
-  static_assert(R >= 3 && R <= 12, "landed counts to R - 2");
 
-  const int U = 2 * kb_n, filled = min(U, R);
+  const int filled = min(U - u0, R);
   v16f acc[SN][SM] = {};
   for (int s = 0; s < filled; ++s) {
 #pragma unroll
@@ -610,17 +622,18 @@ __global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __res
   landed(filled - 2);   // (at least two)
   lds_barrier();
 #pragma unroll
-  for (int r = 0; r < SN + SM; ++r) read_frag(0, r, 0);
+  for (int r = 0; r < SN + SM; ++r) read_frag(0, r, 0, word_at(u0));
   __builtin_amdgcn_s_waitcnt(kLgkmWait0);
   lds_barrier();
 
   // half-step u on stage cur, whose operands are in registers and which all have read:
   // those of u + 1 are read, stage cur takes half-step u + R
-  int cur = 0, u = 0;
+  int cur = 0, u = u0;
   auto half_step = [&](auto half, auto more) __attribute__((always_inline)) {
     constexpr int HF = decltype(half)::value;
     constexpr bool MORE = decltype(more)::value;
     const int shift = (u >> 1 & 3) * 8;   // the block's byte
+    const int word = word_at(u + 1);
     const int oth = cur == (R - 1) * kStage ? 0 : cur + kStage;
     constexpr int kSlots = SN * SM, kReads = (SN + SM + kSlots - 1) / kSlots, kPer = (kDmas + kSlots - 1) / kSlots;
 #pragma unroll
@@ -629,7 +642,7 @@ __global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __res
       acc[i][j] = mfma_fp8(fw[HF][i], fx[HF][j], acc[i][j], sw[HF] >> shift, sx[HF][j] >> shift);
       pin(acc[i][j]);
 #pragma unroll
-      for (int r = k * kReads; r < (k + 1) * kReads; ++r) read_frag(HF ^ 1, r, oth);   // (of the last: not used)
+      for (int r = k * kReads; r < (k + 1) * kReads; ++r) read_frag(HF ^ 1, r, oth, word);   // (of the last: not used)
       if constexpr (MORE) {
 #pragma unroll
         for (int d = k * kPer; d < (k + 1) * kPer; ++d) dma(d, ls + cur);
@@ -659,7 +672,29 @@ __global__ __launch_bounds__(256, OCC) void fp8_ring_kernel(const uint8_t* __res
     half_step(h0{}, no{});
     half_step(h1{}, no{});
   }
-  Out::store(acc, smem + wid * Out::kBytes, bias_lds + wn * 32 * SN, sg.y[tile.seg], nw, mw, N, M);
+  if constexpr (KS > 1) {
+    for (int i = U - u0; i < most; ++i) lds_barrier();   // (as many as the other part)
+    float4* sums = reinterpret_cast<float4*>(smem + wid * kSums) + lane;
+    if (part) {
+#pragma unroll
+      for (int i = 0; i < SN * SM * 4; ++i) {
+        const v16f& a = acc[i / 4 / SM][i / 4 % SM];
+        sums[64 * i] = make_float4(a[i % 4 * 4], a[i % 4 * 4 + 1], a[i % 4 * 4 + 2], a[i % 4 * 4 + 3]);
+      }
+    }
+    __syncthreads();
+    if (part) return;
+#pragma unroll
+    for (int i = 0; i < SN * SM * 4; ++i) {
+      const float4 b = sums[64 * i];
+      v16f& a = acc[i / 4 / SM][i / 4 % SM];
+      a[i % 4 * 4] += b.x;
+      a[i % 4 * 4 + 1] += b.y;
+      a[i % 4 * 4 + 2] += b.z;
+      a[i % 4 * 4 + 3] += b.w;
+    }
+  }
+  Out::store(acc, smem + wid * (KS > 1 ? kSums : Out::kBytes), bias_lds + wn * 32 * SN, sg.y[tile.seg], nw, mw, N, M);
 }
 
 // the weights in bf16, (N, K) row-major; a code times its scale is a bf16 number
@@ -759,43 +794,43 @@ void fp8_large(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStr
   hipLaunchKernelGGL((fp8_large_kernel<SN, SM>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
 }
-template <int SN, int SM, int R, int OCC>
+template <int SN, int SM, int R, int OCC, int KS = 1>
 void fp8_ring(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   cut_tiles(sg, 64 * SN);
   const int mtiles = (M + 64 * SM - 1) / (64 * SM);
   ProfScope prof_("fp8_ring", s);
-  hipLaunchKernelGGL((fp8_ring_kernel<SN, SM, R, OCC>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256), 0, s,
+  hipLaunchKernelGGL((fp8_ring_kernel<SN, SM, R, OCC, KS>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256 * KS), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
 }
 
 // The kernel by the sizes: the least estimate in us, of kb blocks of K, of
 //   tiles <= 256      first(kb), one tile on each CU
 //   more              again + (tiles / 256, between itself and its ceiling) each(kb)
-// fitted to 60 products of 1 to 32768 rows, K 1024 to 11008, N 1024 to 32000; the choice
-// was at most 12 % behind the best of all (linear8 in us, tiles of fp8_few, fp8_ring and
-// fp8_large as rows x columns):
-//   1 row, 1024 -> 1024       16 x 16 3.4   16 x 64 3.7    64 x 64 5.3
-//   64 rows, 4096 -> 4096     16 x 16 15.3  16 x 64 8.1    64 x 64 11.7
-//   200 rows, 8192 -> 1024    16 x 16 25.6  16 x 64 12.6   64 x 64 21.9
-//   32 rows, 4096 -> 32000    16 x 32 42.8  64 x 64 30.3   64 x 128 25.5
-//   500 rows, 1024 -> 4384    32 x 64 24.5  64 x 64 8.2    128 x 128 8.3   256 x 256 16.6
-//   4000 rows, 1024 -> 4384   64 x 64 36    128 x 128 25.8 128 x 256 28.4  256 x 256 34.6
-//   8192 rows, 4096 -> 4096   128 x 128 156 256 x 256 105
+// fitted to 88 products of 1 to 32768 rows, K 1024 to 11008, N 1024 to 32000; the choice
+// was at most 7 % behind the best of all, 0.3 % on average (linear8 in us, tiles of
+// fp8_few, fp8_ring and fp8_large as rows x columns):
+//   1 row, 1024 -> 1024       16 x 16 3.5   16 x 64 3.7    64 x 64 5.1
+//   64 rows, 4096 -> 4096     16 x 16 15.5  16 x 64 8.2    64 x 64 11.0
+//   200 rows, 8192 -> 1024    16 x 16 25.5  16 x 64 12.8   64 x 64 18.4
+//   32 rows, 4096 -> 32000    16 x 32 43.2  64 x 64 28.5   64 x 128 25.5
+//   500 rows, 2050 -> 4383    32 x 64 35.7  64 x 64 14.6   128 x 128 13.7  256 x 256 30.4
+//   4000 rows, 1024 -> 4384   64 x 64 35.7  128 x 128 25.2 128 x 256 28.2  256 x 256 35.3
+//   8192 rows, 4096 -> 4096   128 x 128 138 128 x 256 112  256 x 256 105
 struct Fp8Shape {
   int bm, bn;
   float first0, first1, again, each0, each1;
 };
 constexpr int kFp8Few = 4;   // shapes of fp8_few, then tiles
 constexpr Fp8Shape kFp8Shapes[] = {
-    {16, 16, 2.6f, 0.106f, 1.5f, 0.8f, 0.0725f},
-    {16, 32, 2.5f, 0.119f, 1.5f, 1.0f, 0.115f},
-    {16, 64, 2.8f, 0.146f, 1.5f, 4.4f, 0.0625f},
-    {32, 64, 3.9f, 0.2125f, 1.6f, 1.9f, 0.2375f},
-    {64, 64, 3.0f, 0.30f, 4.0f, -0.2f, 0.255f},
-    {64, 128, 3.0f, 0.40f, 4.0f, -0.2f, 0.39f},
-    {128, 128, 3.0f, 0.60f, 2.9f, 0.5f, 0.58f},
-    {128, 256, 4.0f, 0.93f, 5.3f, 1.3f, 0.87f},
-    {256, 256, 8.0f, 1.06f, 8.0f, 5.0f, 1.48f},   // (full of such tiles the card is bound by power)
+    {16, 16, 3.2f, 0.066f, 1.58f, 0.67f, 0.072f},
+    {16, 32, 3.0f, 0.094f, 2.2f, 0.79f, 0.106f},
+    {16, 64, 3.04f, 0.141f, 0.7f, 4.1f, 0.125f},
+    {32, 64, 3.84f, 0.212f, 1.6f, 1.9f, 0.2f},
+    {64, 64, 3.5f, 0.223f, 3.5f, -0.19f, 0.258f},
+    {64, 128, 4.0f, 0.308f, 4.3f, 0.02f, 0.353f},
+    {128, 128, 4.76f, 0.441f, 3.63f, 0.16f, 0.552f},
+    {128, 256, 8.05f, 0.754f, 4.67f, 1.83f, 0.812f},
+    {256, 256, 8.0f, 1.06f, 2.15f, 6.71f, 1.45f},   // (full of such tiles the card is bound by power)
 };
 int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   // of the first `shapes`
   constexpr int kShapes = sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]);
@@ -824,15 +859,15 @@ int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   /
 
 void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   const Fp8X in{x, xs, 0, 0, 0};
-  // few tiles a CU get deep rings, more of them room beside each other
+  // few tiles a CU get deep rings (the smallest eight waves), more of them room beside each other
   float per_cu = 0.0f;
   switch (fp8_shape(sg, M, kb, sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]), &per_cu)) {
     case 0: return fp8_few<1, 1, 8, kCodes>(in, sg, M, kb, s);
     case 1: return fp8_few<1, 2, 8, kCodes>(in, sg, M, kb, s);
     case 2: return fp8_few<1, 4, 8, kCodes>(in, sg, M, kb, s);
     case 3: return fp8_few<2, 4, 8, kCodes>(in, sg, M, kb, s);
-    case 4: return per_cu <= 2.0f ? fp8_ring<1, 1, 8, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
-    case 5: return per_cu <= 2.0f ? fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 1, 3, 4>(x, xs, sg, M, kb, s);
+    case 4: return per_cu <= 1.0f ? fp8_ring<1, 1, 4, 2, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
+    case 5: return fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s);
     case 6: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
     case 7: return fp8_ring<4, 2, 3, 2>(x, xs, sg, M, kb, s);
     default: return fp8_large<4, 4>(x, xs, sg, M, kb, s);

@@ -446,7 +446,9 @@ TILES = [(61, 4000, [4090], "few"), (120, 3970, [1800, 1, 1000, 1090], "few"), (
          (700, 4200, [1111], "ring"), (70000, 128, [64], "ring"), (8100, 1024, [4384], "ring"),
          (4100, 1408, [4097], "ring"), (8192, 2100, [4104], "ring"), (4095, 4096, [4095], "large"),
          (300, 640, [128, 1, 1000, 333], "ring"), (4096, 2048, [1111, 2000, 77, 900], "ring"), (2040, 6000, [2000, 1027, 77, 900], "large"),
-         (3000, 1, [5000], "ring"), (5000, 130, [5001], "ring")]
+         (3000, 1, [5000], "ring"), (5000, 130, [5001], "ring"), (300, 100, [1111], "ring"), (900, 300, [900], "ring"),
+         (129, 2100, [30001], "ring"), (200, 1300, [9000, 5000], "ring"), (70, 1500, [37000], "ring"), (3000, 5000, [1030], "ring"),
+         (4, 1204, [36073], "ring"), (720, 714, [1933], "ring")]
 
 
 @pytest.mark.gpu
