@@ -511,7 +511,8 @@ __device__ __forceinline__ void pin(v16f& c) { asm volatile("" : "+a"(c)::"memor
 // the cache's time than the operands, each row's word being a line of its own: 1000 rows,
 // 11008 -> 4096 59 us, so 47).
 // KS = 2: eight waves, a ring and one half of K for each four, whose sums meet in LDS:
-// small tiles wait less than their operands take (512 rows, 4096 -> 1024: 12.4 us, so 11.1).
+// small tiles wait less than their operands take (512 rows, 4096 -> 1024: 12.4 us, so 11.1;
+// below eight blocks a half is too short, 512 -> 1024: 4.5, so 4.9).
 template <int SN, int SM, int R, int OCC, int KS>
 __global__ __launch_bounds__(256 * KS, OCC * KS) void fp8_ring_kernel(const uint8_t* __restrict__ x,
                                                                       const uint8_t* __restrict__ xs, const Fp8Segs sg,
@@ -806,8 +807,8 @@ void fp8_ring(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStre
 // The kernel by the sizes: the least estimate in us, of kb blocks of K, of
 //   tiles <= 256      first(kb), one tile on each CU
 //   more              again + (tiles / 256, between itself and its ceiling) each(kb)
-// fitted to 88 products of 1 to 32768 rows, K 1024 to 11008, N 1024 to 32000; the choice
-// was at most 7 % behind the best of all, 0.3 % on average (linear8 in us, tiles of
+// fitted to 131 products of 1 to 32768 rows, K 512 to 11008, N 1024 to 32000; the choice
+// was at most 6 % behind the best of all, 0.5 % on average (linear8 in us, tiles of
 // fp8_few, fp8_ring and fp8_large as rows x columns):
 //   1 row, 1024 -> 1024       16 x 16 3.5   16 x 64 3.7    64 x 64 5.1
 //   64 rows, 4096 -> 4096     16 x 16 15.5  16 x 64 8.2    64 x 64 11.0
@@ -822,15 +823,15 @@ struct Fp8Shape {
 };
 constexpr int kFp8Few = 4;   // shapes of fp8_few, then tiles
 constexpr Fp8Shape kFp8Shapes[] = {
-    {16, 16, 3.2f, 0.066f, 1.58f, 0.67f, 0.072f},
-    {16, 32, 3.0f, 0.094f, 2.2f, 0.79f, 0.106f},
-    {16, 64, 3.04f, 0.141f, 0.7f, 4.1f, 0.125f},
-    {32, 64, 3.84f, 0.212f, 1.6f, 1.9f, 0.2f},
-    {64, 64, 3.5f, 0.223f, 3.5f, -0.19f, 0.258f},
-    {64, 128, 4.0f, 0.308f, 4.3f, 0.02f, 0.353f},
-    {128, 128, 4.76f, 0.441f, 3.63f, 0.16f, 0.552f},
-    {128, 256, 8.05f, 0.754f, 4.67f, 1.83f, 0.812f},
-    {256, 256, 8.0f, 1.06f, 2.15f, 6.71f, 1.45f},   // (full of such tiles the card is bound by power)
+    {16, 16, 3.5f, 0.0577f, 1.65f, 0.549f, 0.0717f},
+    {16, 32, 3.52f, 0.0773f, 3.0f, 0.088f, 0.111f},
+    {16, 64, 3.39f, 0.138f, 0.69f, 3.0f, 0.0957f},
+    {32, 64, 3.83f, 0.219f, 1.6f, 1.9f, 0.2f},
+    {64, 64, 3.2f, 0.235f, 3.55f, -0.17f, 0.258f},
+    {64, 128, 4.0f, 0.321f, 3.84f, 0.109f, 0.38f},
+    {128, 128, 4.64f, 0.461f, 4.0f, 0.26f, 0.574f},
+    {128, 256, 7.76f, 0.745f, 5.17f, 1.94f, 0.865f},
+    {256, 256, 8.2f, 1.1f, 2.2f, 7.8f, 1.43f},   // (full of such tiles the card is bound by power)
 };
 int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   // of the first `shapes`
   constexpr int kShapes = sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]);
@@ -866,7 +867,9 @@ void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream
     case 1: return fp8_few<1, 2, 8, kCodes>(in, sg, M, kb, s);
     case 2: return fp8_few<1, 4, 8, kCodes>(in, sg, M, kb, s);
     case 3: return fp8_few<2, 4, 8, kCodes>(in, sg, M, kb, s);
-    case 4: return per_cu <= 1.0f ? fp8_ring<1, 1, 4, 2, 2>(x, xs, sg, M, kb, s) : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
+    case 4:
+      return per_cu <= 1.0f && kb >= 8 ? fp8_ring<1, 1, 4, 2, 2>(x, xs, sg, M, kb, s)
+                                       : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
     case 5: return fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s);
     case 6: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
     case 7: return fp8_ring<4, 2, 3, 2>(x, xs, sg, M, kb, s);

@@ -439,7 +439,7 @@ def test_linear_of_whole_numbers(M, K, N):
 
 
 # (M, K, [N_i]), the kernel: few rows, tiles of each shape, odd borders, long K, many rows
-TILES = [(61, 4000, [4090], "few"), (120, 3970, [1800, 1, 1000, 1090], "few"), (30, 900, [1, 4000], "few"),
+TILES = [(61, 4000, [4090], "few"), (120, 3970, [1800, 1, 1000, 1090], "ring"), (30, 900, [1, 4000], "few"),
          (16, 1024, [20000], "few"), (32, 11008, [500], "few"), (64, 700, [12287], "ring"), (17, 256, [12289], "ring"),
          (64, 4096, [32000], "ring"), (66, 33000, [70], "few"), (257, 16384, [300], "few"), (500, 2050, [4383], "ring"),
          (1111, 1030, [4383], "ring"), (2001, 1024, [4384], "ring"), (2047, 4096, [4096], "ring"), (2047, 4096, [4100], "large"),
@@ -448,7 +448,8 @@ TILES = [(61, 4000, [4090], "few"), (120, 3970, [1800, 1, 1000, 1090], "few"), (
          (300, 640, [128, 1, 1000, 333], "ring"), (4096, 2048, [1111, 2000, 77, 900], "ring"), (2040, 6000, [2000, 1027, 77, 900], "large"),
          (3000, 1, [5000], "ring"), (5000, 130, [5001], "ring"), (300, 100, [1111], "ring"), (900, 300, [900], "ring"),
          (129, 2100, [30001], "ring"), (200, 1300, [9000, 5000], "ring"), (70, 1500, [37000], "ring"), (3000, 5000, [1030], "ring"),
-         (4, 1204, [36073], "ring"), (720, 714, [1933], "ring")]
+         (4, 1204, [36073], "few"), (720, 714, [1933], "ring"),
+         (100, 11000, [3900], "few"), (97, 9000, [1800, 1, 1000, 1090], "few"), (22001, 1090, [61], "ring"), (20000, 1700, [29, 1], "ring")]
 
 
 @pytest.mark.gpu
