@@ -225,9 +225,10 @@ def _rows(x: Fp8Rows):
     K, codes, scales = x.features, x.codes, x.scales
     shape, s = codes.shape, scales.shape
     Kp = (K + 127) >> 7 << 7
-    if codes.dtype != CODES or not Kp or shape[-1] != Kp:
+    if codes.dtype is not CODES or not Kp or not shape or shape[-1] != Kp:
         raise ValueError(f"fp8_linear: codes must be (..., {Kp}) {CODES}, got {tuple(shape)} {codes.dtype}")
-    if s[:-1] != shape[:-1] or s[-1] != (Kp + 511) >> 9 << 2 or scales.dtype not in _BYTES:
+    beside = len(s) == len(shape) and (s[0] == shape[0] if len(s) == 2 else s[:-1] == shape[:-1])
+    if not beside or s[-1] != (Kp + 511) >> 9 << 2 or scales.dtype not in _BYTES:
         raise ValueError(f"fp8_linear: scales must be (..., {(Kp + 511) >> 9 << 2}) {SCALES} beside codes "
                          f"{tuple(shape)}, got {tuple(s)} {scales.dtype}")
     if not codes.is_contiguous() or codes.data_ptr() & 15:

@@ -185,6 +185,40 @@ def test_linear_refuses(what):
             fp8_linear(x, packed, scales, **kw)
 
 
+def test_rows_of_wrong_shapes():
+    """Codes and scales whose leading sizes or lengths do not belong together."""
+    packed, scales = quantize_fp8(rand(32, 256, dtype=torch.float32))
+    r = make_rows(6, 256)
+    c, s = r.codes, r.scales
+    for codes, sc in ((c, s[0]), (c[0], s), (c[0], s[0, 0]), (c[0, 0], s), (c.view(2, 3, 256), s), (c, s.view(2, 3, 4)),
+                      (c.view(2, 3, 256), s.view(3, 2, 4)), (c, s[:, :2]), (c[:, :128], s)):
+        with pytest.raises(ValueError):
+            fp8_linear(Fp8Rows(codes, sc, 256), packed, scales, out_features=32)
+
+
+@pytest.mark.gpu
+def test_tensors_elsewhere_are_refused():
+    """One tensor of a call on the CPU: told before any launch."""
+    packed, scales = weight(32, 256)
+    x, b = rand(2, 256), rand(32, big=False)
+    r = make_rows(2, 256)
+    w = torch.zeros(256)
+    for i in range(4):
+        at = [t.cuda() if i != j else t for j, t in enumerate((x, packed, scales, b))]
+        with pytest.raises(ValueError):
+            fp8_linear(at[0], *at[1:], out_features=32)
+        with pytest.raises(ValueError):
+            fp8_linear(Fp8Rows(r.codes if i == 0 else r.codes.cuda(), r.scales.cuda(), 256), *at[1:], out_features=32)
+    calls = (lambda: fp8_linear(Fp8Rows(r.codes.cuda(), r.scales, 256), packed.cuda(), scales.cuda()),
+             lambda: fp8_linear(x.cuda(), packed.cuda(), scales.cuda(), xscale=x), lambda: quantize_rows_fp8(x.cuda(), x),
+             lambda: silu_mul_fp8(x, x.cuda()), lambda: rms_norm_fp8(x.cuda(), w), lambda: rms_norm_fp8(x, w.cuda()),
+             lambda: rms_norm_fp8(x.cuda(), w.cuda(), residual=x), lambda: dequantize_fp8(packed.cuda(), scales),
+             lambda: dequantize_fp8(packed, scales))
+    for call in calls:
+        with pytest.raises(ValueError):
+            call()
+
+
 @pytest.mark.parametrize("what", ["norm weight", "norm residual", "norm eps", "norm dtype", "norm wide", "norm cpu",
                                   "norm grad", "silu dtype", "silu shape", "silu grad", "rows dtype", "rows gate",
                                   "rows grad", "rows none", "rows cpu"])
