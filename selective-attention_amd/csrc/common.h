@@ -280,6 +280,11 @@ __device__ __forceinline__ void dma_lds16(const void* base, uint32_t off, uint32
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base),
                "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
 }
+// (past the caches)
+__device__ __forceinline__ void dma_lds16_nt(const void* base, uint32_t off, uint32_t lds) {
+  asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(base),
+               "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");
+}
 __device__ __forceinline__ void dma_lds4(const void* base, uint32_t off, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base),
                "s"(__builtin_amdgcn_readfirstlane(lds)) : "memory", "m0");

@@ -38,6 +38,7 @@ struct Fp8Segs {
   int N[kFp8Segs];
   int blk0[kFp8Segs + 1];
   int nseg;
+  int stream;   // the weights pass the caches by
 };
 
 typedef int v8i __attribute__((ext_vector_type(8)));
@@ -138,12 +139,20 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const Fp8X in, const F
     uint32_t sw[R], sx[CT];
   };
   auto load = [&](int kb, Block& q) __attribute__((always_inline)) {
+    if (sg.stream) {
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
-      q.w[r][0] = wp[r][kb * 128];
-      q.w[r][1] = wp[r][kb * 128 + 64];
-      q.sw[r] = swp[r][kb];
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          q.w[r][i] = __builtin_bit_cast(uint4, __builtin_nontemporal_load(reinterpret_cast<const v4f*>(wp[r] + kb * 128 + 64 * i)));
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) q.w[r][i] = wp[r][kb * 128 + 64 * i];
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r) q.sw[r] = swp[r][kb];
 #pragma unroll
     for (int t = 0; t < CT; ++t) {
       if constexpr (X == kCodes) {
@@ -513,7 +522,7 @@ __device__ __forceinline__ void pin(v16f& c) { asm volatile("" : "+a"(c)::"memor
 // KS = 2: eight waves, a ring and one half of K for each four, whose sums meet in LDS:
 // small tiles wait less than their operands take (512 rows, 4096 -> 1024: 12.4 us, so 11.1;
 // below eight blocks a half is too short, 512 -> 1024: 4.5, so 4.9).
-template <int SN, int SM, int R, int OCC, int KS>
+template <int SN, int SM, int R, int OCC, int KS, bool NT>
 __global__ __launch_bounds__(256 * KS, OCC * KS) void fp8_ring_kernel(const uint8_t* __restrict__ x,
                                                                       const uint8_t* __restrict__ xs, const Fp8Segs sg,
                                                                       int M, int kb_n, int mtiles) {
@@ -569,7 +578,9 @@ __global__ __launch_bounds__(256 * KS, OCC * KS) void fp8_ring_kernel(const uint
     const int q = min(wid + 4 * i, kParts - 1);
     if (i == 0 && ((d_u & 7) == 0 || (KS > 1 && d_u == u0)))
       dma_lds4(d_s + (d_u >> 3) * 4, s_off, ls + kScales + word_at(d_u) + (wid << 8));
-    if (i < kDmas) dma_lds16(q < BN / 16 ? d_w : d_x, off[i], stage + (q << 10));
+    if (i >= kDmas) return;
+    if (NT && i < BN / 64) dma_lds16_nt(d_w, off[i], stage + (q << 10));
+    else dma_lds16(q < BN / 16 ? d_w : d_x, off[i], stage + (q << 10));
   };
   auto advance = [&]() __attribute__((always_inline)) {
     d_w += 1024;
@@ -783,6 +794,7 @@ void cut_tiles(Fp8Segs& sg, int BN) {
 template <int CT, int R, int NW, int X>
 void fp8_few(const Fp8X& in, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   cut_tiles(sg, 16 * R);
+  if (M > 16 * CT) sg.stream = 0;   // (rows of tiles share them)
   ProfScope prof_("fp8_few", s);
   hipLaunchKernelGGL((fp8_few_kernel<CT, R, NW, X>), dim3(sg.blk0[kFp8Segs] * ((M + 16 * CT - 1) / (16 * CT))),
                      dim3(64 * NW), 0, s, in, sg, M, kb);
@@ -795,12 +807,12 @@ void fp8_large(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStr
   hipLaunchKernelGGL((fp8_large_kernel<SN, SM>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
 }
-template <int SN, int SM, int R, int OCC, int KS = 1>
+template <int SN, int SM, int R, int OCC, int KS = 1, bool NT = false>
 void fp8_ring(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   cut_tiles(sg, 64 * SN);
   const int mtiles = (M + 64 * SM - 1) / (64 * SM);
   ProfScope prof_("fp8_ring", s);
-  hipLaunchKernelGGL((fp8_ring_kernel<SN, SM, R, OCC, KS>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256 * KS), 0, s,
+  hipLaunchKernelGGL((fp8_ring_kernel<SN, SM, R, OCC, KS, NT>), dim3(sg.blk0[kFp8Segs] * mtiles), dim3(256 * KS), 0, s,
                      static_cast<const uint8_t*>(x), static_cast<const uint8_t*>(xs), sg, M, kb, mtiles);
 }
 
@@ -858,8 +870,21 @@ int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   /
   return best;
 }
 
+// Weights that one row of tiles reads and that take more than a third of the caches' 256
+// MB pass them by: a model with one such weight has more weights than they hold.  From
+// memory 1 row 4096 -> 32000 takes 26.5 us, so 23.8, 32 rows 27.6, so 24.2, 16 rows 4096 ->
+// 24000 22.0, so 20.4; one weight alone, call after call, comes from the caches, 22.7, so
+// 22.3, 21.6, so 22.8, and 16.8, so 18.2.  Smaller ones lose more there than they gain (64
+// rows, 5120 -> 15000: 25 and 24, 16.3 and 22).
+void fp8_stream(Fp8Segs& sg, int kb) {
+  long bytes = 0;
+  for (int i = 0; i < sg.nseg; ++i) bytes += (sg.N[i] + 15L) / 16 * kb * 2048;
+  sg.stream = 3 * bytes > 256L << 20;
+}
+
 void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   const Fp8X in{x, xs, 0, 0, 0};
+  if (M <= 64) fp8_stream(sg, kb);
   // few tiles a CU get deep rings (the smallest eight waves), more of them room beside each other
   float per_cu = 0.0f;
   switch (fp8_shape(sg, M, kb, sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]), &per_cu)) {
@@ -870,7 +895,9 @@ void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream
     case 4:
       return per_cu <= 1.0f && kb >= 8 ? fp8_ring<1, 1, 4, 2, 2>(x, xs, sg, M, kb, s)
                                        : fp8_ring<1, 1, 3, 5>(x, xs, sg, M, kb, s);
-    case 5: return fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s);
+    case 5:
+      return sg.stream ? fp8_ring<2, 1, 6, 2, 1, true>(x, xs, sg, M, kb, s)
+                                  : fp8_ring<2, 1, 6, 2>(x, xs, sg, M, kb, s);
     case 6: return per_cu <= 2.0f ? fp8_ring<2, 2, 4, 2>(x, xs, sg, M, kb, s) : fp8_ring<2, 2, 3, 3>(x, xs, sg, M, kb, s);
     case 7: return fp8_ring<4, 2, 3, 2>(x, xs, sg, M, kb, s);
     default: return fp8_large<4, 4>(x, xs, sg, M, kb, s);
@@ -881,6 +908,7 @@ void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream
 template <int X>
 void fp8_go_bf16(const Fp8X& in, Fp8Segs& sg, int M, int kb, hipStream_t s) {
   float per_cu = 0.0f;
+  fp8_stream(sg, kb);
   if (fp8_shape(sg, M, kb, 2, &per_cu) == 0) fp8_few<1, 1, 8, X>(in, sg, M, kb, s);
   else fp8_few<1, 2, 8, X>(in, sg, M, kb, s);
 }

@@ -483,7 +483,8 @@ TILES = [(61, 4000, [4090], "few"), (120, 3970, [1800, 1, 1000, 1090], "ring"), 
          (3000, 1, [5000], "ring"), (5000, 130, [5001], "ring"), (300, 100, [1111], "ring"), (900, 300, [900], "ring"),
          (129, 2100, [30001], "ring"), (200, 1300, [9000, 5000], "ring"), (70, 1500, [37000], "ring"), (3000, 5000, [1030], "ring"),
          (4, 1204, [36073], "few"), (720, 714, [1933], "ring"),
-         (100, 11000, [3900], "few"), (97, 9000, [1800, 1, 1000, 1090], "few"), (22001, 1090, [61], "ring"), (20000, 1700, [29, 1], "ring")]
+         (100, 11000, [3900], "few"), (97, 9000, [1800, 1, 1000, 1090], "few"), (22001, 1090, [61], "ring"), (20000, 1700, [29, 1], "ring"),
+         (16, 4100, [24003], "few"), (1, 9000, [8001, 3000], "few"), (33, 4096, [24001], "ring"), (33, 4090, [9000, 14001], "ring")]
 
 
 @pytest.mark.gpu
@@ -511,6 +512,21 @@ def test_linear_tiles(M, K, sizes, kernel):
     assert list(kt.stats) == ["fp8_" + kernel]
     for y, v in zip(ys, want):
         assert torch.equal(y, v.to(torch.bfloat16))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_few_bfloat16_rows_of_a_large_weight(gated):
+    """Whole numbers again: rows rounded by the product, weights that pass the caches by."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    M, K, N = 5, 9001, 11003
+    x = torch.randint(-3, 4, (M, K), generator=g, device="cuda").to(torch.bfloat16)
+    gate = torch.randint(0, 3, (M, K), generator=g, device="cuda").to(torch.bfloat16)
+    w = torch.randint(-3, 4, (N, K), generator=g, device="cuda").float()
+    packed, scales = pack_fp8(w.to(E4), torch.full(((N + 127) // 128, (K + 127) // 128), 127, dtype=torch.uint8, device="cuda"))
+    v = x.double() * gate.double() if gated else x.double()
+    y = fp8_linear(x, packed, scales, out_features=N, xscale=gate if gated else None)
+    assert torch.equal(y, torch.matmul(v, w.double().t().contiguous()).to(torch.bfloat16))
 
 
 @pytest.mark.gpu
