@@ -254,18 +254,30 @@ void norm_go(const void* x, const void* res, const float* w, long rows, long ldx
   // few rows are bound by one row's latency, and take more waves for it: with fewer 1 row
   // of 1024 takes 3.5 us, so 2.7, 1 of 8192 6.4 and 3.8, 512 of 1024 4.9 and 4.0, 512 of 4096
   // 6.3 and 6.5; more rows fill the card either way, and one wave a row needs no barrier
-  const bool few = rows <= kFewRows;
+  if (rows <= kFewRows && dim > 512 && dim <= 8192) {
+    if (dim <= 2048) go(rms_norm_fp8_kernel<T, RES, 1, 4>, 4);
+    else go(rms_norm_fp8_kernel<T, RES, 1, 16>, 16);
+    return;
+  }
+  // lanes without columns cost what the others do: a row takes the sizes that leave few of
+  // them (64 M numbers with residual at dim 1280 95 us, by the sizes of 2048 116, at 5120 92
+  // and 97, at 20000 121 and 220; at 1024 84)
   if (dim <= 512) go(rms_norm_fp8_kernel<T, RES, 1, 1>, 1);
-  else if (dim <= 1024 && !few) go(rms_norm_fp8_kernel<T, RES, 2, 1>, 1);
+  else if (dim <= 1024) go(rms_norm_fp8_kernel<T, RES, 2, 1>, 1);
+  else if (dim <= 1536) go(rms_norm_fp8_kernel<T, RES, 3, 1>, 1);
   else if (dim <= 2048) go(rms_norm_fp8_kernel<T, RES, 1, 4>, 4);
-  else if (dim <= 8192 && few) go(rms_norm_fp8_kernel<T, RES, 1, 16>, 16);
+  else if (dim <= 2560) go(rms_norm_fp8_kernel<T, RES, 5, 1>, 1);
   else if (dim <= 4096) go(rms_norm_fp8_kernel<T, RES, 2, 4>, 4);
+  else if (dim <= 6144) go(rms_norm_fp8_kernel<T, RES, 3, 4>, 4);
   else if (dim <= 8192) go(rms_norm_fp8_kernel<T, RES, 4, 4>, 4);
+  else if (dim <= 10240) go(rms_norm_fp8_kernel<T, RES, 5, 4>, 4);
   else if (dim <= 16384) go(rms_norm_fp8_kernel<T, RES, 2, 16>, 16);
+  else if (dim <= 24576) go(rms_norm_fp8_kernel<T, RES, 3, 16>, 16);
+  else if (dim <= 32768) go(rms_norm_fp8_kernel<T, RES, 4, 16>, 16);
   else go(rms_norm_fp8_kernel<T, RES, 8, 16>, 16);
 }
 constexpr int kMaxNormDim = 65536;
-int norm_waves(int dim) { return dim <= 1024 ? 1 : dim <= 8192 ? 4 : 16; }   // (as norm_go)
+int norm_waves(int dim) { return dim <= 1536 ? 1 : dim <= 10240 ? 4 : 16; }   // at most (as norm_go)
 
 int rows_check(const char* who, int dtype, long rows, int dim, const void* codes, const void* scales) {
   SA_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype code %d", who, dtype);

@@ -386,7 +386,8 @@ def test_silu_mul_where_a_c_passes_fp32():
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("residual", [False, True])
 @pytest.mark.parametrize("shape", SHAPES + [(1, 65536), (2, 33000), (513, 1000), (600, 1024), (530, 1999),
-                                            (520, 4095), (515, 4096), (514, 8191)])
+                                            (520, 4095), (515, 4096), (514, 8191), (523, 1301), (515, 2560), (514, 2057),
+                                            (513, 6100), (3, 10001), (2, 30001)])
 def test_rms_norm(shape, residual, dtype):
     x, w = rand(*shape, seed=13, dtype=dtype), 0.3 * rand(shape[-1], seed=14, dtype=torch.float32)
     res = rand(*shape, seed=15, dtype=dtype) if residual else None
