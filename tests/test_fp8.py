@@ -400,6 +400,21 @@ def test_rms_norm(shape, residual, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape", [(1500, 4096), (6000, 1024), (5, 30000)])
+def test_rms_norm_of_many_numbers(shape, dtype):
+    """Enough numbers that some hundred lie within a few fp32 steps of a tie (2^-19 of
+    them a step), and tiny ones: blocks below fp32's normal numbers, rows below 2^-100."""
+    x, w = rand(*shape, seed=33, dtype=dtype), 0.3 * rand(shape[-1], seed=34, dtype=torch.float32)
+    x[1] *= 2.0 ** -100
+    x[2, :512] *= 2.0 ** -110
+    x[2, 512:1024] *= 2.0 ** -125
+    w[512:640] = -1.0
+    _, v = ref.rms_norm(x, w, 1e-12)
+    same_rows(rms_norm_fp8(x.cuda(), w.cuda(), 1e-12), v)
+
+
+@pytest.mark.gpu
 def test_rms_norm_of_odd_rows():
     """A row of zeros, tiny and large rows, one with an infinity or a NaN; its neighbours stand."""
     x = rand(6, 640, seed=16, dtype=torch.float32)
