@@ -997,7 +997,7 @@ extern "C" size_t sa_colsum_bf16_workspace_size(int64_t M, int N) {
 extern "C" int sa_colsum_bf16(const void* x, int64_t M, int N, void* out, void* workspace, size_t workspace_size,
                               void* stream) {
   const char* who = "sa_colsum_bf16";
-  SA_CHECK_ARG(M >= 1 && M <= (1L << 31) && N >= 1 && N <= (1 << 24), "%s: bad sizes M=%ld N=%d", who,
+  SA_CHECK_ARG(M >= 1 && M < (1L << 31) && N >= 1 && N <= (1 << 24), "%s: bad sizes M=%ld N=%d", who,
                static_cast<long>(M), N);
   SA_CHECK_ARG(x && out, "%s: null pointer", who);
   SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) & 1) == 0 &&
