@@ -144,12 +144,16 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
 }
 
 // 1 / sqrt(ss inv_dim + eps) as hi + lo: the unit's estimate in fp64 (2^-23 off at
-// most) and one Newton step; 0 for a row with an infinity
-__device__ __forceinline__ void rstd_of(double ss, double inv_dim, float eps, float& hi, float& lo) {
+// most) and one Newton step; 0 for a row with an infinity.  For rows that large that hi
+// and lo would lose digits below fp32's normal numbers, 2^64 of it (true)
+__device__ __forceinline__ bool rstd_of(double ss, double inv_dim, float eps, float& hi, float& lo) {
   const double m = fma(ss, inv_dim, static_cast<double>(eps)), e = __builtin_amdgcn_rsq(m);
-  const double r = m == static_cast<double>(__builtin_inff()) ? 0.0 : e * fma(-0.5 * m, e * e, 1.5);
+  double r = m == static_cast<double>(__builtin_inff()) ? 0.0 : e * fma(-0.5 * m, e * e, 1.5);
+  const bool large = r < 0x1p-64;
+  r *= large ? 0x1p64 : 1.0;
   hi = static_cast<float>(r);
   lo = static_cast<float>(r - static_cast<double>(hi));
+  return large;
 }
 
 // Four fp32 roundings leave a value within four of its last steps.  Its code is then the
@@ -210,7 +214,12 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
     for (int i = 0; i < W; ++i) ss += part[i];
   }
   float hi, lo;
-  rstd_of(ss, inv_dim, eps, hi, lo);
+  if (rstd_of(ss, inv_dim, eps, hi, lo)) {
+#pragma unroll
+    for (int j = 0; j < V; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[j][i] *= 0x1p-64f;
+  }
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int p = t + 64 * W * j, k = 8 * p, b = p >> 4;

@@ -406,6 +406,7 @@ def test_rms_norm_of_many_numbers(shape, dtype):
     """Enough numbers that some hundred lie within a few fp32 steps of a tie (2^-19 of
     them a step), and tiny ones: blocks below fp32's normal numbers, rows below 2^-100."""
     x, w = rand(*shape, seed=33, dtype=dtype), 0.3 * rand(shape[-1], seed=34, dtype=torch.float32)
+    x[0] = x[0].double().div(x[0].double().abs().max()).mul(3.2e38).to(dtype)   # (near the type's end)
     x[1] *= 2.0 ** -100
     x[2, :512] *= 2.0 ** -110
     x[2, 512:1024] *= 2.0 ** -125

@@ -170,3 +170,23 @@ def test_seq2seq_generates():
     ids = _prompt(2, 60)
     a = m.generate(ids, gen)
     assert torch.equal(a, m.generate(ids, gen, use_graph=False)) and a.shape == (2, 12)
+
+
+@pytest.mark.gpu
+def test_training_and_ragged_prompts():
+    """In training the layers take tensors and pass their gradient on; a padded prompt's
+    rows stay finite whatever stands behind their lengths, and padding changes nothing
+    before them."""
+    m, ids = _model().quantize_fp8(), _prompt(2, 70)
+    lengths = torch.tensor([70, 33], device="cuda")
+    m.train()
+    y = m(ids, lengths=lengths)
+    y.float().logsumexp(-1).sum().backward()
+    g = m.embedding.weight.grad
+    assert torch.isfinite(y).all() and torch.isfinite(g).all() and g.abs().max() > 0
+    m.eval()
+    other = ids.clone()
+    other[1, 33:] = 7
+    with torch.no_grad():
+        a, b = m(ids, lengths=lengths), m(other, lengths=lengths)
+    assert torch.isfinite(a).all() and torch.equal(a[0], b[0]) and torch.equal(a[1, :33], b[1, :33])
