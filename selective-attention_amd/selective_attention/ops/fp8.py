@@ -26,7 +26,7 @@ import torch
 import torch.nn.functional as F
 
 from ..kernels import fp8 as _k
-from ..kernels.common import in_forward_mode
+from ..kernels.common import in_forward_mode, needs_torch_ops
 from ..kernels.fp8 import CODES, MAX_MATRICES, SCALES
 from ..utils import check_ndim, check_shape
 
@@ -238,6 +238,19 @@ def _rows(x: Fp8Rows):
     return K, codes, scales
 
 
+class _ColumnSumsFn(torch.autograd.Function):
+    """The sums over the rows of (..., N), differentiable any number of times."""
+
+    @staticmethod
+    def forward(ctx, dy):
+        ctx.shape = dy.shape
+        return _k.column_sums(dy)
+
+    @staticmethod
+    def backward(ctx, g):
+        return g.expand(ctx.shape)
+
+
 class _Fp8LinearFn(torch.autograd.Function):
     """x W^T + bias; the gradient passes the rows' rounding as it is."""
 
@@ -256,7 +269,10 @@ class _Fp8LinearFn(torch.autograd.Function):
             w = _k.dequantize(*ctx.saved_tensors, ctx.N, ctx.K)
             dx = (dy.reshape(-1, ctx.N) @ w).view(*dy.shape[:-1], ctx.K)
         if ctx.needs_input_grad[2]:
-            db = _k.column_sums(dy)
+            if needs_torch_ops(dy):
+                db = dy.reshape(-1, ctx.N).sum(0)
+            else:   # (a launch of its own leaves no history)
+                db = _ColumnSumsFn.apply(dy) if torch.is_grad_enabled() else _k.column_sums(dy)
         return dx, None, db, None, None, None
 
 

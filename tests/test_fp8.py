@@ -793,6 +793,76 @@ def test_gradient_is_the_difference():
     assert (dx.cpu().double() * d.double()).sum() == diff
 
 
+def _second(packed, scales, N, K, M, dev):
+    """The gradient by dy of |dx|^2 + |db|^2, whole numbers: dx = dy W and db the column sums."""
+    g = torch.Generator().manual_seed(N)
+    x = torch.randint(-4, 5, (M, K), generator=g).to(torch.bfloat16).to(dev).requires_grad_()
+    b = torch.zeros(N, dtype=torch.bfloat16, device=dev).requires_grad_()
+    dy = torch.randint(-1, 2, (M, N), generator=g).to(torch.bfloat16).to(dev).requires_grad_()
+    w = dequantize_fp8(packed.to(dev), scales.to(dev), N, K).double().cpu()
+    got = []
+    for ts in ((x, b), (b,), (x,)):
+        y = fp8_linear(x, packed.to(dev), scales.to(dev), b, out_features=N)
+        ds = torch.autograd.grad(y, ts, dy, create_graph=True)
+        (d2,) = torch.autograd.grad(sum(d.float().square().sum() for d in ds), dy)
+        d = dy.detach().double().cpu()
+        want = torch.zeros_like(d)
+        if ts[0] is x:
+            want = want + 2 * (d @ w @ w.t())
+        if ts[-1] is b:
+            want = want + 2 * d.sum(0)
+        got.append((d2.cpu().double(), want))
+    return got
+
+
+def _whole_weight(N, K):
+    g = torch.Generator().manual_seed(K)
+    return pack_fp8(torch.randint(-1, 2, (N, K), generator=g).float().to(E4), torch.ones((N + 127) // 128, (K + 127) // 128))
+
+
+def test_second_derivatives_on_the_cpu(monkeypatch):
+    """The launches replaced by their arithmetic, without history as theirs: what is left
+    is how the backward joins them.  Sums below 2^8 are exact in bfloat16."""
+    from selective_attention.ops import fp8 as op
+    packed, scales = _whole_weight(9, 6)
+    w = ref.weight(packed, scales, 9, 6).to(torch.bfloat16)
+    monkeypatch.setattr(op._k, "dequantize", lambda p, s, N, K: w.clone())
+    monkeypatch.setattr(op._k, "linear_multi_bf16", lambda x, g, ws, bs, Ns: [(x.detach() @ w.t() + bs[0].detach())])
+    monkeypatch.setattr(op._k, "column_sums", lambda d: d.detach().reshape(-1, 9).float().sum(0).to(torch.bfloat16))
+    for d2, want in _second(packed, scales, 9, 6, 5, "cpu"):
+        assert want.abs().max() <= 256 and torch.equal(d2, want) and want.any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("M", [5, 40])
+def test_second_derivatives(M):
+    """Of both gradients together and each alone, exact below 2^8."""
+    packed, scales = _whole_weight(9, 6)
+    for d2, want in _second(packed, scales, 9, 6, M, "cuda"):
+        assert want.abs().max() <= 256 and torch.equal(d2, want) and want.any()
+
+
+@pytest.mark.gpu
+def test_tangents_and_batches_of_the_gradient():
+    """A dual dy keeps its tangent through both gradients; dys of a batch likewise."""
+    import torch.autograd.forward_ad as fwd
+    M, N, K = 7, 9, 6
+    packed, scales = (t.cuda() for t in _whole_weight(N, K))
+    g = torch.Generator().manual_seed(1)
+    x = torch.ones(M, K, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    b = torch.zeros(N, dtype=torch.bfloat16, device="cuda").requires_grad_()
+    dys = torch.randint(-1, 2, (3, M, N), generator=g).to(torch.bfloat16).cuda()
+    y = fp8_linear(x, packed, scales, b, out_features=N)
+    one = [torch.autograd.grad(y, (x, b), d, retain_graph=True) for d in dys]
+    both = torch.autograd.grad(y, (x, b), dys, retain_graph=True, is_grads_batched=True)
+    assert all(torch.equal(both[i][j], one[j][i]) for i in range(2) for j in range(3))
+    with fwd.dual_level():
+        ds = torch.autograd.grad(y, (x, b), fwd.make_dual(dys[0], dys[1]))
+        for d, p, t in zip(ds, one[0], one[1]):
+            got = fwd.unpack_dual(d)
+            assert torch.equal(got.primal, p) and torch.equal(got.tangent, t)
+
+
 @pytest.mark.gpu
 def test_forward_mode_is_refused():
     import torch.autograd.forward_ad as fwd
