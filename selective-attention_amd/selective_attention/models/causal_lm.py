@@ -19,7 +19,8 @@ import torch
 import torch.nn as nn
 
 from ..inference import CausalBlockCache, GenerationConfig, InferenceState
-from ..modules.layers import Fp8Linear, Int4Linear, Linear, quantize_linears, quantize_linears_fp8
+from ..modules.layers import (Fp8Linear, Int4Linear, Linear, add_norm_for, norm_for, quantize_linears,
+                              quantize_linears_fp8)
 from ..modules import CausalBlock, RMSNorm
 from ..ops.logprobs import TokenLogprobs, token_logprobs
 from ._graph import graph_decode
@@ -108,7 +109,7 @@ class CausalLM(nn.Module):
                 cache: list | None = None, analysis_cfg=None, stats=None):
         """input_ids (batch_size, seq_len) -> logits (batch_size, seq_len, vocab_size)."""
         h = self._hidden(input_ids, lengths, attn_gate_thresholds, cache)
-        return self.lm_head(self.norm(h, self.lm_head))
+        return self.lm_head(norm_for(self.lm_head, self.norm, h))
 
     def score(self, input_ids: torch.Tensor, lengths: torch.Tensor | None = None,
               attn_gate_thresholds: torch.Tensor | List | None = None, top: int = 0) -> TokenLogprobs:
@@ -138,7 +139,7 @@ class CausalLM(nn.Module):
         pend = None
         for i, layer in enumerate(self.layers):
             h, pend = layer.step(h, cache[i], state, gen_cfg, pending=pend, defer_add=True)
-        return self.lm_head(self.norm.add_forward(h, pend, self.lm_head)[1])
+        return self.lm_head(add_norm_for(self.lm_head, self.norm, h, pend)[1])
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, gen_cfg: GenerationConfig, analysis_cfg=None,
@@ -165,7 +166,7 @@ class CausalLM(nn.Module):
         state = InferenceState(lengths.clone())
         h = self._hidden(input_ids, lengths, gen_cfg.attn_gate_thresholds, cache)
         # logits of each row's last token only (the rows the reference keeps)
-        logits = self.lm_head(self.norm(h[torch.arange(b, device=dev), lengths - 1], self.lm_head))
+        logits = self.lm_head(norm_for(self.lm_head, self.norm, h[torch.arange(b, device=dev), lengths - 1]))
         seq_ids = torch.full((b, L + new), gen_cfg.pad_token_id, dtype=input_ids.dtype, device=dev)
         seq_ids[:, :L] = input_ids
         lps = None if logprobs is None else _LogprobLog(b, max(new, 0), logprobs, dev)

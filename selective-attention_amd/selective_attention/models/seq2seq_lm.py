@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from ..inference import CrossBlockCache, GenerationConfig, InferenceState
-from ..modules.layers import Linear, quantize_linears, quantize_linears_fp8
+from ..modules.layers import Linear, add_norm_for, norm_for, quantize_linears, quantize_linears_fp8
 from ..modules import SSM, BiBlock, CrossBlock, RMSNorm
 from ._graph import graph_decode
 
@@ -96,7 +96,7 @@ class Seq2SeqLM(nn.Module):
         h = self.embedding(input_ids)
         for i, layer in enumerate(self.encoder_layers):
             h, _ = layer(h, lengths=lengths, attn_gate_threshold=_thr(enc_attn_gate_thresholds, i))
-        s, ssm_hiddens = self.ssm(self.norm1(h, self.ssm), lengths=lengths)
+        s, ssm_hiddens = self.ssm(norm_for(self.ssm, self.norm1, h), lengths=lengths)
         h = self.norm2(h + self.dropout(s))
         ssm_hiddens = self.norm3(ssm_hiddens.transpose(1, 2)).transpose(1, 2).contiguous()
         return h, ssm_hiddens
@@ -109,7 +109,7 @@ class Seq2SeqLM(nn.Module):
                       self_attn_gate_threshold=_thr(attn_gate_thresholds, i),
                       cross_attn_gate_threshold=_thr(cross_attn_gate_thresholds, i),
                       cache=cache[i] if cache is not None else None)
-        return self.lm_head(self.norm4(h, self.lm_head))
+        return self.lm_head(norm_for(self.lm_head, self.norm4, h))
 
     def forward(self, input_ids: torch.Tensor, lengths: torch.Tensor,
                 decoder_input_ids: torch.Tensor, enc_attn_gate_thresholds=None,
@@ -129,7 +129,7 @@ class Seq2SeqLM(nn.Module):
         pend = None
         for i, layer in enumerate(self.decoder_layers):
             h, pend = layer.step(h, cache[i], state, gen_cfg, pending=pend, defer_add=True)
-        return self.lm_head(self.norm4.add_forward(h, pend, self.lm_head)[1])
+        return self.lm_head(add_norm_for(self.lm_head, self.norm4, h, pend)[1])
 
     @torch.no_grad()
     def generate(self, input_ids: torch.Tensor, gen_cfg: GenerationConfig, analysis_cfg=None,

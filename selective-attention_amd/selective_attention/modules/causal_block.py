@@ -7,7 +7,7 @@ from __future__ import annotations
 import torch
 import torch.nn as nn
 
-from .layers import RMSNorm, SwiGLU
+from .layers import RMSNorm, SwiGLU, add_norm_for, norm_for
 from .selective_attention import SelectiveMHA
 from .ssm import SSM
 
@@ -34,12 +34,12 @@ class CausalBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor, lengths: torch.Tensor | None = None,
                 attn_gate_threshold=None, cache=None, analysis_cfg=None, stats=None):
         """(batch, seq_len, model_dim) -> (hidden_states, last_ssm_hiddens)."""
-        h, last = self.ssm(self.norm1(hidden_states, self.ssm), lengths=lengths,
+        h, last = self.ssm(norm_for(self.ssm, self.norm1, hidden_states), lengths=lengths,
                            cache=cache.ssm_cache if cache is not None else None)
-        hidden_states, n = self.norm2.add_forward(hidden_states, self.dropout(h), self.mha)
+        hidden_states, n = add_norm_for(self.mha, self.norm2, hidden_states, self.dropout(h))
         h = self.mha(n, lengths=lengths, attn_gate_threshold=attn_gate_threshold,
                      cache=cache.attn_cache if cache is not None else None)
-        hidden_states, n = self.norm3.add_forward(hidden_states, self.dropout(h), self.ffn)
+        hidden_states, n = add_norm_for(self.ffn, self.norm3, hidden_states, self.dropout(h))
         hidden_states = hidden_states + self.dropout(self.ffn(n))
         return hidden_states, last
 
@@ -50,12 +50,12 @@ class CausalBlock(nn.Module):
         is added to hidden_states first (with norm1, one kernel), and with
         defer_add the block returns (hidden_states, ffn output) unsummed."""
         if pending is None:
-            n = self.norm1(hidden_states, self.ssm)
+            n = norm_for(self.ssm, self.norm1, hidden_states)
         else:
-            hidden_states, n = self.norm1.add_forward(hidden_states, pending, self.ssm)
+            hidden_states, n = add_norm_for(self.ssm, self.norm1, hidden_states, pending)
         h = self.ssm.step(n, cache.ssm_cache)
-        hidden_states, n = self.norm2.add_forward(hidden_states, self.dropout(h), self.mha)
+        hidden_states, n = add_norm_for(self.mha, self.norm2, hidden_states, self.dropout(h))
         h = self.mha.step(n, cache.attn_cache, state, gen_cfg)
-        hidden_states, n = self.norm3.add_forward(hidden_states, self.dropout(h), self.ffn)
+        hidden_states, n = add_norm_for(self.ffn, self.norm3, hidden_states, self.dropout(h))
         f = self.dropout(self.ffn(n))
         return (hidden_states, f) if defer_add else hidden_states + f

@@ -253,7 +253,20 @@ class RMSNorm(nn.Module):
                          and (x.requires_grad or y.requires_grad or self.weight.requires_grad))):
             return add_rms_norm(x, y, self.weight, self.eps)
         s = x + y
-        return s, self(s, layer)
+        return s, self(s) if layer is None else self(s, layer)
+
+
+def norm_for(layer, norm, x: torch.Tensor):
+    """norm(x), in 8 bits where `layer`, which is behind it, takes such rows: any module
+    may stand for a norm, and it is called with x alone where they are not asked for."""
+    return norm(x, layer) if isinstance(norm, RMSNorm) and getattr(layer, "takes_rows", False) else norm(x)
+
+
+def add_norm_for(layer, norm, x: torch.Tensor, y: torch.Tensor):
+    """norm.add_forward(x, y), likewise."""
+    if isinstance(norm, RMSNorm) and getattr(layer, "takes_rows", False):
+        return norm.add_forward(x, y, layer)
+    return norm.add_forward(x, y)
 
 
 def _rotate_half(x: torch.Tensor) -> torch.Tensor:

@@ -9,7 +9,7 @@ import torch
 import torch.nn as nn
 
 from .cross_selective_attention import CrossSelectiveMHA
-from .layers import RMSNorm, SwiGLU
+from .layers import RMSNorm, SwiGLU, add_norm_for, norm_for
 from .selective_attention import SelectiveMHA
 from .ssm import SSM
 
@@ -38,10 +38,10 @@ class BiBlock(nn.Module):
     def forward(self, hidden_states: torch.Tensor, lengths: torch.Tensor | None = None,
                 attn_gate_threshold=None, analysis_cfg=None, stats=None):
         """(batch, seq_len, model_dim) -> (hidden_states, last_ssm_hiddens)."""
-        h, last = self.ssm(self.norm1(hidden_states, self.ssm), lengths=lengths)
-        hidden_states, n = self.norm2.add_forward(hidden_states, self.dropout(h), self.mha)
+        h, last = self.ssm(norm_for(self.ssm, self.norm1, hidden_states), lengths=lengths)
+        hidden_states, n = add_norm_for(self.mha, self.norm2, hidden_states, self.dropout(h))
         h = self.mha(n, lengths=lengths, attn_gate_threshold=attn_gate_threshold)
-        hidden_states, n = self.norm3.add_forward(hidden_states, self.dropout(h), self.ffn)
+        hidden_states, n = add_norm_for(self.ffn, self.norm3, hidden_states, self.dropout(h))
         hidden_states = hidden_states + self.dropout(self.ffn(n))
         return hidden_states, last
 
@@ -69,16 +69,16 @@ class CrossBlock(nn.Module):
                 self_attn_gate_threshold=None, cross_attn_gate_threshold=None, cache=None,
                 analysis_cfg=None, stats=None):
         """(batch, seq_len, model_dim) -> (batch, seq_len, model_dim)."""
-        h, _ = self.ssm(self.norm1(hidden_states, self.ssm), ssm_hiddens=ssm_hiddens,
+        h, _ = self.ssm(norm_for(self.ssm, self.norm1, hidden_states), ssm_hiddens=ssm_hiddens,
                         cache=cache.ssm_cache if cache is not None else None)
-        hidden_states, n = self.norm2.add_forward(hidden_states, self.dropout(h), self.mha)
+        hidden_states, n = add_norm_for(self.mha, self.norm2, hidden_states, self.dropout(h))
         h = self.mha(n, attn_gate_threshold=self_attn_gate_threshold,
                      cache=cache.attn_cache if cache is not None else None)
-        hidden_states, n = self.norm3.add_forward(hidden_states, self.dropout(h), self.cross_mha)
+        hidden_states, n = add_norm_for(self.cross_mha, self.norm3, hidden_states, self.dropout(h))
         h = self.cross_mha(n, context=context, context_lengths=context_lengths,
                            attn_gate_threshold=cross_attn_gate_threshold,
                            cache=cache.cross_attn_cache if cache is not None else None)
-        hidden_states, n = self.norm4.add_forward(hidden_states, self.dropout(h), self.ffn)
+        hidden_states, n = add_norm_for(self.ffn, self.norm4, hidden_states, self.dropout(h))
         return hidden_states + self.dropout(self.ffn(n))
 
     def step(self, hidden_states: torch.Tensor, cache, state, gen_cfg, analysis_cfg=None,
@@ -86,14 +86,14 @@ class CrossBlock(nn.Module):
         """(batch, model_dim) -> (batch, model_dim); pending / defer_add as in
         CausalBlock.step (the last residual add left to the next block)."""
         if pending is None:
-            n = self.norm1(hidden_states, self.ssm)
+            n = norm_for(self.ssm, self.norm1, hidden_states)
         else:
-            hidden_states, n = self.norm1.add_forward(hidden_states, pending, self.ssm)
+            hidden_states, n = add_norm_for(self.ssm, self.norm1, hidden_states, pending)
         h = self.ssm.step(n, cache.ssm_cache)
-        hidden_states, n = self.norm2.add_forward(hidden_states, self.dropout(h), self.mha)
+        hidden_states, n = add_norm_for(self.mha, self.norm2, hidden_states, self.dropout(h))
         h = self.mha.step(n, cache.attn_cache, state, gen_cfg)
-        hidden_states, n = self.norm3.add_forward(hidden_states, self.dropout(h), self.cross_mha)
+        hidden_states, n = add_norm_for(self.cross_mha, self.norm3, hidden_states, self.dropout(h))
         h = self.cross_mha.step(n, cache.cross_attn_cache, gen_cfg)
-        hidden_states, n = self.norm4.add_forward(hidden_states, self.dropout(h), self.ffn)
+        hidden_states, n = add_norm_for(self.ffn, self.norm4, hidden_states, self.dropout(h))
         f = self.dropout(self.ffn(n))
         return (hidden_states, f) if defer_add else hidden_states + f

@@ -52,6 +52,75 @@ def test_every_linear_layer_is_replaced():
     assert quantize_linears_fp8(m).w1 is kept
 
 
+class _Mixer(torch.nn.Module):
+    """Stands for an SSM, an attention or a feed-forward that takes a tensor."""
+
+    def __init__(self, two):
+        super().__init__()
+        self.two = two
+
+    def forward(self, x, **kw):
+        assert isinstance(x, torch.Tensor)
+        return (x, None) if self.two else x
+
+
+class _Sum(torch.nn.Identity):
+    """A norm of another kind, with the two calls that a block makes of one."""
+
+    def add_forward(self, x, y):
+        return x + y, self(x + y)
+
+
+def _plain_blocks():
+    from selective_attention.modules import BiBlock, CausalBlock, CrossBlock
+    kw = dict(layer_idx=0, model_dim=64, head_dim=32, ssm_state_dim=16, ssm_chunk_size=16, device="cpu")
+    for cls in (CausalBlock, BiBlock, CrossBlock):
+        b = cls(**kw).eval()
+        b.ssm, b.mha, b.ffn = _Mixer(True), _Mixer(False), _Mixer(False)
+        if cls is CrossBlock:
+            b.cross_mha = _Mixer(False)
+        yield b, dict(context=None, context_lengths=None, ssm_hiddens=None) if cls is CrossBlock else {}
+
+
+def test_norms_are_called_as_norms():
+    """Where no layer takes rows in 8 bits a norm is called with x alone: its hooks see one
+    argument, and any module may stand in its place."""
+    seen = []
+    for block, kw in _plain_blocks():
+        norms = [m for m in block.modules() if isinstance(m, RMSNorm)]
+        for m in norms:
+            m.register_forward_pre_hook(lambda m, args: seen.append(len(args)))
+        x = torch.randn(2, 5, 64)
+        block(x, **kw)                       # (with a gradient wanted, add_forward calls the norm)
+        assert seen == [1] * len(norms) and len(norms) >= 3
+        seen.clear()
+        for name, m in list(block.named_children()):
+            if isinstance(m, RMSNorm):
+                setattr(block, name, _Sum())
+        y = block(x, **kw)
+        y = y if torch.is_tensor(y) else y[0]
+        assert torch.equal(y, x * 2 ** len(norms))
+
+
+def test_models_with_a_norm_of_another_kind():
+    m = CausalLM(CausalLMConfig(vocab_size=20, model_dim=64, head_dim=32, ssm_state_dim=16, ssm_chunk_size=16,
+                                num_layers=0, device="cpu")).eval()
+    ids = torch.tensor([[3, 4, 5]])
+    m.norm = torch.nn.LayerNorm(64)
+    assert torch.equal(m(ids), m.lm_head(m.norm(m.embedding(ids))))
+    quantize_linears_fp8(m)                  # (a layer that takes rows, a norm that has none)
+    m.lm_head.forward = lambda x: x
+    assert torch.equal(m(ids), m.norm(m.embedding(ids)))
+    s = Seq2SeqLM(Seq2SeqLMConfig(vocab_size=20, model_dim=64, head_dim=32, ssm_state_dim=16, ssm_chunk_size=16,
+                                  num_layers=0, device="cpu")).eval()
+    s.ssm, s.norm1, s.norm4 = _Mixer(True), torch.nn.Identity(), torch.nn.Identity()
+    s.norm3.forward = lambda x: x
+    s.ssm.forward = lambda x, **kw: (x, torch.zeros(1, 4, 32, 16))
+    h = s.embedding(ids)
+    assert torch.equal(s.encode(ids, None)[0], s.norm2(h + h))
+    assert torch.equal(s.decode(ids, None, None, None), s.lm_head(h))
+
+
 # --- modules ------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("rows", [3, 100])
