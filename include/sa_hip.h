@@ -361,8 +361,10 @@ int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zer
  * Rows in 8 bits, the inputs of sa_fp8_linear (the reference has none).  For each
  * block of 128 columns of a row v of `dim` columns, e4m3 codes c and one scale s = 2^e,
  * the smallest power of two with max|v| <= 448 s (1 for a block of zeros, at least
- * 2^-126); c is v / s rounded to nearest, v not rounded before.  Infinities and
- * NaN give NaN codes, the scale goes by what is finite.  kb = ceil(dim / 128):
+ * 2^-126); c is v / s rounded to nearest, v not rounded before (with `silu` v is off by
+ * at most 8 2^-24 of itself).  Infinities and NaN give NaN codes, the scale goes by what
+ * is finite.  A v beyond float's range counts as infinite, one of 2^-150 and less as 0.
+ * kb = ceil(dim / 128):
  *   codes (rows, 128 kb), 16-byte aligned, zeros behind dim;
  *   scales (rows, 4 ceil(kb / 4)) e8m0 bytes, 2^(byte - 127), 127 behind block kb - 1.
  * sa_rows_fp8: v = x, x * gate (gate not NULL), or with `silu` (bfloat16)

@@ -18,6 +18,14 @@ __device__ __forceinline__ float to_odd(float y, float lo) {
   return __uint_as_float(lo != 0.0f && fabsf(lo) < fabsf(y) && (b & 1u) == 0u ? b + step : b);
 }
 
+// v rounded to fp32 to odd; beyond its range infinite, below it 0
+__device__ __forceinline__ float to_odd(double v) {
+  const float y = static_cast<float>(v);
+  const uint32_t b = __float_as_uint(y);
+  const bool moves = static_cast<double>(y) != v && (b & 1u) == 0u && y != 0.0f && fabsf(y) < __builtin_inff();
+  return __uint_as_float(!moves ? b : fabs(v) > fabs(static_cast<double>(y)) ? b + 1 : b - 1);
+}
+
 // e8m0 byte of the scale of a block with the largest finite magnitude top
 __device__ __forceinline__ uint32_t scale_byte(float top) {
   const uint32_t b = __float_as_uint(top);

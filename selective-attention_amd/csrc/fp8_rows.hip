@@ -17,6 +17,7 @@
 // Rounding: v is computed to within a few 2^-48 (rows, rms_norm; silu_mul 8 2^-24)
 // and rounded to fp32 to odd, so that the one rounding that counts, to e4m3, is that
 // of v itself: rounding to nearest twice would send values next to a tie the wrong way.
+// A v beyond fp32's range counts as infinite, one below it (2^-150 at most) as 0.
 //
 // Streams of memory: 16 lanes a block, 8 columns a lane, so that a block's maximum is
 // four rotations within a row of lanes and its codes leave as 128 bytes.  Large calls
@@ -31,11 +32,14 @@
 namespace sa {
 namespace {
 
-// the block's scale and the lane's eight codes; all 16 lanes of the block are here
-__device__ __forceinline__ uint2 encode_block(float (&v)[8], uint32_t& byte) {
+__device__ __forceinline__ float top_of(const float (&v)[8]) {
   float top = 0.0f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(v[i]));   // (a NaN is passed over)
+  return top;
+}
+// the block's scale and the lane's eight codes, of top_of(v); all 16 lanes of the block are here
+__device__ __forceinline__ uint2 encode_block(float (&v)[8], float top, uint32_t& byte) {
   if (__any(top == __builtin_inff())) {
     top = 0.0f;
 #pragma unroll
@@ -107,6 +111,26 @@ __device__ __forceinline__ void store8(T* row, int k, int dim, const float (&v)[
   }
 }
 
+// x - t ln 2, for t next to x log2 e, ln 2 in two words
+__device__ __forceinline__ float left_of(float x, float t) {
+  return fmaf(t, 1.9046542999e-9f, fmaf(t, -0.693147182464599609375f, x));
+}
+// a c / (1 + e^-c) in fp64 but for the exponential and the reciprocal, 5 2^-24 off at most:
+// for gates so far that e^-c nears fp32's end, and where fp32 runs out below.  e is e^-|c|,
+// times 2^164 where the unit would drop its digits; of e^-200 nothing is left whatever a is
+__device__ __forceinline__ double silu64(float a, float c) {
+  const float b = fminf(fabsf(c), 200.0f);
+  const float t = -b * kLog2e;
+  const bool far = t < -115.0f;
+  float e = fast_exp2(far ? t + 164.0f : t);
+  e = fmaf(e, left_of(-b, t), e);
+  const float d = 1.0f + (far ? 0.0f : e);
+  float r = __builtin_amdgcn_rcpf(d);
+  r = fmaf(fmaf(-d, r, 1.0f), r, r);
+  const double s = c >= 0.0f ? 1.0 : c < -200.0f ? 0.0 : static_cast<double>(e) * (far ? 0x1p-164 : 1.0);
+  return static_cast<double>(a) * c * (r * s);
+}
+
 // v = x, x * gate, or x * silu(gate); 16 lanes a block, blocks in order
 enum { kPlain = 0, kGated = 1, kSilu = 2 };
 template <typename T, int MODE>
@@ -117,29 +141,46 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
   if (q >= blocks) return;   // (16 lanes at a time)
   const uint32_t row = q / static_cast<uint32_t>(o.kb);
   const int b = static_cast<int>(q - row * o.kb), k = kQBlock * b + 8 * l16;
-  float v[8];
+  float v[8], top;
   load8<T>(v, x + row * ldx, k, dim);
   if constexpr (MODE != kPlain) {
     float c[8];
     load8<T>(c, gate + row * ldg, k, dim);
+    if constexpr (MODE == kGated) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if constexpr (MODE == kGated) {
+      for (int i = 0; i < 8; ++i) {
         const float y = v[i] * c[i];
         v[i] = to_odd(y, fmaf(v[i], c[i], -y));   // (exact for bf16)
-      } else {
+      }
+    } else {
+      float y[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
         // e^-c by the transcendental unit (2^t, 1 ulp), with what t's rounding leaves
-        const float t = -c[i] * kLog2e, dt = fmaf(-c[i], kLog2e, -t) + -c[i] * 1.925963033500642e-8f;
-        const float e = fast_exp2(t), d = 1.0f + fmaf(e, dt * 0.6931471805599453f, e);
+        const float t = -c[i] * kLog2e, e = fast_exp2(t), d = 1.0f + fmaf(e, left_of(-c[i], t), e);
         float r = __builtin_amdgcn_rcpf(d);
         r = fmaf(fmaf(-d, r, 1.0f), r, r);
-        r = d < __builtin_inff() ? r : 0.0f;   // (c below -88: 0, as with e^-c infinite; no NaN of inf - inf)
-        v[i] = v[i] * r * c[i];   // (a c may pass fp32's range where the result does not)
+        y[i] = v[i] * r * c[i];   // (a c may pass fp32's range where the result does not)
       }
+      top = top_of(y);
+      // by the lane's own numbers: a row's codes do not depend on those beside it
+      bool ends = top_of(c) > 80.0f;
+      if (top < 0x1p-100f) {   // (with a product that is not 0)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) ends |= v[i] != 0.0f && c[i] != 0.0f;
+      }
+      if (ends) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = to_odd(silu64(v[i], c[i]));
+        top = top_of(y);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = y[i];
     }
   }
+  if constexpr (MODE != kSilu) top = top_of(v);
   uint32_t byte;
-  const uint2 c = encode_block(v, byte);
+  const uint2 c = encode_block(v, top, byte);
   put_block(o, row, b, l16, c, byte);
 }
 
@@ -246,7 +287,7 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
     for (int i = 0; i < 8; ++i) v[j][i] = k + i < dim ? y[i] : 0.0f;
     if (b < o.kb) {   // (16 lanes at a time)
       uint32_t byte;
-      const uint2 c = encode_block(v[j], byte);
+      const uint2 c = encode_block(v[j], top_of(v[j]), byte);
       put_block(o, row, b, l16, c, byte);
     }
   }

@@ -10,7 +10,8 @@ The rows are rounded by the op before the layer, in the pass that makes them:
 rms_norm_fp8 (with the residual's addition), silu_mul_fp8 (SwiGLU's product) or
 quantize_rows_fp8 (as they are, or times a gate); each code is the nearest to the
 op's own value, not to that value rounded to bfloat16 first.  Infinities and NaN
-become NaN codes, which make their row's outputs NaN and no other's.  fp8_linear
+become NaN codes, which make their row's outputs NaN and no other's; a value beyond
+float32's range counts as infinite, one of 2^-150 and less as 0.  fp8_linear
 takes such Fp8Rows, or a bfloat16 tensor that it rounds itself; a row's outputs do
 not depend on the rows beside it, but for the order of fp32 sums.  It is
 differentiable in x (a tensor) and bias: the gradient passes the rounding as it

@@ -382,6 +382,61 @@ def test_silu_mul_where_a_c_passes_fp32():
     assert not r.codes.float().any() and (r.scales.float() == 1).all()
 
 
+def check_silu_of_all(r, a, c):
+    """check_silu where a product may lie below fp32's range: 2^-150 and less counts as 0."""
+    v = a.double() * c.double() * torch.sigmoid(c.double())
+    check_silu(r, torch.where(v.abs() <= 2.0 ** -150, 0.0, a.double()), c)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", range(-30, 101, 10))
+def test_silu_mul_of_far_gates(shift):
+    """Gates to both ends of bfloat16 beside every size of a that leaves a finite product: a
+    product from 2^-136 on, half a step of the smallest scale, has its code."""
+    big = torch.tensor([17.0, 88.0, 100.0, 127.0, 128.0, 200.0, 2.3e38, 2.4e38, 3.38e38])
+    far = -torch.cat([torch.arange(80, 92, 0.5), torch.arange(92, 200, 4.0), torch.tensor([1e3, 1e30, 2.4e38, 3.38e38])])
+    c = torch.cat([big, far, torch.linspace(-79, 16, 20)]).to(torch.bfloat16)
+    top = torch.where(c > 1, 2.0 ** 127 / c.double(), 2.0 ** 127)
+    a = (top * 2.0 ** -shift if shift >= 0 else torch.full_like(top, 2.0 ** (4 * shift))).clamp(max=2.0 ** 127)
+    a = (a * torch.where(torch.arange(len(c)) % 2 == 0, 1.0, -1.0)).to(torch.bfloat16)
+    assert torch.isfinite((a.double() * c.double() * torch.sigmoid(c.double())).float()).all()
+    # a block for each pair, so that each has the scale of its own
+    x, g = torch.zeros(len(c), 128).to(torch.bfloat16), torch.ones(len(c), 128).to(torch.bfloat16)
+    x[:, 9], g[:, 9] = a, c
+    check_silu_of_all(silu_mul_fp8(x.cuda(), g.cuda()), x, g)
+    # and all in one row, beside ordinary ones, which stay as they are alone
+    x, g = rand(2, 256, seed=1), rand(2, 256, seed=2, big=False)
+    alone = silu_mul_fp8(x[1:].cuda(), g[1:].cuda())
+    x[0, :len(c)], g[0, :len(c)] = a, c
+    r = silu_mul_fp8(x.cuda(), g.cuda())
+    check_silu_of_all(r, x, g)
+    assert torch.equal(r.codes[1:].view(torch.uint8), alone.codes.view(torch.uint8))
+
+
+@pytest.mark.gpu
+def test_silu_mul_of_tiny_numbers():
+    """Products below fp32's normal numbers, of tiny factors of either kind."""
+    g = torch.Generator().manual_seed(3)
+    e = torch.arange(-133, -60).double()[:, None]
+    x = (torch.randn(len(e), 128, generator=g).double() * torch.exp2(e)).to(torch.bfloat16)
+    for c in (torch.randn(len(e), 128, generator=g) * 4 - 2, -80 - 8 * torch.rand(len(e), 128, generator=g)):
+        check_silu_of_all(silu_mul_fp8(x.cuda(), c.to(torch.bfloat16).cuda()), x, c.to(torch.bfloat16))
+    c = (torch.randn(len(e), 128, generator=g).double() * torch.exp2(-60 - e / 2)).to(torch.bfloat16)
+    check_silu_of_all(silu_mul_fp8(x.cuda(), c.cuda()), x, c)
+    check_silu_of_all(silu_mul_fp8(c.cuda(), x.cuda()), c, x)
+
+
+@pytest.mark.gpu
+def test_silu_mul_of_gates_without_end():
+    """An infinite or NaN gate, or a, gives NaN, beside far gates too."""
+    inf = math.inf
+    a = torch.tensor([[1.0, 1.0, 1.0, inf, -inf, math.nan, inf, 0.0, 1.0, 2.0]]).to(torch.bfloat16)
+    c = torch.tensor([[inf, -inf, math.nan, -100.0, 100.0, -100.0, -3e38, inf, -100.0, 1.0]]).to(torch.bfloat16)
+    for x, y in ((a, c), (a[:, :8], c[:, :8])):
+        r = silu_mul_fp8(x.cuda(), y.cuda())
+        assert torch.isnan(r.codes.float().cpu()[0, :8]).all() and not torch.isnan(r.codes[0, 8:].float()).any()
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("residual", [False, True])
