@@ -184,25 +184,20 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
   put_block(o, row, b, l16, c, byte);
 }
 
-// 1 / sqrt(ss inv_dim + eps) as hi + lo: the unit's estimate in fp64 (2^-23 off at
-// most) and one Newton step; 0 for a row with an infinity.  For rows that large that hi
-// and lo would lose digits below fp32's normal numbers, 2^64 of it (true)
-__device__ __forceinline__ bool rstd_of(double ss, double inv_dim, float eps, float& hi, float& lo) {
+// 1 / sqrt(ss inv_dim + eps): the unit's estimate in fp64 (2^-23 off at most) and one Newton
+// step; 0 for a row with an infinity
+__device__ __forceinline__ double rstd_of(double ss, double inv_dim, float eps) {
   const double m = fma(ss, inv_dim, static_cast<double>(eps)), e = __builtin_amdgcn_rsq(m);
-  double r = m == static_cast<double>(__builtin_inff()) ? 0.0 : e * fma(-0.5 * m, e * e, 1.5);
-  const bool large = r < 0x1p-64;
-  r *= large ? 0x1p64 : 1.0;
-  hi = static_cast<float>(r);
-  lo = static_cast<float>(r - static_cast<double>(hi));
-  return large;
+  return m == static_cast<double>(__builtin_inff()) ? 0.0 : e * fma(-0.5 * m, e * e, 1.5);
 }
 
 // Four fp32 roundings leave a value within four of its last steps.  Its code is then the
 // exact value's unless a border of the codes or of the scale lies that near.  All have the
 // last 19 bits zero: ties have five significant bits, four or fewer below 2^-6 of the
-// scale, and 448 has three.  So a wave takes the remainders along (to_odd) only where one
-// of its numbers lies within six steps of such bits, a piece of 512 in 80, or where fp32
-// runs out below (64 M numbers of dim 1024 without residual 45 us, with them always 54).
+// scale, and 448 has three.  So a wave takes them in fp64 (to_odd) only where one of its
+// numbers lies within six steps of such bits, a piece of 512 in 80, or where fp32 runs out:
+// for small values, and for rows whose factor is beyond 2^-64 or 2^64 (64 M numbers of dim
+// 1024 without residual 48 us, all in fp64 63).
 // A row stays in registers between its sum of squares and its codes: W waves a row
 // and V pieces of 8 columns a lane (W = 1: four rows a workgroup).  The squares are
 // summed in fp64, at fp32's rate but for the widening: in fp32 the row's factor is off
@@ -251,36 +246,34 @@ __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
     if (lane == 0) part[tid >> 6] = ss;
     __syncthreads();
     ss = 0.0;
-#pragma unroll
+#pragma unroll 4   // (16 at a time take the registers of a second workgroup on the CU)
     for (int i = 0; i < W; ++i) ss += part[i];
   }
-  float hi, lo;
-  if (rstd_of(ss, inv_dim, eps, hi, lo)) {
-#pragma unroll
-    for (int j = 0; j < V; ++j)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[j][i] *= 0x1p-64f;
-  }
+  const double rstd = rstd_of(ss, inv_dim, eps);
+  const float hi = static_cast<float>(rstd);
+  const bool far = !(rstd >= 0x1p-64 && rstd <= 0x1p64);
 #pragma unroll
   for (int j = 0; j < V; ++j) {
     const int p = t + 64 * W * j, k = 8 * p, b = p >> 4;
     if constexpr (V > 2) load8<float>(w[j], weight, k, dim);
     float y[8], top = 0.0f;
-    bool near = false;
+    bool near = far;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       y[i] = v[j][i] * hi * (1.0f + w[j][i]);
       near |= ((__float_as_uint(y[i]) + 6u) & 0x7ffffu) <= 12u && y[i] != 0.0f;
       top = fmaxf(top, fabsf(y[i]));
     }
-    if (__any(near || (top < 0x1p-80f && top != 0.0f))) {
+    if (top < 0x1p-80f) {   // (with a number that is not 0)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) near |= v[j][i] != 0.0f;
+    }
+    if (__any(near)) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        // (q + e) (g + gl) with q + e = v rstd and g + gl = 1 + w
-        const float g = 1.0f + w[j][i], gl = w[j][i] - (g - 1.0f);
-        const float q = v[j][i] * hi, e = fmaf(v[j][i], hi, -q) + v[j][i] * lo;
-        const float c = fmaf(e, g, q * gl), t = fmaf(q, g, c);
-        y[i] = to_odd(t, fmaf(q, g, -t) + c);
+        float a = v[j][i];
+        asm volatile("" : "+v"(a));   // (widened anew: the squares' fp64 copies would fill the registers)
+        y[i] = to_odd(static_cast<double>(a) * rstd * (1.0 + static_cast<double>(w[j][i])));
       }
     }
 #pragma unroll

@@ -497,6 +497,41 @@ def test_rms_norm_of_odd_rows():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dim", [1, 130, 640, 1500, 2500, 9000])
+def test_rms_norm_of_tiny_rows(dim, residual, dtype):
+    """Rows below fp32's normal numbers, whose factor passes fp32, with eps 0 and near it."""
+    x = rand(6, dim, seed=18, dtype=torch.float32, big=False)
+    for i, e in enumerate((-126, -130, -133, -140, -143, 0)):
+        x[i] *= 2.0 ** e
+    x[4, 0] = 2.0 ** -133 if dtype == torch.bfloat16 else 1e-45     # (not all zeros)
+    x = x.to(dtype)
+    res = rand(6, dim, seed=19, dtype=dtype, big=False) * 2.0 ** -130 if residual else None
+    w = 0.3 * rand(dim, seed=20, dtype=torch.float32, big=False)
+    for eps in (0.0, 2.0 ** -149):
+        t, v = ref.rms_norm(x, w, eps, res)
+        got = rms_norm_fp8(x.cuda(), w.cuda(), eps, residual=None if res is None else res.cuda())
+        if residual:
+            assert torch.equal(got[0].cpu(), t)
+            got = got[1]
+        keep = t.double().abs().sum(1) > 0 if eps == 0 else torch.ones(6, dtype=torch.bool)
+        assert keep.sum() >= 4
+        same_rows(Fp8Rows(got.codes.cpu()[keep], got.scales.cpu().view(torch.uint8)[keep].view(E8), dim), v[keep])
+        assert torch.isnan(got.codes.float().cpu()[~keep, :dim]).all()      # (0 / 0)
+
+
+@pytest.mark.gpu
+def test_rms_norm_of_large_weights():
+    """Numbers that the factor takes below fp32 and the weight brings back."""
+    x, w = rand(3, 512, seed=21, dtype=torch.float32, big=False) * 1e-18, rand(512, seed=22, dtype=torch.float32, big=False)
+    x[:, 3] = 1e30
+    w[128:256] *= 1e25
+    w[256:] *= 1e10
+    same_rows(rms_norm_fp8(x.cuda(), w.cuda(), 1e-6), ref.rms_norm(x, w, 1e-6)[1])
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("fn", [lambda x: quantize_rows_fp8(x), lambda x: silu_mul_fp8(x, x),
                                 lambda x: rms_norm_fp8(x, torch.zeros(200, device="cuda"))])
 def test_no_rows(fn):
