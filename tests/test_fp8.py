@@ -3,7 +3,7 @@ oracle/fp8.py in float64.
 
 Rows: quantize_rows_fp8 and rms_norm_fp8 round a value known to some 2^-45 of itself
 (products of two fp32 or bf16 numbers are taken with their remainder, the norm's
-factor in two words) to odd and then to e4m3, so the codes and scales are the
+in fp64 where fp32 may not do) to odd and then to e4m3, so the codes and scales are the
 oracle's own, bit for bit; the inputs here are random, no exact norm lies within
 2^-40 of a tie.  silu_mul_fp8's value has seven fp32 roundings (e^-c 1 ulp and the
 remainder's product, the sum, a reciprocal with one correction, two products): it
