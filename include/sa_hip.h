@@ -377,7 +377,7 @@ int sa_int4_dequant_bf16(const void* packed, const void* scales, const void* zer
 int sa_rows_fp8(int dtype, const void* x, const void* gate, int silu, int64_t rows, int dim,
                 int64_t ldx, int64_t ldg, void* codes, void* scales, void* stream);
 int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, const float* weight,
-                    int64_t rows, int dim, int64_t ldx, float eps, void* sum, void* codes,
+                    int64_t rows, int dim, int64_t ldx, double eps, void* sum, void* codes,
                     void* scales, void* stream);
 
 /*

@@ -186,8 +186,8 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
 
 // 1 / sqrt(ss inv_dim + eps): the unit's estimate in fp64 (2^-23 off at most) and one Newton
 // step; 0 for a row with an infinity
-__device__ __forceinline__ double rstd_of(double ss, double inv_dim, float eps) {
-  const double m = fma(ss, inv_dim, static_cast<double>(eps)), e = __builtin_amdgcn_rsq(m);
+__device__ __forceinline__ double rstd_of(double ss, double inv_dim, double eps) {
+  const double m = fma(ss, inv_dim, eps), e = __builtin_amdgcn_rsq(m);
   return m == static_cast<double>(__builtin_inff()) ? 0.0 : e * fma(-0.5 * m, e * e, 1.5);
 }
 
@@ -205,7 +205,7 @@ __device__ __forceinline__ double rstd_of(double ss, double inv_dim, float eps) 
 template <typename T, bool RES, int V, int W>
 __global__ __launch_bounds__(W == 1 ? 256 : 64 * W) void rms_norm_fp8_kernel(
     const T* __restrict__ x, const T* __restrict__ res, const float* __restrict__ weight, long rows, long ldx,
-    int dim, double inv_dim, float eps, T* __restrict__ sum, const RowsOut o) {
+    int dim, double inv_dim, double eps, T* __restrict__ sum, const RowsOut o) {
   const int tid = threadIdx.x, lane = tid & 63;
   const long row = W == 1 ? blockIdx.x * 4L + (tid >> 6) : static_cast<long>(blockIdx.x);
   const int t = W == 1 ? lane : tid, l16 = tid & 15;
@@ -305,7 +305,7 @@ void rows_go(int mode, const void* x, const void* gate, long ldx, long ldg, int 
 
 constexpr long kFewRows = 512;
 template <typename T, bool RES>
-void norm_go(const void* x, const void* res, const float* w, long rows, long ldx, int dim, float eps, void* sum,
+void norm_go(const void* x, const void* res, const float* w, long rows, long ldx, int dim, double eps, void* sum,
              const RowsOut& o, hipStream_t s) {
   auto go = [&](auto kern, int waves) {
     const long grid = waves == 1 ? (rows + 3) / 4 : rows;
@@ -378,7 +378,7 @@ extern "C" int sa_rows_fp8(int dtype, const void* x, const void* gate, int silu,
 }
 
 extern "C" int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, const float* weight, int64_t rows,
-                               int dim, int64_t ldx, float eps, void* sum, void* codes, void* scales, void* stream) {
+                               int dim, int64_t ldx, double eps, void* sum, void* codes, void* scales, void* stream) {
   const char* who = "sa_rms_norm_fp8";
   if (const int rc = sa::rows_check(who, dtype, rows, dim, codes, scales)) return rc;
   if (rows == 0) return 0;

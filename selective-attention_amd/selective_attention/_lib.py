@@ -18,6 +18,7 @@ _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _i64 = ctypes.c_int64
 _f = ctypes.c_float
+_d = ctypes.c_double
 _sz = ctypes.c_size_t
 
 # name -> argtypes; kept in the same order as include/sa_hip.h
@@ -76,7 +77,7 @@ SIGNATURES: dict[str, list] = {
     "sa_int4_linear_bf16": [_vp, _vp, _i, _i, _i, _i, _i, ctypes.POINTER(_i64), _vp],
     "sa_int4_dequant_bf16": [_vp, _vp, _vp, _i, _i, _i, _vp, _vp],
     "sa_rows_fp8": [_i, _vp, _vp, _i, _i64, _i, _i64, _i64, _vp, _vp, _vp],
-    "sa_rms_norm_fp8": [_i, _vp, _vp, _vp, _i64, _i, _i64, _f, _vp, _vp, _vp, _vp],
+    "sa_rms_norm_fp8": [_i, _vp, _vp, _vp, _i64, _i, _i64, _d, _vp, _vp, _vp, _vp],
     "sa_fp8_linear": [_vp, _vp, _i64, _i, _i, ctypes.POINTER(_i64), _vp],
     "sa_fp8_linear_bf16": [_vp, _vp, _i, _i, _i64, _i64, _i, ctypes.POINTER(_i64), _vp],
     "sa_fp8_dequant_bf16": [_vp, _vp, _i, _i, _vp, _vp],

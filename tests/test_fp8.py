@@ -522,6 +522,24 @@ def test_rms_norm_of_tiny_rows(dim, residual, dtype):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("eps", [1e-6, 1e-5, 1e-60])
+def test_rms_norm_takes_eps_as_given(eps):
+    """Rows that eps alone scales, each number next to a tie, on the side that the given eps
+    puts it on: half as far from it as eps in fp32 would move it."""
+    e32 = float(torch.tensor(eps, dtype=torch.float32))
+    off = (eps / e32) ** 0.5 - 1 if e32 else 1e-9
+    side = 1e-9 if abs(off) < 1e-10 else off
+    tie = (torch.arange(8, 16).double() + 0.5).repeat(16) * 2.0 ** -20
+    g = torch.Generator().manual_seed(7)
+    w = 1e-3 * (0.5 + torch.rand(128, generator=g).double())
+    x = (tie * eps ** 0.5 / (1 + w)).float()
+    w = (tie * (1 - side / 2) * eps ** 0.5 / x.double() - 1).float()      # (finer than x: its steps are 2^-33)
+    v = ref.rms_norm(x[None], w, eps)[1]
+    assert ((v / tie - 1).abs() < abs(side)).all() and ((v < tie) == (side > 0)).all()
+    same_rows(rms_norm_fp8(x[None].cuda(), w.cuda(), eps), v)
+
+
+@pytest.mark.gpu
 def test_rms_norm_of_large_weights():
     """Numbers that the factor takes below fp32 and the weight brings back."""
     x, w = rand(3, 512, seed=21, dtype=torch.float32, big=False) * 1e-18, rand(512, seed=22, dtype=torch.float32, big=False)
