@@ -340,11 +340,12 @@ void norm_go(const void* x, const void* res, const float* w, long rows, long ldx
 constexpr int kMaxNormDim = 65536;
 int norm_waves(int dim) { return dim <= 1536 ? 1 : dim <= 10240 ? 4 : 16; }   // at most (as norm_go)
 
+constexpr long kMaxBlocks = ((1L << 24) - 1) * 16;   // 16 a workgroup of 256, a grid of less than 2^32 threads
 int rows_check(const char* who, int dtype, long rows, int dim, const void* codes, const void* scales) {
   SA_CHECK_ARG(dtype == kF32 || dtype == kBF16, "%s: dtype code %d", who, dtype);
   SA_CHECK_ARG(rows >= 0 && dim > 0 && dim <= (1 << 26), "%s: bad sizes rows=%ld dim=%d", who, rows, dim);
-  SA_CHECK_ARG(rows * ((dim + kQBlock - 1L) / kQBlock) < (1L << 28), "%s: %ld rows of %d columns are too many", who,
-               rows, dim);   // (2^32 threads a grid)
+  SA_CHECK_ARG(rows < (1L << 28) && rows * ((dim + kQBlock - 1L) / kQBlock) <= kMaxBlocks,
+               "%s: %ld rows of %d columns are too many", who, rows, dim);
   SA_CHECK_ARG(rows == 0 || (codes && scales), "%s: null pointer", who);
   SA_CHECK_ARG(((reinterpret_cast<uintptr_t>(codes) & 15) | (reinterpret_cast<uintptr_t>(scales) & 3)) == 0,
                "%s: codes or scales are not aligned", who);
@@ -383,8 +384,9 @@ extern "C" int sa_rms_norm_fp8(int dtype, const void* x, const void* residual, c
   if (const int rc = sa::rows_check(who, dtype, rows, dim, codes, scales)) return rc;
   if (rows == 0) return 0;
   SA_CHECK_ARG(dim <= sa::kMaxNormDim, "%s: dim %d above %d", who, dim, sa::kMaxNormDim);
-  SA_CHECK_ARG(rows * 64 * sa::norm_waves(dim) < (1L << 32), "%s: %ld rows of %d columns are too many", who,
-               static_cast<long>(rows), dim);   // (2^32 threads a grid)
+  const int waves = sa::norm_waves(dim);   // (four rows a workgroup where that is one)
+  SA_CHECK_ARG((waves == 1 ? (rows + 3) / 4 * 256 : rows * 64 * waves) < (1L << 32),
+               "%s: %ld rows of %d columns are too many", who, static_cast<long>(rows), dim);
   SA_CHECK_ARG(x && weight && (!residual == !sum), "%s: null pointer, or one of residual and sum without the other", who);
   SA_CHECK_ARG(ldx >= dim, "%s: row stride %ld below dim %d", who, static_cast<long>(ldx), dim);
   const uintptr_t size = dtype == sa::kF32 ? 4 : 2;

@@ -239,6 +239,29 @@ def test_rows_refuse(what):
         calls[what]()
 
 
+def test_grids_stay_below_their_limit():
+    """2^24 workgroups of 256 are 2^32 threads, one more than a grid may have: the calls
+    that would launch them are refused by their sizes (nothing is read: the addresses
+    are none), the largest that would not pass this check and fail the next."""
+    from selective_attention import _lib
+
+    def rows(n, dim, ldx):
+        return lambda: _lib.call("sa_rows_fp8", 1, 4096, None, 0, n, dim, ldx, dim, 4096, 4096, None)
+
+    def norm(n, dim, ldx):
+        return lambda: _lib.call("sa_rms_norm_fp8", 1, 4096, None, 4096, n, dim, ldx, 1e-6, None, 4096, 4096, None)
+    most = (1 << 24) - 1
+    for make, n, dim in ((rows, 16 * most, 128), (rows, 16 * most, 5), (rows, most, 2048), (rows, 5 * most, 300),
+                         (norm, 4 * most, 100), (norm, 4 * most, 512), (norm, (1 << 24) - 1, 2000), (norm, (1 << 21) - 1, 16384),
+                         (norm, 16 * most // 12, 1536)):
+        with pytest.raises(RuntimeError, match="row stride"):
+            make(n, dim, dim - 1)()
+    for make, n, dim in ((rows, 16 * most + 1, 128), (rows, (1 << 28) - 1, 7), (rows, most + 1, 2048), (norm, 4 * most + 1, 100),
+                         (norm, (1 << 26) - 1, 512), (norm, 1 << 24, 2000), (norm, 1 << 22, 16384), (rows, 1 << 40, 1 << 26)):
+        with pytest.raises(RuntimeError, match="too many"):
+            make(n, dim, dim - 1)()
+
+
 # --- rows on the GPU ---------------------------------------------------------------
 SHAPES = [(1, 1), (3, 127), (2, 128), (5, 130), (1, 512), (4, 1000), (7, 1024), (3, 2056), (65, 4096), (2, 4100),
           (3, 8200), (2, 16384), (1, 20000)]
