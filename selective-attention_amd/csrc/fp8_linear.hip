@@ -729,7 +729,7 @@ __global__ __launch_bounds__(128) void fp8_dequant_kernel(const uint8_t* __restr
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       v[e] = ldexpf(__builtin_amdgcn_cvt_f32_fp8(static_cast<int>(u[e >> 2] >> (8 * (e & 3))), 0), static_cast<int>(byte) - 127);
-    if (k + 8 <= K) {
+    if (k <= K - 8) {   // (K may be int's last)
       *reinterpret_cast<v4u_any*>(o) =
           v4u_any{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
     } else {

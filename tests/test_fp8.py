@@ -816,6 +816,20 @@ def test_dequantize(N, K):
         dequantize_fp8(packed.cuda(), scales.cuda(), N + 16, K)
 
 
+@pytest.mark.gpu
+def test_dequantize_of_the_widest_weight():
+    """2^31 - 1 columns: the last piece of a row stops at its end."""
+    from selective_attention import _lib
+    K = (1 << 31) - 1
+    packed = torch.zeros(1, 1 << 24, 8, 16, 16, dtype=torch.uint8, device="cuda")
+    packed[0, -1, :, 0] = torch.ones(8, 16).to(E4).view(torch.uint8)
+    scales = torch.full((1, 1 << 24), 128, dtype=torch.uint8, device="cuda")
+    pool = torch.full((K + 9,), 7.0, dtype=torch.bfloat16, device="cuda")
+    _lib.call("sa_fp8_dequant_bf16", packed.data_ptr(), scales.data_ptr(), 1, K, pool.data_ptr(), _lib.stream_of(pool))
+    assert (pool[K:] == 7).all() and (pool[K - 127:K] == 2).all() and not pool[K - 4096:K - 127].any()
+    assert not pool[:4096].any()
+
+
 # --- gradients -------------------------------------------------------------------------
 @pytest.mark.gpu
 @pytest.mark.parametrize("M", [3, 100])
