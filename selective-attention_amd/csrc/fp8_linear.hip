@@ -89,15 +89,15 @@ __device__ __forceinline__ void load16(uint4 (&q)[2], const bf16* row, int k, in
     }
   }
 }
+__device__ __forceinline__ uint32_t word_of(const uint4 (&q)[2], int i) {
+  const uint4& u = q[i >> 2];
+  return (i & 3) == 0 ? u.x : (i & 3) == 1 ? u.y : (i & 3) == 2 ? u.z : u.w;
+}
 __device__ __forceinline__ void widen16(float* v, const uint4 (&q)[2]) {
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t u[4] = {q[i].x, q[i].y, q[i].z, q[i].w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[8 * i + 2 * e] = bf16lo_to_f32(u[e]);
-      v[8 * i + 2 * e + 1] = bf16hi_to_f32(u[e]);
-    }
+  for (int i = 0; i < 8; ++i) {
+    v[2 * i] = bf16lo_to_f32(word_of(q, i));
+    v[2 * i + 1] = bf16hi_to_f32(word_of(q, i));
   }
 }
 template <int CT, int R, int NW, int X>
@@ -191,10 +191,23 @@ __global__ __launch_bounds__(64 * NW) void fp8_few_kernel(const Fp8X in, const F
 #pragma unroll
           for (int i = 0; i < 2; ++i) widen16(f + 16 * i, q.gate[t][i]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] *= f[i];   // (exact)
+          for (int i = 0; i < 32; ++i) v[i] *= f[i];   // (exact but for those below fp32's normal numbers)
         }
 #pragma unroll
         for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));   // (a NaN is passed over)
+        if constexpr (X == kGated) {
+          if (__any(top < 0x1p-100f && top != 0.0f)) {
+            top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              uint32_t a = word_of(q.x[t][i >> 3], i & 7), b = word_of(q.gate[t][i >> 3], i & 7);
+              asm volatile("" : "+v"(a), "+v"(b));   // (widened anew: the first copies would stay in registers)
+              v[2 * i] = to_odd(static_cast<double>(bf16lo_to_f32(a)) * bf16lo_to_f32(b));
+              v[2 * i + 1] = to_odd(static_cast<double>(bf16hi_to_f32(a)) * bf16hi_to_f32(b));
+              top = fmaxf(top, fmaxf(fabsf(v[2 * i]), fabsf(v[2 * i + 1])));
+            }
+          }
+        }
         const bool rare = __any(top == __builtin_inff());
         if (rare) {
           top = 0.0f;

@@ -146,14 +146,20 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
   if constexpr (MODE != kPlain) {
     float c[8];
     load8<T>(c, gate + row * ldg, k, dim);
+    float y[8];
     if constexpr (MODE == kGated) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float y = v[i] * c[i];
-        v[i] = to_odd(y, fmaf(v[i], c[i], -y));   // (exact for bf16)
+        const float p = v[i] * c[i];
+        y[i] = to_odd(p, fmaf(v[i], c[i], -p));   // (exact for bf16)
+      }
+      top = top_of(y);
+      if (top < 0x1p-100f && top != 0.0f) {   // (fp32 loses the remainder)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = to_odd(static_cast<double>(v[i]) * c[i]);
+        top = top_of(y);
       }
     } else {
-      float y[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         // e^-c by the transcendental unit (2^t, 1 ulp), with what t's rounding leaves
@@ -174,11 +180,12 @@ __global__ __launch_bounds__(256) void rows_kernel(const T* __restrict__ x, cons
         for (int i = 0; i < 8; ++i) y[i] = to_odd(silu64(v[i], c[i]));
         top = top_of(y);
       }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = y[i];
     }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = y[i];
+  } else {
+    top = top_of(v);
   }
-  if constexpr (MODE != kSilu) top = top_of(v);
   uint32_t byte;
   const uint2 c = encode_block(v, top, byte);
   put_block(o, row, b, l16, c, byte);

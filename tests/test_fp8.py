@@ -311,6 +311,37 @@ def test_quantize_rows_next_to_ties():
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_tiny_gated_rows_next_to_ties(dtype):
+    """Products below fp32's normal numbers, beside ties of the smallest scale by less than
+    half of fp32's last step there, or half of it: fp32's own product is the tie.  Up to 16 rows of bfloat16 in the product too, whose
+    weight of ones and twos adds codes that fp32 holds."""
+    e = torch.exp2(torch.linspace(20, 60, 128).floor().double())
+    if dtype == torch.bfloat16:     # 145 226 = 2^15 (1 + 2^-14): half of fp32's last step above half of the codes'
+        tie = torch.full((128,), 2.0 ** -136).double()
+        over, f = torch.full((128,), 2.0 ** -14).double(), (145 / 128, 226 / 256)
+    else:
+        tie = ((torch.arange(8) * 2.0 + 1.0) * 2.0 ** -136).double().repeat(16)
+        over = torch.where(torch.arange(128) % 3 == 0, -1.0, 1.0).double() * 2.0 ** -20
+        f = 1 + over, 1.0
+    sign = torch.where(torch.arange(128) % 5 == 0, -1.0, 1.0).double()
+    x = torch.stack([f[0] / e, 1 / e, torch.zeros(128).double()]).to(dtype)
+    gate = torch.stack([f[1] * tie * e * sign, tie * e, torch.ones(128).double()]).to(dtype)
+    v = x.double() * gate.double()
+    assert torch.equal(v[0], tie * (1 + over) * sign) and torch.equal(v[1], tie)
+    assert ((x.float() * gate.float()).double()[0] == tie * sign).all()
+    v = torch.where(v.abs() <= 2.0 ** -150, 0.0, v)
+    r = quantize_rows_fp8(x.cuda(), gate.cuda())
+    same_rows(r, v)
+    if dtype == torch.bfloat16:
+        ws = tuple(t.cuda() for t in pack_fp8(torch.ones(16, 128).to(E4), torch.full((1, 1), 247, dtype=torch.uint8)))
+        for rows in (1, 2, 3):
+            got = fp8_linear(x[:rows].cuda(), *ws, xscale=gate[:rows].cuda())
+            assert torch.equal(got, fp8_linear(Fp8Rows(r.codes[:rows], r.scales[:rows]), *ws))
+            assert torch.equal(got.double().cpu()[:, 0], (ref.values(r.codes[:rows], r.scales[:rows], 128).sum(1) * 2.0 ** 120).to(torch.bfloat16).double())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_rows_that_are_not_finite(dtype):
     x = rand(6, 300, seed=8, dtype=dtype)
     x[1, 7], x[2, 140], x[3, 299] = math.inf, -math.inf, math.nan
