@@ -239,6 +239,212 @@ def test_rows_refuse(what):
         calls[what]()
 
 
+def off_by(t, n):
+    """t's values n bytes behind a 16-byte boundary."""
+    raw = torch.empty(t.numel() * t.element_size() + 16 + n, dtype=torch.uint8)
+    at = -raw.data_ptr() % 16 + n
+    out = raw[at:at + t.numel() * t.element_size()].view(t.dtype).view(t.shape)
+    return out.copy_(t)
+
+
+# what is wrong, and what the call says of it; "" names nothing: the call is whole, and
+# only a device is missing
+LINEAR_SAYS = {
+    "": "no CPU path", "bias given": "no CPU path", "gated": "no CPU path", "rows": "no CPU path", "one row": "no CPU path",
+    "uint8 scales": "no CPU path",
+    "dtype": "x must be bfloat16", "features": "packed must be", "more features": "packed must be", "outs": "packed must be",
+    "no outs": "packed must be", "packed type": "packed must be", "packed layout": "packed must be",
+    "packed flat": "packed must be", "packed strides": "must be contiguous on 16- and 4-byte", "packed place": "must be contiguous on 16- and 4-byte",
+    "scales": "scales must be", "scales rows": "scales must be", "scale type": "scales must be .* or its bytes",
+    "scales strides": "must be contiguous on 16- and 4-byte", "scales place": "must be contiguous on 16- and 4-byte",
+    "bias": r"\[bias\] Shape mismatch", "bias type": "bias must be bfloat16", "xscale": "xscale must be", "xscale type": "xscale must be",
+    "rows xscale": "xscale goes with x as a tensor", "codes": "codes must be", "codes short": "codes must be", "codes long": "codes must be",
+    "rows scales": "scales must be .* beside codes", "rows scales short": "scales must be .* beside codes",
+    "rows scales type": "scales must be .* beside codes", "no features": "x must have features", "no x": "x must have features",
+    "none": "1..4 weights", "five": "1..4 weights", "biases": "1..4 weights", "sizes": "1..4 weights", "second": "packed must be",
+}
+
+
+@pytest.mark.parametrize("what", LINEAR_SAYS)
+def test_linear_says_what_is_wrong(what):
+    """Each check by its own words: without it the call would get as far as its device."""
+    packed, scales = quantize_fp8(rand(160, 256, dtype=torch.float32))
+    x, bias, xscale, N = torch.zeros(3, 256, dtype=torch.bfloat16), None, None, 160
+    r = make_rows(3, 256)
+    if what == "bias given":
+        bias = torch.zeros(160, dtype=torch.bfloat16)
+    elif what == "gated":
+        xscale = x
+    elif what == "rows":
+        x = r
+    elif what == "one row":
+        x = Fp8Rows(r.codes[0], r.scales[0])
+    elif what == "uint8 scales":
+        x, scales = Fp8Rows(r.codes, r.scales.view(torch.uint8)), scales.view(torch.uint8)
+    elif what == "dtype":
+        x = x.float()
+    elif what == "features":
+        x = x[:, :128]
+    elif what == "more features":
+        x = torch.zeros(3, 257, dtype=torch.bfloat16)
+    elif what == "outs":
+        N = 161
+    elif what == "no outs":
+        packed, scales, N = packed[:0], scales[:0], 0
+    elif what == "packed type":
+        packed = packed.view(torch.int8)
+    elif what == "packed layout":
+        packed = packed.transpose(2, 3)
+    elif what == "packed flat":
+        packed = packed.flatten(3)
+    elif what == "packed strides":
+        packed = packed.transpose(3, 4)
+    elif what == "packed place":
+        packed = off_by(packed, 8)
+    elif what == "scales":
+        scales = scales[:, :2]
+    elif what == "scales rows":
+        scales = scales[:1]
+    elif what == "scale type":
+        scales = scales.float()
+    elif what == "scales strides":
+        scales = scales.view(torch.uint8).t().contiguous().t()
+    elif what == "scales place":
+        scales = off_by(scales.view(torch.uint8), 2)
+    elif what == "bias":
+        bias = torch.zeros(159, dtype=torch.bfloat16)
+    elif what == "bias type":
+        bias = torch.zeros(160)
+    elif what == "xscale":
+        xscale = x[:1]
+    elif what == "xscale type":
+        xscale = x.float()
+    elif what == "rows xscale":
+        x, xscale = r, x
+    elif what == "codes":
+        x = Fp8Rows(r.codes.float(), r.scales)
+    elif what == "codes short":
+        x = Fp8Rows(r.codes[:, :128], r.scales, 256)
+    elif what == "codes long":
+        x = Fp8Rows(r.codes, r.scales, 128)
+    elif what == "rows scales":
+        x = Fp8Rows(r.codes, r.scales[:1])
+    elif what == "rows scales short":
+        x = Fp8Rows(r.codes, r.scales[:, :2])
+    elif what == "rows scales type":
+        x = Fp8Rows(r.codes, r.scales.float())
+    elif what == "no features":
+        x = x[:, :0]
+    elif what == "no x":
+        x = x[0, 0]
+    ws, bs, sizes = [(packed, scales)], [bias], [N]
+    if what == "none":
+        ws, bs, sizes = [], [], []
+    elif what == "five":
+        ws, bs, sizes = ws * 5, bs * 5, sizes * 5
+    elif what == "biases":
+        bs = []
+    elif what == "sizes":
+        sizes = sizes * 2
+    elif what == "second":
+        ws, bs, sizes = ws * 2, bs * 2, [160, 176]
+    calls = [lambda: fp8_linear_multi(x, ws, bs, sizes, xscale)]
+    if len(ws) == len(bs) == len(sizes) == 1:
+        calls.append(lambda: fp8_linear(x, packed, scales, bias, N, xscale))
+    for call in calls:
+        with pytest.raises((ValueError, TypeError), match=LINEAR_SAYS[what]):
+            call()
+
+
+def test_rows_that_do_not_belong_together_are_named():
+    """Codes and scales of different leading sizes, each by the words of its own check."""
+    packed, scales = quantize_fp8(rand(32, 256, dtype=torch.float32))
+    r = make_rows(6, 256)
+    c, s = r.codes, r.scales
+    for codes, sc in ((c, s[0]), (c[0], s), (c[0], s[0, 0]), (c, s.view(2, 3, 4)), (c.view(2, 3, 256), s),
+                      (c.view(2, 3, 256), s.view(3, 2, 4)), (c, s[:, :2]), (c, s[:5]), (c[:5], s)):
+        with pytest.raises(ValueError, match="beside codes"):
+            fp8_linear(Fp8Rows(codes, sc, 256), packed, scales, out_features=32)
+    for codes in (c[:, :128], c[0, 0], c.view(6, 2, 128)):
+        with pytest.raises(ValueError, match="codes must be"):
+            fp8_linear(Fp8Rows(codes, s, 256), packed, scales, out_features=32)
+    with pytest.raises(ValueError, match="no CPU path"):
+        fp8_linear(Fp8Rows(c, s, 256), packed, scales, out_features=32)
+
+
+def test_rows_say_what_is_wrong():
+    x, w = torch.zeros(2, 8), torch.zeros(8)
+    h = x.to(torch.bfloat16)
+    g, hg = x.clone().requires_grad_(), h.clone().requires_grad_()
+    wide = torch.zeros(1, 65537)
+    says = [
+        ("no CPU path", lambda: quantize_rows_fp8(x)), ("no CPU path", lambda: quantize_rows_fp8(h, h)),
+        ("no CPU path", lambda: silu_mul_fp8(h, h)), ("no CPU path", lambda: rms_norm_fp8(x, w)),
+        ("no CPU path", lambda: rms_norm_fp8(h, w, 0.0, h)), ("no CPU path", lambda: rms_norm_fp8(wide[:, 1:], wide[0, 1:])),
+        ("no CPU path", lambda: rms_norm_fp8(x, w.to(torch.bfloat16))),
+        ("x must have features", lambda: quantize_rows_fp8(x[:, :0])), ("x must have features", lambda: quantize_rows_fp8(x[0, 0])),
+        ("x must have features", lambda: silu_mul_fp8(h[:, :0], h[:, :0])), ("x must have features", lambda: rms_norm_fp8(x[:, :0], w[:0])),
+        ("xscale must be", lambda: quantize_rows_fp8(x, h)), ("xscale must be", lambda: quantize_rows_fp8(x, x[:1])),
+        ("c must be", lambda: silu_mul_fp8(h, h[:1])), ("c must be", lambda: silu_mul_fp8(h, x)),
+        ("a and c must be bfloat16", lambda: silu_mul_fp8(x, x)),
+        ("residual must be", lambda: rms_norm_fp8(x, w, residual=h)), ("residual must be", lambda: rms_norm_fp8(x, w, residual=x[:1])),
+        (r"\[weight\] Shape mismatch", lambda: rms_norm_fp8(x, w[:7])), (r"\[weight\] Shape mismatch", lambda: rms_norm_fp8(x, w[None])),
+        ("at most 65536", lambda: rms_norm_fp8(wide, wide[0])),
+        ("must not be negative", lambda: rms_norm_fp8(x, w, -1e-9)), ("must not be negative", lambda: rms_norm_fp8(x, w, math.nan)),
+        ("codes have no gradient", lambda: quantize_rows_fp8(g)), ("codes have no gradient", lambda: quantize_rows_fp8(x, g)),
+        ("codes have no gradient", lambda: silu_mul_fp8(hg, h)), ("codes have no gradient", lambda: silu_mul_fp8(h, hg)),
+        ("codes have no gradient", lambda: rms_norm_fp8(g, w)), ("codes have no gradient", lambda: rms_norm_fp8(x, g[0])),
+        ("codes have no gradient", lambda: rms_norm_fp8(x, w, residual=g)),
+    ]
+    for words, call in says:
+        with pytest.raises((ValueError, TypeError, RuntimeError), match=words):
+            call()
+    with torch.no_grad():
+        for call in (lambda: quantize_rows_fp8(g), lambda: silu_mul_fp8(hg, hg), lambda: rms_norm_fp8(g, g[0], residual=g)):
+            with pytest.raises(ValueError, match="no CPU path"):
+                call()
+
+
+def test_weights_say_what_is_wrong():
+    codes, ones = torch.zeros(130, 128).to(E4), torch.ones(2, 1)
+    w = torch.zeros(4, 4)
+    packed, scales = quantize_fp8(torch.ones(32, 256))
+    x = torch.zeros(3, 256, dtype=torch.bfloat16)
+    bad = w.clone()
+    bad[1, 2] = math.inf
+    says = [
+        (r"\[codes\] Dim mismatch", lambda: pack_fp8(codes[0], ones)), ("pack_fp8: empty weight", lambda: pack_fp8(codes[:0], ones[:0])),
+        ("pack_fp8: empty weight", lambda: pack_fp8(codes[:, :0], ones[:, :0])),
+        ("codes must be", lambda: pack_fp8(codes.float(), ones)), (r"\[scales\] Shape mismatch", lambda: pack_fp8(codes, ones[:1])),
+        ("codes hold NaN", lambda: pack_fp8(torch.full((130, 128), math.nan).to(E4), ones)),
+        ("powers of two", lambda: pack_fp8(codes, 3 * ones)), ("powers of two", lambda: pack_fp8(codes, -ones)),
+        ("powers of two", lambda: pack_fp8(codes, 2.0 ** -127 * ones.double())), ("floating or e8m0", lambda: pack_fp8(codes, ones.long())),
+        (r"scales must be 2\^-126", lambda: pack_fp8(codes, torch.zeros(2, 1, dtype=torch.uint8))),
+        (r"\[weight\] Dim mismatch", lambda: quantize_fp8(w[0])), ("quantize_fp8: empty weight", lambda: quantize_fp8(w[:0])),
+        ("quantize_fp8: empty weight", lambda: quantize_fp8(w[:, :0])), ("quantize_fp8: the weight holds", lambda: quantize_fp8(bad)),
+        ("packed must be", lambda: dequantize_fp8(packed.flatten(3), scales)), ("packed must be", lambda: dequantize_fp8(packed, scales, 33, 256)),
+        ("packed must be", lambda: dequantize_fp8(packed, scales, 32, 257)), ("scales must be", lambda: dequantize_fp8(packed, scales[:, :1])),
+        ("no CPU path", lambda: dequantize_fp8(packed, scales)), ("no CPU path", lambda: dequantize_fp8(packed, scales, 17, 129)),
+        ("packed must be", lambda: dequantize_fp8(packed.flatten()[0], scales)),
+        ("packed must be", lambda: fp8_linear(x, packed.flatten()[0], scales)),
+        ("packed must be", lambda: fp8_linear(x, packed.flatten(3), scales)), ("no CPU path", lambda: fp8_linear(x, packed, scales)),
+    ]
+    for words, call in says:
+        with pytest.raises((ValueError, TypeError), match=words):
+            call()
+
+
+@pytest.mark.gpu
+def test_rows_of_other_types_are_refused():
+    x, w = torch.zeros(2, 8, device="cuda"), torch.zeros(8, device="cuda")
+    for t in (torch.float64, torch.float16, torch.int32):
+        y = x.to(t)
+        for call in (lambda: quantize_rows_fp8(y), lambda: quantize_rows_fp8(y, y), lambda: rms_norm_fp8(y, w),
+                     lambda: rms_norm_fp8(y, w, residual=y)):
+            with pytest.raises(TypeError, match="unsupported activation dtype"):
+                call()
+
+
 def test_grids_stay_below_their_limit():
     """2^24 workgroups of 256 are 2^32 threads, one more than a grid may have: the calls
     that would launch them are refused by their sizes (nothing is read: the addresses
