@@ -858,22 +858,24 @@ constexpr Fp8Shape kFp8Shapes[] = {
     {128, 256, 7.76f, 0.745f, 5.17f, 1.94f, 0.865f},
     {256, 256, 8.2f, 1.1f, 2.2f, 7.8f, 1.43f},   // (full of such tiles the card is bound by power)
 };
-int fp8_shape(const Fp8Segs& sg, int M, int kb, int shapes, float* per_cu) {   // of the first `shapes`
+int fp8_shape(const Fp8Segs& sg, int M, int kb, float* per_cu) {
   constexpr int kShapes = sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]);
   int best = 0;
   float least = 0.0f;
-  for (int i = 0; i < shapes; ++i) {
+  for (int i = 0; i < kShapes; ++i) {
     const Fp8Shape& p = kFp8Shapes[i];
     long tiles = 0;
     for (int k = 0; k < sg.nseg; ++k) tiles += (sg.N[k] + p.bn - 1) / p.bn;
     tiles *= (M + p.bm - 1) / p.bm;
     if (tiles >= 1 << 23) continue;   // (2^32 threads a grid, of up to 512 a tile)
-    if ((i == 2 || i == 3) && tiles > 256) continue;   // (1 row, 4096 -> 32000: 16 x 64 25.6, 64 x 128 24.7)
+    // (their line holds for one tile a CU alone: with more, 64 rows, 1024 -> 4384 would take
+    // 16 x 64, 8.0 us, for 64 x 64, 5.4, and 400 rows, 4096 -> 1024 14.5 for 11.2)
+    if ((i == 2 || i == 3) && tiles > 256) continue;
     const float r = static_cast<float>(tiles) / 256.0f, k = static_cast<float>(kb), each = p.each0 + p.each1 * k;
     float us = p.first0 + p.first1 * k;
     if (i < kFp8Few) us = std::max(us, p.again + r * each);
     else if (r > 1.0f) us = p.again + 0.5f * (r + static_cast<float>((tiles + 255) / 256)) * each;
-    else if (i == kShapes - 1) us = std::max(us, r * (each + 2.0f));
+    else if (i == kShapes - 1) us = std::max(us, r * (each + 2.0f));   // (300 rows, 1024 -> 32000: 20.8, for 19.0)
     if (least == 0.0f || us < least) {
       least = us;
       best = i;
@@ -900,7 +902,7 @@ void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream
   if (M <= 64) fp8_stream(sg, kb);
   // few tiles a CU get deep rings (the smallest eight waves), more of them room beside each other
   float per_cu = 0.0f;
-  switch (fp8_shape(sg, M, kb, sizeof(kFp8Shapes) / sizeof(kFp8Shapes[0]), &per_cu)) {
+  switch (fp8_shape(sg, M, kb, &per_cu)) {
     case 0: return fp8_few<1, 1, 8, kCodes>(in, sg, M, kb, s);
     case 1: return fp8_few<1, 2, 8, kCodes>(in, sg, M, kb, s);
     case 2: return fp8_few<1, 4, 8, kCodes>(in, sg, M, kb, s);
@@ -917,12 +919,16 @@ void fp8_go(const void* x, const void* xs, Fp8Segs& sg, int M, int kb, hipStream
   }
 }
 
-// up to 16 rows in bfloat16
+// up to 16 rows in bfloat16, which every workgroup rounds again: tiles of 32 columns where
+// those of 16 are more than the CUs (16 gated rows, 1024 -> 4384 4.9 us, by 16 7.6, 8192 -> 8192
+// 20.8 and 36.3; 1 row without gate between 6 % less and 8 % more, 4096 -> 32000 29.1 and 27.0),
+// of 16 where they are not (4096 -> 4096 11.2, by 32 11.5, 1 row 1024 -> 1024 3.05 and 3.65)
 template <int X>
 void fp8_go_bf16(const Fp8X& in, Fp8Segs& sg, int M, int kb, hipStream_t s) {
-  float per_cu = 0.0f;
   fp8_stream(sg, kb);
-  if (fp8_shape(sg, M, kb, 2, &per_cu) == 0) fp8_few<1, 1, 8, X>(in, sg, M, kb, s);
+  long tiles = 0;
+  for (int i = 0; i < sg.nseg; ++i) tiles += (sg.N[i] + 15) / 16;
+  if (tiles <= 256) fp8_few<1, 1, 8, X>(in, sg, M, kb, s);
   else fp8_few<1, 2, 8, X>(in, sg, M, kb, s);
 }
 
