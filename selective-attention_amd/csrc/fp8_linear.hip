@@ -543,7 +543,7 @@ __global__ __launch_bounds__(256 * KS, OCC * KS) void fp8_ring_kernel(const uint
   constexpr int kScales = R * kStage, kRing = kScales + 2048, kSums = SN * SM * 4096;   // (a wave's sums, in bytes)
   constexpr int kParts = (BN + BM) / 16, kDmas = (kParts + 3) / 4;   // DMA instructions of a stage, and of a wave
   static_assert(BM <= 128 && BN <= 256, "a word's scales: two waves' rows, one's columns");
-  static_assert(R >= 3 && R <= 8, "the word after the next comes when the last half-step of this one has been read");
+  static_assert(R >= 3 && R <= 6, "landed knows them; the word after the next comes when this one's has been read");
   static_assert((R - 1) * kDmas + 1 < 63, "vmcnt counts them");
   using Out = Fp8Out<SN, SM>;
   static_assert(4 * Out::kBytes <= R * kStage, "y fits the stages");
@@ -631,7 +631,7 @@ __global__ __launch_bounds__(256 * KS, OCC * KS) void fp8_ring_kernel(const uint
   case k: \
     if constexpr (k < R - 1) __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<(k < R - 1 ? k : 0) * kDmas>()); \
     break;
-      SA_FP8_WAIT(1) SA_FP8_WAIT(2) SA_FP8_WAIT(3) SA_FP8_WAIT(4) SA_FP8_WAIT(5) SA_FP8_WAIT(6)
+      SA_FP8_WAIT(1) SA_FP8_WAIT(2) SA_FP8_WAIT(3) SA_FP8_WAIT(4)
 #undef SA_FP8_WAIT
       default: __builtin_amdgcn_s_waitcnt(vm_lgkm_wait<0>());
     }
