@@ -757,7 +757,7 @@ __global__ __launch_bounds__(128) void fp8_dequant_kernel(const uint8_t* __restr
 // columns of `chunk` rows, eight columns a thread (128 bytes of a row, a line) and every
 // 32nd row, whose sums meet in LDS; more chunks than one go to a second pass over their
 // sums, in order.  32768 x 4096 46 us, 5.8 TB/s; 32768 x 1024 15.5, where 256 columns a
-// workgroup and 256 chunks took 47 in the second pass; 4095 columns 119, no row on a line.
+// workgroup and 256 chunks took 47 in the second pass; 4095 columns 112, no row on a line.
 constexpr int kSumCols = 64, kSumRows = 32;
 template <typename TI, typename TO>
 __global__ __launch_bounds__(256) void colsum_kernel(const TI* __restrict__ x, TO* __restrict__ out, long rows, int N,

@@ -21,7 +21,7 @@
 //
 // Streams of memory: 16 lanes a block, 8 columns a lane, so that a block's maximum is
 // four rotations within a row of lanes and its codes leave as 128 bytes.  Large calls
-// run at the rate of a copy (5.1 TB/s): silu_mul 32768 x 4096 120 us, 5.6 TB/s; norm
+// run at the rate of a copy (5.1 TB/s): silu_mul 32768 x 4096 120 to 126 us, 5.5 TB/s; norm
 // with residual 32768 x 1024 45.8 us, 5.1; rows 8191 x 2056 9.9 us, 5.1.  Few rows are
 // one latency after another: 4 rows 2.3 to 3.4 us, and the call's host time above that.
 #include "fp8.h"

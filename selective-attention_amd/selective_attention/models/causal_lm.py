@@ -89,8 +89,8 @@ class CausalLM(nn.Module):
 
     def quantize_fp8(self) -> "CausalLM":
         """Every linear layer and the head to 8 bits (Fp8Linear), in place, for inference in
-        bfloat16: the norms and SwiGLU's product then leave in 8 bits too, and the
-        products run at twice bfloat16's rate.  The embedding keeps its own table."""
+        bfloat16: the norms and SwiGLU's product then leave in 8 bits too, and large
+        products take 0.55 to 0.6 of bfloat16's time.  The embedding keeps its own table."""
         quantize_linears_fp8(self.layers)
         if isinstance(self.lm_head, nn.Linear):
             self.lm_head = Fp8Linear.from_linear(self.lm_head)
