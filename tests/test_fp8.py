@@ -988,6 +988,30 @@ def test_few_rows_are_rounded_as_by_the_rows_op(M, K, gated):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("gated", [False, True])
+def test_few_rows_at_both_ends_of_their_type(gated):
+    """Subnormal bfloat16 numbers and those next to its end, rounded by the product as by the
+    rows op, which is the oracle's: a weight of one code a row brings each block's codes out."""
+    e = torch.tensor([-133, -130, -127, -126, -124, -120, -100, 100, 120, 125, 126, 127])
+    g = torch.Generator().manual_seed(2)
+    x = ((torch.rand(12, 384, generator=g) + 1).double() * torch.exp2(e.double())[:, None]
+         * torch.exp2(-torch.randint(0, 9, (12, 384), generator=g).double())).to(torch.bfloat16)
+    x[:, ::7] *= -1
+    assert torch.isfinite(x).all()
+    gate = (2.0 ** torch.randint(-1, 1, (12, 384), generator=g)).to(torch.bfloat16) if gated else None
+    v = x.double() if gate is None else x.double() * gate.double()
+    codes, s = ref.rows(v)
+    w = torch.zeros(384, 384)
+    w[torch.arange(384), torch.arange(384)] = 1.0
+    # one scale for both ends would leave bf16: two weights
+    for byte, at in ((247, slice(0, 7)), (7, slice(7, 12))):
+        packed, ws = pack_fp8(w.to(E4), torch.full((3, 3), byte, dtype=torch.uint8))
+        y = fp8_linear(x[at].cuda(), packed.cuda(), ws.cuda(), xscale=None if gate is None else gate[at].cuda())
+        want = codes[at] * s[at, :3].repeat_interleave(128, 1) * 2.0 ** (byte - 127)
+        assert torch.equal(y.cpu().double(), want.to(torch.bfloat16).double())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("M", [1, 20, 300])
 def test_linear_multi(M):
     K, sizes = 600, [128, 1, 300, 513]
